@@ -413,6 +413,83 @@ int fdi4_dequantize_int4(const uint8_t* q, int64_t rows, int num_channels, int64
                          int64_t s_row_stride, int64_t s_channel_stride, float* out,
                          int64_t out_row_stride, hipStream_t stream);
 
+/* Largest number of drafted tokens of fdi4_decode_tree. */
+#define FDI4_MAX_NODES (1024)
+
+/* Workspace for fdi4_decode_window (nodes = 1) and fdi4_decode_tree with the same
+ * arguments (0: none needed). num_splits <= 0 selects the split count. */
+size_t fdi4_decode_rows_workspace_bytes(int batch, int num_q_heads, int nodes, int window,
+                                        int sinks, int num_splits,
+                                        const fdi4_paged_cache* cache);
+
+/* fdi4_decode_paged_ex over a sliding window with sinks: query [b, h] (element
+ * strides, channel stride 1) attends the rows t of sequence b with t < sinks or
+ * t >= n - window, n its length (the query is that of its last token); window >= 1,
+ * sinks >= 0. Only the pages of those rows are read. The cache has group-indexed
+ * scales (s_page_stride 0) and no page_lens. out is contiguous [batch,
+ * num_q_heads, head_dim]; a sequence with no row gives zeros. lens_out as in
+ * fdi4_decode_paged_advance, or NULL. float32 logits from
+ * queries times scales held to 23 bits of their largest, probabilities and sums in
+ * 24 bits or more (16 against 16-bit values that are rounded to 8 on output). */
+int fdi4_decode_window(const void* query, int query_dtype, int batch, int num_q_heads,
+                       int64_t q_batch_stride, int64_t q_head_stride,
+                       const fdi4_paged_cache* cache, int window, int sinks, void* out,
+                       int out_dtype, int num_splits, void* workspace, size_t workspace_bytes,
+                       int32_t* lens_out, hipStream_t stream);
+
+/* Attention of a tree of drafted tokens over the cache and over each other, with
+ * nothing written: query [b, h, i] (i < nodes <= FDI4_MAX_NODES) attends the cached
+ * rows of sequence b and the drafts j with mask[b, i, j] != 0 (a node's ancestors and
+ * itself, for a tree; any mask is taken as it is). k_draft [b, hk, j] is float32,
+ * v_draft the cache's value type (as fdi4_append_paged takes them), element strides,
+ * channel stride 1, rows starting on 16-byte boundaries; mask bytes with byte strides
+ * over sequences and nodes, columns apart by 1 (a batch stride of 0 shares one mask).
+ * window 0: all cached rows; otherwise (window >= nodes) node i, which sees d_i
+ * drafts, attends the cached rows t < sinks and t >= n + d_i - window: the last
+ * `window` tokens of the sequence that it ends. out is contiguous [batch,
+ * num_q_heads, nodes, head_dim]; a node that sees no row and no draft gives zeros.
+ * The accepted drafts go to the cache with fdi4_extend_paged. */
+int fdi4_decode_tree(const void* query, int query_dtype, int batch, int num_q_heads, int nodes,
+                     int64_t q_batch_stride, int64_t q_head_stride, int64_t q_node_stride,
+                     const float* k_draft, int64_t kd_batch_stride, int64_t kd_head_stride,
+                     int64_t kd_node_stride, const void* v_draft, int64_t vd_batch_stride,
+                     int64_t vd_head_stride, int64_t vd_node_stride, const uint8_t* mask,
+                     int64_t mask_batch_stride, int64_t mask_row_stride,
+                     const fdi4_paged_cache* cache, int window, int sinks, void* out,
+                     int out_dtype, int num_splits, void* workspace, size_t workspace_bytes,
+                     hipStream_t stream);
+
+/* fdi4_append_paged of several tokens: sequence b takes counts[b] (clamped to
+ * [0, max_new]) of its new rows k_new[b, h, j] (float32) and v_new[b, h, j] (the
+ * cache's value type) at positions seq_lens[b] .., in order, or, with index (int32
+ * [batch, index_batch_stride], entries clamped to [0, max_new)), token j is new row
+ * index[b, j]. Every scale group touched is quantized over its valid rows, the keys of
+ * the group that is open afterwards go to k_stage; the result equals
+ * fdi4_quantize_paged over the whole sequences. lens_next[b] = seq_lens[b] + the
+ * tokens taken; the cache's lengths are not changed (copy lens_next to them
+ * afterwards). A count that does not fit the cache, or a length outside
+ * [0, max_pages * page_rows], takes nothing. lens_next overlaps neither the
+ * lengths nor the counts; the pages are mapped by the caller. */
+int fdi4_extend_paged(const float* k_new, int64_t kn_batch_stride, int64_t kn_head_stride,
+                      int64_t kn_row_stride, const void* v_new, int64_t vn_batch_stride,
+                      int64_t vn_head_stride, int64_t vn_row_stride, int batch, int max_new,
+                      const int32_t* counts, const int32_t* index, int64_t index_batch_stride,
+                      float* k_stage, int64_t st_batch_stride, int64_t st_head_stride,
+                      int64_t st_row_stride, int group_rows, const fdi4_paged_cache* cache,
+                      int32_t* lens_next, hipStream_t stream);
+
+/* Rows [start, start + length) of every sequence as dense tensors: k_out[b, h, i, :]
+ * = nib*scale - zp*scale in float32 (fdi4_dequantize_int4), rounded once to out_dtype,
+ * and v_out[b, h, i, :] the stored values converted to it, for token start + i; zeros
+ * behind a sequence's end. start[b] from the device (clamped to [0, max_pages *
+ * page_rows]), or start0 for all when start is NULL. Element strides, channel stride
+ * 1, rows on 16-byte boundaries. Group-indexed scales, no page_lens. */
+int fdi4_read_paged(const fdi4_paged_cache* cache, int batch, const int32_t* start, int start0,
+                    int length, void* k_out, int64_t ko_batch_stride, int64_t ko_head_stride,
+                    int64_t ko_row_stride, void* v_out, int64_t vo_batch_stride,
+                    int64_t vo_head_stride, int64_t vo_row_stride, int out_dtype,
+                    hipStream_t stream);
+
 /* Device nibble packing: out[r, j] = q[r, 2j] | q[r, 2j+1] << 4 for
  * j < ceil(C/2) (odd C zero-padded), zero for ceil(C/2) <= j < out_cols.
  * Values are taken modulo 16. Counterpart of pack_int4 (reference

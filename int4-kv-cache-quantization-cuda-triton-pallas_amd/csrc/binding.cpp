@@ -632,6 +632,237 @@ void decode_paged_partials(torch::Tensor query, torch::Tensor k_pages, torch::Te
            "decode_paged_partials");
 }
 
+// Checks shared by decode_window and decode_tree: group-indexed scales and a row of
+// every per-sequence tensor for each of B sequences.
+fdi4_paged_cache make_rows_cache(const torch::Tensor& k_pages, const torch::Tensor& v_pages,
+                                 const torch::Tensor& k_scale, const torch::Tensor& k_zp,
+                                 const c10::optional<torch::Tensor>& page_table,
+                                 const torch::Tensor& seq_lens, int64_t pages_per_group,
+                                 int64_t max_pages, int64_t B) {
+  TORCH_CHECK(pages_per_group >= 1 && pages_per_group <= INT32_MAX && max_pages >= 0 &&
+                  max_pages <= INT32_MAX,
+              "pages_per_group and max_pages are out of range");
+  TORCH_CHECK(k_scale.dim() == 4 && k_scale.size(0) >= B &&
+                  k_scale.size(1) == k_pages.size(1) &&
+                  k_scale.size(2) * pages_per_group >= max_pages,
+              "k_scale must be [batch, kv_heads, >= ceil(max_pages / pages_per_group), head_dim]");
+  TORCH_CHECK(seq_lens.dim() == 1 && seq_lens.size(0) >= B,
+              "seq_lens must have an entry per sequence");
+  if (page_table && page_table->defined()) {
+    TORCH_CHECK(page_table->size(0) >= B, "page_table must have a row per sequence");
+  }
+  return make_cache(k_pages, &v_pages, k_scale, k_zp, page_table, seq_lens, c10::nullopt,
+                    pages_per_group, max_pages);
+}
+
+// Attention of query [B, Hq, D] over the first `sinks` and last `window` rows of
+// every sequence (see fdi4_decode_window); returns [B, Hq, D]. lens_out receives the
+// lengths read, when given.
+torch::Tensor decode_window(torch::Tensor query, torch::Tensor k_pages, torch::Tensor v_pages,
+                            torch::Tensor k_scale, torch::Tensor k_zp,
+                            c10::optional<torch::Tensor> page_table, torch::Tensor seq_lens,
+                            int64_t pages_per_group, int64_t max_pages, int64_t window,
+                            int64_t sinks, int64_t num_splits,
+                            c10::optional<torch::Tensor> lens_out) {
+  CHECK_DEV(query);
+  const int qcode = elem_code(query, "query");
+  TORCH_CHECK(query.dim() == 3 && query.stride(2) == 1,
+              "query must be [batch, heads, head_dim] with contiguous rows");
+  TORCH_CHECK(query.size(2) == k_pages.size(3) * 2, "query head_dim must match the cache");
+  TORCH_CHECK(query.size(1) % k_pages.size(1) == 0, "query heads must be a multiple of kv_heads");
+  TORCH_CHECK(window >= 1 && window <= INT32_MAX && sinks >= 0 && sinks <= INT32_MAX,
+              "window must be >= 1 and sinks >= 0");
+  CHECK_SAME_DEVICE(query, k_pages);
+  const int64_t B = query.size(0);
+  fdi4_paged_cache c = make_rows_cache(k_pages, v_pages, k_scale, k_zp, page_table, seq_lens,
+                                       pages_per_group, max_pages, B);
+  const DeviceGuard guard(query.device());
+  const int Hq = (int)query.size(1), D = (int)query.size(2);
+  int32_t* back = nullptr;
+  if (lens_out && lens_out->defined()) {
+    const torch::Tensor& t = *lens_out;
+    CHECK_INPUT(t);
+    CHECK_SAME_DEVICE(query, t);
+    TORCH_CHECK(t.scalar_type() == torch::kInt32 && t.dim() == 1 && t.size(0) >= B,
+                "lens_out must be int32 [>= batch]");
+    back = t.data_ptr<int32_t>();
+  }
+  auto out = torch::empty({B, Hq, D}, query.options());
+  if (out.numel() == 0) return out;
+  auto ws = workspace(query, fdi4_decode_rows_workspace_bytes((int)B, Hq, 1, (int)window,
+                                                              (int)sinks, (int)num_splits, &c));
+  check_rc(fdi4_decode_window(query.data_ptr(), qcode, (int)B, Hq, query.stride(0),
+                              query.stride(1), &c, (int)window, (int)sinks, out.data_ptr(), qcode,
+                              (int)num_splits, ws.data_ptr(), ws.numel(), back, stream()),
+           "decode_window");
+  return out;
+}
+
+// Attention of query [B, Hq, N, D], the nodes of a drafted tree, over the cache and
+// the drafts that mask [B or 1, N, N] shows (see fdi4_decode_tree); window 0: the whole
+// cache. Returns [B, Hq, N, D].
+torch::Tensor decode_tree(torch::Tensor query, torch::Tensor k_draft, torch::Tensor v_draft,
+                          torch::Tensor mask, torch::Tensor k_pages, torch::Tensor v_pages,
+                          torch::Tensor k_scale, torch::Tensor k_zp,
+                          c10::optional<torch::Tensor> page_table, torch::Tensor seq_lens,
+                          int64_t pages_per_group, int64_t max_pages, int64_t window,
+                          int64_t sinks, int64_t num_splits) {
+  CHECK_DEV(query);
+  CHECK_DEV(k_draft);
+  CHECK_DEV(v_draft);
+  CHECK_DEV(mask);
+  const int qcode = elem_code(query, "query");
+  TORCH_CHECK(query.dim() == 4 && query.stride(3) == 1,
+              "query must be [batch, heads, nodes, head_dim] with contiguous rows");
+  const int64_t B = query.size(0), N = query.size(2);
+  TORCH_CHECK(query.size(3) == k_pages.size(3) * 2, "query head_dim must match the cache");
+  TORCH_CHECK(query.size(1) % k_pages.size(1) == 0, "query heads must be a multiple of kv_heads");
+  TORCH_CHECK(N >= 1 && N <= FDI4_MAX_NODES, "a tree has 1 to ", FDI4_MAX_NODES, " nodes, got ", N);
+  TORCH_CHECK(k_draft.scalar_type() == torch::kFloat32 && k_draft.dim() == 4 &&
+                  k_draft.size(0) == B && k_draft.size(1) == k_pages.size(1) &&
+                  k_draft.size(2) == N && k_draft.size(3) == query.size(3) &&
+                  k_draft.stride(3) == 1,
+              "k_draft must be float32 [batch, kv_heads, nodes, head_dim] with contiguous rows");
+  TORCH_CHECK(v_draft.scalar_type() == v_pages.scalar_type() && v_draft.dim() == 4 &&
+                  v_draft.sizes() == k_draft.sizes() && v_draft.stride(3) == 1,
+              "v_draft must be [batch, kv_heads, nodes, head_dim] in the cache's value dtype");
+  TORCH_CHECK((mask.scalar_type() == torch::kBool || mask.scalar_type() == torch::kUInt8) &&
+                  mask.dim() == 3 && (mask.size(0) == B || mask.size(0) == 1) &&
+                  mask.size(1) == N && mask.size(2) == N && (mask.stride(2) == 1 || N == 1),
+              "mask must be bool [nodes, nodes] or [batch, nodes, nodes] with contiguous rows");
+  TORCH_CHECK(window >= 0 && window <= INT32_MAX && sinks >= 0 && sinks <= INT32_MAX,
+              "window must be >= 1 and sinks >= 0");
+  TORCH_CHECK(window == 0 || window >= N, "a window must hold the nodes: ", window, " < ", N);
+  TORCH_CHECK(window > 0 || sinks == 0, "sinks need a window");
+  CHECK_SAME_DEVICE(query, k_draft);
+  CHECK_SAME_DEVICE(query, v_draft);
+  CHECK_SAME_DEVICE(query, mask);
+  CHECK_SAME_DEVICE(query, k_pages);
+  fdi4_paged_cache c = make_rows_cache(k_pages, v_pages, k_scale, k_zp, page_table, seq_lens,
+                                       pages_per_group, max_pages, B);
+  const DeviceGuard guard(query.device());
+  const int Hq = (int)query.size(1), D = (int)query.size(3);
+  auto out = torch::empty({B, Hq, N, D}, query.options());
+  if (out.numel() == 0) return out;
+  auto ws = workspace(query, fdi4_decode_rows_workspace_bytes((int)B, Hq, (int)N, (int)window,
+                                                              (int)sinks, (int)num_splits, &c));
+  check_rc(fdi4_decode_tree(query.data_ptr(), qcode, (int)B, Hq, (int)N, query.stride(0),
+                            query.stride(1), query.stride(2), k_draft.data_ptr<float>(),
+                            k_draft.stride(0), k_draft.stride(1), k_draft.stride(2),
+                            v_draft.data_ptr(), v_draft.stride(0), v_draft.stride(1),
+                            v_draft.stride(2), static_cast<const uint8_t*>(mask.data_ptr()),
+                            mask.size(0) == 1 ? 0 : mask.stride(0), mask.stride(1), &c,
+                            (int)window, (int)sinks, out.data_ptr(), qcode, (int)num_splits,
+                            ws.data_ptr(), ws.numel(), stream()),
+           "decode_tree");
+  return out;
+}
+
+// Several tokens per sequence into the cache (see fdi4_extend_paged).
+void extend_paged(torch::Tensor k_new, torch::Tensor v_new, torch::Tensor counts,
+                  torch::Tensor k_stage, torch::Tensor k_pages, torch::Tensor v_pages,
+                  torch::Tensor k_scale, torch::Tensor k_zp, torch::Tensor page_table,
+                  torch::Tensor seq_lens, torch::Tensor lens_next, int64_t group_rows,
+                  c10::optional<torch::Tensor> index) {
+  CHECK_DEV(k_new);
+  CHECK_DEV(v_new);
+  CHECK_DEV(k_stage);
+  TORCH_CHECK(k_new.scalar_type() == torch::kFloat32 && k_new.dim() == 4 && k_new.stride(3) == 1,
+              "k_new must be float32 [batch, kv_heads, tokens, head_dim] with contiguous rows");
+  TORCH_CHECK(v_new.scalar_type() == v_pages.scalar_type() && v_new.dim() == 4 &&
+                  v_new.stride(3) == 1 && v_new.sizes() == k_new.sizes(),
+              "v_new must be [batch, kv_heads, tokens, head_dim] in the cache's value dtype");
+  TORCH_CHECK(k_stage.scalar_type() == torch::kFloat32 && k_stage.dim() == 4 &&
+                  k_stage.stride(3) == 1 && k_stage.size(2) >= group_rows,
+              "k_stage must be float32 [batch, kv_heads, >= group_rows, head_dim]");
+  TORCH_CHECK(k_new.size(1) == k_pages.size(1) && k_new.size(3) == k_pages.size(3) * 2 &&
+                  k_stage.size(1) == k_pages.size(1) && k_stage.size(3) == k_new.size(3),
+              "k_new / k_stage heads and head_dim must match the cache");
+  const int64_t B = k_new.size(0), N = k_new.size(2);
+  TORCH_CHECK(N <= INT32_MAX, "too many tokens");
+  TORCH_CHECK(k_stage.size(0) >= B && page_table.size(0) >= B && k_scale.dim() == 4 &&
+                  k_scale.size(0) >= B && k_scale.size(1) == k_pages.size(1),
+              "k_stage, page_table and k_scale need a row per sequence");
+  TORCH_CHECK(group_rows > 0 && group_rows % k_pages.size(2) == 0,
+              "group_rows must be a multiple of page_rows");
+  const int64_t max_pages = page_table.size(1);
+  TORCH_CHECK(k_scale.size(2) * (group_rows / k_pages.size(2)) >= max_pages,
+              "k_scale has fewer than ceil(max_pages / pages_per_group) groups");
+  for (const torch::Tensor* t : {&counts, &seq_lens, &lens_next}) {
+    CHECK_INPUT(*t);
+    TORCH_CHECK(t->scalar_type() == torch::kInt32 && t->dim() == 1 && t->size(0) >= B,
+                "counts, seq_lens and lens_next must be int32 [>= batch]");
+    CHECK_SAME_DEVICE(k_new, *t);
+  }
+  const int32_t* ix = nullptr;
+  int64_t ix_b = 0;
+  if (index && index->defined()) {
+    CHECK_DEV(*index);
+    CHECK_SAME_DEVICE(k_new, *index);
+    TORCH_CHECK(index->scalar_type() == torch::kInt32 && index->dim() == 2 &&
+                    index->size(0) == B && index->size(1) >= N &&
+                    (index->stride(1) == 1 || N <= 1),
+                "index must be int32 [batch, >= tokens] with contiguous rows");
+    ix = index->data_ptr<int32_t>();
+    ix_b = index->stride(0);
+  }
+  CHECK_SAME_DEVICE(k_new, v_new);
+  CHECK_SAME_DEVICE(k_new, k_stage);
+  CHECK_SAME_DEVICE(k_new, k_pages);
+  if (B == 0) return;
+  fdi4_paged_cache c = make_cache(k_pages, &v_pages, k_scale, k_zp, page_table, seq_lens,
+                                  c10::nullopt, group_rows / k_pages.size(2), max_pages);
+  const DeviceGuard guard(k_new.device());
+  // Empty tensors have no address: any will do where no row is read.
+  const void* kp = N ? k_new.data_ptr() : k_stage.data_ptr();
+  const void* vp = N ? v_new.data_ptr() : k_stage.data_ptr();
+  check_rc(fdi4_extend_paged(static_cast<const float*>(kp), N ? k_new.stride(0) : 0,
+                             N ? k_new.stride(1) : 0, N ? k_new.stride(2) : 0, vp,
+                             N ? v_new.stride(0) : 0, N ? v_new.stride(1) : 0,
+                             N ? v_new.stride(2) : 0, (int)B, (int)N,
+                             counts.data_ptr<int32_t>(), ix, ix_b, k_stage.data_ptr<float>(),
+                             k_stage.stride(0), k_stage.stride(1), k_stage.stride(2),
+                             (int)group_rows, &c, lens_next.data_ptr<int32_t>(), stream()),
+           "extend_paged");
+}
+
+// Rows [start, start + length) of sequences 0..B-1 as dense k and v [B, kv_heads,
+// length, head_dim] of type dtype (see fdi4_read_paged); start_t, int32 [B],
+// in the place of start when given.
+std::vector<torch::Tensor> read_paged(torch::Tensor k_pages, torch::Tensor v_pages,
+                                      torch::Tensor k_scale, torch::Tensor k_zp,
+                                      c10::optional<torch::Tensor> page_table,
+                                      torch::Tensor seq_lens, int64_t pages_per_group,
+                                      int64_t max_pages, int64_t start,
+                                      c10::optional<torch::Tensor> start_t, int64_t length,
+                                      at::ScalarType dtype) {
+  const int64_t B = seq_lens.size(0);
+  fdi4_paged_cache c = make_rows_cache(k_pages, v_pages, k_scale, k_zp, page_table, seq_lens,
+                                       pages_per_group, max_pages, B);
+  TORCH_CHECK(start >= 0 && start <= INT32_MAX && length >= 0 && length <= INT32_MAX,
+              "start and length must be non-negative");
+  const int32_t* st = nullptr;
+  if (start_t && start_t->defined()) {
+    CHECK_INPUT(*start_t);
+    CHECK_SAME_DEVICE(k_pages, *start_t);
+    TORCH_CHECK(start_t->scalar_type() == torch::kInt32 && start_t->dim() == 1 &&
+                    start_t->size(0) == B,
+                "start must be an int or int32 [batch]");
+    st = start_t->data_ptr<int32_t>();
+  }
+  const DeviceGuard guard(k_pages.device());
+  auto k = torch::empty({B, k_pages.size(1), length, k_pages.size(3) * 2},
+                        k_pages.options().dtype(dtype));
+  auto v = torch::empty_like(k);
+  const int code = elem_code(k, "dtype");
+  if (k.numel() == 0) return {k, v};
+  check_rc(fdi4_read_paged(&c, (int)B, st, (int)start, (int)length, k.data_ptr(), k.stride(0),
+                           k.stride(1), k.stride(2), v.data_ptr(), v.stride(0), v.stride(1),
+                           v.stride(2), code, stream()),
+           "read_paged");
+  return {k, v};
+}
+
 torch::Tensor merge_splits(torch::Tensor partials, int64_t batch, int64_t q_heads,
                            int64_t head_dim, int64_t num_splits) {
   CHECK_INPUT(partials);
@@ -772,6 +1003,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "Decode-time append that writes the advanced lengths to a second array (HIP)");
   m.def("decode_paged_advance", &decode_paged_advance,
         "decode_paged that copies the lengths it reads to a second array (HIP)");
+  m.def("decode_window", &decode_window,
+        "Decode over a sliding window and the first tokens of paged keys (HIP)");
+  m.def("decode_tree", &decode_tree,
+        "Attention of a tree of drafted tokens over paged keys and the drafts (HIP)");
+  m.def("extend_paged", &extend_paged,
+        "Several tokens per sequence into the cache, touched groups re-quantized (HIP)");
+  m.def("read_paged", &read_paged, "Rows of the cache as dense keys and values (HIP)");
   m.def("decode_paged_partials", &decode_paged_partials,
         "Decode kernel alone, writing split partials (HIP)");
   m.def("merge_splits", &merge_splits, "Log-sum-exp merge of split partials (HIP)");

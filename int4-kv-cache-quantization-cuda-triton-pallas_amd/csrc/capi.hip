@@ -887,6 +887,186 @@ int fdi4_decode_paged_partials(const float* query, int batch, int num_q_heads,
 
 }  // extern "C"
 
+// ---- attention of several rows over part of the cache and over drafts ---------
+
+namespace {
+
+// Validate and fill the argument block of fdi4_decode_window and fdi4_decode_tree.
+int make_rows_args(const void* query, int q_dtype, int batch, int num_q_heads, int nodes,
+                   int64_t q_batch_stride, int64_t q_head_stride, int64_t q_node_stride,
+                   const fdi4_paged_cache* cache, int window, int sinks, void* out, int out_dtype,
+                   fdi4::RowsArgs* r) {
+  *r = fdi4::RowsArgs{};
+  int rc = make_decode_args(query, q_dtype, batch, num_q_heads, q_batch_stride, q_head_stride,
+                            cache, 1, &r->c);
+  if (rc != hipSuccess) return rc;
+  // One scale group per pages_per_group pages of a sequence, valid rows by length.
+  if (cache->s_page_stride != 0 || cache->page_lens) return hipErrorInvalidValue;
+  if ((int64_t)cache->pages_per_group * cache->page_rows > INT32_MAX) return hipErrorInvalidValue;
+  if (nodes < 1 || nodes > FDI4_MAX_NODES || (int64_t)num_q_heads * nodes > INT32_MAX ||
+      window < 0 || sinks < 0 || (sinks > 0 && window == 0) || (window > 0 && window < nodes))
+    return hipErrorInvalidValue;
+  if (!out || !valid_elem_dtype(out_dtype)) return hipErrorInvalidValue;
+  r->nodes = nodes;
+  r->q_n = q_node_stride;
+  r->window = window;
+  r->sinks = sinks;
+  r->c.out = out;
+  r->c.out_dtype = out_dtype;
+  return hipSuccess;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fdi4_decode_rows_workspace_bytes(int batch, int num_q_heads, int nodes, int window,
+                                        int sinks, int num_splits,
+                                        const fdi4_paged_cache* cache) {
+  return 0;
+}
+
+int fdi4_decode_window(const void* query, int query_dtype, int batch, int num_q_heads,
+                       int64_t q_batch_stride, int64_t q_head_stride,
+                       const fdi4_paged_cache* cache, int window, int sinks, void* out,
+                       int out_dtype, int num_splits, void* workspace, size_t workspace_bytes,
+                       int32_t* lens_out, hipStream_t stream) {
+  if (window < 1 || (lens_out && (!cache || !cache->seq_lens || !aligned(lens_out, 4) ||
+                                  batch < 0 || !disjoint_lens(lens_out, cache->seq_lens, batch))))
+    return hipErrorInvalidValue;
+  fdi4::RowsArgs r;
+  const int rc = make_rows_args(query, query_dtype, batch, num_q_heads, 1, q_batch_stride,
+                                q_head_stride, 0, cache, window, sinks, out, out_dtype, &r);
+  if (rc != hipSuccess) return rc;
+  r.c.lens_out = lens_out;
+  return fdi4::launch_decode_rows(r, cache->head_dim, cache->v_dtype, batch, stream);
+}
+
+int fdi4_decode_tree(const void* query, int query_dtype, int batch, int num_q_heads, int nodes,
+                     int64_t q_batch_stride, int64_t q_head_stride, int64_t q_node_stride,
+                     const float* k_draft, int64_t kd_batch_stride, int64_t kd_head_stride,
+                     int64_t kd_node_stride, const void* v_draft, int64_t vd_batch_stride,
+                     int64_t vd_head_stride, int64_t vd_node_stride, const uint8_t* mask,
+                     int64_t mask_batch_stride, int64_t mask_row_stride,
+                     const fdi4_paged_cache* cache, int window, int sinks, void* out,
+                     int out_dtype, int num_splits, void* workspace, size_t workspace_bytes,
+                     hipStream_t stream) {
+  fdi4::RowsArgs r;
+  const int rc = make_rows_args(query, query_dtype, batch, num_q_heads, nodes, q_batch_stride,
+                                q_head_stride, q_node_stride, cache, window, sinks, out,
+                                out_dtype, &r);
+  if (rc != hipSuccess) return rc;
+  const int veb = cache->v_dtype == FDI4_V_F32 ? 4 : 2;
+  // 16-byte loads of the drafts' key and value rows.
+  if (!k_draft || !v_draft || !mask || !aligned(k_draft, 16) || kd_batch_stride % 4 ||
+      kd_head_stride % 4 || kd_node_stride % 4 || !aligned(v_draft, 16) ||
+      (vd_batch_stride * veb) % 16 || (vd_head_stride * veb) % 16 || (vd_node_stride * veb) % 16)
+    return hipErrorInvalidValue;
+  r.kd = k_draft;
+  r.kd_b = kd_batch_stride;
+  r.kd_h = kd_head_stride;
+  r.kd_n = kd_node_stride;
+  r.vd = static_cast<const uint8_t*>(v_draft);
+  r.vd_b = vd_batch_stride * veb;
+  r.vd_h = vd_head_stride * veb;
+  r.vd_n = vd_node_stride * veb;
+  r.mask = mask;
+  r.mk_b = mask_batch_stride;
+  r.mk_i = mask_row_stride;
+  return fdi4::launch_decode_rows(r, cache->head_dim, cache->v_dtype, batch, stream);
+}
+
+int fdi4_extend_paged(const float* k_new, int64_t kn_batch_stride, int64_t kn_head_stride,
+                      int64_t kn_row_stride, const void* v_new, int64_t vn_batch_stride,
+                      int64_t vn_head_stride, int64_t vn_row_stride, int batch, int max_new,
+                      const int32_t* counts, const int32_t* index, int64_t index_batch_stride,
+                      float* k_stage, int64_t st_batch_stride, int64_t st_head_stride,
+                      int64_t st_row_stride, int group_rows, const fdi4_paged_cache* cache,
+                      int32_t* lens_next, hipStream_t stream) {
+  // (With no new rows the lengths are still written; nothing is read from k_new.)
+  fdi4::AppendArgs ap;
+  const int rc = make_append_args(k_new, kn_batch_stride, kn_head_stride, v_new, vn_batch_stride,
+                                  vn_head_stride, batch, k_stage, st_batch_stride,
+                                  st_head_stride, st_row_stride, group_rows, cache, &ap);
+  if (rc != hipSuccess) return rc;
+  const int veb = cache->v_dtype == FDI4_V_F32 ? 4 : 2;
+  if (!counts || !lens_next || max_new < 0 || kn_row_stride % 4 || (vn_row_stride * veb) % 16 ||
+      !disjoint_lens(lens_next, cache->seq_lens, batch) ||
+      !disjoint_lens(lens_next, counts, batch))
+    return hipErrorInvalidValue;
+  if ((int64_t)max_new + ap.capacity > INT32_MAX - 2 * group_rows) return hipErrorInvalidValue;
+  fdi4::ExtendArgs a;
+  a.q = ap.q;
+  a.q.k = k_new;
+  a.q.k_b = kn_batch_stride;
+  a.q.k_h = kn_head_stride;
+  a.q.k_t = kn_row_stride;
+  a.q.max_tokens = max_new;
+  a.counts = counts;
+  a.index = index;
+  a.ix_b = index_batch_stride;
+  a.v = ap.v_new;
+  a.v_b = ap.vn_b;
+  a.v_h = ap.vn_h;
+  a.v_t = vn_row_stride * veb;
+  a.v_pages = ap.v_pages;
+  a.vp_page = ap.vp_page;
+  a.vp_head = ap.vp_head;
+  a.vp_row = ap.vp_row;
+  a.v_row_bytes = ap.v_row_bytes;
+  a.stage = ap.stage;
+  a.st_b = ap.st_b;
+  a.st_h = ap.st_h;
+  a.st_r = ap.st_r;
+  a.capacity = ap.capacity;
+  a.lens_next = lens_next;
+  return fdi4::launch_extend_paged(a, cache->head_dim, group_rows, batch, cache->num_kv_heads,
+                                   stream);
+}
+
+int fdi4_read_paged(const fdi4_paged_cache* cache, int batch, const int32_t* start, int start0,
+                    int length, void* k_out, int64_t ko_batch_stride, int64_t ko_head_stride,
+                    int64_t ko_row_stride, void* v_out, int64_t vo_batch_stride,
+                    int64_t vo_head_stride, int64_t vo_row_stride, int out_dtype,
+                    hipStream_t stream) {
+  int rc = check_cache(cache, true);
+  if (rc != hipSuccess) return rc;
+  if (cache->s_page_stride != 0 || cache->page_lens || batch < 0 || batch > 65535 ||
+      start0 < 0 || length < 0 || !valid_elem_dtype(out_dtype))
+    return hipErrorInvalidValue;
+  const int64_t G = (int64_t)cache->pages_per_group * cache->page_rows;
+  const int64_t cap = (int64_t)cache->max_pages * cache->page_rows;
+  // Token positions, and the groups that a range reaches past the end, in 32 bits.
+  if (G > INT32_MAX / 4 || std::max<int64_t>(cap, start0) + length > INT32_MAX - 2 * G)
+    return hipErrorInvalidValue;
+  if (batch == 0 || length == 0) return hipSuccess;
+  const int oeb = out_dtype == FDI4_K_F32 ? 4 : 2;
+  if (!k_out || !v_out || !aligned(k_out, 16) || !aligned(v_out, 16) ||
+      (ko_batch_stride * oeb) % 16 || (ko_head_stride * oeb) % 16 || (ko_row_stride * oeb) % 16 ||
+      (vo_batch_stride * oeb) % 16 || (vo_head_stride * oeb) % 16 || (vo_row_stride * oeb) % 16)
+    return hipErrorInvalidValue;
+  fdi4::ReadArgs a = {};
+  // The cache part of a decode's arguments (the query is not used).
+  rc = make_decode_args(k_out, FDI4_K_F32, batch, cache->num_kv_heads, 0, 0, cache, 1, &a.c);
+  if (rc != hipSuccess) return rc;
+  a.start = start;
+  a.start0 = start0;
+  a.length = length;
+  a.k_out = k_out;
+  a.ko_b = ko_batch_stride;
+  a.ko_h = ko_head_stride;
+  a.ko_t = ko_row_stride;
+  a.v_out = v_out;
+  a.vo_b = vo_batch_stride;
+  a.vo_h = vo_head_stride;
+  a.vo_t = vo_row_stride;
+  a.out_dtype = out_dtype;
+  return fdi4::launch_read_paged(a, cache->head_dim, cache->v_dtype, batch, cache->num_kv_heads,
+                                 stream);
+}
+
+}  // extern "C"
+
 // ---- decode with its split partials in a static device array ------------------
 
 namespace {

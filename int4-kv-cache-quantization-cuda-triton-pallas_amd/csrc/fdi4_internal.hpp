@@ -143,6 +143,54 @@ struct DecodeArgs {
   StepAppend step;                      // the fused serving step (step.k_new != null)
 };
 
+// Several query rows of every (sequence, kv-head) over part of the cache and over
+// drafted tokens: row r of a kv-head is (q-head r / nodes of its group, node
+// r % nodes). c holds the cache, the queries and the split partials; the window
+// and the drafts are beside it.
+struct RowsArgs {
+  DecodeArgs c;                         // c.q_h / c.q_b: heads, sequences; out contiguous
+  int nodes;                            // drafted tokens per sequence (1: no drafts, one query)
+  int64_t q_n;                          // query node stride, elements
+  const float* kd;                      // drafts' keys, null: none
+  int64_t kd_b, kd_h, kd_n;             // elements
+  const uint8_t* vd;                    // drafts' values, the cache's type
+  int64_t vd_b, vd_h, vd_n;             // bytes
+  const uint8_t* mask;                  // [b, i, j] != 0: node i sees draft j
+  int64_t mk_b, mk_i;                   // bytes
+  int window;                           // 0: the whole cache
+  int sinks;
+};
+
+// Several tokens per sequence appended: counts[b] of the new rows (by index when
+// given), the touched scale groups re-quantized, the open group staged.
+struct ExtendArgs {
+  QuantPagedArgs q;                     // pages, scales, table, lengths; k: the new keys
+  const int32_t* counts;                // [B]
+  const int32_t* index;                 // null, or [B, ix_b]: the new row of each token
+  int64_t ix_b;
+  const uint8_t* v;
+  int64_t v_b, v_h, v_t;                // bytes
+  uint8_t* v_pages;
+  int64_t vp_page, vp_head, vp_row;     // bytes
+  int v_row_bytes;
+  float* stage;
+  int64_t st_b, st_h, st_r;             // elements
+  int capacity;                         // max_pages * page_rows
+  int32_t* lens_next;                   // [B]
+};
+
+// Rows [start_b, start_b + length) of every sequence as dense keys and values.
+struct ReadArgs {
+  DecodeArgs c;                         // the cache part
+  const int32_t* start;                 // null: start0 for every sequence
+  int start0, length;
+  void* k_out;
+  int64_t ko_b, ko_h, ko_t;             // elements
+  void* v_out;
+  int64_t vo_b, vo_h, vo_t;             // elements
+  int out_dtype;                        // EDtype
+};
+
 // Quantize-dequantize of keys [B, H, T, D] (channel stride 1) in blocks of
 // `block` positions into out (same type and shape, own strides).
 struct FakeQuantArgs {
@@ -192,6 +240,14 @@ hipError_t launch_decode_mfma(const DecodeArgs& a, int D, int v_dtype, int batch
 hipError_t launch_merge(const float* ws_acc, const double* ws_ml, int batch, int hq, int D,
                         int splits, void* out, int out_dtype, int64_t o_b, int64_t o_h,
                         hipStream_t st);
+
+hipError_t launch_decode_rows(const RowsArgs& a, int D, int v_dtype, int batch, hipStream_t st);
+
+hipError_t launch_extend_paged(const ExtendArgs& a, int D, int group, int batch, int heads,
+                               hipStream_t st);
+
+hipError_t launch_read_paged(const ReadArgs& a, int D, int v_dtype, int batch, int heads,
+                             hipStream_t st);
 
 hipError_t launch_fake_quant(const FakeQuantArgs& a, int key_dtype, int rounding, int batch,
                              int heads, hipStream_t st);

@@ -33,7 +33,12 @@
 //       staging rows of the open group) and re-quantizes that group over its
 //       valid rows, exactly what the grouped quantizer gives for the whole
 //       sequence; optionally writes the advanced length to a second array.
+//   extend_paged_kernel<D, GROUP>
+//       several tokens per sequence (a chunk, or drafts picked by index): every
+//       touched group re-quantized over its valid rows, one workgroup each.
 //   pack_kernel   device form of the nibble packing (reference src/int4_pack.py:14-29)
+
+#include <algorithm>
 
 #include "fdi4_device.hpp"
 #include "fdi4_internal.hpp"
@@ -892,6 +897,101 @@ __global__ __launch_bounds__(kQThreads) void append_paged_kernel(AppendArgs a) {
     x[i] = *reinterpret_cast<const float4*>(src + 4 * cq);
   }
   quantize_group<D, GROUP>(a.q, b, h, g, g * GROUP, rnew + 1, x);
+}
+
+// Several tokens appended to every sequence: token j < counts[b] of sequence b,
+// at position L + j (L = seq_lens[b]), is new row j, or index[b, j]. One workgroup
+// per (touched scale group, kv-head, sequence) loads the group's rows -- the open
+// group's earlier ones from the staging rows, the others from the new keys --
+// with the values' copies in flight, and quantizes them as the grouped quantizer
+// does the whole sequence. The rows that are open afterwards go to the staging
+// rows; the workgroup of the first group, the only reader of those, writes them
+// when its own loads are done (the quantizer's barriers lie between). A count
+// that does not fit the cache, or a length out of range, appends nothing.
+template <int D, int GROUP>
+__global__ __launch_bounds__(kQThreads) void extend_paged_kernel(ExtendArgs p, int slots,
+                                                                 int heads) {
+  using G = QGeo<D, GROUP>;
+  const QuantPagedArgs& a = p.q;
+  const unsigned wi = xcd_run_item(blockIdx.x, gridDim.x, kQRun);
+  const int slot = (int)(wi % (unsigned)slots);
+  const int h = (int)(wi / (unsigned)slots % (unsigned)heads);
+  const int b = (int)(wi / ((unsigned)slots * (unsigned)heads));
+  const int tid = threadIdx.x;
+  const int L = a.seq_lens[b];
+  int n = min(max(p.counts[b], 0), a.max_tokens);
+  if (L < 0 || L > p.capacity || n > p.capacity - L) n = 0;
+  if (slot == 0 && h == 0 && tid == 0) p.lens_next[b] = L + n;
+  if (n == 0) return;
+  const int end = L + n;
+  const int g = L / GROUP + slot, r0 = g * GROUP;
+  if (r0 >= end) return;
+  const int nrows = min(GROUP, end - r0);
+  const int32_t* index = p.index ? p.index + (int64_t)b * p.ix_b : nullptr;
+  // New row of token t >= L.
+  auto new_row = [&](int t) -> int64_t {
+    const int j = t - L;
+    return index ? min(max(index[j], 0), a.max_tokens - 1) : j;
+  };
+  const int cq = tid % G::VPR, rsub = tid / G::VPR;
+  const float* knew = a.k + (int64_t)b * a.k_b + (int64_t)h * a.k_h;
+  float* stage = p.stage + (int64_t)b * p.st_b + (int64_t)h * p.st_h;
+  float4 x[G::NI];
+#pragma unroll
+  for (int i = 0; i < G::NI; ++i) {
+    const int r = min(rsub + i * G::RPI, nrows - 1);
+    const float* src = r0 + r < L ? stage + (int64_t)r * p.st_r : knew + new_row(r0 + r) * a.k_t;
+    x[i] = *reinterpret_cast<const float4*>(src + 4 * cq);
+  }
+
+  // The new values of this group, 16 bytes a piece.
+  {
+    const uint8_t* vsrc = p.v + (int64_t)b * p.v_b + (int64_t)h * p.v_h;
+    uint8_t* vdst = p.v_pages + (int64_t)h * p.vp_head;
+    const int ppr = p.v_row_bytes / 16, lg = __builtin_ctz(ppr);
+    const int t0 = max(r0, L), npiece = (r0 + nrows - t0) << lg;
+    for (int pc = tid; pc < npiece; pc += kQThreads) {
+      const int t = t0 + (pc >> lg), o = (pc & (ppr - 1)) * 16;
+      const int lp = fdiv(t, a.div_rows), row = t - lp * a.page_rows;
+      const int64_t phys =
+          (int64_t)min(max(a.page_table[(int64_t)b * a.pt_b + lp], 0), a.num_pages - 1);
+      st16(vdst + phys * p.vp_page + (int64_t)row * p.vp_row + o,
+           ld16(vsrc + new_row(t) * p.v_t + o));
+    }
+  }
+
+  quantize_group<D, GROUP>(a, b, h, g, r0, nrows, x);
+
+  // The open group's new rows to the staging rows.
+  if (slot == 0) {
+    const int open0 = end / GROUP * GROUP, t0 = max(open0, L);
+    for (int i = tid; i < (end - t0) * G::VPR; i += kQThreads) {
+      const int t = t0 + i / G::VPR, c = 4 * (i % G::VPR);
+      *reinterpret_cast<float4*>(stage + (int64_t)(t - open0) * p.st_r + c) =
+          *reinterpret_cast<const float4*>(knew + new_row(t) * a.k_t + c);
+    }
+  }
+}
+
+hipError_t launch_extend_paged(const ExtendArgs& a, int D, int group, int batch, int heads,
+                               hipStream_t st) {
+  if (batch == 0 || heads == 0) return hipSuccess;
+  // Groups that max_tokens new ones can touch from any position in a group.
+  const int slots = (int)(((int64_t)a.q.max_tokens + 2 * group - 2) / group);
+  const int64_t items = (int64_t)std::max(slots, 1) * heads * batch;
+  if (items > INT32_MAX) return hipErrorInvalidValue;
+  dim3 grid((unsigned)items);
+#define FDI4_EX(DD, GG)                                                                  \
+  if (D == DD && group == GG) {                                                          \
+    hipLaunchKernelGGL((extend_paged_kernel<DD, GG>), grid, dim3(kQThreads), 0, st, a,     \
+                       std::max(slots, 1), heads);                                       \
+    return hipGetLastError();                                                            \
+  }
+  FDI4_EX(64, 64) FDI4_EX(64, 128) FDI4_EX(64, 256)
+  FDI4_EX(128, 64) FDI4_EX(128, 128) FDI4_EX(128, 256)
+  FDI4_EX(256, 64) FDI4_EX(256, 128) FDI4_EX(256, 256)
+#undef FDI4_EX
+  return hipErrorInvalidValue;
 }
 
 hipError_t launch_quantize_paged(const QuantPagedArgs& a, int D, int group, int batch, int heads,

@@ -1,0 +1,132 @@
+// Rows of the paged INT4 cache back as dense tensors (gfx950): for token t in
+// [start_b, start_b + length) of sequence b
+//   k[b, h, t - start_b, d] = q*s - zp*s     (two rounded float32 products and a
+//                                             rounded difference, then one rounding
+//                                             to the output type)
+//   v[b, h, t - start_b, d] = the stored value, converted
+// and zeros behind the sequence's end. The arithmetic is that of
+// dequant_kernel (reference src/quantize_int4_ref.py:87-136).
+//
+// One workgroup per (scale group, kv-head, sequence): a thread owns eight channels,
+// whose scales it loads once, and walks the group's rows. Bound by memory: every
+// byte is read once and written once.
+
+#include "decode_common.hpp"
+
+namespace fdi4 {
+
+constexpr int kReadThreads = 256;
+
+// Eight consecutive elements of type OUT at p.
+template <int OUT>
+__device__ __forceinline__ void store8(uint8_t* p, const float* x) {
+  if constexpr (OUT == kEF32) {
+    st16_stream(p, U32x4{f2u(x[0]), f2u(x[1]), f2u(x[2]), f2u(x[3])});
+    st16_stream(p + 16, U32x4{f2u(x[4]), f2u(x[5]), f2u(x[6]), f2u(x[7])});
+  } else {
+    unsigned w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      unsigned lo, hi;
+      if constexpr (OUT == kEF16) {
+        lo = __builtin_bit_cast(unsigned short, (_Float16)x[2 * k]);
+        hi = __builtin_bit_cast(unsigned short, (_Float16)x[2 * k + 1]);
+      } else {
+        lo = bf16_rne(x[2 * k]);
+        hi = bf16_rne(x[2 * k + 1]);
+      }
+      w[k] = lo | hi << 16;
+    }
+    st16_stream(p, U32x4{w[0], w[1], w[2], w[3]});
+  }
+}
+
+template <int D, int VDT, int OUT>
+__global__ __launch_bounds__(kReadThreads) void read_paged_kernel(ReadArgs a, int slots,
+                                                                  int heads) {
+  constexpr int TPR = D / 8;                  // threads per row
+  constexpr int RPS = kReadThreads / TPR;     // rows per sweep
+  constexpr int VEB = VDT == kVF32 ? 4 : 2;
+  constexpr int OEB = OUT == kEF32 ? 4 : 2;
+  const DecodeArgs& c = a.c;
+  const int slot = (int)(blockIdx.x % (unsigned)slots);
+  const int h = (int)(blockIdx.x / (unsigned)slots % (unsigned)heads);
+  const int b = (int)(blockIdx.x / ((unsigned)slots * (unsigned)heads));
+  const int cap = c.max_pages * c.page_rows;
+  const int G = c.pages_per_group * c.page_rows;
+  const int start = a.start ? min(max(a.start[b], 0), cap) : a.start0;
+  const int T = seq_len_of(c, b);
+  // Rows of this slot: the part of its group within the range (64 bits: a range
+  // may end anywhere), counted from the range's start.
+  const int g = start / G + slot;
+  const int64_t g0 = (int64_t)g * G;
+  const int i0 = (int)max(g0 - start, (int64_t)0);
+  const int i1 = (int)min(g0 + G - start, (int64_t)a.length);
+  const int tid = threadIdx.x, oct = tid % TPR, rsub = tid / TPR;
+  uint8_t* ko = reinterpret_cast<uint8_t*>(a.k_out) +
+                ((int64_t)b * a.ko_b + (int64_t)h * a.ko_h + 8 * oct) * OEB;
+  uint8_t* vo = reinterpret_cast<uint8_t*>(a.v_out) +
+                ((int64_t)b * a.vo_b + (int64_t)h * a.vo_h + 8 * oct) * OEB;
+  float s[8], zs[8];
+  if (g0 < T) {
+    const int64_t so = (int64_t)b * c.s_b + (int64_t)h * c.s_h + (int64_t)g * c.s_g + 8 * oct;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      s[k] = c.k_scale[so + k];
+      zs[k] = __fmul_rn(c.k_zp[so + k], s[k]);
+    }
+  }
+  for (int i = i0 + rsub; i < i1; i += RPS) {
+    const int t = start + i;
+    float k[8], v[8];
+    if (t < T) {
+      const int lp = fdiv(t, c.div_rows), row = t - lp * c.page_rows;
+      const int pg = c.page_table ? c.page_table[(int64_t)b * c.pt_b + lp] : lp;
+      const int64_t phys = (int64_t)min(max(pg, 0), c.num_pages - 1);
+      const unsigned q = __builtin_nontemporal_load(reinterpret_cast<const unsigned*>(
+          c.k_pages + phys * c.k_page + (int64_t)h * c.k_head + (int64_t)row * c.k_row + 4 * oct));
+      const uint8_t* vp = reinterpret_cast<const uint8_t*>(c.v_pages) +
+                          (phys * c.v_page + (int64_t)h * c.v_head + (int64_t)row * c.v_row +
+                           8 * oct) * VEB;
+      if constexpr (VDT == kVF32) {
+        widen_values<VDT>(ld16_stream(vp), v);
+        widen_values<VDT>(ld16_stream(vp + 16), v + 4);
+      } else {
+        widen_values<VDT>(ld16_stream(vp), v);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        k[j] = __fsub_rn(__fmul_rn((float)((q >> (4 * j)) & 15u), s[j]), zs[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) k[j] = v[j] = 0.f;
+    }
+    store8<OUT>(ko + (int64_t)i * a.ko_t * OEB, k);
+    store8<OUT>(vo + (int64_t)i * a.vo_t * OEB, v);
+  }
+}
+
+hipError_t launch_read_paged(const ReadArgs& a, int D, int v_dtype, int batch, int heads,
+                             hipStream_t st) {
+  if (batch == 0 || heads == 0 || a.length == 0) return hipSuccess;
+  const int64_t G = (int64_t)a.c.pages_per_group * a.c.page_rows;
+  // Groups that a range of this length touches from any start.
+  const int64_t slots = (a.length + 2 * G - 2) / G;
+  const int64_t items = slots * heads * batch;
+  if (items > INT32_MAX) return hipErrorInvalidValue;
+#define FDI4_RD(DD, VV, OO)                                                               \
+  if (D == DD && v_dtype == VV && a.out_dtype == OO) {                                    \
+    hipLaunchKernelGGL((read_paged_kernel<DD, VV, OO>), dim3((unsigned)items),            \
+                       dim3(kReadThreads), 0, st, a, (int)slots, heads);                  \
+    return hipGetLastError();                                                             \
+  }
+#define FDI4_RD_O(DD, VV) FDI4_RD(DD, VV, kEF32) FDI4_RD(DD, VV, kEF16) FDI4_RD(DD, VV, kEBF16)
+#define FDI4_RD_V(DD) FDI4_RD_O(DD, kVF32) FDI4_RD_O(DD, kVF16) FDI4_RD_O(DD, kVBF16)
+  FDI4_RD_V(64) FDI4_RD_V(128) FDI4_RD_V(256)
+#undef FDI4_RD_V
+#undef FDI4_RD_O
+#undef FDI4_RD
+  return hipErrorInvalidValue;
+}
+
+}  // namespace fdi4

@@ -17,7 +17,10 @@ backend is delivered or refused, never substituted (reference
 src/ops.py:90-108).
 
 Beyond the reference: ``quantize_int4_paged`` / ``flash_decode_paged`` (the
-per-sequence paged layout with 128-token scale groups and packed keys) and
+per-sequence paged layout with 128-token scale groups and packed keys, the
+latter also over a sliding window with sinks), ``flash_decode_paged_tree``
+(drafted tokens over that cache), ``extend_int4_paged`` (several tokens per
+sequence into it), ``dequantize_int4_paged`` (and out of it) and
 ``pack_int4_device``.
 """
 
@@ -340,7 +343,8 @@ def quantize_int4_paged(k, seq_lens, page_table, k_pages, k_scale, k_zp,
 
 def flash_decode_paged(query, k_pages, v_pages, k_scale, k_zp, page_table, seq_lens,
                        group_rows: int = 128, num_splits: int = 0, page_lens=None,
-                       max_pages: Optional[int] = None):
+                       max_pages: Optional[int] = None, window: Optional[int] = None,
+                       sinks: int = 0):
     """Split-K fused INT4 flash decoding over the paged layout (all GPU tensors).
 
     query float32, float16 or bfloat16 [B, Hq, D]; k_pages uint8 [P, Hkv,
@@ -350,6 +354,109 @@ def flash_decode_paged(query, k_pages, v_pages, k_scale, k_zp, page_table, seq_l
     kv-head h // (Hq // Hkv). Returns [B, Hq, D] on the GPU in the query's
     dtype: float32 arithmetic, 16-bit queries widened exactly, one rounding
     (to nearest even) of each output element.
+
+    ``window``: attend only the last ``window`` tokens of each sequence (the
+    query is that of its last token) and its first ``sinks``; the pages between
+    are not read. It needs seq_lens and the grouped scales, not page_lens.
+    """
+    _check_window(window, sinks)
+    _require_device(None)
+    page_rows = k_pages.shape[2]
+    if group_rows % page_rows:
+        raise ValueError("group_rows must be a multiple of the page size")
+    if max_pages is None:
+        max_pages = page_table.shape[1] if page_table is not None else k_pages.shape[0]
+    if window is not None:
+        if page_lens is not None or seq_lens is None or k_scale.dim() != 4:
+            raise ValueError("a window needs seq_lens and scales [batch, kv_heads, groups, "
+                             "head_dim], without page_lens")
+        return load_binding().decode_window(query, k_pages, v_pages, k_scale, k_zp, page_table,
+                                            seq_lens, group_rows // page_rows, int(max_pages),
+                                            int(window), int(sinks), int(num_splits), None)
+    return load_binding().decode_paged(query, k_pages, v_pages, k_scale, k_zp, page_table,
+                                       seq_lens, page_lens, group_rows // page_rows,
+                                       int(max_pages), int(num_splits))
+
+
+def _check_window(window: Optional[int], sinks: int, least: int = 1) -> None:
+    if window is None:
+        if sinks:
+            raise ValueError("sinks need a window")
+    elif window < least:
+        raise ValueError(f"window must be at least {least}, got {window}")
+    if sinks < 0:
+        raise ValueError(f"sinks must not be negative, got {sinks}")
+
+
+def flash_decode_paged_tree(query, k_draft, v_draft, mask, k_pages, v_pages, k_scale, k_zp,
+                            page_table, seq_lens, group_rows: int = 128, num_splits: int = 0,
+                            max_pages: Optional[int] = None, window: Optional[int] = None,
+                            sinks: int = 0):
+    """Attention of drafted tokens over the paged INT4 cache and over each other.
+
+    query float32, float16 or bfloat16 [B, Hq, N, D]: N <= 1024 drafted tokens
+    (nodes) per sequence, none of them in the cache; k_draft float32 and v_draft
+    (the cache's value dtype) [B, Hkv, N, D], their keys and values (any strides
+    with rows on 16-byte boundaries); mask bool [N, N] or [B, N, N]: node i sees
+    draft j where mask[.., i, j]. For a tree that is a node's ancestors and itself,
+    for a chunk of a prompt the lower triangle; any mask is taken as it is. The
+    cache's tensors are those of ``flash_decode_paged``. Returns [B, Hq, N, D] in
+    the query's dtype; a node that sees no cached token and no draft gives zeros.
+
+    ``window`` (at least N): node i, seeing d drafts, attends the cache's last
+    ``window - d`` tokens, which with its drafts are the last ``window`` tokens of
+    the sequence that it ends, and the first ``sinks``.
+
+    Nothing is written; ``extend_int4_paged`` puts the accepted drafts into the
+    cache.
+    """
+    if query.dim() != 4:
+        raise ValueError(f"query must be [batch, heads, nodes, head_dim], got "
+                         f"{tuple(query.shape)}")
+    _check_window(window, sinks, query.shape[2])
+    _require_device(None)
+    page_rows = k_pages.shape[2]
+    if group_rows % page_rows:
+        raise ValueError("group_rows must be a multiple of the page size")
+    if max_pages is None:
+        max_pages = page_table.shape[1] if page_table is not None else k_pages.shape[0]
+    if mask.dim() == 2:
+        mask = mask.unsqueeze(0)
+    return load_binding().decode_tree(query, k_draft, v_draft, mask, k_pages, v_pages, k_scale,
+                                      k_zp, page_table, seq_lens, group_rows // page_rows,
+                                      int(max_pages), int(window or 0), int(sinks),
+                                      int(num_splits))
+
+
+def extend_int4_paged(k_new, v_new, counts, k_stage, k_pages, v_pages, k_scale, k_zp, page_table,
+                      seq_lens, lens_next, group_rows: int = 128, index=None) -> None:
+    """Append several tokens to every sequence: the grouped write of
+    ``quantize_int4_paged`` continued from a sequence's open scale group.
+
+    k_new float32 and v_new (the cache's value dtype) [B, Hkv, N, D]; counts int32
+    [B], the tokens each sequence takes (clamped to [0, N]), in order, or with index
+    (int32 [B, N], clamped) token j from new row index[b, j] -- the accepted path of
+    a tree of drafts. They are written at positions seq_lens[b] ..; every touched
+    group is quantized over its valid rows, bit-exact with the whole sequence's
+    quantization; k_stage float32 [B, Hkv, group_rows, D] holds the open group's
+    keys before and after. lens_next int32 [B] receives the new lengths; seq_lens is
+    left for the caller to advance. A count that does not fit the pages mapped by
+    page_table's columns takes nothing.
+    """
+    _require_device(None)
+    load_binding().extend_paged(k_new, v_new, counts, k_stage, k_pages, v_pages, k_scale, k_zp,
+                                page_table, seq_lens, lens_next, group_rows, index)
+
+
+def dequantize_int4_paged(k_pages, v_pages, k_scale, k_zp, page_table, seq_lens, start,
+                          length: int, group_rows: int = 128, dtype=None,
+                          max_pages: Optional[int] = None):
+    """Tokens start .. start + length - 1 of every sequence as dense keys and values.
+
+    start is an int, or int32 [B] (clamped to the pages). Returns (k, v), both
+    [B, Hkv, length, D] of dtype (float32, the default, float16 or bfloat16): keys
+    ``q*scale - zp*scale`` as ``dequantize_int4`` computes them, rounded once; values
+    converted; zeros behind a sequence's end.
     """
     _require_device(None)
     page_rows = k_pages.shape[2]
@@ -357,9 +464,12 @@ def flash_decode_paged(query, k_pages, v_pages, k_scale, k_zp, page_table, seq_l
         raise ValueError("group_rows must be a multiple of the page size")
     if max_pages is None:
         max_pages = page_table.shape[1] if page_table is not None else k_pages.shape[0]
-    return load_binding().decode_paged(query, k_pages, v_pages, k_scale, k_zp, page_table,
-                                       seq_lens, page_lens, group_rows // page_rows,
-                                       int(max_pages), int(num_splits))
+    is_tensor = isinstance(start, torch.Tensor)
+    k, v = load_binding().read_paged(k_pages, v_pages, k_scale, k_zp, page_table, seq_lens,
+                                     group_rows // page_rows, int(max_pages),
+                                     0 if is_tensor else int(start), start if is_tensor else None,
+                                     int(length), torch.float32 if dtype is None else dtype)
+    return k, v
 
 
 def backend_status() -> dict:

@@ -444,6 +444,69 @@ class INT4PagedSequenceCache:
         self.seq_lens[:B] += 1
         self._lens[:B] += 1
 
+    def extend(self, k_new, v_new, counts=None, index=None) -> None:
+        """Append counts[b] of the tokens k_new, v_new [B, kv_heads, N, D] (keys
+        float32, values converted to the cache's dtype) to sequence b: a chunk of a
+        prompt, or the accepted ones of a tree of drafts. counts: None (all N), host
+        integers, or int32 [B] on the GPU; index: None (in order) or [B, N], token j
+        being new row index[b, j].
+
+        With counts on the host the pages are mapped here. With counts on the GPU
+        nothing goes through the host, so the call can be captured into a graph; the
+        pages of N tokens per sequence must be reserved (reserve), and the lengths
+        are known to the host only after sync_lengths(), as after step()."""
+        import torch
+        if k_new.dim() != 4 or k_new.shape[1] != self.num_kv_heads or \
+                k_new.shape[3] != self.head_dim or tuple(v_new.shape) != tuple(k_new.shape):
+            raise ValueError("k_new and v_new must be [batch, kv_heads, tokens, head_dim] of "
+                             "this cache")
+        B, _, N, _ = k_new.shape
+        if B > self.max_seqs:
+            raise ValueError(f"{B} sequences, the cache holds {self.max_seqs}")
+        if k_new.dtype != torch.float32:
+            raise TypeError(f"k_new must be float32, got {k_new.dtype}")
+        on_device = isinstance(counts, torch.Tensor) and counts.is_cuda
+        if on_device:
+            if counts.dtype != torch.int32 or tuple(counts.shape) != (B,):
+                raise ValueError("counts on the GPU must be int32 [batch]")
+            short = np.nonzero(self._lens[:B] + self._unsynced_steps + N > self._mapped[:B])[0]
+            if len(short):
+                raise RuntimeError(f"extend() could write past the pages reserved for sequence "
+                                   f"{int(short[0])}; call reserve() first")
+            n = None
+        else:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("extend() with host counts cannot be captured into a graph")
+            n = np.full(B, N, np.int64) if counts is None else np.asarray(
+                counts, np.int64).reshape(-1)
+            if n.shape != (B,) or (n < 0).any() or (n > N).any():
+                raise ValueError(f"counts must be one of 0 .. {N} per sequence")
+        if index is not None:
+            if not isinstance(index, torch.Tensor):
+                index = torch.as_tensor(np.asarray(index, np.int64))
+            if index.dim() != 2 or tuple(index.shape) != (B, N):
+                raise ValueError("index must be [batch, tokens]")
+            if not index.is_cuda:
+                taken = torch.arange(N)[None] < torch.from_numpy(n)[:, None] if n is not None \
+                    else torch.ones(B, N, dtype=torch.bool)
+                if ((index < 0) | (index >= N))[taken].any():
+                    raise ValueError(f"index must lie in 0 .. {N - 1}")
+            index = index.to(device=k_new.device, dtype=torch.int32)
+        if n is not None:
+            self._sync_if_stepped()
+            self._grow_all((b, int(self._lens[b]) + int(n[b])) for b in range(B))
+            counts = torch.from_numpy(n.astype(np.int32)).to(k_new.device)
+        load_binding().extend_paged(k_new, v_new.to(self.v_pages.dtype), counts, self.k_stage,
+                                    self.k_pages, self.v_pages, self.k_scale, self.k_zp,
+                                    self.page_table, self.seq_lens, self._lens_next,
+                                    self.group_rows, index)
+        # (An addition, not a copy: a kernel of its own in a captured graph.)
+        torch.add(self._lens_next[:B], 0, out=self.seq_lens[:B])
+        if n is not None:
+            self._lens[:B] += n
+        else:
+            self._unsynced_steps += N
+
     # ---- device-only decode steps (graph capture) ----------------------------
 
     def reserve(self, batch: int, n_tokens: int) -> None:
@@ -452,7 +515,7 @@ class INT4PagedSequenceCache:
         self._sync_if_stepped()
         self._grow_all((b, int(self._lens[b]) + n_tokens) for b in range(batch))
 
-    def step(self, k_new, v_new, query, num_splits: int = 0):
+    def step(self, k_new, v_new, query, num_splits: int = 0, window=None, sinks: int = 0):
         """One decode step on the device alone: append (k_new, v_new) [B,
         kv_heads, D] at each sequence's length, advance the lengths on the
         device, attend with query [B, Hq, D] (float32, float16 or bfloat16);
@@ -470,7 +533,9 @@ class INT4PagedSequenceCache:
         An eager call whose token would fall outside the reserved pages raises
         RuntimeError before anything is launched (the host knows the lengths up
         to the eager steps since the last sync; replays are the caller's to
-        keep within the reservation)."""
+        keep within the reservation). window, sinks: attend as decode() does with
+        them."""
+        ops._check_window(window, sinks)
         B = k_new.shape[0]
         if B > self.max_seqs or tuple(k_new.shape) != (B, self.num_kv_heads, self.head_dim):
             raise ValueError("k_new must be [batch <= max_seqs, kv_heads, head_dim]")
@@ -479,6 +544,15 @@ class INT4PagedSequenceCache:
             raise RuntimeError(f"step() would write past the pages reserved for sequence "
                                f"{int(short[0])}; call reserve() first")
         self._unsynced_steps += 1
+        if window is not None:
+            C = load_binding()
+            C.append_paged_advance(k_new, v_new, self.k_stage[:B], self.k_pages, self.v_pages,
+                                   self.k_scale[:B], self.k_zp[:B], self.page_table[:B],
+                                   self.seq_lens[:B], self.group_rows, self._lens_next[:B])
+            return C.decode_window(query, self.k_pages, self.v_pages, self.k_scale[:B],
+                                   self.k_zp[:B], self.page_table[:B], self._lens_next[:B],
+                                   self.group_rows // self.page_rows, self.max_pages_per_seq,
+                                   int(window), int(sinks), int(num_splits), self.seq_lens[:B])
         if num_splits:
             # An explicit split count: the two-launch form (the append writes
             # seq_lens + 1 to _lens_next, the decode attends over it with the
@@ -508,15 +582,49 @@ class INT4PagedSequenceCache:
 
     # ---- reads -------------------------------------------------------------
 
-    def decode(self, query, num_splits: int = 0):
+    def decode(self, query, num_splits: int = 0, window=None, sinks: int = 0):
         """Fused INT4 attention of query [B, Hq, D] (float32, float16 or bfloat16;
         Hq a multiple of kv_heads) over sequences 0..B-1; returns [B, Hq, D] in
-        the query's dtype (float32 arithmetic, one rounding at the end)."""
+        the query's dtype (float32 arithmetic, one rounding at the end). With a
+        window only over each sequence's last ``window`` and first ``sinks``
+        tokens."""
         B = query.shape[0]
         return ops.flash_decode_paged(query, self.k_pages, self.v_pages, self.k_scale[:B],
                                       self.k_zp[:B], self.page_table[:B], self.seq_lens[:B],
                                       self.group_rows, num_splits,
-                                      max_pages=self.max_pages_per_seq)
+                                      max_pages=self.max_pages_per_seq, window=window,
+                                      sinks=sinks)
+
+    def tree_attention(self, query, k_draft, v_draft, mask, window=None, sinks: int = 0,
+                       num_splits: int = 0):
+        """Attention of drafted tokens, query [B, Hq, N, D] with k_draft (float32)
+        and v_draft (the cache's value dtype) [B, kv_heads, N, D], over sequences
+        0..B-1 and the drafts that mask ([N, N] or [B, N, N] bool) shows each of them
+        (ops.flash_decode_paged_tree). Writes nothing; extend() takes the accepted
+        drafts."""
+        B = query.shape[0]
+        return ops.flash_decode_paged_tree(
+            query, k_draft, v_draft, mask, self.k_pages, self.v_pages, self.k_scale[:B],
+            self.k_zp[:B], self.page_table[:B], self.seq_lens[:B], self.group_rows, num_splits,
+            max_pages=self.max_pages_per_seq, window=window, sinks=sinks)
+
+    def read(self, batch: int, start=0, length=None, dtype=None):
+        """Tokens start .. start + length - 1 (to the longest sequence's end by
+        default) of sequences 0..batch-1 as dense (k, v) [batch, kv_heads, length, D]
+        of dtype (float32 by default): dequantized keys, stored values, zeros behind a
+        sequence's end. start: an int, or int32 [batch] on the GPU (then length is
+        needed)."""
+        if not 0 <= batch <= self.max_seqs:
+            raise ValueError(f"batch must lie in 0 .. {self.max_seqs}")
+        if length is None:
+            if not isinstance(start, int):
+                raise ValueError("length is needed with a start per sequence")
+            self._sync_if_stepped()
+            length = max(0, int(self._lens[:batch].max(initial=0)) - start)
+        return ops.dequantize_int4_paged(
+            self.k_pages, self.v_pages, self.k_scale[:batch], self.k_zp[:batch],
+            self.page_table[:batch], self.seq_lens[:batch], start, length, self.group_rows, dtype,
+            max_pages=self.max_pages_per_seq)
 
     def lengths(self) -> np.ndarray:
         return self._lens.copy()
