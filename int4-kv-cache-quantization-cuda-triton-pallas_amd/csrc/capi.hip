@@ -891,29 +891,82 @@ int fdi4_decode_paged_partials(const float* query, int batch, int num_q_heads,
 
 namespace {
 
+// Launch shape of a windowed or tree attention: 16-row tiles per workgroup, workgroups
+// for a kv-head's rows, and splits of a sequence's items (scale groups, and 64 drafts).
+struct RowsPlan {
+  int row_tiles, tiles, splits;
+};
+
+RowsPlan plan_rows(int batch, int num_q_heads, int nodes, int window, int sinks, int num_splits,
+                   const fdi4_paged_cache* cache) {
+  RowsPlan p;
+  const int most = cache->head_dim == 256 ? 2 : 4;
+  const int64_t rows = (int64_t)(num_q_heads / cache->num_kv_heads) * nodes;
+  const int64_t t16 = (rows + 15) / 16;
+  p.tiles = (int)((t16 + most - 1) / most);
+  p.row_tiles = (int)((t16 + p.tiles - 1) / p.tiles);
+  // The most items a sequence can have.
+  const int64_t cap = (int64_t)cache->max_pages * cache->page_rows;
+  const int64_t G = (int64_t)std::min(cache->pages_per_group, std::max(cache->max_pages, 1)) *
+                    cache->page_rows;
+  int64_t items = (cap + G - 1) / G;
+  if (window)
+    items = std::min(items, ((int64_t)sinks + G - 1) / G + ((int64_t)window + G - 1) / G + 1);
+  if (nodes > 1) items += (nodes + 63) / 64;
+  items = std::max<int64_t>(items, 1);
+  const int64_t streams = (int64_t)batch * cache->num_kv_heads * p.tiles;
+  const int64_t slots = p.row_tiles == 1 ? 2 * kCUs : kCUs;
+  const int64_t s = num_splits > 0 ? num_splits : slots / std::max<int64_t>(streams, 1);
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(s, items), kMaxSplits));
+  return p;
+}
+
 // Validate and fill the argument block of fdi4_decode_window and fdi4_decode_tree.
 int make_rows_args(const void* query, int q_dtype, int batch, int num_q_heads, int nodes,
                    int64_t q_batch_stride, int64_t q_head_stride, int64_t q_node_stride,
                    const fdi4_paged_cache* cache, int window, int sinks, void* out, int out_dtype,
-                   fdi4::RowsArgs* r) {
+                   int num_splits, fdi4::RowsArgs* r) {
   *r = fdi4::RowsArgs{};
   int rc = make_decode_args(query, q_dtype, batch, num_q_heads, q_batch_stride, q_head_stride,
                             cache, 1, &r->c);
   if (rc != hipSuccess) return rc;
   // One scale group per pages_per_group pages of a sequence, valid rows by length.
   if (cache->s_page_stride != 0 || cache->page_lens) return hipErrorInvalidValue;
-  if ((int64_t)cache->pages_per_group * cache->page_rows > INT32_MAX) return hipErrorInvalidValue;
+  // (A position and a group's rows add up in 32 bits.)
+  if ((int64_t)cache->max_pages * cache->page_rows > (1 << 30)) return hipErrorInvalidValue;
   if (nodes < 1 || nodes > FDI4_MAX_NODES || (int64_t)num_q_heads * nodes > INT32_MAX ||
       window < 0 || sinks < 0 || (sinks > 0 && window == 0) || (window > 0 && window < nodes))
     return hipErrorInvalidValue;
   if (!out || !valid_elem_dtype(out_dtype)) return hipErrorInvalidValue;
+  // A group larger than a sequence is the one group that the sequence has.
+  r->c.pages_per_group = std::min(cache->pages_per_group, std::max(cache->max_pages, 1));
+  r->c.div_ppg = fdi4::make_fast_div(r->c.pages_per_group);
+  r->div_group = fdi4::make_fast_div(r->c.pages_per_group * cache->page_rows);
   r->nodes = nodes;
   r->q_n = q_node_stride;
   r->window = window;
   r->sinks = sinks;
+  const RowsPlan p = plan_rows(batch, num_q_heads, nodes, window, sinks, num_splits, cache);
+  r->row_tiles = p.row_tiles;
+  r->tiles = p.tiles;
+  r->c.num_splits = p.splits;
+  r->c.final_out = p.splits == 1 ? 1 : 0;
   r->c.out = out;
   r->c.out_dtype = out_dtype;
   return hipSuccess;
+}
+
+int launch_rows(fdi4::RowsArgs* r, int batch, const fdi4_paged_cache* cache, void* workspace,
+                size_t workspace_bytes, hipStream_t stream) {
+  const int d = cache->head_dim, rows = r->c.num_q_heads * r->nodes;
+  if (r->c.num_splits > 1) {
+    const int rc = carve_partials(workspace, workspace_bytes, batch, rows, d, &r->c);
+    if (rc != hipSuccess) return rc;
+  }
+  const hipError_t e = fdi4::launch_decode_rows(*r, d, cache->v_dtype, batch, stream);
+  if (e != hipSuccess || r->c.num_splits == 1) return e;
+  return fdi4::launch_merge(r->c.ws_acc, r->c.ws_ml, batch, rows, d, r->c.num_splits, r->c.out,
+                            r->c.out_dtype, (int64_t)rows * d, d, stream);
 }
 
 }  // namespace
@@ -923,7 +976,14 @@ extern "C" {
 size_t fdi4_decode_rows_workspace_bytes(int batch, int num_q_heads, int nodes, int window,
                                         int sinks, int num_splits,
                                         const fdi4_paged_cache* cache) {
-  return 0;
+  if (!cache || batch <= 0 || num_q_heads <= 0 || nodes < 1 || nodes > FDI4_MAX_NODES ||
+      window < 0 || sinks < 0 || cache->num_kv_heads < 1 ||
+      num_q_heads % cache->num_kv_heads || cache->page_rows < 1 || cache->pages_per_group < 1 ||
+      cache->max_pages < 0 || !valid_head_dim(cache->head_dim) ||
+      (int64_t)num_q_heads * nodes > INT32_MAX)
+    return 0;
+  const int s = plan_rows(batch, num_q_heads, nodes, window, sinks, num_splits, cache).splits;
+  return s > 1 ? decode_ws_bytes(batch, num_q_heads * nodes, cache->head_dim, s) : 0;
 }
 
 int fdi4_decode_window(const void* query, int query_dtype, int batch, int num_q_heads,
@@ -936,10 +996,11 @@ int fdi4_decode_window(const void* query, int query_dtype, int batch, int num_q_
     return hipErrorInvalidValue;
   fdi4::RowsArgs r;
   const int rc = make_rows_args(query, query_dtype, batch, num_q_heads, 1, q_batch_stride,
-                                q_head_stride, 0, cache, window, sinks, out, out_dtype, &r);
+                                q_head_stride, 0, cache, window, sinks, out, out_dtype,
+                                num_splits, &r);
   if (rc != hipSuccess) return rc;
   r.c.lens_out = lens_out;
-  return fdi4::launch_decode_rows(r, cache->head_dim, cache->v_dtype, batch, stream);
+  return launch_rows(&r, batch, cache, workspace, workspace_bytes, stream);
 }
 
 int fdi4_decode_tree(const void* query, int query_dtype, int batch, int num_q_heads, int nodes,
@@ -954,7 +1015,7 @@ int fdi4_decode_tree(const void* query, int query_dtype, int batch, int num_q_he
   fdi4::RowsArgs r;
   const int rc = make_rows_args(query, query_dtype, batch, num_q_heads, nodes, q_batch_stride,
                                 q_head_stride, q_node_stride, cache, window, sinks, out,
-                                out_dtype, &r);
+                                out_dtype, num_splits, &r);
   if (rc != hipSuccess) return rc;
   const int veb = cache->v_dtype == FDI4_V_F32 ? 4 : 2;
   // 16-byte loads of the drafts' key and value rows.
@@ -973,7 +1034,7 @@ int fdi4_decode_tree(const void* query, int query_dtype, int batch, int num_q_he
   r.mask = mask;
   r.mk_b = mask_batch_stride;
   r.mk_i = mask_row_stride;
-  return fdi4::launch_decode_rows(r, cache->head_dim, cache->v_dtype, batch, stream);
+  return launch_rows(&r, batch, cache, workspace, workspace_bytes, stream);
 }
 
 int fdi4_extend_paged(const float* k_new, int64_t kn_batch_stride, int64_t kn_head_stride,

@@ -1,6 +1,6 @@
-// Attention of several query rows per sequence over part of the paged INT4 cache
-// and over drafted tokens (gfx950). For the row of node i and q-head h of sequence
-// b, with n cached tokens and d_i drafts that node i sees,
+// Attention of several query rows per (sequence, kv-head) over part of the paged INT4
+// cache and over drafted tokens, on the matrix cores (gfx950). For the row of node i
+// and q-head h of sequence b, with n cached tokens and d_i drafts that node i sees,
 //
 //   out = sum_t p_t v_t / sum_t p_t,   p_t = exp(q . k_t - max)
 //
@@ -9,112 +9,835 @@
 // k_t = nib*scale - zp*scale, and over the drafts j with mask[i, j]. A row that sees
 // nothing is zero.
 //
-// The plain form: one workgroup per row, a wave takes every fourth key.
+// A workgroup of four waves serves RT tiles of 16 rows of one kv-head over a range of
+// scale groups (and drafts, 64 an item, at the range's end). Its 16-row chunks of keys
+// go to the waves in turn, so the cache is read once for all rows, straight to
+// registers; the waves meet at the end, in LDS, and splits in the merge kernel.
+//
+//   digits: q . k_t = sum_d v_d (nib_td - zp_d), v = q*s. Per group and row, v is taken
+//      relative to the largest |q| of the row and the largest s of the group, as a
+//      32-bit integer |v| < 2^30 in four balanced base-256 digits; one product and
+//      one conversion per element, shared by the 128 keys of the group, where
+//      dequantized keys would need three 8-bit terms against three of the query.
+//      v_mfma_i32_16x16x64_i8 multiplies the nibbles of 16 keys (A) by a digit of 16
+//      rows (B); the digits' exact sums meet in float32 (28 bits of each pair), and
+//      the constant sum_d v_d zp_d, in float32, goes in with the exponent's FMA. A
+//      logit is off by what float32 products of q and k would be.
+//      The digits are built by the whole workgroup for the next group while the
+//      present one is multiplied (two LDS buffers, one barrier a group).
+//   softmax: lane (g, r) of a wave holds the logits of row r with keys 4g .. 4g+3, and
+//      the value product wants its B operand in the same lanes, so probabilities never
+//      leave their registers. The shift is a whole number that moves only when a logit
+//      passes it by kSlack (a power of two, so probabilities stay in their type's
+//      range); the accumulators are rescaled then and not for every new maximum.
+//   values: lane (g, r) loads the channels 8r.. of rows 4g .. 4g+3, byte permutes pair
+//      the rows, and one product takes 32 keys. A probability is the sum of two
+//      (float16: 22 bits; bfloat16: 16) or three (bfloat16 values, float32 output:
+//      24) terms. float32 values: v_mfma_f32_16x16x4_f32.
+//
+// A non-finite value times a probability of zero is NaN, though the row does not see
+// it: a workgroup that ends with a NaN goes through its range again, row by row and key
+// by key (rare, slow).
 
 #include "decode_common.hpp"
 
 namespace fdi4 {
 
-template <int D, int VDT>
-__global__ __launch_bounds__(256) void decode_rows_kernel(RowsArgs a) {
-  constexpr int CH = D / 64, W = 4;
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+constexpr int kRowWaves = 4;
+
+template <int D, int VDT, int RT, int TERMS>
+struct RowsGeo {
+  static constexpr int NB = D / 64;                // 64-channel blocks of the key product
+  static constexpr int KW = D / 32;                // packed key words per lane per row
+  static constexpr int VEB = VDT == kVF32 ? 4 : 2;
+  static constexpr int PB = D * VEB / 16 < 16 ? D * VEB / 16 : 16;  // bytes per value load
+  static constexpr int NP = D * VEB / (16 * PB);   // value loads per lane per row
+  static constexpr int CPP = PB / VEB;             // channels per value load
+  static constexpr int NA = D / 16;                // 16-channel output tiles
+  static constexpr int CPS = VDT == kVF32 ? 1 : 2; // chunks per step
+  static constexpr int M = 16 * RT;                // rows of the workgroup
+  static constexpr int DS = D + 16;                // bytes per row of a digit (padded)
+  static constexpr int kDig = 4 * M * DS;          // a buffer of digits
+  static constexpr int AS = D + 4;                 // floats per row of a wave's output
+  static constexpr int kAcc = kRowWaves * M * AS * 4;
+  static constexpr int kSmem = 2 * kDig > kAcc ? 2 * kDig : kAcc;
+};
+
+__device__ __forceinline__ int row_slot(int d) {
+  return (d & ~15) | ((d & 1) << 3) | ((d & 15) >> 1);
+}
+
+__device__ __forceinline__ int row_channel(int s) {
+  return (s & ~15) | ((s & 7) << 1) | ((s >> 3) & 1);
+}
+
+// Maximum and sum over the four 16-lane groups.
+__device__ __forceinline__ float over_groups_max(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(f2u(x), f2u(x), false, false);
+  x = fmaxf(u2f(r[0]), u2f(r[1]));
+  auto s = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
+  return fmaxf(u2f(s[0]), u2f(s[1]));
+}
+
+__device__ __forceinline__ float over_groups_sum(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(f2u(x), f2u(x), false, false);
+  x = u2f(r[0]) + u2f(r[1]);
+  auto s = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
+  return u2f(s[0]) + u2f(s[1]);
+}
+
+template <int D, int VDT, int RT, int TERMS>
+__global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a) {
+  using G = RowsGeo<D, VDT, RT, TERMS>;
+  constexpr int NB = G::NB, CPS = G::CPS, NA = G::NA, M = G::M;
+  // Threads that build digits take whole rows: TPR (a power of two) per row.
+  constexpr int TPR = RT == 1 ? 16 : RT == 2 ? 8 : 4;
+  constexpr int SPT = D / TPR;                     // channels of a row per thread
+  constexpr int kWidth = kRowWaves * 64 / TPR;     // rows the threads cover: >= M
+  static_assert(kWidth >= M, "rows");
+  // Shift of the probabilities: largest logit + kUp at most kSlack above the shift's.
+  // float16 terms need the headroom (p * 2^kUp < 2^16) and the small end (quantum
+  // 2^-24): a probability's terms are exact to 2^-37 of the largest.
+  constexpr float kUp = VDT == kVF16 ? 13.f : 0.f;
+  constexpr float kSlack = VDT == kVF16 ? 2.f : 8.f;
+  constexpr float kLeast = -3.4028235e38f;
+  constexpr float kLog2e = 1.44269504088896f;
+
   const DecodeArgs& c = a.c;
-  const int row = blockIdx.x, b = blockIdx.y;
-  const int hq = row / a.nodes, node = row % a.nodes;
-  const int hk = hq / c.hq_per_kv;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n16 = lane & 15, grp = lane >> 4;
+
+  // Tiles of one (sequence, kv-head, split) run on one XCD, one after the other: they
+  // read the same pages.
+  unsigned wi = xcd_run_item(blockIdx.x, gridDim.x, (unsigned)a.tiles);
+  const int tile = (int)(wi % (unsigned)a.tiles);
+  wi /= (unsigned)a.tiles;
+  const int split = (int)(wi % (unsigned)c.num_splits);
+  wi /= (unsigned)c.num_splits;
+  const int hkv = c.num_q_heads / c.hq_per_kv;
+  const int hk = (int)(wi % (unsigned)hkv), b = (int)(wi / (unsigned)hkv);
+  const int rows = c.hq_per_kv * a.nodes;          // rows of this kv-head
+  const int row0 = tile * M;
+
+  __shared__ __align__(16) uint8_t smem[G::kSmem];
+  __shared__ __align__(16) float sz_s[2][2 * D];   // scaled scales, zero-points (slot order)
+  __shared__ float cs_s[2];                        // a group's scale unit
+  __shared__ float2 cc_s[2][M];                    // a row's logit unit and constant
+  __shared__ float qm_s[M];                        // a row's query unit
+  __shared__ int low_s[M];                         // first cached token in a row's window
+  __shared__ int ext_s[2];                         // smallest and largest of them
+  __shared__ float m_s[kRowWaves][M], l_s[kRowWaves][M];
+  __shared__ int bad_s;
+
   const int n = seq_len_of(c, b);
-  float q[CH];
+  if (c.lens_out && tile == 0 && split == 0 && hk == 0 && tid == 0)
+    c.lens_out[b] = c.seq_lens[b];
+
+  // ---- the rows: queries to registers (slot order, relative to the row's largest) ----
+  const int brow = tid / TPR, part = tid % TPR;
+  const bool builds = brow < M;
+  const int R = row0 + min(brow, M - 1);
+  const int node = R % a.nodes;
+  float qn[SPT];
+  {
+    const bool real = builds && R < rows;
+    const int64_t q0 = (int64_t)b * c.q_b +
+                       (int64_t)(hk * c.hq_per_kv + (real ? R / a.nodes : 0)) * c.q_h +
+                       (int64_t)(real ? node : 0) * a.q_n;
+    unsigned mx = 0;
 #pragma unroll
-  for (int i = 0; i < CH; ++i)
-    q[i] = load_elem(c.q, (int64_t)b * c.q_b + (int64_t)hq * c.q_h + (int64_t)node * a.q_n +
-                              lane * CH + i, c.q_dtype);
-  const uint8_t* mask =
-      a.mask ? a.mask + (int64_t)b * a.mk_b + (int64_t)node * a.mk_i : nullptr;
-  int mine = 0;
-  if (mask)
-    for (int j = 0; j < a.nodes; ++j) mine += mask[j] != 0;
-  const int low = a.window ? min(max((int64_t)n + mine - a.window, (int64_t)0), (int64_t)n) : 0;
-  const int sinks = min(a.sinks, low);
-  const int cached = sinks + n - low;
-  const int drafts = mask ? a.nodes : 0;
-  float m = -INFINITY, l = 0.f, acc[CH] = {};
-  for (int e = w; e < cached + drafts; e += W) {
-    float k[CH], v[CH];
-    if (e < cached) {
-      const int t = e < sinks ? e : low + e - sinks;
-      const int lp = t / c.page_rows, r = t % c.page_rows;
-      const int pg = c.page_table ? c.page_table[(int64_t)b * c.pt_b + lp] : lp;
-      const int64_t phys = min(max(pg, 0), c.num_pages - 1);
-      const uint8_t* kp = c.k_pages + phys * c.k_page + (int64_t)hk * c.k_head +
-                          (int64_t)r * c.k_row;
-      const int64_t so = (int64_t)b * c.s_b + (int64_t)hk * c.s_h +
-                         (int64_t)(lp / c.pages_per_group) * c.s_g;
-      const int64_t vo = phys * c.v_page + (int64_t)hk * c.v_head + (int64_t)r * c.v_row;
+    for (int i = 0; i < SPT; ++i) {
+      const float x = load_elem(c.q, q0 + row_channel(part * SPT + i), c.q_dtype);
+      qn[i] = real ? x : 0.f;
+      mx = max(mx, f2u(qn[i]) & 0x7FFFFFFFu);
+    }
+    if constexpr (TPR > 1) mx = max(mx, xchg_u32<1>(mx));
+    if constexpr (TPR > 2) mx = max(mx, xchg_u32<2>(mx));
+    if constexpr (TPR > 4) mx = max(mx, xchg_u32<4>(mx));
+    if constexpr (TPR > 8) mx = max(mx, xchg_u32<8>(mx));
+    // (As bits, so that NaN is the largest and makes the row NaN.)
+    const float unit = u2f(max(mx, f2u(1e-30f)));
+    const float inv = 1.f / unit;
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const int d = lane * CH + i;
-        const float s = c.k_scale[so + d], z = c.k_zp[so + d];
-        k[i] = (float)((kp[d >> 1] >> (4 * (d & 1))) & 15) * s - z * s;
-        v[i] = load_elem(c.v_pages, vo + d, VDT);
+    for (int i = 0; i < SPT; ++i) qn[i] *= inv;
+    if (builds && part == 0) qm_s[brow] = unit;
+    // The window of each row.
+    int low = 0;
+    if (a.window) {
+      int mine = 0;
+      if (a.mask && real) {
+        const uint8_t* mk = a.mask + (int64_t)b * a.mk_b + (int64_t)node * a.mk_i;
+        for (int j = part; j < a.nodes; j += TPR) mine += mk[j] != 0;
       }
-    } else {
-      const int j = e - cached;
-      if (!mask[j]) continue;
-      const float* kd = a.kd + (int64_t)b * a.kd_b + (int64_t)hk * a.kd_h + (int64_t)j * a.kd_n;
-      const uint8_t* vd = a.vd + (int64_t)b * a.vd_b + (int64_t)hk * a.vd_h + (int64_t)j * a.vd_n;
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        k[i] = kd[lane * CH + i];
-        v[i] = load_elem(vd, lane * CH + i, VDT);
+      if constexpr (TPR > 1) mine += (int)xchg_u32<1>((unsigned)mine);
+      if constexpr (TPR > 2) mine += (int)xchg_u32<2>((unsigned)mine);
+      if constexpr (TPR > 4) mine += (int)xchg_u32<4>((unsigned)mine);
+      if constexpr (TPR > 8) mine += (int)xchg_u32<8>((unsigned)mine);
+      low = (int)min(max((int64_t)n + mine - a.window, (int64_t)0), (int64_t)n);
+    }
+    if (tid == 0) {
+      ext_s[0] = 0x7FFFFFFF;
+      ext_s[1] = 0;
+      bad_s = 0;
+    }
+    __syncthreads();
+    if (builds && part == 0) {
+      low_s[brow] = low;
+      if (real) {
+        atomicMin(&ext_s[0], low);
+        atomicMax(&ext_s[1], low);
       }
     }
-    float x = 0.f;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) x = __builtin_fmaf(q[i], k[i], x);
-    x = allreduce_sum<1, 64>(x);
-    const float mn = fmaxf(m, x);
-    const float f = exp2_of((double)m - (double)mn), p = exp2_of((double)x - (double)mn);
-    m = mn;
-    l = __builtin_fmaf(l, f, p);
-#pragma unroll
-    for (int i = 0; i < CH; ++i) acc[i] = __builtin_fmaf(acc[i], f, p * v[i]);
+    __syncthreads();
   }
-  if (c.lens_out && blockIdx.x == 0 && threadIdx.x == 0) c.lens_out[b] = c.seq_lens[b];
-  __shared__ float m_s[W], l_s[W], acc_s[W][D];
+  const int low_min = __builtin_amdgcn_readfirstlane(ext_s[0]);
+  const int low_max = __builtin_amdgcn_readfirstlane(ext_s[1]);
+
+  // ---- the items: scale groups of the sinks, of the window, and 64 drafts each ----
+  const int group_rows = c.pages_per_group * c.page_rows;
+  const int cpp = (c.page_rows + 15) >> 4, cpg = cpp * c.pages_per_group;
+  const int gend = fdiv(n, a.div_group) + (n % group_rows != 0);
+  const int gw0 = a.sinks >= low_min ? 0 : fdiv(low_min, a.div_group);
+  const int nsg = min(fdiv(min(a.sinks, n) + group_rows - 1, a.div_group), gw0);
+  const int ng = nsg + max(gend - gw0, 0);
+  const int nd = a.mask ? (a.nodes + 63) >> 6 : 0;
+  const int tot = ng + nd;
+  const int i0 = (int)((int64_t)split * tot / c.num_splits);
+  const int i1 = (int)((int64_t)(split + 1) * tot / c.num_splits);
+  const int it0 = min(i0, ng), it1 = min(i1, ng);
+  const int dr0 = max(i0, ng) - ng, dr1 = max(i1, ng) - ng;
+  auto group_of = [&](int it) { return it < nsg ? it : it - nsg + gw0; };
+
+  const float* sbase = c.k_scale + (int64_t)b * c.s_b + (int64_t)hk * c.s_h;
+  const float* zbase = c.k_zp + (int64_t)b * c.s_b + (int64_t)hk * c.s_h;
+  const uint8_t* kbase = c.k_pages + (int64_t)hk * c.k_head;
+  const uint8_t* vbase = reinterpret_cast<const uint8_t*>(c.v_pages) +
+                         (int64_t)hk * c.v_head * G::VEB;
+  const unsigned krow_b = (unsigned)c.k_row, vrow_b = (unsigned)(c.v_row * G::VEB);
+  const unsigned k_lane = grp * (D / 8), v_lane = n16 * G::PB;
+  const int32_t* table = c.page_table ? c.page_table + (int64_t)b * c.pt_b : nullptr;
+
+  // ---- a step: CPS chunks of 16 rows of a group, for this wave ----
+  struct Meta {
+    unsigned phys[CPS];
+    int r0[CPS], nval[CPS], tok0[CPS];
+  };
+  auto meta_of = [&](int it, int p) __attribute__((always_inline)) -> Meta {
+    Meta m;
+    const int g = group_of(it);
 #pragma unroll
-  for (int i = 0; i < CH; ++i) acc_s[w][lane * CH + i] = acc[i];
-  if (lane == 0) {
-    m_s[w] = m;
-    l_s[w] = l;
+    for (int e = 0; e < CPS; ++e) {
+      const int j = (p * CPS + e) * kRowWaves + w;
+      const int pj = fdiv(j, c.div_cpp);
+      const int lp = g * c.pages_per_group + pj;
+      const int r0 = (j - pj * cpp) * 16;
+      const int tok0 = lp * c.page_rows + r0;
+      int nval = j < cpg ? min(min(16, c.page_rows - r0), n - tok0) : 0;
+      // Behind the sinks and before every row's window.
+      if (tok0 >= a.sinks && tok0 + nval <= low_min) nval = 0;
+      const bool some = nval > 0;
+      const int pg = some ? (table ? ld_ro(table, lp) : lp) : 0;
+      m.phys[e] = (unsigned)min(max(pg, 0), c.num_pages - 1);
+      m.r0[e] = some ? r0 : 0;
+      m.nval[e] = nval;
+      m.tok0[e] = tok0;
+    }
+    return m;
+  };
+
+  struct Buf {
+    unsigned k[CPS][G::KW];
+    unsigned v[CPS][4][G::NP][G::PB / 4];
+  };
+  // Rows past the valid count are loaded from the last valid row, a chunk of none from
+  // the first row of some page (never out of bounds, and its values are dropped).
+  auto load_step = [&](const Meta& m, Buf& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < CPS; ++e) {
+      const int last = max(m.nval[e] - 1, 0);
+      const uint8_t* kb = kbase + ((uint64_t)m.phys[e] * (uint64_t)c.k_page +
+                                   (uint64_t)(unsigned)m.r0[e] * krow_b);
+      const unsigned ko = k_lane + (unsigned)min(n16, last) * krow_b;
+      constexpr int KL = G::KW < 4 ? G::KW : 4;
+#pragma unroll
+      for (int i = 0; i < G::KW / KL; ++i) {
+        const KVec<KL> x = load_k<KL>(kb + (ko + 16 * i));
+#pragma unroll
+        for (int k = 0; k < KL; ++k) f.k[e][KL * i + k] = x.w[k];
+      }
+      const uint8_t* vb = vbase + ((uint64_t)m.phys[e] * (uint64_t)(c.v_page * G::VEB) +
+                                   (uint64_t)(unsigned)m.r0[e] * vrow_b);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned vo = v_lane + (unsigned)min(4 * grp + i, last) * vrow_b;
+#pragma unroll
+        for (int u = 0; u < G::NP; ++u) {
+          const KVec<G::PB / 4> x = load_k<G::PB / 4>(vb + (vo + 16 * G::PB * u));
+#pragma unroll
+          for (int k = 0; k < G::PB / 4; ++k) f.v[e][i][u][k] = x.w[k];
+        }
+      }
+    }
+  };
+
+  // ---- scales of a group to LDS, and the rows' digits ----
+  // Thread t < D / 2 holds 16 bytes: scales 4t .. (t < D / 4), or zero-points.
+  auto load_sz = [&](int it) __attribute__((always_inline)) -> U32x4 {
+    const int g = group_of(max(min(it, it1 - 1), 0));
+    const int e = tid % (D / 2);
+    const float* src = e < D / 4 ? sbase + 4 * e : zbase + 4 * (e - D / 4);
+    return ld16(src + (uint64_t)(unsigned)g * (uint64_t)c.s_g);
+  };
+  auto stage_sz = [&](const U32x4& x, int buf) __attribute__((always_inline)) {
+    if (tid >= (D / 2 + 63) / 64 * 64) return;     // whole waves
+    const bool is_s = tid < D / 4;
+    float4 y = make_float4(u2f(x.x), u2f(x.y), u2f(x.z), u2f(x.w));
+    if (w == 0) {
+      unsigned mx = is_s ? max(max(x.x & 0x7FFFFFFFu, x.y & 0x7FFFFFFFu),
+                               max(x.z & 0x7FFFFFFFu, x.w & 0x7FFFFFFFu))
+                         : 0u;
+      mx = max(mx, xchg_u32<1>(mx));
+      mx = max(mx, xchg_u32<2>(mx));
+      mx = max(mx, xchg_u32<4>(mx));
+      mx = max(mx, xchg_u32<8>(mx));
+      mx = max(mx, xchg_u32<16>(mx));
+      mx = max(mx, xchg_u32<32>(mx));
+      const float unit = u2f(max(mx, f2u(1e-28f))) * 0x1p-30f;
+      const float inv = (1.f - 0x1p-20f) / unit;
+      if (is_s) {
+        y.x *= inv;
+        y.y *= inv;
+        y.z *= inv;
+        y.w *= inv;
+      }
+      if (tid == 0) cs_s[buf] = unit * (1.f + 0x1p-20f);
+    }
+    if (tid < D / 2) {
+      float* dst = sz_s[buf] + (is_s ? 0 : D) + row_slot(4 * (tid % (D / 4)));
+      *reinterpret_cast<float2*>(dst) = make_float2(y.x, y.z);
+      *reinterpret_cast<float2*>(dst + 8) = make_float2(y.y, y.w);
+    }
+  };
+  auto build = [&](int buf) __attribute__((always_inline)) {
+    const float* s = sz_s[buf] + part * SPT;
+    const float* z = s + D;
+    uint8_t* dst = smem + buf * G::kDig + min(brow, M - 1) * G::DS + part * SPT;
+    float cg[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < SPT; i += 4) {
+      const float4 s4 = *reinterpret_cast<const float4*>(s + i);
+      const float4 z4 = *reinterpret_cast<const float4*>(z + i);
+      const float v0 = qn[i] * s4.x, v1 = qn[i + 1] * s4.y, v2 = qn[i + 2] * s4.z,
+                  v3 = qn[i + 3] * s4.w;
+      cg[0] = __builtin_fmaf(v0, z4.x, cg[0]);
+      cg[1] = __builtin_fmaf(v1, z4.y, cg[1]);
+      cg[2] = __builtin_fmaf(v2, z4.z, cg[2]);
+      cg[3] = __builtin_fmaf(v3, z4.w, cg[3]);
+      const unsigned x0 = (unsigned)(int)v0 + 0x808080u, x1 = (unsigned)(int)v1 + 0x808080u,
+                     x2 = (unsigned)(int)v2 + 0x808080u, x3 = (unsigned)(int)v3 + 0x808080u;
+      const unsigned t0 = __builtin_amdgcn_perm(x1, x0, 0x05010400u);
+      const unsigned t1 = __builtin_amdgcn_perm(x1, x0, 0x07030602u);
+      const unsigned u0 = __builtin_amdgcn_perm(x3, x2, 0x05010400u);
+      const unsigned u1 = __builtin_amdgcn_perm(x3, x2, 0x07030602u);
+      const unsigned dg[4] = {__builtin_amdgcn_perm(u0, t0, 0x05040100u) ^ 0x80808080u,
+                              __builtin_amdgcn_perm(u0, t0, 0x07060302u) ^ 0x80808080u,
+                              __builtin_amdgcn_perm(u1, t1, 0x05040100u) ^ 0x80808080u,
+                              __builtin_amdgcn_perm(u1, t1, 0x07060302u)};
+      if (builds) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<unsigned*>(dst + k * M * G::DS + i) = dg[k];
+      }
+    }
+    float cgs = (cg[0] + cg[1]) + (cg[2] + cg[3]);
+    if constexpr (TPR > 1) cgs += xchg<1>(cgs);
+    if constexpr (TPR > 2) cgs += xchg<2>(cgs);
+    if constexpr (TPR > 4) cgs += xchg<4>(cgs);
+    if constexpr (TPR > 8) cgs += xchg<8>(cgs);
+    if (builds && part == 0) {
+      const float c1 = qm_s[brow] * cs_s[buf] * kLog2e;
+      cc_s[buf][brow] = make_float2(c1, cgs * c1);
+    }
+  };
+
+  // ---- softmax and values ----
+  float m_run[RT], l_run[RT];
+  v4f acc[RT][NA];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m_run[rt] = kLeast;
+    l_run[rt] = 0.f;
+#pragma unroll
+    for (int t = 0; t < NA; ++t) acc[rt][t] = v4f{0.f, 0.f, 0.f, 0.f};
   }
+
+  // Value operands of a step, the same for all row tiles.
+  constexpr int AW = VDT == kVF32 ? 1 : 4;
+  auto value_op = [&](const Buf& f, int t, unsigned* o) __attribute__((always_inline)) {
+    const int u = t / G::CPP, j = t % G::CPP;
+    const unsigned sel = j & 1 ? 0x07060302u : 0x05040100u;
+#pragma unroll
+    for (int e = 0; e < CPS; ++e) {
+      o[2 * e] = __builtin_amdgcn_perm(f.v[e][1][u][j / 2], f.v[e][0][u][j / 2], sel);
+      o[2 * e + 1] = __builtin_amdgcn_perm(f.v[e][3][u][j / 2], f.v[e][2][u][j / 2], sel);
+    }
+  };
+  // Element (chunk e, row 4 grp + i) of output tile t's channel of this lane.
+  auto value_at = [&](const Buf& f, int t, int e, int i) __attribute__((always_inline)) -> float {
+    const int u = t / G::CPP, j = t % G::CPP;
+    if constexpr (VDT == kVF32) return u2f(f.v[e][i][u][j]);
+    const unsigned x = f.v[e][i][u][j / 2];
+    if constexpr (VDT == kVF16)
+      return (float)__builtin_bit_cast(_Float16, (unsigned short)(x >> (16 * (j & 1))));
+    return u2f(j & 1 ? x & 0xFFFF0000u : x << 16);
+  };
+
+  // Row tile rt takes the step's keys: scores s (logit = s * c1 - cc, log2 units) of
+  // keys 4 grp + i of chunk e in s[4 e + i], of which those in vis are seen.
+  auto take = [&](int rt, const Buf& f, const unsigned (*va)[AW], const float* s, float c1,
+                  float cc, bool masked, unsigned vis) __attribute__((always_inline)) {
+    constexpr int NS = 4 * CPS;
+    float x[NS];
+#pragma unroll
+    for (int k = 0; k < NS; ++k) x[k] = s[k];
+    if (masked) {
+#pragma unroll
+      for (int k = 0; k < NS; ++k) x[k] = (vis >> k) & 1u ? x[k] : kLeast;
+    }
+    float mx = x[0];
+#pragma unroll
+    for (int k = 1; k < NS; ++k) mx = fmaxf(mx, x[k]);
+    mx = over_groups_max(mx);
+    // (A row that sees none of them has mx = kLeast: no new shift.)
+    const float top = mx == kLeast ? kLeast : __builtin_fmaf(mx, c1, -cc);
+    const bool up = top > m_run[rt] + (kUp + kSlack);
+    if (__builtin_amdgcn_ballot_w64(up)) {
+      const float m_new = up ? __builtin_ceilf(top) - kUp : m_run[rt];
+      const float corr = __builtin_amdgcn_exp2f(m_run[rt] - m_new);
+      m_run[rt] = m_new;
+      l_run[rt] *= corr;
+#pragma unroll
+      for (int t = 0; t < NA; ++t) acc[rt][t] *= corr;
+    }
+    const float sub = -cc - m_run[rt];
+    float p[NS], ps = 0.f;
+#pragma unroll
+    for (int k = 0; k < NS; ++k) {
+      p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], c1, sub));
+    }
+    if (masked) {
+#pragma unroll
+      for (int k = 0; k < NS; ++k) p[k] = (vis >> k) & 1u ? p[k] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < NS; ++k) ps += p[k];
+    l_run[rt] += ps;
+    if constexpr (VDT == kVF32) {
+#pragma unroll
+      for (int t = 0; t < NA; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(value_at(f, t, 0, i), p[i],
+                                                            acc[rt][t], 0, 0, 0);
+    } else {
+      unsigned bt[TERMS][4];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        float y0 = p[2 * h], y1 = p[2 * h + 1];
+#pragma unroll
+        for (int q = 0; q < TERMS; ++q) {
+          if constexpr (VDT == kVF16) {
+            const float h0 = q == TERMS - 1 ? y0 : u2f(f2u(y0) & 0xFFFFE000u);
+            const float h1 = q == TERMS - 1 ? y1 : u2f(f2u(y1) & 0xFFFFE000u);
+            bt[q][h] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(h0, h1));
+            y0 -= h0;
+            y1 -= h1;
+          } else {
+            const v2bf r = __builtin_convertvector(v2f{y0, y1}, v2bf);
+            bt[q][h] = __builtin_bit_cast(unsigned, r);
+            y0 -= u2f(bt[q][h] << 16);
+            y1 -= u2f(bt[q][h] & 0xFFFF0000u);
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NA; ++t)
+#pragma unroll
+        for (int q = 0; q < TERMS; ++q) {
+          const uint4 av = make_uint4(va[t][0], va[t][1], va[t][2], va[t][3]);
+          const uint4 bv = make_uint4(bt[q][0], bt[q][1], bt[q][2], bt[q][3]);
+          if constexpr (VDT == kVF16)
+            acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, av),
+                                                                __builtin_bit_cast(v8h, bv),
+                                                                acc[rt][t], 0, 0, 0);
+          else
+            acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, av),
+                                                                 __builtin_bit_cast(v8bf, bv),
+                                                                 acc[rt][t], 0, 0, 0);
+        }
+    }
+  };
+
+  // Digit sums of row tile rt with the step's keys.
+  auto scores = [&](int rt, int buf, const v4i (*ak)[NB], v4i (*ds)[4])
+      __attribute__((always_inline)) {
+    const uint8_t* dg = smem + buf * G::kDig + (rt * 16 + n16) * G::DS + grp * (D / 4);
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const v4i bq = *reinterpret_cast<const v4i*>(dg + k * M * G::DS + 16 * kb);
+#pragma unroll
+        for (int e = 0; e < CPS; ++e)
+          ds[e][k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+              ak[e][kb], bq, kb == 0 ? v4i{0, 0, 0, 0} : ds[e][k], 0, 0, 0);
+      }
+  };
+
+  auto consume = [&](Buf& f, const Meta& m, int buf) __attribute__((always_inline)) {
+    bool any = false, masked = false;
+#pragma unroll
+    for (int e = 0; e < CPS; ++e) {
+      any |= m.nval[e] > 0;
+      masked |= m.nval[e] < 16 || (m.tok0[e] < low_max && m.tok0[e] + 16 > a.sinks);
+    }
+    if (!any) return;
+    // Keys that no row sees keep no value: a probability of zero times what lies
+    // there (a chunk of none holds anything) would be NaN where that is not finite.
+    if (masked) {
+#pragma unroll
+      for (int e = 0; e < CPS; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 4 * grp + i, t = m.tok0[e] + r;
+          const unsigned keep =
+              r < m.nval[e] && (t < a.sinks || t >= low_min) ? ~0u : 0u;
+#pragma unroll
+          for (int u = 0; u < G::NP; ++u)
+#pragma unroll
+            for (int k = 0; k < G::PB / 4; ++k) f.v[e][i][u][k] &= keep;
+        }
+    }
+    v4i ak[CPS][NB];
+#pragma unroll
+    for (int e = 0; e < CPS; ++e)
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb) {
+        const unsigned w0 = f.k[e][2 * kb], w1 = f.k[e][2 * kb + 1];
+        ak[e][kb] = v4i{(int)(w0 & 0x0F0F0F0Fu), (int)(w1 & 0x0F0F0F0Fu),
+                        (int)((w0 >> 4) & 0x0F0F0F0Fu), (int)((w1 >> 4) & 0x0F0F0F0Fu)};
+      }
+    unsigned va[NA][AW];
+    if constexpr (VDT != kVF32) {
+#pragma unroll
+      for (int t = 0; t < NA; ++t) value_op(f, t, va[t]);
+    }
+    v4i ds[2][CPS][4];
+    scores(0, buf, ak, ds[0]);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (rt + 1 < RT) scores(rt + 1, buf, ak, ds[(rt + 1) & 1]);
+      float s[4 * CPS];
+#pragma unroll
+      for (int e = 0; e < CPS; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const v4i* d = ds[rt & 1][e];
+          s[4 * e + i] = __builtin_fmaf((float)((d[3][i] << 8) + d[2][i]), 65536.f,
+                                        (float)((d[1][i] << 8) + d[0][i]));
+        }
+      const float2 cc = cc_s[buf][rt * 16 + n16];
+      unsigned vis = 0;
+      if (masked) {
+        const int low = low_s[rt * 16 + n16];
+#pragma unroll
+        for (int e = 0; e < CPS; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 4 * grp + i, t = m.tok0[e] + r;
+            vis |= (r < m.nval[e] && (t < a.sinks || t >= low) ? 1u : 0u) << (4 * e + i);
+          }
+      }
+      take(rt, f, va, s, cc.x, cc.y, masked, vis);
+    }
+  };
+
+  // ---- drafts: 16 of them a wave and item ----
+  auto drafts = [&](int item) __attribute__((always_inline)) {
+    const int j0 = (item * kRowWaves + w) * 16;
+    const int nval = min(16, a.nodes - j0);
+    if (nval <= 0) return;
+    Buf f;
+    const uint8_t* vb = a.vd + (int64_t)b * a.vd_b + (int64_t)hk * a.vd_h + v_lane;
+#pragma unroll
+    for (int e = 0; e < CPS; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int u = 0; u < G::NP; ++u) {
+          KVec<G::PB / 4> x = {};
+          if (e == 0)
+            x = load_k<G::PB / 4>(vb + (int64_t)(j0 + min(4 * grp + i, nval - 1)) * a.vd_n +
+                                  16 * G::PB * u);
+#pragma unroll
+          for (int k = 0; k < G::PB / 4; ++k) f.v[e][i][u][k] = x.w[k];
+        }
+    unsigned va[NA][AW];
+    if constexpr (VDT != kVF32) {
+#pragma unroll
+      for (int t = 0; t < NA; ++t) value_op(f, t, va[t]);
+    }
+    const float* kd = a.kd + (int64_t)b * a.kd_b + (int64_t)hk * a.kd_h +
+                      (int64_t)(j0 + min(n16, nval - 1)) * a.kd_n + grp * (D / 4);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int Rq = min(row0 + rt * 16 + n16, rows - 1);
+      const int i = Rq % a.nodes;
+      const int64_t q0 = (int64_t)b * c.q_b + (int64_t)(hk * c.hq_per_kv + Rq / a.nodes) * c.q_h +
+                         (int64_t)i * a.q_n + grp * (D / 4);
+      v4f ds = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int d = 0; d < D / 4; d += 4) {
+        const float4 k4 = *reinterpret_cast<const float4*>(kd + d);
+        ds = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.x, load_elem(c.q, q0 + d, c.q_dtype), ds, 0, 0, 0);
+        ds = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.y, load_elem(c.q, q0 + d + 1, c.q_dtype), ds, 0, 0, 0);
+        ds = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.z, load_elem(c.q, q0 + d + 2, c.q_dtype), ds, 0, 0, 0);
+        ds = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.w, load_elem(c.q, q0 + d + 3, c.q_dtype), ds, 0, 0, 0);
+      }
+      const uint8_t* mk = a.mask + (int64_t)b * a.mk_b + (int64_t)i * a.mk_i + j0;
+      unsigned vis = 0;
+      float s[4 * CPS];
+#pragma unroll
+      for (int k = 0; k < 4 * CPS; ++k) s[k] = kLeast;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = 4 * grp + k;
+        vis |= (mk[min(r, nval - 1)] != 0 && r < nval ? 1u : 0u) << k;
+        s[k] = ds[k];
+      }
+      take(rt, f, va, s, kLog2e, 0.f, true, vis);
+    }
+  };
+
+  // ---- the range ----
+  const int spg = (cpg + CPS * kRowWaves - 1) / (CPS * kRowWaves);
+  const int steps = (it1 - it0) * spg;
+  if (steps > 0) {
+    U32x4 szr;
+    {
+      const U32x4 x0 = load_sz(it0), x1 = load_sz(it0 + 1);
+      szr = load_sz(it0 + 2);
+      stage_sz(x0, 0);
+      stage_sz(x1, 1);
+    }
+    Buf f[2];
+    int li = it0, lp = 0;                          // item and step of the next metadata
+    auto next_meta = [&]() __attribute__((always_inline)) -> Meta {
+      // (Behind the last item: chunks of none.)
+      const Meta m = meta_of(min(li, it1 - 1), li < it1 ? lp : spg);
+      if (++lp == spg) {
+        lp = 0;
+        ++li;
+      }
+      return m;
+    };
+    Meta cur = next_meta(), nxt = next_meta();
+    load_step(cur, f[0]);
+    __syncthreads();
+    build(0);
+    int it = it0, p = 0, done = 0;
+    auto step = [&](Buf& now, Buf& then) __attribute__((always_inline)) -> bool {
+      const int buf = (it - it0) & 1;
+      if (p == 0) {
+        __syncthreads();
+        if (it + 1 < it1) build(buf ^ 1);
+        stage_sz(szr, buf);                        // of item it + 2
+      }
+      szr = load_sz(it + 3);
+      load_step(nxt, then);
+      const Meta ahead = next_meta();
+      consume(now, cur, buf);
+      cur = nxt;
+      nxt = ahead;
+      if (++p == spg) {
+        p = 0;
+        ++it;
+      }
+      return ++done == steps;
+    };
+    while (true) {
+      if (step(f[0], f[1])) break;
+      if (step(f[1], f[0])) break;
+    }
+  }
+  for (int i = dr0; i < dr1; ++i) drafts(i);
+
+  // The range again for every row by itself, a wave a row and key after key, for the
+  // rare workgroup with a NaN: a key that a row does not see takes no part in it.
+  auto plain_rows = [&]() {
+    constexpr int CH = D / 64;
+    float* part0 = reinterpret_cast<float*>(smem);
+    __syncthreads();
+    for (int i = tid; i < kRowWaves * M; i += kRowWaves * 64) {
+      m_s[i / M][i % M] = kLeast;
+      l_s[i / M][i % M] = 0.f;
+    }
+    for (int i = tid; i < kRowWaves * M * G::AS; i += kRowWaves * 64) part0[i] = 0.f;
+    __syncthreads();
+    for (int r = w; r < M && row0 + r < rows; r += kRowWaves) {
+      const int i = (row0 + r) % a.nodes;
+      const int64_t q0 = (int64_t)b * c.q_b +
+                         (int64_t)(hk * c.hq_per_kv + (row0 + r) / a.nodes) * c.q_h +
+                         (int64_t)i * a.q_n + lane * CH;
+      float q[CH], o[CH];
+      for (int k = 0; k < CH; ++k) {
+        q[k] = load_elem(c.q, q0 + k, c.q_dtype);
+        o[k] = 0.f;
+      }
+      float m = kLeast, l = 0.f;
+      auto key = [&](const float* k, const float* v) {
+        float x = 0.f;
+        for (int d = 0; d < CH; ++d) x = __builtin_fmaf(q[d], k[d], x);
+        x = allreduce_sum<1, 64>(x) * kLog2e;
+        const float mn = fmaxf(m, x);
+        const float f = __builtin_amdgcn_exp2f(m - mn), p = __builtin_amdgcn_exp2f(x - mn);
+        m = mn;
+        l = __builtin_fmaf(l, f, p);
+        for (int d = 0; d < CH; ++d) o[d] = __builtin_fmaf(o[d], f, p * v[d]);
+      };
+      for (int it = it0; it < it1; ++it) {
+        const int g = group_of(it);
+        for (int t = g * group_rows; t < min((g + 1) * group_rows, n); ++t) {
+          if (t >= a.sinks && t < low_s[r]) continue;
+          const int lp = fdiv(t, c.div_rows), tr = t - lp * c.page_rows;
+          const int64_t phys = min(max(table ? table[lp] : lp, 0), c.num_pages - 1);
+          const uint8_t* kp = kbase + phys * c.k_page + (int64_t)tr * c.k_row;
+          const int64_t vo = phys * c.v_page + (int64_t)hk * c.v_head + (int64_t)tr * c.v_row;
+          float k[CH], v[CH];
+          for (int j = 0; j < CH; ++j) {
+            const int d = lane * CH + j;
+            const float s = sbase[(int64_t)g * c.s_g + d], z = zbase[(int64_t)g * c.s_g + d];
+            k[j] = (float)((kp[d >> 1] >> (4 * (d & 1))) & 15) * s - z * s;
+            v[j] = load_elem(c.v_pages, vo + d, VDT);
+          }
+          key(k, v);
+        }
+      }
+      for (int j = dr0 * 64; j < min(dr1 * 64, a.nodes); ++j) {
+        if (!a.mask[(int64_t)b * a.mk_b + (int64_t)i * a.mk_i + j]) continue;
+        const float* kd = a.kd + (int64_t)b * a.kd_b + (int64_t)hk * a.kd_h + (int64_t)j * a.kd_n;
+        const uint8_t* vd = a.vd + (int64_t)b * a.vd_b + (int64_t)hk * a.vd_h + (int64_t)j * a.vd_n;
+        float v[CH];
+        for (int d = 0; d < CH; ++d) v[d] = load_elem(vd, lane * CH + d, VDT);
+        key(kd + lane * CH, v);
+      }
+      for (int k = 0; k < CH; ++k) part0[r * G::AS + lane * CH + k] = o[k];
+      if (lane == 0) {
+        m_s[0][r] = m;
+        l_s[0][r] = l;
+      }
+    }
+    __syncthreads();
+  };
+
+  // ---- the waves' parts ----
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const float l = over_groups_sum(l_run[rt]);
+    if (grp == 0) {
+      m_s[w][rt * 16 + n16] = m_run[rt];
+      l_s[w][rt * 16 + n16] = l;
+    }
+  }
+  __syncthreads();                                 // (the digits are no longer read)
+  float* out_w = reinterpret_cast<float*>(smem) + w * M * G::AS;
+  float any_nan = 0.f;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = rt * 16 + n16;
+    float top = m_s[0][r];
+#pragma unroll
+    for (int i = 1; i < kRowWaves; ++i) top = fmaxf(top, m_s[i][r]);
+    const float f = __builtin_amdgcn_exp2f(m_run[rt] - top);
+#pragma unroll
+    for (int u = 0; u < G::NP; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float* dst = out_w + r * G::AS + u * 16 * G::CPP + (4 * grp + i) * G::CPP;
+#pragma unroll
+        for (int j = 0; j < G::CPP; j += 4) {
+          const float4 x =
+              make_float4(acc[rt][u * G::CPP + j][i] * f, acc[rt][u * G::CPP + j + 1][i] * f,
+                          acc[rt][u * G::CPP + j + 2][i] * f, acc[rt][u * G::CPP + j + 3][i] * f);
+          *reinterpret_cast<float4*>(dst + j) = x;
+          any_nan += (x.x + x.y) + (x.z + x.w);
+        }
+      }
+  }
+  if (!(any_nan == any_nan)) bad_s = 1;
   __syncthreads();
-  if (w) return;
-  const float ms = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3]));
-  float lt = 0.f, o[CH] = {};
-  for (int i = 0; i < W; ++i) {
-    if (m_s[i] == -INFINITY && l_s[i] == 0.f) continue;
-    const float f = exp2_of((double)m_s[i] - (double)ms);
-    lt = __builtin_fmaf(l_s[i], f, lt);
+  if (bad_s) plain_rows();
+  const float* parts = reinterpret_cast<const float*>(smem);
+  const int64_t o0 = ((int64_t)b * c.num_q_heads + (int64_t)hk * c.hq_per_kv) * a.nodes + row0;
+  for (int idx = tid * 4; idx < M * D; idx += kRowWaves * 64 * 4) {
+    const int r = idx / D, d = idx % D;
+    if (row0 + r >= rows) continue;
+    float top = m_s[0][r];
 #pragma unroll
-    for (int k = 0; k < CH; ++k) o[k] = __builtin_fmaf(acc_s[i][lane * CH + k], f, o[k]);
+    for (int i = 1; i < kRowWaves; ++i) top = fmaxf(top, m_s[i][r]);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < kRowWaves; ++i) {
+      l = __builtin_fmaf(__builtin_amdgcn_exp2f(m_s[i][r] - top), l_s[i][r], l);
+      const float4 x = *reinterpret_cast<const float4*>(parts + (i * M + r) * G::AS + d);
+      o.x += x.x;
+      o.y += x.y;
+      o.z += x.z;
+      o.w += x.w;
+    }
+    if (c.final_out) {
+      const float os[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        store_elem(c.out, (o0 + r) * D + d + k, c.out_dtype, l == 0.f ? 0.f : os[k] / l);
+    } else {
+      const int64_t pi = (o0 + r) * c.num_splits + split;
+      *reinterpret_cast<float4*>(c.ws_acc + pi * D + d) = o;
+      if (d == 0) {
+        c.ws_ml[2 * pi] = l == 0.f ? -INFINITY : (double)top * 0.6931471805599453;
+        c.ws_ml[2 * pi + 1] = (double)l;
+      }
+    }
   }
-#pragma unroll
-  for (int k = 0; k < CH; ++k)
-    store_elem(c.out, ((int64_t)b * gridDim.x + row) * D + lane * CH + k, c.out_dtype,
-               lt == 0.f ? 0.f : o[k] / lt);
 }
 
 hipError_t launch_decode_rows(const RowsArgs& a, int D, int v_dtype, int batch, hipStream_t st) {
-  dim3 grid(a.c.num_q_heads * a.nodes, batch);
-#define FDI4_RW(DD, VV)                                                                     \
-  if (D == DD && v_dtype == VV) {                                                           \
-    hipLaunchKernelGGL((decode_rows_kernel<DD, VV>), grid, dim3(256), 0, st, a);            \
-    return hipGetLastError();                                                               \
+  const int64_t wgs = (int64_t)a.tiles * a.c.num_splits * (a.c.num_q_heads / a.c.hq_per_kv) *
+                      batch;
+  if (wgs > INT32_MAX) return hipErrorInvalidValue;
+  const bool wide = a.c.out_dtype == kEF32;
+#define FDI4_RW(DD, VV, RR, TT)                                                              \
+  if (D == DD && v_dtype == VV && a.row_tiles == RR && (VV != kVBF16 || wide == (TT == 3))) { \
+    hipLaunchKernelGGL((decode_rows_kernel<DD, VV, RR, TT>), dim3((unsigned)wgs),             \
+                       dim3(kRowWaves * 64), 0, st, a);                                       \
+    return hipGetLastError();                                                                 \
   }
-  FDI4_RW(64, kVF32) FDI4_RW(64, kVF16) FDI4_RW(64, kVBF16)
-  FDI4_RW(128, kVF32) FDI4_RW(128, kVF16) FDI4_RW(128, kVBF16)
-  FDI4_RW(256, kVF32) FDI4_RW(256, kVF16) FDI4_RW(256, kVBF16)
+#define FDI4_RW_V(DD, RR) \
+  FDI4_RW(DD, kVF32, RR, 1) FDI4_RW(DD, kVF16, RR, 2) FDI4_RW(DD, kVBF16, RR, 2) \
+  FDI4_RW(DD, kVBF16, RR, 3)
+  FDI4_RW_V(64, 1) FDI4_RW_V(64, 2) FDI4_RW_V(64, 3) FDI4_RW_V(64, 4)
+  FDI4_RW_V(128, 1) FDI4_RW_V(128, 2) FDI4_RW_V(128, 3) FDI4_RW_V(128, 4)
+  FDI4_RW_V(256, 1) FDI4_RW_V(256, 2)
+#undef FDI4_RW_V
 #undef FDI4_RW
   return hipErrorInvalidValue;
 }

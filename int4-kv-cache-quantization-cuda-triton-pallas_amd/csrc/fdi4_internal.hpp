@@ -159,6 +159,9 @@ struct RowsArgs {
   int64_t mk_b, mk_i;                   // bytes
   int window;                           // 0: the whole cache
   int sinks;
+  FastDiv div_group;                    // by the rows of a scale group
+  int row_tiles;                        // 16-row tiles per workgroup
+  int tiles;                            // workgroups for the rows of a kv-head
 };
 
 // Several tokens per sequence appended: counts[b] of the new rows (by index when
