@@ -903,8 +903,8 @@ RowsPlan plan_rows(int batch, int num_q_heads, int nodes, int window, int sinks,
   const int most = cache->head_dim == 256 ? 2 : 4;
   const int64_t rows = (int64_t)(num_q_heads / cache->num_kv_heads) * nodes;
   const int64_t t16 = (rows + 15) / 16;
-  p.tiles = (int)((t16 + most - 1) / most);
-  p.row_tiles = (int)((t16 + p.tiles - 1) / p.tiles);
+  p.row_tiles = t16 >= 3 ? most : (int)std::min<int64_t>(t16, most);
+  p.tiles = (int)((t16 + p.row_tiles - 1) / p.row_tiles);
   // The most items a sequence can have.
   const int64_t cap = (int64_t)cache->max_pages * cache->page_rows;
   const int64_t G = (int64_t)std::min(cache->pages_per_group, std::max(cache->max_pages, 1)) *
@@ -915,7 +915,7 @@ RowsPlan plan_rows(int batch, int num_q_heads, int nodes, int window, int sinks,
   if (nodes > 1) items += (nodes + 63) / 64;
   items = std::max<int64_t>(items, 1);
   const int64_t streams = (int64_t)batch * cache->num_kv_heads * p.tiles;
-  const int64_t slots = p.row_tiles == 1 ? 2 * kCUs : kCUs;
+  const int64_t slots = p.row_tiles < most ? 2 * kCUs : kCUs;
   const int64_t s = num_splits > 0 ? num_splits : slots / std::max<int64_t>(streams, 1);
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(s, items), kMaxSplits));
   return p;

@@ -50,9 +50,9 @@ typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
-constexpr int kRowWaves = 4;
+constexpr int kKeyWaves = 4;   // waves that share a step's chunks (per row group)
 
-template <int D, int VDT, int RT, int TERMS>
+template <int D, int VDT, int RT, int RW>
 struct RowsGeo {
   static constexpr int NB = D / 64;                // 64-channel blocks of the key product
   static constexpr int KW = D / 32;                // packed key words per lane per row
@@ -62,12 +62,20 @@ struct RowsGeo {
   static constexpr int CPP = PB / VEB;             // channels per value load
   static constexpr int NA = D / 16;                // 16-channel output tiles
   static constexpr int CPS = VDT == kVF32 ? 1 : 2; // chunks per step
-  static constexpr int M = 16 * RT;                // rows of the workgroup
+  static constexpr int M = 16 * RT * RW;           // rows of the workgroup
+  static constexpr int NT = kKeyWaves * 64 * RW;   // threads
+  static constexpr int TPR = NT / M;               // threads per row that build digits
+  static constexpr int SPT = D / TPR;              // channels each
   static constexpr int DS = D + 16;                // bytes per row of a digit (padded)
   static constexpr int kDig = 4 * M * DS;          // a buffer of digits
-  static constexpr int AS = D + 4;                 // floats per row of a wave's output
-  static constexpr int kAcc = kRowWaves * M * AS * 4;
-  static constexpr int kSmem = 2 * kDig > kAcc ? 2 * kDig : kAcc;
+  static constexpr int AS = D + 4;                 // floats per row of queries and outputs
+  // LDS: two buffers of digits and the queries while the keys stream, then the waves'
+  // outputs.
+  static constexpr int kQ = 2 * kDig;
+  static constexpr int kStream = kQ + M * AS * 4;
+  static constexpr int kAcc = kKeyWaves * M * AS * 4;
+  static constexpr int kSmem = kStream > kAcc ? kStream : kAcc;
+  static_assert(TPR >= 4 && TPR <= 16 && (TPR & (TPR - 1)) == 0 && SPT % 4 == 0, "threads");
 };
 
 __device__ __forceinline__ int row_slot(int d) {
@@ -93,18 +101,16 @@ __device__ __forceinline__ float over_groups_sum(float x) {
   return u2f(s[0]) + u2f(s[1]);
 }
 
-template <int D, int VDT, int RT, int TERMS>
-__global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a) {
-  using G = RowsGeo<D, VDT, RT, TERMS>;
-  constexpr int NB = G::NB, CPS = G::CPS, NA = G::NA, M = G::M;
-  // Threads that build digits take whole rows: TPR (a power of two) per row.
-  constexpr int TPR = RT == 1 ? 16 : RT == 2 ? 8 : 4;
-  constexpr int SPT = D / TPR;                     // channels of a row per thread
-  constexpr int kWidth = kRowWaves * 64 / TPR;     // rows the threads cover: >= M
-  static_assert(kWidth >= M, "rows");
-  // Shift of the probabilities: largest logit + kUp at most kSlack above the shift's.
-  // float16 terms need the headroom (p * 2^kUp < 2^16) and the small end (quantum
-  // 2^-24): a probability's terms are exact to 2^-37 of the largest.
+// TERMS: 16-bit terms of a probability. RT row tiles a wave, RW row groups of four
+// waves: wave w takes key chunks w % 4 and row group w / 4.
+template <int D, int VDT, int RT, int RW, int TERMS>
+__global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(RowsArgs a) {
+  using G = RowsGeo<D, VDT, RT, RW>;
+  constexpr int NB = G::NB, CPS = G::CPS, NA = G::NA, M = G::M, NT = G::NT;
+  constexpr int TPR = G::TPR, SPT = G::SPT, NS = 4 * CPS;
+  // Shift of the probabilities: the largest is 2^kUp when the shift moves, and stays
+  // below 2^(kUp + kSlack). float16 terms need the headroom (2^16) and the small end
+  // (quantum 2^-24): a probability's terms are exact to 2^-37 of the largest.
   constexpr float kUp = VDT == kVF16 ? 13.f : 0.f;
   constexpr float kSlack = VDT == kVF16 ? 2.f : 8.f;
   constexpr float kLeast = -3.4028235e38f;
@@ -113,7 +119,9 @@ __global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a)
   const DecodeArgs& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kw = w & (kKeyWaves - 1), rg = w / kKeyWaves;
   const int n16 = lane & 15, grp = lane >> 4;
+  const int rbase = rg * 16 * RT;                  // first row of this wave's tiles
 
   // Tiles of one (sequence, kv-head, split) run on one XCD, one after the other: they
   // read the same pages.
@@ -126,85 +134,62 @@ __global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a)
   const int hk = (int)(wi % (unsigned)hkv), b = (int)(wi / (unsigned)hkv);
   const int rows = c.hq_per_kv * a.nodes;          // rows of this kv-head
   const int row0 = tile * M;
+  const int live = min(rows - row0, M);            // rows of this workgroup
 
   __shared__ __align__(16) uint8_t smem[G::kSmem];
   __shared__ __align__(16) float sz_s[2][2 * D];   // scaled scales, zero-points (slot order)
   __shared__ float cs_s[2];                        // a group's scale unit
   __shared__ float2 cc_s[2][M];                    // a row's logit unit and constant
-  __shared__ float qm_s[M];                        // a row's query unit
   __shared__ int low_s[M];                         // first cached token in a row's window
   __shared__ int ext_s[2];                         // smallest and largest of them
-  __shared__ float m_s[kRowWaves][M], l_s[kRowWaves][M];
+  __shared__ float m_s[kKeyWaves][M], l_s[kKeyWaves][M];
   __shared__ int bad_s;
+  float* const q_s = reinterpret_cast<float*>(smem + G::kQ);
 
   const int n = seq_len_of(c, b);
   if (c.lens_out && tile == 0 && split == 0 && hk == 0 && tid == 0)
     c.lens_out[b] = c.seq_lens[b];
 
-  // ---- the rows: queries to registers (slot order, relative to the row's largest) ----
-  const int brow = tid / TPR, part = tid % TPR;
-  const bool builds = brow < M;
-  const int R = row0 + min(brow, M - 1);
-  const int node = R % a.nodes;
-  float qn[SPT];
-  {
-    const bool real = builds && R < rows;
-    const int64_t q0 = (int64_t)b * c.q_b +
-                       (int64_t)(hk * c.hq_per_kv + (real ? R / a.nodes : 0)) * c.q_h +
-                       (int64_t)(real ? node : 0) * a.q_n;
-    unsigned mx = 0;
-#pragma unroll
-    for (int i = 0; i < SPT; ++i) {
-      const float x = load_elem(c.q, q0 + row_channel(part * SPT + i), c.q_dtype);
-      qn[i] = real ? x : 0.f;
-      mx = max(mx, f2u(qn[i]) & 0x7FFFFFFFu);
-    }
-    if constexpr (TPR > 1) mx = max(mx, xchg_u32<1>(mx));
-    if constexpr (TPR > 2) mx = max(mx, xchg_u32<2>(mx));
-    if constexpr (TPR > 4) mx = max(mx, xchg_u32<4>(mx));
-    if constexpr (TPR > 8) mx = max(mx, xchg_u32<8>(mx));
-    // (As bits, so that NaN is the largest and makes the row NaN.)
-    const float unit = u2f(max(mx, f2u(1e-30f)));
-    const float inv = 1.f / unit;
-#pragma unroll
-    for (int i = 0; i < SPT; ++i) qn[i] *= inv;
-    if (builds && part == 0) qm_s[brow] = unit;
-    // The window of each row.
-    int low = 0;
-    if (a.window) {
+  // ---- each row's window ----
+  const int brow = tid / TPR, part = tid % TPR;    // this thread's row of digits
+  int low_min = 0, low_max = 0;
+  if (a.window) {
+    low_min = low_max = max(n - a.window, 0);
+    if (a.mask) {
+      // It ends at the node, whose visible drafts count.
+      const int node = (row0 + min(brow, live - 1)) % a.nodes;
+      const uint8_t* mk = a.mask + (int64_t)b * a.mk_b + (int64_t)node * a.mk_i;
       int mine = 0;
-      if (a.mask && real) {
-        const uint8_t* mk = a.mask + (int64_t)b * a.mk_b + (int64_t)node * a.mk_i;
-        for (int j = part; j < a.nodes; j += TPR) mine += mk[j] != 0;
-      }
-      if constexpr (TPR > 1) mine += (int)xchg_u32<1>((unsigned)mine);
-      if constexpr (TPR > 2) mine += (int)xchg_u32<2>((unsigned)mine);
+      for (int j = part; j < a.nodes; j += TPR) mine += mk[j] != 0;
+      mine += (int)xchg_u32<1>((unsigned)mine);
+      mine += (int)xchg_u32<2>((unsigned)mine);
       if constexpr (TPR > 4) mine += (int)xchg_u32<4>((unsigned)mine);
       if constexpr (TPR > 8) mine += (int)xchg_u32<8>((unsigned)mine);
-      low = (int)min(max((int64_t)n + mine - a.window, (int64_t)0), (int64_t)n);
-    }
-    if (tid == 0) {
-      ext_s[0] = 0x7FFFFFFF;
-      ext_s[1] = 0;
-      bad_s = 0;
-    }
-    __syncthreads();
-    if (builds && part == 0) {
-      low_s[brow] = low;
-      if (real) {
+      const int low = (int)min(max((int64_t)n + mine - a.window, (int64_t)0), (int64_t)n);
+      if (tid == 0) {
+        ext_s[0] = 0x7FFFFFFF;
+        ext_s[1] = 0;
+      }
+      __syncthreads();
+      if (part == 0) {
+        low_s[brow] = low;
         atomicMin(&ext_s[0], low);
         atomicMax(&ext_s[1], low);
       }
+      __syncthreads();
+      low_min = __builtin_amdgcn_readfirstlane(ext_s[0]);
+      low_max = __builtin_amdgcn_readfirstlane(ext_s[1]);
+    } else if (tid < M) {
+      low_s[tid] = low_min;
     }
-    __syncthreads();
+  } else if (tid < M) {
+    low_s[tid] = 0;
   }
-  const int low_min = __builtin_amdgcn_readfirstlane(ext_s[0]);
-  const int low_max = __builtin_amdgcn_readfirstlane(ext_s[1]);
 
   // ---- the items: scale groups of the sinks, of the window, and 64 drafts each ----
   const int group_rows = c.pages_per_group * c.page_rows;
   const int cpp = (c.page_rows + 15) >> 4, cpg = cpp * c.pages_per_group;
-  const int gend = fdiv(n, a.div_group) + (n % group_rows != 0);
+  const int gend = fdiv(n + group_rows - 1, a.div_group);
   const int gw0 = a.sinks >= low_min ? 0 : fdiv(low_min, a.div_group);
   const int nsg = min(fdiv(min(a.sinks, n) + group_rows - 1, a.div_group), gw0);
   const int ng = nsg + max(gend - gw0, 0);
@@ -215,6 +200,7 @@ __global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a)
   const int it0 = min(i0, ng), it1 = min(i1, ng);
   const int dr0 = max(i0, ng) - ng, dr1 = max(i1, ng) - ng;
   auto group_of = [&](int it) { return it < nsg ? it : it - nsg + gw0; };
+  const int64_t o0 = ((int64_t)b * c.num_q_heads + (int64_t)hk * c.hq_per_kv) * a.nodes + row0;
 
   const float* sbase = c.k_scale + (int64_t)b * c.s_b + (int64_t)hk * c.s_h;
   const float* zbase = c.k_zp + (int64_t)b * c.s_b + (int64_t)hk * c.s_h;
@@ -226,53 +212,66 @@ __global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a)
   const int32_t* table = c.page_table ? c.page_table + (int64_t)b * c.pt_b : nullptr;
 
   // ---- a step: CPS chunks of 16 rows of a group, for this wave ----
+  const int spg = (cpg + CPS * kKeyWaves - 1) / (CPS * kKeyWaves);
   struct Meta {
     unsigned phys[CPS];
     int r0[CPS], nval[CPS], tok0[CPS];
   };
-  auto meta_of = [&](int it, int p) __attribute__((always_inline)) -> Meta {
+  int li = it0, lp = 0;                            // item and step of the next metadata
+  auto next_meta = [&]() __attribute__((always_inline)) -> Meta {
     Meta m;
-    const int g = group_of(it);
+    const int g = group_of(min(li, it1 - 1));
 #pragma unroll
     for (int e = 0; e < CPS; ++e) {
-      const int j = (p * CPS + e) * kRowWaves + w;
+      const int j = (lp * CPS + e) * kKeyWaves + kw;
       const int pj = fdiv(j, c.div_cpp);
-      const int lp = g * c.pages_per_group + pj;
+      const int page = g * c.pages_per_group + pj;
       const int r0 = (j - pj * cpp) * 16;
-      const int tok0 = lp * c.page_rows + r0;
-      int nval = j < cpg ? min(min(16, c.page_rows - r0), n - tok0) : 0;
+      const int tok0 = page * c.page_rows + r0;
+      int nval = j < cpg && li < it1 ? min(min(16, c.page_rows - r0), n - tok0) : 0;
       // Behind the sinks and before every row's window.
       if (tok0 >= a.sinks && tok0 + nval <= low_min) nval = 0;
       const bool some = nval > 0;
-      const int pg = some ? (table ? ld_ro(table, lp) : lp) : 0;
+      const int pg = some ? (table ? ld_ro(table, page) : page) : 0;
       m.phys[e] = (unsigned)min(max(pg, 0), c.num_pages - 1);
       m.r0[e] = some ? r0 : 0;
       m.nval[e] = nval;
       m.tok0[e] = tok0;
     }
+    if (++lp == spg) {
+      lp = 0;
+      ++li;
+    }
     return m;
   };
 
-  struct Buf {
-    unsigned k[CPS][G::KW];
-    unsigned v[CPS][4][G::NP][G::PB / 4];
-  };
   // Rows past the valid count are loaded from the last valid row, a chunk of none from
   // the first row of some page (never out of bounds, and its values are dropped).
-  auto load_step = [&](const Meta& m, Buf& f) __attribute__((always_inline)) {
+  struct Keys {
+    unsigned w[CPS][G::KW];
+  };
+  struct Vals {
+    unsigned w[CPS][4][G::NP][G::PB / 4];
+  };
+  auto load_keys = [&](const Meta& m, Keys& f) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < CPS; ++e) {
-      const int last = max(m.nval[e] - 1, 0);
       const uint8_t* kb = kbase + ((uint64_t)m.phys[e] * (uint64_t)c.k_page +
                                    (uint64_t)(unsigned)m.r0[e] * krow_b);
-      const unsigned ko = k_lane + (unsigned)min(n16, last) * krow_b;
+      const unsigned ko = k_lane + (unsigned)min(n16, max(m.nval[e] - 1, 0)) * krow_b;
       constexpr int KL = G::KW < 4 ? G::KW : 4;
 #pragma unroll
       for (int i = 0; i < G::KW / KL; ++i) {
         const KVec<KL> x = load_k<KL>(kb + (ko + 16 * i));
 #pragma unroll
-        for (int k = 0; k < KL; ++k) f.k[e][KL * i + k] = x.w[k];
+        for (int k = 0; k < KL; ++k) f.w[e][KL * i + k] = x.w[k];
       }
+    }
+  };
+  auto load_values = [&](const Meta& m, Vals& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < CPS; ++e) {
+      const int last = max(m.nval[e] - 1, 0);
       const uint8_t* vb = vbase + ((uint64_t)m.phys[e] * (uint64_t)(c.v_page * G::VEB) +
                                    (uint64_t)(unsigned)m.r0[e] * vrow_b);
 #pragma unroll
@@ -282,7 +281,7 @@ __global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a)
         for (int u = 0; u < G::NP; ++u) {
           const KVec<G::PB / 4> x = load_k<G::PB / 4>(vb + (vo + 16 * G::PB * u));
 #pragma unroll
-          for (int k = 0; k < G::PB / 4; ++k) f.v[e][i][u][k] = x.w[k];
+          for (int k = 0; k < G::PB / 4; ++k) f.w[e][i][u][k] = x.w[k];
         }
       }
     }
@@ -291,13 +290,13 @@ __global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a)
   // ---- scales of a group to LDS, and the rows' digits ----
   // Thread t < D / 2 holds 16 bytes: scales 4t .. (t < D / 4), or zero-points.
   auto load_sz = [&](int it) __attribute__((always_inline)) -> U32x4 {
-    const int g = group_of(max(min(it, it1 - 1), 0));
+    const int g = group_of(min(it, it1 - 1));
     const int e = tid % (D / 2);
     const float* src = e < D / 4 ? sbase + 4 * e : zbase + 4 * (e - D / 4);
     return ld16(src + (uint64_t)(unsigned)g * (uint64_t)c.s_g);
   };
   auto stage_sz = [&](const U32x4& x, int buf) __attribute__((always_inline)) {
-    if (tid >= (D / 2 + 63) / 64 * 64) return;     // whole waves
+    if (w >= (D / 2 + 63) / 64) return;
     const bool is_s = tid < D / 4;
     float4 y = make_float4(u2f(x.x), u2f(x.y), u2f(x.z), u2f(x.w));
     if (w == 0) {
@@ -326,10 +325,11 @@ __global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a)
       *reinterpret_cast<float2*>(dst + 8) = make_float2(y.y, y.w);
     }
   };
+  float qn[SPT], q_unit;                           // the row relative to its largest
   auto build = [&](int buf) __attribute__((always_inline)) {
     const float* s = sz_s[buf] + part * SPT;
     const float* z = s + D;
-    uint8_t* dst = smem + buf * G::kDig + min(brow, M - 1) * G::DS + part * SPT;
+    uint8_t* dst = smem + buf * G::kDig + brow * G::DS + part * SPT;
     float cg[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < SPT; i += 4) {
@@ -347,23 +347,22 @@ __global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a)
       const unsigned t1 = __builtin_amdgcn_perm(x1, x0, 0x07030602u);
       const unsigned u0 = __builtin_amdgcn_perm(x3, x2, 0x05010400u);
       const unsigned u1 = __builtin_amdgcn_perm(x3, x2, 0x07030602u);
-      const unsigned dg[4] = {__builtin_amdgcn_perm(u0, t0, 0x05040100u) ^ 0x80808080u,
-                              __builtin_amdgcn_perm(u0, t0, 0x07060302u) ^ 0x80808080u,
-                              __builtin_amdgcn_perm(u1, t1, 0x05040100u) ^ 0x80808080u,
-                              __builtin_amdgcn_perm(u1, t1, 0x07060302u)};
-      if (builds) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          *reinterpret_cast<unsigned*>(dst + k * M * G::DS + i) = dg[k];
-      }
+      *reinterpret_cast<unsigned*>(dst + i) =
+          __builtin_amdgcn_perm(u0, t0, 0x05040100u) ^ 0x80808080u;
+      *reinterpret_cast<unsigned*>(dst + M * G::DS + i) =
+          __builtin_amdgcn_perm(u0, t0, 0x07060302u) ^ 0x80808080u;
+      *reinterpret_cast<unsigned*>(dst + 2 * M * G::DS + i) =
+          __builtin_amdgcn_perm(u1, t1, 0x05040100u) ^ 0x80808080u;
+      *reinterpret_cast<unsigned*>(dst + 3 * M * G::DS + i) =
+          __builtin_amdgcn_perm(u1, t1, 0x07060302u);
     }
     float cgs = (cg[0] + cg[1]) + (cg[2] + cg[3]);
-    if constexpr (TPR > 1) cgs += xchg<1>(cgs);
-    if constexpr (TPR > 2) cgs += xchg<2>(cgs);
+    cgs += xchg<1>(cgs);
+    cgs += xchg<2>(cgs);
     if constexpr (TPR > 4) cgs += xchg<4>(cgs);
     if constexpr (TPR > 8) cgs += xchg<8>(cgs);
-    if (builds && part == 0) {
-      const float c1 = qm_s[brow] * cs_s[buf] * kLog2e;
+    if (part == 0) {
+      const float c1 = q_unit * cs_s[buf] * kLog2e;
       cc_s[buf][brow] = make_float2(c1, cgs * c1);
     }
   };
@@ -378,43 +377,22 @@ __global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a)
 #pragma unroll
     for (int t = 0; t < NA; ++t) acc[rt][t] = v4f{0.f, 0.f, 0.f, 0.f};
   }
+  // Probabilities of a step as the value product's operands.
+  constexpr int PW = VDT == kVF32 ? 4 : 4 * TERMS;
+  unsigned pr[RT][PW];
 
-  // Value operands of a step, the same for all row tiles.
-  constexpr int AW = VDT == kVF32 ? 1 : 4;
-  auto value_op = [&](const Buf& f, int t, unsigned* o) __attribute__((always_inline)) {
-    const int u = t / G::CPP, j = t % G::CPP;
-    const unsigned sel = j & 1 ? 0x07060302u : 0x05040100u;
-#pragma unroll
-    for (int e = 0; e < CPS; ++e) {
-      o[2 * e] = __builtin_amdgcn_perm(f.v[e][1][u][j / 2], f.v[e][0][u][j / 2], sel);
-      o[2 * e + 1] = __builtin_amdgcn_perm(f.v[e][3][u][j / 2], f.v[e][2][u][j / 2], sel);
-    }
-  };
-  // Element (chunk e, row 4 grp + i) of output tile t's channel of this lane.
-  auto value_at = [&](const Buf& f, int t, int e, int i) __attribute__((always_inline)) -> float {
-    const int u = t / G::CPP, j = t % G::CPP;
-    if constexpr (VDT == kVF32) return u2f(f.v[e][i][u][j]);
-    const unsigned x = f.v[e][i][u][j / 2];
-    if constexpr (VDT == kVF16)
-      return (float)__builtin_bit_cast(_Float16, (unsigned short)(x >> (16 * (j & 1))));
-    return u2f(j & 1 ? x & 0xFFFF0000u : x << 16);
-  };
-
-  // Row tile rt takes the step's keys: scores s (logit = s * c1 - cc, log2 units) of
-  // keys 4 grp + i of chunk e in s[4 e + i], of which those in vis are seen.
-  auto take = [&](int rt, const Buf& f, const unsigned (*va)[AW], const float* s, float c1,
-                  float cc, bool masked, unsigned vis) __attribute__((always_inline)) {
-    constexpr int NS = 4 * CPS;
-    float x[NS];
-#pragma unroll
-    for (int k = 0; k < NS; ++k) x[k] = s[k];
+  // Row tile rt and scores s (logit = s * c1 - cc, log2 units) of keys 4 grp + i of
+  // chunk e in s[4 e + i], of which those in vis are seen.
+  auto softmax = [&](int rt, const float* s, float c1, float cc, bool masked, unsigned vis)
+      __attribute__((always_inline)) {
+    float mx = kLeast;
     if (masked) {
 #pragma unroll
-      for (int k = 0; k < NS; ++k) x[k] = (vis >> k) & 1u ? x[k] : kLeast;
-    }
-    float mx = x[0];
+      for (int k = 0; k < NS; ++k) mx = fmaxf(mx, (vis >> k) & 1u ? s[k] : kLeast);
+    } else {
 #pragma unroll
-    for (int k = 1; k < NS; ++k) mx = fmaxf(mx, x[k]);
+      for (int k = 0; k < NS; ++k) mx = fmaxf(mx, s[k]);
+    }
     mx = over_groups_max(mx);
     // (A row that sees none of them has mx = kLeast: no new shift.)
     const float top = mx == kLeast ? kLeast : __builtin_fmaf(mx, c1, -cc);
@@ -430,9 +408,7 @@ __global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a)
     const float sub = -cc - m_run[rt];
     float p[NS], ps = 0.f;
 #pragma unroll
-    for (int k = 0; k < NS; ++k) {
-      p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], c1, sub));
-    }
+    for (int k = 0; k < NS; ++k) p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], c1, sub));
     if (masked) {
 #pragma unroll
       for (int k = 0; k < NS; ++k) p[k] = (vis >> k) & 1u ? p[k] : 0.f;
@@ -442,13 +418,8 @@ __global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a)
     l_run[rt] += ps;
     if constexpr (VDT == kVF32) {
 #pragma unroll
-      for (int t = 0; t < NA; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(value_at(f, t, 0, i), p[i],
-                                                            acc[rt][t], 0, 0, 0);
+      for (int k = 0; k < 4; ++k) pr[rt][k] = f2u(p[k]);
     } else {
-      unsigned bt[TERMS][4];
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
         float y0 = p[2 * h], y1 = p[2 * h + 1];
@@ -457,228 +428,258 @@ __global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a)
           if constexpr (VDT == kVF16) {
             const float h0 = q == TERMS - 1 ? y0 : u2f(f2u(y0) & 0xFFFFE000u);
             const float h1 = q == TERMS - 1 ? y1 : u2f(f2u(y1) & 0xFFFFE000u);
-            bt[q][h] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(h0, h1));
+            pr[rt][4 * q + h] =
+                __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(h0, h1));
             y0 -= h0;
             y1 -= h1;
           } else {
-            const v2bf r = __builtin_convertvector(v2f{y0, y1}, v2bf);
-            bt[q][h] = __builtin_bit_cast(unsigned, r);
-            y0 -= u2f(bt[q][h] << 16);
-            y1 -= u2f(bt[q][h] & 0xFFFF0000u);
+            const unsigned r =
+                __builtin_bit_cast(unsigned, __builtin_convertvector(v2f{y0, y1}, v2bf));
+            pr[rt][4 * q + h] = r;
+            y0 -= u2f(r << 16);
+            y1 -= u2f(r & 0xFFFF0000u);
           }
         }
       }
-#pragma unroll
-      for (int t = 0; t < NA; ++t)
-#pragma unroll
-        for (int q = 0; q < TERMS; ++q) {
-          const uint4 av = make_uint4(va[t][0], va[t][1], va[t][2], va[t][3]);
-          const uint4 bv = make_uint4(bt[q][0], bt[q][1], bt[q][2], bt[q][3]);
-          if constexpr (VDT == kVF16)
-            acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, av),
-                                                                __builtin_bit_cast(v8h, bv),
-                                                                acc[rt][t], 0, 0, 0);
-          else
-            acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, av),
-                                                                 __builtin_bit_cast(v8bf, bv),
-                                                                 acc[rt][t], 0, 0, 0);
-        }
     }
   };
 
-  // Digit sums of row tile rt with the step's keys.
-  auto scores = [&](int rt, int buf, const v4i (*ak)[NB], v4i (*ds)[4])
-      __attribute__((always_inline)) {
-    const uint8_t* dg = smem + buf * G::kDig + (rt * 16 + n16) * G::DS + grp * (D / 4);
+  auto add_values = [&](const Vals& f) __attribute__((always_inline)) {
 #pragma unroll
-    for (int kb = 0; kb < NB; ++kb)
+    for (int t = 0; t < NA; ++t) {
+      const int u = t / G::CPP, j = t % G::CPP;
+      if constexpr (VDT == kVF32) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const v4i bq = *reinterpret_cast<const v4i*>(dg + k * M * G::DS + 16 * kb);
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < CPS; ++e)
-          ds[e][k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-              ak[e][kb], bq, kb == 0 ? v4i{0, 0, 0, 0} : ds[e][k], 0, 0, 0);
-      }
-  };
-
-  auto consume = [&](Buf& f, const Meta& m, int buf) __attribute__((always_inline)) {
-    bool any = false, masked = false;
+          for (int rt = 0; rt < RT; ++rt)
+            acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                u2f(f.w[0][i][u][j]), u2f(pr[rt][i]), acc[rt][t], 0, 0, 0);
+      } else {
+        const unsigned sel = j & 1 ? 0x07060302u : 0x05040100u;
+        const uint4 av =
+            make_uint4(__builtin_amdgcn_perm(f.w[0][1][u][j / 2], f.w[0][0][u][j / 2], sel),
+                       __builtin_amdgcn_perm(f.w[0][3][u][j / 2], f.w[0][2][u][j / 2], sel),
+                       __builtin_amdgcn_perm(f.w[CPS - 1][1][u][j / 2],
+                                             f.w[CPS - 1][0][u][j / 2], sel),
+                       __builtin_amdgcn_perm(f.w[CPS - 1][3][u][j / 2],
+                                             f.w[CPS - 1][2][u][j / 2], sel));
 #pragma unroll
-    for (int e = 0; e < CPS; ++e) {
-      any |= m.nval[e] > 0;
-      masked |= m.nval[e] < 16 || (m.tok0[e] < low_max && m.tok0[e] + 16 > a.sinks);
-    }
-    if (!any) return;
-    // Keys that no row sees keep no value: a probability of zero times what lies
-    // there (a chunk of none holds anything) would be NaN where that is not finite.
-    if (masked) {
+        for (int q = 0; q < TERMS; ++q)
 #pragma unroll
-      for (int e = 0; e < CPS; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 4 * grp + i, t = m.tok0[e] + r;
-          const unsigned keep =
-              r < m.nval[e] && (t < a.sinks || t >= low_min) ? ~0u : 0u;
-#pragma unroll
-          for (int u = 0; u < G::NP; ++u)
-#pragma unroll
-            for (int k = 0; k < G::PB / 4; ++k) f.v[e][i][u][k] &= keep;
-        }
-    }
-    v4i ak[CPS][NB];
-#pragma unroll
-    for (int e = 0; e < CPS; ++e)
-#pragma unroll
-      for (int kb = 0; kb < NB; ++kb) {
-        const unsigned w0 = f.k[e][2 * kb], w1 = f.k[e][2 * kb + 1];
-        ak[e][kb] = v4i{(int)(w0 & 0x0F0F0F0Fu), (int)(w1 & 0x0F0F0F0Fu),
-                        (int)((w0 >> 4) & 0x0F0F0F0Fu), (int)((w1 >> 4) & 0x0F0F0F0Fu)};
-      }
-    unsigned va[NA][AW];
-    if constexpr (VDT != kVF32) {
-#pragma unroll
-      for (int t = 0; t < NA; ++t) value_op(f, t, va[t]);
-    }
-    v4i ds[2][CPS][4];
-    scores(0, buf, ak, ds[0]);
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      if (rt + 1 < RT) scores(rt + 1, buf, ak, ds[(rt + 1) & 1]);
-      float s[4 * CPS];
-#pragma unroll
-      for (int e = 0; e < CPS; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const v4i* d = ds[rt & 1][e];
-          s[4 * e + i] = __builtin_fmaf((float)((d[3][i] << 8) + d[2][i]), 65536.f,
-                                        (float)((d[1][i] << 8) + d[0][i]));
-        }
-      const float2 cc = cc_s[buf][rt * 16 + n16];
-      unsigned vis = 0;
-      if (masked) {
-        const int low = low_s[rt * 16 + n16];
-#pragma unroll
-        for (int e = 0; e < CPS; ++e)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = 4 * grp + i, t = m.tok0[e] + r;
-            vis |= (r < m.nval[e] && (t < a.sinks || t >= low) ? 1u : 0u) << (4 * e + i);
+          for (int rt = 0; rt < RT; ++rt) {
+            const uint4 bv = make_uint4(pr[rt][4 * q], pr[rt][4 * q + 1], pr[rt][4 * q + 2],
+                                        pr[rt][4 * q + 3]);
+            if constexpr (VDT == kVF16)
+              acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  __builtin_bit_cast(v8h, av), __builtin_bit_cast(v8h, bv), acc[rt][t], 0, 0, 0);
+            else
+              acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  __builtin_bit_cast(v8bf, av), __builtin_bit_cast(v8bf, bv), acc[rt][t], 0, 0, 0);
           }
       }
-      take(rt, f, va, s, cc.x, cc.y, masked, vis);
     }
   };
 
-  // ---- drafts: 16 of them a wave and item ----
-  auto drafts = [&](int item) __attribute__((always_inline)) {
-    const int j0 = (item * kRowWaves + w) * 16;
-    const int nval = min(16, a.nodes - j0);
-    if (nval <= 0) return;
-    Buf f;
-    const uint8_t* vb = a.vd + (int64_t)b * a.vd_b + (int64_t)hk * a.vd_h + v_lane;
-#pragma unroll
-    for (int e = 0; e < CPS; ++e)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int u = 0; u < G::NP; ++u) {
-          KVec<G::PB / 4> x = {};
-          if (e == 0)
-            x = load_k<G::PB / 4>(vb + (int64_t)(j0 + min(4 * grp + i, nval - 1)) * a.vd_n +
-                                  16 * G::PB * u);
-#pragma unroll
-          for (int k = 0; k < G::PB / 4; ++k) f.v[e][i][u][k] = x.w[k];
-        }
-    unsigned va[NA][AW];
-    if constexpr (VDT != kVF32) {
-#pragma unroll
-      for (int t = 0; t < NA; ++t) value_op(f, t, va[t]);
+  if (i0 < i1) {
+    const int steps = (it1 - it0) * spg;
+    Keys kf;
+    Vals vf;
+    Meta cur, nxt;
+    U32x4 sz0, sz1, szr;
+    if (steps > 0) {
+      cur = next_meta();
+      nxt = next_meta();
+      sz0 = load_sz(it0);
+      load_keys(cur, kf);
+      load_values(cur, vf);
+      sz1 = load_sz(it0 + 1);
+      szr = load_sz(it0 + 2);
     }
-    const float* kd = a.kd + (int64_t)b * a.kd_b + (int64_t)hk * a.kd_h +
-                      (int64_t)(j0 + min(n16, nval - 1)) * a.kd_n + grp * (D / 4);
+    // The queries to LDS (zeros behind the last row), and from there each thread's part
+    // of a row, relative to the row's largest, in slot order.
+    for (int i = tid; i < M * D; i += NT) {
+      const int r = i / D, d = i % D, R = row0 + r;
+      float x = 0.f;
+      if (r < live)
+        x = load_elem(c.q, (int64_t)b * c.q_b +
+                               (int64_t)(hk * c.hq_per_kv + R / a.nodes) * c.q_h +
+                               (int64_t)(R % a.nodes) * a.q_n + d, c.q_dtype);
+      q_s[r * G::AS + d] = x;
+    }
+    if (tid == 0) bad_s = 0;
+    if (steps > 0) {
+      stage_sz(sz0, 0);
+      stage_sz(sz1, 1);
+    }
+    __syncthreads();
+    if (steps > 0) {
+      unsigned mx = 0;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int Rq = min(row0 + rt * 16 + n16, rows - 1);
-      const int i = Rq % a.nodes;
-      const int64_t q0 = (int64_t)b * c.q_b + (int64_t)(hk * c.hq_per_kv + Rq / a.nodes) * c.q_h +
-                         (int64_t)i * a.q_n + grp * (D / 4);
-      v4f ds = {0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < SPT; ++i) {
+        qn[i] = q_s[brow * G::AS + row_channel(part * SPT + i)];
+        mx = max(mx, f2u(qn[i]) & 0x7FFFFFFFu);
+      }
+      mx = max(mx, xchg_u32<1>(mx));
+      mx = max(mx, xchg_u32<2>(mx));
+      if constexpr (TPR > 4) mx = max(mx, xchg_u32<4>(mx));
+      if constexpr (TPR > 8) mx = max(mx, xchg_u32<8>(mx));
+      // (As bits, so that NaN is the largest and makes the row NaN.)
+      q_unit = u2f(max(mx, f2u(1e-30f)));
+      const float inv = 1.f / q_unit;
+#pragma unroll
+      for (int i = 0; i < SPT; ++i) qn[i] *= inv;
+      build(0);
+      int it = it0, p = 0;
+      for (int done = 0; done < steps; ++done) {
+        const int buf = (it - it0) & 1;
+        if (p == 0) {
+          __syncthreads();
+          if (it + 1 < it1) build(buf ^ 1);
+          stage_sz(szr, buf);                      // of item it + 2
+          szr = load_sz(it + 3);
+        }
+        v4i ak[CPS][NB];
+#pragma unroll
+        for (int e = 0; e < CPS; ++e)
+#pragma unroll
+          for (int kb = 0; kb < NB; ++kb) {
+            const unsigned w0 = kf.w[e][2 * kb], w1 = kf.w[e][2 * kb + 1];
+            ak[e][kb] = v4i{(int)(w0 & 0x0F0F0F0Fu), (int)(w1 & 0x0F0F0F0Fu),
+                            (int)((w0 >> 4) & 0x0F0F0F0Fu), (int)((w1 >> 4) & 0x0F0F0F0Fu)};
+          }
+        load_keys(nxt, kf);
+        bool any = false, masked = false;
+#pragma unroll
+        for (int e = 0; e < CPS; ++e) {
+          any |= cur.nval[e] > 0;
+          masked |= cur.nval[e] < 16 || (cur.tok0[e] < low_max && cur.tok0[e] + 16 > a.sinks);
+        }
+        if (any) {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            const int r = rbase + rt * 16 + n16;
+            const uint8_t* dg = smem + buf * G::kDig + r * G::DS + grp * (D / 4);
+            v4i ds[CPS][4];
+#pragma unroll
+            for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const v4i bq = *reinterpret_cast<const v4i*>(dg + k * M * G::DS + 16 * kb);
+#pragma unroll
+                for (int e = 0; e < CPS; ++e)
+                  ds[e][k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                      ak[e][kb], bq, kb == 0 ? v4i{0, 0, 0, 0} : ds[e][k], 0, 0, 0);
+              }
+            float s[NS];
+#pragma unroll
+            for (int e = 0; e < CPS; ++e)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                s[4 * e + i] =
+                    __builtin_fmaf((float)((ds[e][3][i] << 8) + ds[e][2][i]), 65536.f,
+                                   (float)((ds[e][1][i] << 8) + ds[e][0][i]));
+            const float2 cc = cc_s[buf][r];
+            unsigned vis = 0;
+            if (masked) {
+              const int low = low_s[r];
+#pragma unroll
+              for (int e = 0; e < CPS; ++e)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int k = 4 * grp + i, t = cur.tok0[e] + k;
+                  vis |= (k < cur.nval[e] && (t < a.sinks || t >= low) ? 1u : 0u) << (4 * e + i);
+                }
+            }
+            softmax(rt, s, cc.x, cc.y, masked, vis);
+          }
+          // Keys that no row sees keep no value: a probability of zero times what lies
+          // there (a chunk of none holds anything) would be NaN where that is not
+          // finite.
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < CPS; ++e)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int k = 4 * grp + i, t = cur.tok0[e] + k;
+                const unsigned keep =
+                    k < cur.nval[e] && (t < a.sinks || t >= low_min) ? ~0u : 0u;
+#pragma unroll
+                for (int u = 0; u < G::NP; ++u)
+#pragma unroll
+                  for (int x = 0; x < G::PB / 4; ++x) vf.w[e][i][u][x] &= keep;
+              }
+          }
+          add_values(vf);
+        }
+        load_values(nxt, vf);
+        cur = nxt;
+        nxt = next_meta();
+        if (++p == spg) {
+          p = 0;
+          ++it;
+        }
+      }
+    }
+
+    // ---- drafts: 16 of them a wave and item, float32 products ----
+    for (int item = dr0; item < dr1; ++item) {
+      const int j0 = (item * kKeyWaves + kw) * 16;
+      const int nval = min(16, a.nodes - j0);
+      if (nval <= 0) break;
+      const uint8_t* vb = a.vd + (int64_t)b * a.vd_b + (int64_t)hk * a.vd_h + v_lane;
+#pragma unroll
+      for (int e = 0; e < CPS; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int u = 0; u < G::NP; ++u) {
+            KVec<G::PB / 4> x = {};
+            if (e == 0)
+              x = load_k<G::PB / 4>(vb + (int64_t)(j0 + min(4 * grp + i, nval - 1)) * a.vd_n +
+                                    16 * G::PB * u);
+#pragma unroll
+            for (int k = 0; k < G::PB / 4; ++k) vf.w[e][i][u][k] = x.w[k];
+          }
+      const float* kd = a.kd + (int64_t)b * a.kd_b + (int64_t)hk * a.kd_h +
+                        (int64_t)(j0 + min(n16, nval - 1)) * a.kd_n + grp * (D / 4);
+      v4f ds[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) ds[rt] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
       for (int d = 0; d < D / 4; d += 4) {
         const float4 k4 = *reinterpret_cast<const float4*>(kd + d);
-        ds = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.x, load_elem(c.q, q0 + d, c.q_dtype), ds, 0, 0, 0);
-        ds = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.y, load_elem(c.q, q0 + d + 1, c.q_dtype), ds, 0, 0, 0);
-        ds = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.z, load_elem(c.q, q0 + d + 2, c.q_dtype), ds, 0, 0, 0);
-        ds = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.w, load_elem(c.q, q0 + d + 3, c.q_dtype), ds, 0, 0, 0);
-      }
-      const uint8_t* mk = a.mask + (int64_t)b * a.mk_b + (int64_t)i * a.mk_i + j0;
-      unsigned vis = 0;
-      float s[4 * CPS];
 #pragma unroll
-      for (int k = 0; k < 4 * CPS; ++k) s[k] = kLeast;
+        for (int rt = 0; rt < RT; ++rt) {
+          const float4 q4 = *reinterpret_cast<const float4*>(
+              q_s + (rbase + rt * 16 + n16) * G::AS + grp * (D / 4) + d);
+          ds[rt] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.x, q4.x, ds[rt], 0, 0, 0);
+          ds[rt] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.y, q4.y, ds[rt], 0, 0, 0);
+          ds[rt] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.z, q4.z, ds[rt], 0, 0, 0);
+          ds[rt] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.w, q4.w, ds[rt], 0, 0, 0);
+        }
+      }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int r = 4 * grp + k;
-        vis |= (mk[min(r, nval - 1)] != 0 && r < nval ? 1u : 0u) << k;
-        s[k] = ds[k];
+      for (int rt = 0; rt < RT; ++rt) {
+        const int R = row0 + min(rbase + rt * 16 + n16, live - 1);
+        const uint8_t* mk = a.mask + (int64_t)b * a.mk_b + (int64_t)(R % a.nodes) * a.mk_i + j0;
+        unsigned vis = 0;
+        float s[NS];
+#pragma unroll
+        for (int k = 0; k < NS; ++k) s[k] = kLeast;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = 4 * grp + k;
+          vis |= (mk[min(r, nval - 1)] != 0 && r < nval ? 1u : 0u) << k;
+          s[k] = ds[rt][k];
+        }
+        softmax(rt, s, kLog2e, 0.f, true, vis);
       }
-      take(rt, f, va, s, kLog2e, 0.f, true, vis);
+      add_values(vf);
     }
-  };
-
-  // ---- the range ----
-  const int spg = (cpg + CPS * kRowWaves - 1) / (CPS * kRowWaves);
-  const int steps = (it1 - it0) * spg;
-  if (steps > 0) {
-    U32x4 szr;
-    {
-      const U32x4 x0 = load_sz(it0), x1 = load_sz(it0 + 1);
-      szr = load_sz(it0 + 2);
-      stage_sz(x0, 0);
-      stage_sz(x1, 1);
-    }
-    Buf f[2];
-    int li = it0, lp = 0;                          // item and step of the next metadata
-    auto next_meta = [&]() __attribute__((always_inline)) -> Meta {
-      // (Behind the last item: chunks of none.)
-      const Meta m = meta_of(min(li, it1 - 1), li < it1 ? lp : spg);
-      if (++lp == spg) {
-        lp = 0;
-        ++li;
-      }
-      return m;
-    };
-    Meta cur = next_meta(), nxt = next_meta();
-    load_step(cur, f[0]);
-    __syncthreads();
-    build(0);
-    int it = it0, p = 0, done = 0;
-    auto step = [&](Buf& now, Buf& then) __attribute__((always_inline)) -> bool {
-      const int buf = (it - it0) & 1;
-      if (p == 0) {
-        __syncthreads();
-        if (it + 1 < it1) build(buf ^ 1);
-        stage_sz(szr, buf);                        // of item it + 2
-      }
-      szr = load_sz(it + 3);
-      load_step(nxt, then);
-      const Meta ahead = next_meta();
-      consume(now, cur, buf);
-      cur = nxt;
-      nxt = ahead;
-      if (++p == spg) {
-        p = 0;
-        ++it;
-      }
-      return ++done == steps;
-    };
-    while (true) {
-      if (step(f[0], f[1])) break;
-      if (step(f[1], f[0])) break;
-    }
+  } else if (tid == 0) {
+    bad_s = 0;
   }
-  for (int i = dr0; i < dr1; ++i) drafts(i);
 
   // The range again for every row by itself, a wave a row and key after key, for the
   // rare workgroup with a NaN: a key that a row does not see takes no part in it.
@@ -686,13 +687,13 @@ __global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a)
     constexpr int CH = D / 64;
     float* part0 = reinterpret_cast<float*>(smem);
     __syncthreads();
-    for (int i = tid; i < kRowWaves * M; i += kRowWaves * 64) {
+    for (int i = tid; i < kKeyWaves * M; i += NT) {
       m_s[i / M][i % M] = kLeast;
       l_s[i / M][i % M] = 0.f;
     }
-    for (int i = tid; i < kRowWaves * M * G::AS; i += kRowWaves * 64) part0[i] = 0.f;
+    for (int i = tid; i < kKeyWaves * M * G::AS; i += NT) part0[i] = 0.f;
     __syncthreads();
-    for (int r = w; r < M && row0 + r < rows; r += kRowWaves) {
+    for (int r = w; r < live; r += NT / 64) {
       const int i = (row0 + r) % a.nodes;
       const int64_t q0 = (int64_t)b * c.q_b +
                          (int64_t)(hk * c.hq_per_kv + (row0 + r) / a.nodes) * c.q_h +
@@ -753,19 +754,19 @@ __global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a)
   for (int rt = 0; rt < RT; ++rt) {
     const float l = over_groups_sum(l_run[rt]);
     if (grp == 0) {
-      m_s[w][rt * 16 + n16] = m_run[rt];
-      l_s[w][rt * 16 + n16] = l;
+      m_s[kw][rbase + rt * 16 + n16] = m_run[rt];
+      l_s[kw][rbase + rt * 16 + n16] = l;
     }
   }
   __syncthreads();                                 // (the digits are no longer read)
-  float* out_w = reinterpret_cast<float*>(smem) + w * M * G::AS;
+  float* out_w = reinterpret_cast<float*>(smem) + kw * M * G::AS;
   float any_nan = 0.f;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int r = rt * 16 + n16;
+    const int r = rbase + rt * 16 + n16;
     float top = m_s[0][r];
 #pragma unroll
-    for (int i = 1; i < kRowWaves; ++i) top = fmaxf(top, m_s[i][r]);
+    for (int i = 1; i < kKeyWaves; ++i) top = fmaxf(top, m_s[i][r]);
     const float f = __builtin_amdgcn_exp2f(m_run[rt] - top);
 #pragma unroll
     for (int u = 0; u < G::NP; ++u)
@@ -774,9 +775,9 @@ __global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a)
         float* dst = out_w + r * G::AS + u * 16 * G::CPP + (4 * grp + i) * G::CPP;
 #pragma unroll
         for (int j = 0; j < G::CPP; j += 4) {
-          const float4 x =
-              make_float4(acc[rt][u * G::CPP + j][i] * f, acc[rt][u * G::CPP + j + 1][i] * f,
-                          acc[rt][u * G::CPP + j + 2][i] * f, acc[rt][u * G::CPP + j + 3][i] * f);
+          const int t = u * G::CPP + j;
+          const float4 x = make_float4(acc[rt][t][i] * f, acc[rt][t + 1][i] * f,
+                                       acc[rt][t + 2][i] * f, acc[rt][t + 3][i] * f);
           *reinterpret_cast<float4*>(dst + j) = x;
           any_nan += (x.x + x.y) + (x.z + x.w);
         }
@@ -786,17 +787,15 @@ __global__ __launch_bounds__(kRowWaves * 64) void decode_rows_kernel(RowsArgs a)
   __syncthreads();
   if (bad_s) plain_rows();
   const float* parts = reinterpret_cast<const float*>(smem);
-  const int64_t o0 = ((int64_t)b * c.num_q_heads + (int64_t)hk * c.hq_per_kv) * a.nodes + row0;
-  for (int idx = tid * 4; idx < M * D; idx += kRowWaves * 64 * 4) {
+  for (int idx = tid * 4; idx < live * D; idx += NT * 4) {
     const int r = idx / D, d = idx % D;
-    if (row0 + r >= rows) continue;
     float top = m_s[0][r];
 #pragma unroll
-    for (int i = 1; i < kRowWaves; ++i) top = fmaxf(top, m_s[i][r]);
+    for (int i = 1; i < kKeyWaves; ++i) top = fmaxf(top, m_s[i][r]);
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < kRowWaves; ++i) {
+    for (int i = 0; i < kKeyWaves; ++i) {
       l = __builtin_fmaf(__builtin_amdgcn_exp2f(m_s[i][r] - top), l_s[i][r], l);
       const float4 x = *reinterpret_cast<const float4*>(parts + (i * M + r) * G::AS + d);
       o.x += x.x;
@@ -825,18 +824,19 @@ hipError_t launch_decode_rows(const RowsArgs& a, int D, int v_dtype, int batch, 
                       batch;
   if (wgs > INT32_MAX) return hipErrorInvalidValue;
   const bool wide = a.c.out_dtype == kEF32;
-#define FDI4_RW(DD, VV, RR, TT)                                                              \
-  if (D == DD && v_dtype == VV && a.row_tiles == RR && (VV != kVBF16 || wide == (TT == 3))) { \
-    hipLaunchKernelGGL((decode_rows_kernel<DD, VV, RR, TT>), dim3((unsigned)wgs),             \
-                       dim3(kRowWaves * 64), 0, st, a);                                       \
-    return hipGetLastError();                                                                 \
+#define FDI4_RW(DD, VV, RR, WW, TT)                                                       \
+  if (D == DD && v_dtype == VV && a.row_tiles == RR * WW &&                               \
+      (VV != kVBF16 || wide == (TT == 3))) {                                              \
+    hipLaunchKernelGGL((decode_rows_kernel<DD, VV, RR, WW, TT>), dim3((unsigned)wgs),      \
+                       dim3(kKeyWaves * 64 * WW), 0, st, a);                              \
+    return hipGetLastError();                                                             \
   }
-#define FDI4_RW_V(DD, RR) \
-  FDI4_RW(DD, kVF32, RR, 1) FDI4_RW(DD, kVF16, RR, 2) FDI4_RW(DD, kVBF16, RR, 2) \
-  FDI4_RW(DD, kVBF16, RR, 3)
-  FDI4_RW_V(64, 1) FDI4_RW_V(64, 2) FDI4_RW_V(64, 3) FDI4_RW_V(64, 4)
-  FDI4_RW_V(128, 1) FDI4_RW_V(128, 2) FDI4_RW_V(128, 3) FDI4_RW_V(128, 4)
-  FDI4_RW_V(256, 1) FDI4_RW_V(256, 2)
+#define FDI4_RW_V(DD, RR, WW) \
+  FDI4_RW(DD, kVF32, RR, WW, 1) FDI4_RW(DD, kVF16, RR, WW, 2) \
+  FDI4_RW(DD, kVBF16, RR, WW, 2) FDI4_RW(DD, kVBF16, RR, WW, 3)
+  FDI4_RW_V(64, 1, 1) FDI4_RW_V(64, 2, 1) FDI4_RW_V(64, 2, 2)
+  FDI4_RW_V(128, 1, 1) FDI4_RW_V(128, 2, 1) FDI4_RW_V(128, 2, 2)
+  FDI4_RW_V(256, 1, 1) FDI4_RW_V(256, 1, 2)
 #undef FDI4_RW_V
 #undef FDI4_RW
   return hipErrorInvalidValue;
