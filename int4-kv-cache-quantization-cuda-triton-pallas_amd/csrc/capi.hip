@@ -947,6 +947,13 @@ int make_rows_args(const void* query, int q_dtype, int batch, int num_q_heads, i
   r->window = window;
   r->sinks = sinks;
   const RowsPlan p = plan_rows(batch, num_q_heads, nodes, window, sinks, num_splits, cache);
+  r->c.div_splits = fdi4::make_fast_div(p.splits);
+  r->div_nodes = fdi4::make_fast_div(nodes);
+  r->div_heads = fdi4::make_fast_div(cache->num_kv_heads);
+  r->kv_heads = cache->num_kv_heads;
+  const int qeb = q_dtype == FDI4_K_F32 ? 4 : 2;
+  r->q_vec = aligned(query, 16) && (q_batch_stride * qeb) % 16 == 0 &&
+             (q_head_stride * qeb) % 16 == 0 && (q_node_stride * qeb) % 16 == 0;
   r->row_tiles = p.row_tiles;
   r->tiles = p.tiles;
   r->c.num_splits = p.splits;

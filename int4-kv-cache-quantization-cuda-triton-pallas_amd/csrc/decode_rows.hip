@@ -78,20 +78,42 @@ struct RowsGeo {
   static_assert(TPR >= 4 && TPR <= 16 && (TPR & (TPR - 1)) == 0 && SPT % 4 == 0, "threads");
 };
 
+// Position of channel d in the operands' order: of every eight channels (a word of
+// nibbles) the even ones (low nibbles) before the odd ones.
 __device__ __forceinline__ int row_slot(int d) {
-  return (d & ~15) | ((d & 1) << 3) | ((d & 15) >> 1);
+  return (d & ~7) | ((d & 1) << 2) | ((d & 7) >> 1);
 }
 
-__device__ __forceinline__ int row_channel(int s) {
-  return (s & ~15) | ((s & 7) << 1) | ((s >> 3) & 1);
+// Eight channels of a query as float32, from 16-byte loads (VEC) or element by element.
+__device__ __forceinline__ void load_query8(const void* q, int64_t i, int dt, bool vec, float* x) {
+  if (!vec) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = load_elem(q, i + k, dt);
+  } else if (dt == kEF32) {
+    const float* p = static_cast<const float*>(q) + i;
+    widen_values<kVF32>(ld16(p), x);
+    widen_values<kVF32>(ld16(p + 4), x + 4);
+  } else {
+    const U32x4 v = ld16(static_cast<const unsigned short*>(q) + i);
+    if (dt == kEF16) widen_values<kVF16>(v, x);
+    else widen_values<kVBF16>(v, x);
+  }
 }
 
 // Maximum and sum over the four 16-lane groups.
+// (The maximum without the quieting moves that fmax puts before operands of unknown
+// origin; the instruction quiets them itself.)
+__device__ __forceinline__ float max_of(float x, float y) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(y));
+  return r;
+}
+
 __device__ __forceinline__ float over_groups_max(float x) {
   auto r = __builtin_amdgcn_permlane16_swap(f2u(x), f2u(x), false, false);
-  x = fmaxf(u2f(r[0]), u2f(r[1]));
+  x = max_of(u2f(r[0]), u2f(r[1]));
   auto s = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
-  return fmaxf(u2f(s[0]), u2f(s[1]));
+  return max_of(u2f(s[0]), u2f(s[1]));
 }
 
 __device__ __forceinline__ float over_groups_sum(float x) {
@@ -125,13 +147,15 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
 
   // Tiles of one (sequence, kv-head, split) run on one XCD, one after the other: they
   // read the same pages.
-  unsigned wi = xcd_run_item(blockIdx.x, gridDim.x, (unsigned)a.tiles);
-  const int tile = (int)(wi % (unsigned)a.tiles);
-  wi /= (unsigned)a.tiles;
-  const int split = (int)(wi % (unsigned)c.num_splits);
-  wi /= (unsigned)c.num_splits;
-  const int hkv = c.num_q_heads / c.hq_per_kv;
-  const int hk = (int)(wi % (unsigned)hkv), b = (int)(wi / (unsigned)hkv);
+  int wi = (int)blockIdx.x, tile = 0;
+  if (a.tiles > 1) {
+    const int L = (int)xcd_run_item(blockIdx.x, gridDim.x, (unsigned)a.tiles);
+    wi = L / a.tiles;
+    tile = L - wi * a.tiles;
+  }
+  int wj = fdiv(wi, c.div_splits);
+  const int split = wi - wj * c.num_splits;
+  const int b = fdiv(wj, a.div_heads), hk = wj - b * a.kv_heads;
   const int rows = c.hq_per_kv * a.nodes;          // rows of this kv-head
   const int row0 = tile * M;
   const int live = min(rows - row0, M);            // rows of this workgroup
@@ -146,18 +170,30 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
   __shared__ int bad_s;
   float* const q_s = reinterpret_cast<float*>(smem + G::kQ);
 
+  // This thread's part of a row of digits: brow's channels part * SPT .. (of eight, the
+  // even or the odd ones where SPT is four).
+  const int brow = tid / TPR, part = tid % TPR;
+  constexpr int NQ = SPT / 8 > 0 ? SPT / 8 : 1;
+  float qv[NQ][8];
+  {
+    const int R = row0 + min(brow, live - 1), hr = fdiv(R, a.div_nodes);
+    const int64_t q0 = (int64_t)b * c.q_b + (int64_t)(hk * c.hq_per_kv + hr) * c.q_h +
+                       (int64_t)(R - hr * a.nodes) * a.q_n + (part * SPT & ~7);
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) load_query8(c.q, q0 + 8 * i, c.q_dtype, a.q_vec, qv[i]);
+  }
+
   const int n = seq_len_of(c, b);
   if (c.lens_out && tile == 0 && split == 0 && hk == 0 && tid == 0)
     c.lens_out[b] = c.seq_lens[b];
 
   // ---- each row's window ----
-  const int brow = tid / TPR, part = tid % TPR;    // this thread's row of digits
   int low_min = 0, low_max = 0;
   if (a.window) {
     low_min = low_max = max(n - a.window, 0);
     if (a.mask) {
       // It ends at the node, whose visible drafts count.
-      const int node = (row0 + min(brow, live - 1)) % a.nodes;
+      const int R = row0 + min(brow, live - 1), node = R - fdiv(R, a.div_nodes) * a.nodes;
       const uint8_t* mk = a.mask + (int64_t)b * a.mk_b + (int64_t)node * a.mk_i;
       int mine = 0;
       for (int j = part; j < a.nodes; j += TPR) mine += mk[j] != 0;
@@ -233,10 +269,10 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
       if (tok0 >= a.sinks && tok0 + nval <= low_min) nval = 0;
       const bool some = nval > 0;
       const int pg = some ? (table ? ld_ro(table, page) : page) : 0;
-      m.phys[e] = (unsigned)min(max(pg, 0), c.num_pages - 1);
-      m.r0[e] = some ? r0 : 0;
-      m.nval[e] = nval;
-      m.tok0[e] = tok0;
+      m.phys[e] = (unsigned)__builtin_amdgcn_readfirstlane(min(max(pg, 0), c.num_pages - 1));
+      m.r0[e] = __builtin_amdgcn_readfirstlane(some ? r0 : 0);
+      m.nval[e] = __builtin_amdgcn_readfirstlane(nval);
+      m.tok0[e] = __builtin_amdgcn_readfirstlane(tok0);
     }
     if (++lp == spg) {
       lp = 0;
@@ -322,7 +358,7 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
     if (tid < D / 2) {
       float* dst = sz_s[buf] + (is_s ? 0 : D) + row_slot(4 * (tid % (D / 4)));
       *reinterpret_cast<float2*>(dst) = make_float2(y.x, y.z);
-      *reinterpret_cast<float2*>(dst + 8) = make_float2(y.y, y.w);
+      *reinterpret_cast<float2*>(dst + 4) = make_float2(y.y, y.w);
     }
   };
   float qn[SPT], q_unit;                           // the row relative to its largest
@@ -385,17 +421,16 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
   // chunk e in s[4 e + i], of which those in vis are seen.
   auto softmax = [&](int rt, const float* s, float c1, float cc, bool masked, unsigned vis)
       __attribute__((always_inline)) {
-    float mx = kLeast;
+    float p[NS], top = kLeast, ps = 0.f;
+#pragma unroll
+    for (int k = 0; k < NS; ++k) p[k] = __builtin_fmaf(s[k], c1, -cc);
     if (masked) {
 #pragma unroll
-      for (int k = 0; k < NS; ++k) mx = fmaxf(mx, (vis >> k) & 1u ? s[k] : kLeast);
-    } else {
-#pragma unroll
-      for (int k = 0; k < NS; ++k) mx = fmaxf(mx, s[k]);
+      for (int k = 0; k < NS; ++k) p[k] = (vis >> k) & 1u ? p[k] : -INFINITY;
     }
-    mx = over_groups_max(mx);
-    // (A row that sees none of them has mx = kLeast: no new shift.)
-    const float top = mx == kLeast ? kLeast : __builtin_fmaf(mx, c1, -cc);
+#pragma unroll
+    for (int k = 0; k < NS; ++k) top = fmaxf(top, p[k]);
+    top = over_groups_max(top);
     const bool up = top > m_run[rt] + (kUp + kSlack);
     if (__builtin_amdgcn_ballot_w64(up)) {
       const float m_new = up ? __builtin_ceilf(top) - kUp : m_run[rt];
@@ -405,14 +440,8 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
 #pragma unroll
       for (int t = 0; t < NA; ++t) acc[rt][t] *= corr;
     }
-    const float sub = -cc - m_run[rt];
-    float p[NS], ps = 0.f;
 #pragma unroll
-    for (int k = 0; k < NS; ++k) p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], c1, sub));
-    if (masked) {
-#pragma unroll
-      for (int k = 0; k < NS; ++k) p[k] = (vis >> k) & 1u ? p[k] : 0.f;
-    }
+    for (int k = 0; k < NS; ++k) p[k] = __builtin_amdgcn_exp2f(p[k] - m_run[rt]);
 #pragma unroll
     for (int k = 0; k < NS; ++k) ps += p[k];
     l_run[rt] += ps;
@@ -496,16 +525,39 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
       sz1 = load_sz(it0 + 1);
       szr = load_sz(it0 + 2);
     }
-    // The queries to LDS (zeros behind the last row), and from there each thread's part
-    // of a row, relative to the row's largest, in slot order.
-    for (int i = tid; i < M * D; i += NT) {
-      const int r = i / D, d = i % D, R = row0 + r;
-      float x = 0.f;
-      if (r < live)
-        x = load_elem(c.q, (int64_t)b * c.q_b +
-                               (int64_t)(hk * c.hq_per_kv + R / a.nodes) * c.q_h +
-                               (int64_t)(R % a.nodes) * a.q_n + d, c.q_dtype);
-      q_s[r * G::AS + d] = x;
+    // The row relative to its largest, in slot order (zeros behind the last row), and
+    // as it is to LDS for the drafts.
+    unsigned mx = 0;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        qv[i][k] = brow < live ? qv[i][k] : 0.f;
+        mx = max(mx, f2u(qv[i][k]) & 0x7FFFFFFFu);
+      }
+    mx = max(mx, xchg_u32<1>(mx));
+    mx = max(mx, xchg_u32<2>(mx));
+    if constexpr (TPR > 4) mx = max(mx, xchg_u32<4>(mx));
+    if constexpr (TPR > 8) mx = max(mx, xchg_u32<8>(mx));
+    // (As bits, so that NaN is the largest and makes the row NaN.)
+    q_unit = u2f(max(mx, f2u(1e-30f)));
+    const float inv = 1.f / q_unit;
+#pragma unroll
+    for (int i = 0; i < SPT; ++i) {
+      if constexpr (SPT >= 8) {
+        qn[i] = qv[i / 8][2 * (i % 4) + ((i >> 2) & 1)] * inv;
+      } else {
+        const unsigned odd = part & 1 ? ~0u : 0u;
+        qn[i] = u2f((f2u(qv[0][2 * i + 1]) & odd) | (f2u(qv[0][2 * i]) & ~odd)) * inv;
+      }
+    }
+    if (dr0 < dr1) {
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        float* dst = q_s + brow * G::AS + (part * SPT & ~7) + 8 * i;
+        *reinterpret_cast<float4*>(dst) = make_float4(qv[i][0], qv[i][1], qv[i][2], qv[i][3]);
+        *reinterpret_cast<float4*>(dst + 4) = make_float4(qv[i][4], qv[i][5], qv[i][6], qv[i][7]);
+      }
     }
     if (tid == 0) bad_s = 0;
     if (steps > 0) {
@@ -514,21 +566,6 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
     }
     __syncthreads();
     if (steps > 0) {
-      unsigned mx = 0;
-#pragma unroll
-      for (int i = 0; i < SPT; ++i) {
-        qn[i] = q_s[brow * G::AS + row_channel(part * SPT + i)];
-        mx = max(mx, f2u(qn[i]) & 0x7FFFFFFFu);
-      }
-      mx = max(mx, xchg_u32<1>(mx));
-      mx = max(mx, xchg_u32<2>(mx));
-      if constexpr (TPR > 4) mx = max(mx, xchg_u32<4>(mx));
-      if constexpr (TPR > 8) mx = max(mx, xchg_u32<8>(mx));
-      // (As bits, so that NaN is the largest and makes the row NaN.)
-      q_unit = u2f(max(mx, f2u(1e-30f)));
-      const float inv = 1.f / q_unit;
-#pragma unroll
-      for (int i = 0; i < SPT; ++i) qn[i] *= inv;
       build(0);
       int it = it0, p = 0;
       for (int done = 0; done < steps; ++done) {
@@ -539,21 +576,28 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
           stage_sz(szr, buf);                      // of item it + 2
           szr = load_sz(it + 3);
         }
+        // Nibbles of key block kb of chunk e.
+        auto key_op = [&](int e, int kb) __attribute__((always_inline)) -> v4i {
+          const unsigned w0 = kf.w[e][2 * kb], w1 = kf.w[e][2 * kb + 1];
+          return v4i{(int)(w0 & 0x0F0F0F0Fu), (int)((w0 >> 4) & 0x0F0F0F0Fu),
+                     (int)(w1 & 0x0F0F0F0Fu), (int)((w1 >> 4) & 0x0F0F0F0Fu)};
+        };
+        // With one row tile they are made where they are used (registers), with two
+        // once for both, and the next keys are loaded over the words.
         v4i ak[CPS][NB];
+        if constexpr (RT > 1) {
 #pragma unroll
-        for (int e = 0; e < CPS; ++e)
+          for (int e = 0; e < CPS; ++e)
 #pragma unroll
-          for (int kb = 0; kb < NB; ++kb) {
-            const unsigned w0 = kf.w[e][2 * kb], w1 = kf.w[e][2 * kb + 1];
-            ak[e][kb] = v4i{(int)(w0 & 0x0F0F0F0Fu), (int)(w1 & 0x0F0F0F0Fu),
-                            (int)((w0 >> 4) & 0x0F0F0F0Fu), (int)((w1 >> 4) & 0x0F0F0F0Fu)};
-          }
-        load_keys(nxt, kf);
+            for (int kb = 0; kb < NB; ++kb) ak[e][kb] = key_op(e, kb);
+          load_keys(nxt, kf);
+        }
         bool any = false, masked = false;
 #pragma unroll
         for (int e = 0; e < CPS; ++e) {
           any |= cur.nval[e] > 0;
-          masked |= cur.nval[e] < 16 || (cur.tok0[e] < low_max && cur.tok0[e] + 16 > a.sinks);
+          masked |= (cur.nval[e] < 16) |
+                    ((cur.tok0[e] < low_max) & (cur.tok0[e] + 16 > a.sinks));
         }
         if (any) {
 #pragma unroll
@@ -562,15 +606,20 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
             const uint8_t* dg = smem + buf * G::kDig + r * G::DS + grp * (D / 4);
             v4i ds[CPS][4];
 #pragma unroll
-            for (int kb = 0; kb < NB; ++kb)
+            for (int kb = 0; kb < NB; ++kb) {
+              v4i kop[CPS];
+#pragma unroll
+              for (int e = 0; e < CPS; ++e) kop[e] = RT > 1 ? ak[e][kb] : key_op(e, kb);
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const v4i bq = *reinterpret_cast<const v4i*>(dg + k * M * G::DS + 16 * kb);
 #pragma unroll
                 for (int e = 0; e < CPS; ++e)
                   ds[e][k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-                      ak[e][kb], bq, kb == 0 ? v4i{0, 0, 0, 0} : ds[e][k], 0, 0, 0);
+                      kop[e], bq, kb == 0 ? v4i{0, 0, 0, 0} : ds[e][k], 0, 0, 0);
               }
+            }
+            if constexpr (RT == 1) load_keys(nxt, kf);
             float s[NS];
 #pragma unroll
             for (int e = 0; e < CPS; ++e)
@@ -588,7 +637,8 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   const int k = 4 * grp + i, t = cur.tok0[e] + k;
-                  vis |= (k < cur.nval[e] && (t < a.sinks || t >= low) ? 1u : 0u) << (4 * e + i);
+                  vis |= (unsigned)((k < cur.nval[e]) & ((t < a.sinks) | (t >= low)))
+                         << (4 * e + i);
                 }
             }
             softmax(rt, s, cc.x, cc.y, masked, vis);
@@ -603,7 +653,7 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
               for (int i = 0; i < 4; ++i) {
                 const int k = 4 * grp + i, t = cur.tok0[e] + k;
                 const unsigned keep =
-                    k < cur.nval[e] && (t < a.sinks || t >= low_min) ? ~0u : 0u;
+                    (k < cur.nval[e]) & ((t < a.sinks) | (t >= low_min)) ? ~0u : 0u;
 #pragma unroll
                 for (int u = 0; u < G::NP; ++u)
 #pragma unroll
@@ -611,6 +661,8 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
               }
           }
           add_values(vf);
+        } else if constexpr (RT == 1) {
+          load_keys(nxt, kf);
         }
         load_values(nxt, vf);
         cur = nxt;
@@ -662,7 +714,8 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         const int R = row0 + min(rbase + rt * 16 + n16, live - 1);
-        const uint8_t* mk = a.mask + (int64_t)b * a.mk_b + (int64_t)(R % a.nodes) * a.mk_i + j0;
+        const int node = R - fdiv(R, a.div_nodes) * a.nodes;
+        const uint8_t* mk = a.mask + (int64_t)b * a.mk_b + (int64_t)node * a.mk_i + j0;
         unsigned vis = 0;
         float s[NS];
 #pragma unroll
@@ -670,7 +723,7 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int r = 4 * grp + k;
-          vis |= (mk[min(r, nval - 1)] != 0 && r < nval ? 1u : 0u) << k;
+          vis |= (unsigned)((mk[min(r, nval - 1)] != 0) & (r < nval)) << k;
           s[k] = ds[rt][k];
         }
         softmax(rt, s, kLog2e, 0.f, true, vis);

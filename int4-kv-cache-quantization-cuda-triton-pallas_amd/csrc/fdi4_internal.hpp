@@ -160,6 +160,9 @@ struct RowsArgs {
   int window;                           // 0: the whole cache
   int sinks;
   FastDiv div_group;                    // by the rows of a scale group
+  FastDiv div_nodes, div_heads;         // by nodes, kv_heads
+  int kv_heads;
+  int q_vec;                            // query rows start on 16-byte boundaries
   int row_tiles;                        // 16-row tiles per workgroup
   int tiles;                            // workgroups for the rows of a kv-head
 };
