@@ -52,7 +52,7 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kKeyWaves = 4;   // waves that share a step's chunks (per row group)
 
-template <int D, int VDT, int RT, int RW>
+template <int D, int VDT, int RT, int RW, int ND>
 struct RowsGeo {
   static constexpr int NB = D / 64;                // 64-channel blocks of the key product
   static constexpr int KW = D / 32;                // packed key words per lane per row
@@ -67,7 +67,7 @@ struct RowsGeo {
   static constexpr int TPR = NT / M;               // threads per row that build digits
   static constexpr int SPT = D / TPR;              // channels each
   static constexpr int DS = D + 16;                // bytes per row of a digit (padded)
-  static constexpr int kDig = 4 * M * DS;          // a buffer of digits
+  static constexpr int kDig = ND * M * DS;         // a buffer of digits
   static constexpr int AS = D + 4;                 // floats per row of queries and outputs
   // LDS: two buffers of digits and the queries while the keys stream, then the waves'
   // outputs.
@@ -100,6 +100,14 @@ __device__ __forceinline__ void load_query8(const void* q, int64_t i, int dt, bo
   }
 }
 
+// KW words of a key or value row: streamed (non-temporal) where one wave reads them,
+// through the caches where the second row group, or another tile's workgroup, does too.
+template <int KW, bool STREAM>
+__device__ __forceinline__ KVec<KW> load_words(const uint8_t* p) {
+  if constexpr (STREAM) return load_k<KW>(p);
+  return *reinterpret_cast<const KVec<KW>*>(__builtin_assume_aligned(p, 4 * KW));
+}
+
 // Maximum and sum over the four 16-lane groups.
 // (The maximum without the quieting moves that fmax puts before operands of unknown
 // origin; the instruction quiets them itself.)
@@ -123,11 +131,14 @@ __device__ __forceinline__ float over_groups_sum(float x) {
   return u2f(s[0]) + u2f(s[1]);
 }
 
-// TERMS: 16-bit terms of a probability. RT row tiles a wave, RW row groups of four
-// waves: wave w takes key chunks w % 4 and row group w / 4.
-template <int D, int VDT, int RT, int RW, int TERMS>
+// RT row tiles a wave, RW row groups of four waves: wave w takes key chunks w % 4 and
+// row group w / 4. WIDE: float32 outputs (four digits of q*s, all 24 bits of a
+// probability); otherwise three digits and at least 16 bits.
+template <int D, int VDT, int RT, int RW, bool WIDE>
 __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(RowsArgs a) {
-  using G = RowsGeo<D, VDT, RT, RW>;
+  constexpr int ND = WIDE ? 4 : 3;
+  constexpr int TERMS = WIDE && VDT == kVBF16 ? 3 : 2;   // 16-bit terms of a probability
+  using G = RowsGeo<D, VDT, RT, RW, ND>;
   constexpr int NB = G::NB, CPS = G::CPS, NA = G::NA, M = G::M, NT = G::NT;
   constexpr int TPR = G::TPR, SPT = G::SPT, NS = 4 * CPS;
   // Shift of the probabilities: the largest is 2^kUp when the shift moves, and stays
@@ -245,13 +256,16 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
                          (int64_t)hk * c.v_head * G::VEB;
   const unsigned krow_b = (unsigned)c.k_row, vrow_b = (unsigned)(c.v_row * G::VEB);
   const unsigned k_lane = grp * (D / 8), v_lane = n16 * G::PB;
-  const int32_t* table = c.page_table ? c.page_table + (int64_t)b * c.pt_b : nullptr;
+  // (An absent table is read at element 0 of some valid array and the value dropped.)
+  const int32_t* table = c.page_table ? c.page_table + (int64_t)b * c.pt_b
+                                      : reinterpret_cast<const int32_t*>(c.k_scale);
+  const int table_mul = c.page_table ? 1 : 0;
 
   // ---- a step: CPS chunks of 16 rows of a group, for this wave ----
   const int spg = (cpg + CPS * kKeyWaves - 1) / (CPS * kKeyWaves);
+  // The table entries are loaded with the metadata and first used a step later.
   struct Meta {
-    unsigned phys[CPS];
-    int r0[CPS], nval[CPS], tok0[CPS];
+    int entry[CPS], page[CPS], r0[CPS], nval[CPS], tok0[CPS];
   };
   int li = it0, lp = 0;                            // item and step of the next metadata
   auto next_meta = [&]() __attribute__((always_inline)) -> Meta {
@@ -267,10 +281,9 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
       int nval = j < cpg && li < it1 ? min(min(16, c.page_rows - r0), n - tok0) : 0;
       // Behind the sinks and before every row's window.
       if (tok0 >= a.sinks && tok0 + nval <= low_min) nval = 0;
-      const bool some = nval > 0;
-      const int pg = some ? (table ? ld_ro(table, page) : page) : 0;
-      m.phys[e] = (unsigned)__builtin_amdgcn_readfirstlane(min(max(pg, 0), c.num_pages - 1));
-      m.r0[e] = __builtin_amdgcn_readfirstlane(some ? r0 : 0);
+      m.page[e] = min(page, c.max_pages - 1);
+      m.entry[e] = ld_ro(table, __builtin_amdgcn_readfirstlane(m.page[e] * table_mul));
+      m.r0[e] = r0;
       m.nval[e] = __builtin_amdgcn_readfirstlane(nval);
       m.tok0[e] = __builtin_amdgcn_readfirstlane(tok0);
     }
@@ -280,9 +293,12 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
     }
     return m;
   };
+  auto phys_of = [&](const Meta& m, int e) __attribute__((always_inline)) -> uint64_t {
+    return (uint64_t)(unsigned)min(max(table_mul ? m.entry[e] : m.page[e], 0), c.num_pages - 1);
+  };
 
   // Rows past the valid count are loaded from the last valid row, a chunk of none from
-  // the first row of some page (never out of bounds, and its values are dropped).
+  // its first (never out of bounds, and its values are dropped).
   struct Keys {
     unsigned w[CPS][G::KW];
   };
@@ -292,13 +308,13 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
   auto load_keys = [&](const Meta& m, Keys& f) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < CPS; ++e) {
-      const uint8_t* kb = kbase + ((uint64_t)m.phys[e] * (uint64_t)c.k_page +
+      const uint8_t* kb = kbase + (phys_of(m, e) * (uint64_t)c.k_page +
                                    (uint64_t)(unsigned)m.r0[e] * krow_b);
       const unsigned ko = k_lane + (unsigned)min(n16, max(m.nval[e] - 1, 0)) * krow_b;
       constexpr int KL = G::KW < 4 ? G::KW : 4;
 #pragma unroll
       for (int i = 0; i < G::KW / KL; ++i) {
-        const KVec<KL> x = load_k<KL>(kb + (ko + 16 * i));
+        const KVec<KL> x = load_words<KL, RW == 1>(kb + (ko + 16 * i));
 #pragma unroll
         for (int k = 0; k < KL; ++k) f.w[e][KL * i + k] = x.w[k];
       }
@@ -308,14 +324,15 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
 #pragma unroll
     for (int e = 0; e < CPS; ++e) {
       const int last = max(m.nval[e] - 1, 0);
-      const uint8_t* vb = vbase + ((uint64_t)m.phys[e] * (uint64_t)(c.v_page * G::VEB) +
+      const uint8_t* vb = vbase + (phys_of(m, e) * (uint64_t)(c.v_page * G::VEB) +
                                    (uint64_t)(unsigned)m.r0[e] * vrow_b);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const unsigned vo = v_lane + (unsigned)min(4 * grp + i, last) * vrow_b;
 #pragma unroll
         for (int u = 0; u < G::NP; ++u) {
-          const KVec<G::PB / 4> x = load_k<G::PB / 4>(vb + (vo + 16 * G::PB * u));
+          const KVec<G::PB / 4> x =
+              load_words<G::PB / 4, RW == 1>(vb + (vo + 16 * G::PB * u));
 #pragma unroll
           for (int k = 0; k < G::PB / 4; ++k) f.w[e][i][u][k] = x.w[k];
         }
@@ -324,41 +341,38 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
   };
 
   // ---- scales of a group to LDS, and the rows' digits ----
-  // Thread t < D / 2 holds 16 bytes: scales 4t .. (t < D / 4), or zero-points.
-  auto load_sz = [&](int it) __attribute__((always_inline)) -> U32x4 {
-    const int g = group_of(min(it, it1 - 1));
-    const int e = tid % (D / 2);
-    const float* src = e < D / 4 ? sbase + 4 * e : zbase + 4 * (e - D / 4);
-    return ld16(src + (uint64_t)(unsigned)g * (uint64_t)c.s_g);
+  // Thread t < D / 4, all of wave 0, holds the scales and zero-points of channels 4t ..
+  struct Scales {
+    U32x4 s, z;
   };
-  auto stage_sz = [&](const U32x4& x, int buf) __attribute__((always_inline)) {
-    if (w >= (D / 2 + 63) / 64) return;
-    const bool is_s = tid < D / 4;
-    float4 y = make_float4(u2f(x.x), u2f(x.y), u2f(x.z), u2f(x.w));
-    if (w == 0) {
-      unsigned mx = is_s ? max(max(x.x & 0x7FFFFFFFu, x.y & 0x7FFFFFFFu),
-                               max(x.z & 0x7FFFFFFFu, x.w & 0x7FFFFFFFu))
-                         : 0u;
-      mx = max(mx, xchg_u32<1>(mx));
-      mx = max(mx, xchg_u32<2>(mx));
-      mx = max(mx, xchg_u32<4>(mx));
-      mx = max(mx, xchg_u32<8>(mx));
-      mx = max(mx, xchg_u32<16>(mx));
-      mx = max(mx, xchg_u32<32>(mx));
-      const float unit = u2f(max(mx, f2u(1e-28f))) * 0x1p-30f;
-      const float inv = (1.f - 0x1p-20f) / unit;
-      if (is_s) {
-        y.x *= inv;
-        y.y *= inv;
-        y.z *= inv;
-        y.w *= inv;
-      }
-      if (tid == 0) cs_s[buf] = unit * (1.f + 0x1p-20f);
-    }
-    if (tid < D / 2) {
-      float* dst = sz_s[buf] + (is_s ? 0 : D) + row_slot(4 * (tid % (D / 4)));
-      *reinterpret_cast<float2*>(dst) = make_float2(y.x, y.z);
-      *reinterpret_cast<float2*>(dst + 4) = make_float2(y.y, y.w);
+  auto load_sz = [&](int it) __attribute__((always_inline)) -> Scales {
+    const uint64_t off = (uint64_t)(unsigned)group_of(min(it, it1 - 1)) * (uint64_t)c.s_g +
+                         4 * (tid % (D / 4));
+    return Scales{ld16(sbase + off), ld16(zbase + off)};
+  };
+  // The scales in units of 2^-30 (2^-22) of the largest, and zero-points times them.
+  auto stage_sz = [&](const Scales& x, int buf) __attribute__((always_inline)) {
+    if (w != 0) return;
+    unsigned mx = max(max(x.s.x & 0x7FFFFFFFu, x.s.y & 0x7FFFFFFFu),
+                      max(x.s.z & 0x7FFFFFFFu, x.s.w & 0x7FFFFFFFu));
+    mx = max(mx, xchg_u32<1>(mx));
+    mx = max(mx, xchg_u32<2>(mx));
+    mx = max(mx, xchg_u32<4>(mx));
+    mx = max(mx, xchg_u32<8>(mx));
+    if constexpr (D > 64) mx = max(mx, xchg_u32<16>(mx));
+    if constexpr (D > 128) mx = max(mx, xchg_u32<32>(mx));
+    const float unit = u2f(max(mx, f2u(1e-28f))) * (WIDE ? 0x1p-30f : 0x1p-22f);
+    // (A little less than all the bits, so that no rounding reaches beyond them.)
+    const float inv = (1.f - 0x1p-20f) / unit;
+    if (tid == 0) cs_s[buf] = unit * (1.f + 0x1p-20f);
+    if (tid < D / 4) {
+      const float s0 = u2f(x.s.x) * inv, s1 = u2f(x.s.y) * inv, s2 = u2f(x.s.z) * inv,
+                  s3 = u2f(x.s.w) * inv;
+      float* dst = sz_s[buf] + row_slot(4 * tid);
+      *reinterpret_cast<float2*>(dst) = make_float2(s0, s2);
+      *reinterpret_cast<float2*>(dst + 4) = make_float2(s1, s3);
+      *reinterpret_cast<float2*>(dst + D) = make_float2(u2f(x.z.x) * s0, u2f(x.z.z) * s2);
+      *reinterpret_cast<float2*>(dst + D + 4) = make_float2(u2f(x.z.y) * s1, u2f(x.z.w) * s3);
     }
   };
   float qn[SPT], q_unit;                           // the row relative to its largest
@@ -371,26 +385,31 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
     for (int i = 0; i < SPT; i += 4) {
       const float4 s4 = *reinterpret_cast<const float4*>(s + i);
       const float4 z4 = *reinterpret_cast<const float4*>(z + i);
-      const float v0 = qn[i] * s4.x, v1 = qn[i + 1] * s4.y, v2 = qn[i + 2] * s4.z,
-                  v3 = qn[i + 3] * s4.w;
-      cg[0] = __builtin_fmaf(v0, z4.x, cg[0]);
-      cg[1] = __builtin_fmaf(v1, z4.y, cg[1]);
-      cg[2] = __builtin_fmaf(v2, z4.z, cg[2]);
-      cg[3] = __builtin_fmaf(v3, z4.w, cg[3]);
-      const unsigned x0 = (unsigned)(int)v0 + 0x808080u, x1 = (unsigned)(int)v1 + 0x808080u,
-                     x2 = (unsigned)(int)v2 + 0x808080u, x3 = (unsigned)(int)v3 + 0x808080u;
-      const unsigned t0 = __builtin_amdgcn_perm(x1, x0, 0x05010400u);
-      const unsigned t1 = __builtin_amdgcn_perm(x1, x0, 0x07030602u);
-      const unsigned u0 = __builtin_amdgcn_perm(x3, x2, 0x05010400u);
-      const unsigned u1 = __builtin_amdgcn_perm(x3, x2, 0x07030602u);
-      *reinterpret_cast<unsigned*>(dst + i) =
-          __builtin_amdgcn_perm(u0, t0, 0x05040100u) ^ 0x80808080u;
-      *reinterpret_cast<unsigned*>(dst + M * G::DS + i) =
-          __builtin_amdgcn_perm(u0, t0, 0x07060302u) ^ 0x80808080u;
-      *reinterpret_cast<unsigned*>(dst + 2 * M * G::DS + i) =
-          __builtin_amdgcn_perm(u1, t1, 0x05040100u) ^ 0x80808080u;
-      *reinterpret_cast<unsigned*>(dst + 3 * M * G::DS + i) =
-          __builtin_amdgcn_perm(u1, t1, 0x07060302u);
+      const float ss[4] = {s4.x, s4.y, s4.z, s4.w}, zz[4] = {z4.x, z4.y, z4.z, z4.w};
+      unsigned x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        cg[k] = __builtin_fmaf(qn[i + k], zz[k], cg[k]);
+        // The integer plus a bias that makes its lower bytes digits + 128.
+        if constexpr (WIDE) {
+          x[k] = (unsigned)(int)(qn[i + k] * ss[k]) + 0x808080u;
+        } else {
+          // (Rounded by the addition of 1.5 * 2^23, whose bits go again; |v| < 2^22.)
+          x[k] = f2u(__builtin_fmaf(qn[i + k], ss[k], 12582912.f)) - (0x4B400000u - 0x8080u);
+        }
+      }
+      const unsigned t0 = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u);
+      const unsigned u0 = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u);
+      const unsigned t1 = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u);
+      const unsigned u1 = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
+      unsigned dg[4] = {__builtin_amdgcn_perm(u0, t0, 0x05040100u) ^ 0x80808080u,
+                        __builtin_amdgcn_perm(u0, t0, 0x07060302u) ^ 0x80808080u,
+                        __builtin_amdgcn_perm(u1, t1, 0x05040100u),
+                        __builtin_amdgcn_perm(u1, t1, 0x07060302u)};
+      if constexpr (WIDE) dg[2] ^= 0x80808080u;
+#pragma unroll
+      for (int k = 0; k < ND; ++k)
+        *reinterpret_cast<unsigned*>(dst + k * M * G::DS + i) = dg[k];
     }
     float cgs = (cg[0] + cg[1]) + (cg[2] + cg[3]);
     cgs += xchg<1>(cgs);
@@ -515,7 +534,7 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
     Keys kf;
     Vals vf;
     Meta cur, nxt;
-    U32x4 sz0, sz1, szr;
+    Scales sz0, sz1, szr;
     if (steps > 0) {
       cur = next_meta();
       nxt = next_meta();
@@ -572,9 +591,11 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
         const int buf = (it - it0) & 1;
         if (p == 0) {
           __syncthreads();
-          if (it + 1 < it1) build(buf ^ 1);
           stage_sz(szr, buf);                      // of item it + 2
           szr = load_sz(it + 3);
+          if (RW == 1 || rg == 0) {
+            if (it + 1 < it1) build(buf ^ 1);
+          }
         }
         // Nibbles of key block kb of chunk e.
         auto key_op = [&](int e, int kb) __attribute__((always_inline)) -> v4i {
@@ -600,18 +621,19 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
                     ((cur.tok0[e] < low_max) & (cur.tok0[e] + 16 > a.sinks));
         }
         if (any) {
+          v4i ds_all[RT][CPS][ND];
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) {
-            const int r = rbase + rt * 16 + n16;
-            const uint8_t* dg = smem + buf * G::kDig + r * G::DS + grp * (D / 4);
-            v4i ds[CPS][4];
+            const uint8_t* dg =
+                smem + buf * G::kDig + (rbase + rt * 16 + n16) * G::DS + grp * (D / 4);
+            v4i (&ds)[CPS][ND] = ds_all[rt];
 #pragma unroll
             for (int kb = 0; kb < NB; ++kb) {
               v4i kop[CPS];
 #pragma unroll
               for (int e = 0; e < CPS; ++e) kop[e] = RT > 1 ? ak[e][kb] : key_op(e, kb);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
+              for (int k = 0; k < ND; ++k) {
                 const v4i bq = *reinterpret_cast<const v4i*>(dg + k * M * G::DS + 16 * kb);
 #pragma unroll
                 for (int e = 0; e < CPS; ++e)
@@ -619,15 +641,24 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
                       kop[e], bq, kb == 0 ? v4i{0, 0, 0, 0} : ds[e][k], 0, 0, 0);
               }
             }
-            if constexpr (RT == 1) load_keys(nxt, kf);
+          }
+          if constexpr (RT == 1) load_keys(nxt, kf);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            const int r = rbase + rt * 16 + n16;
+            const v4i (&ds)[CPS][ND] = ds_all[rt];
             float s[NS];
 #pragma unroll
             for (int e = 0; e < CPS; ++e)
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                s[4 * e + i] =
-                    __builtin_fmaf((float)((ds[e][3][i] << 8) + ds[e][2][i]), 65536.f,
-                                   (float)((ds[e][1][i] << 8) + ds[e][0][i]));
+              for (int i = 0; i < 4; ++i) {
+                const float hi = (float)((ds[e][ND - 1][i] << 8) + ds[e][ND - 2][i]);
+                if constexpr (WIDE)
+                  s[4 * e + i] =
+                      __builtin_fmaf(hi, 65536.f, (float)((ds[e][1][i] << 8) + ds[e][0][i]));
+                else
+                  s[4 * e + i] = __builtin_fmaf(hi, 256.f, (float)ds[e][0][i]);
+              }
             const float2 cc = cc_s[buf][r];
             unsigned vis = 0;
             if (masked) {
@@ -660,13 +691,18 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
                   for (int x = 0; x < G::PB / 4; ++x) vf.w[e][i][u][x] &= keep;
               }
           }
-          add_values(vf);
         } else if constexpr (RT == 1) {
           load_keys(nxt, kf);
         }
+        // The table entries of the step after the next: no LDS access, whose waits
+        // would wait for them too, follows before the value products.
+        const Meta ahead = next_meta();
+        if (any) add_values(vf);
         load_values(nxt, vf);
+        // The second row group, on the same SIMDs, builds while the first multiplies.
+        if (RW > 1 && rg != 0 && p == 0 && it + 1 < it1) build(buf ^ 1);
         cur = nxt;
-        nxt = next_meta();
+        nxt = ahead;
         if (++p == spg) {
           p = 0;
           ++it;
@@ -772,7 +808,7 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
         for (int t = g * group_rows; t < min((g + 1) * group_rows, n); ++t) {
           if (t >= a.sinks && t < low_s[r]) continue;
           const int lp = fdiv(t, c.div_rows), tr = t - lp * c.page_rows;
-          const int64_t phys = min(max(table ? table[lp] : lp, 0), c.num_pages - 1);
+          const int64_t phys = min(max(table_mul ? table[lp] : lp, 0), c.num_pages - 1);
           const uint8_t* kp = kbase + phys * c.k_page + (int64_t)tr * c.k_row;
           const int64_t vo = phys * c.v_page + (int64_t)hk * c.v_head + (int64_t)tr * c.v_row;
           float k[CH], v[CH];
@@ -877,16 +913,16 @@ hipError_t launch_decode_rows(const RowsArgs& a, int D, int v_dtype, int batch, 
                       batch;
   if (wgs > INT32_MAX) return hipErrorInvalidValue;
   const bool wide = a.c.out_dtype == kEF32;
-#define FDI4_RW(DD, VV, RR, WW, TT)                                                       \
-  if (D == DD && v_dtype == VV && a.row_tiles == RR * WW &&                               \
-      (VV != kVBF16 || wide == (TT == 3))) {                                              \
-    hipLaunchKernelGGL((decode_rows_kernel<DD, VV, RR, WW, TT>), dim3((unsigned)wgs),      \
+#define FDI4_RW(DD, VV, RR, WW, OO)                                                       \
+  if (D == DD && v_dtype == VV && a.row_tiles == RR * WW && wide == OO) {                 \
+    hipLaunchKernelGGL((decode_rows_kernel<DD, VV, RR, WW, OO>), dim3((unsigned)wgs),      \
                        dim3(kKeyWaves * 64 * WW), 0, st, a);                              \
     return hipGetLastError();                                                             \
   }
 #define FDI4_RW_V(DD, RR, WW) \
-  FDI4_RW(DD, kVF32, RR, WW, 1) FDI4_RW(DD, kVF16, RR, WW, 2) \
-  FDI4_RW(DD, kVBF16, RR, WW, 2) FDI4_RW(DD, kVBF16, RR, WW, 3)
+  FDI4_RW(DD, kVF32, RR, WW, false) FDI4_RW(DD, kVF16, RR, WW, false) \
+  FDI4_RW(DD, kVBF16, RR, WW, false) FDI4_RW(DD, kVF32, RR, WW, true) \
+  FDI4_RW(DD, kVF16, RR, WW, true) FDI4_RW(DD, kVBF16, RR, WW, true)
   FDI4_RW_V(64, 1, 1) FDI4_RW_V(64, 2, 1) FDI4_RW_V(64, 2, 2)
   FDI4_RW_V(128, 1, 1) FDI4_RW_V(128, 2, 1) FDI4_RW_V(128, 2, 2)
   FDI4_RW_V(256, 1, 1) FDI4_RW_V(256, 1, 2)
