@@ -900,10 +900,10 @@ struct RowsPlan {
 RowsPlan plan_rows(int batch, int num_q_heads, int nodes, int window, int sinks, int num_splits,
                    const fdi4_paged_cache* cache) {
   RowsPlan p;
-  const int most = cache->head_dim == 256 ? 2 : 4;
+  const int most = cache->head_dim == 256 ? 1 : 2;
   const int64_t rows = (int64_t)(num_q_heads / cache->num_kv_heads) * nodes;
   const int64_t t16 = (rows + 15) / 16;
-  p.row_tiles = t16 >= 3 ? most : (int)std::min<int64_t>(t16, most);
+  p.row_tiles = (int)std::min<int64_t>(t16, most);
   p.tiles = (int)((t16 + p.row_tiles - 1) / p.row_tiles);
   // The most items a sequence can have.
   const int64_t cap = (int64_t)cache->max_pages * cache->page_rows;
@@ -915,7 +915,7 @@ RowsPlan plan_rows(int batch, int num_q_heads, int nodes, int window, int sinks,
   if (nodes > 1) items += (nodes + 63) / 64;
   items = std::max<int64_t>(items, 1);
   const int64_t streams = (int64_t)batch * cache->num_kv_heads * p.tiles;
-  const int64_t slots = p.row_tiles < most ? 2 * kCUs : kCUs;
+  const int64_t slots = 2 * kCUs;
   const int64_t s = num_splits > 0 ? num_splits : slots / std::max<int64_t>(streams, 1);
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(s, items), kMaxSplits));
   return p;

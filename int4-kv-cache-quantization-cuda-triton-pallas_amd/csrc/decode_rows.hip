@@ -50,9 +50,9 @@ typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
-constexpr int kKeyWaves = 4;   // waves that share a step's chunks (per row group)
+constexpr int kWaves = 4;
 
-template <int D, int VDT, int RT, int RW, int ND>
+template <int D, int VDT, int RT, int ND>
 struct RowsGeo {
   static constexpr int NB = D / 64;                // 64-channel blocks of the key product
   static constexpr int KW = D / 32;                // packed key words per lane per row
@@ -62,8 +62,8 @@ struct RowsGeo {
   static constexpr int CPP = PB / VEB;             // channels per value load
   static constexpr int NA = D / 16;                // 16-channel output tiles
   static constexpr int CPS = VDT == kVF32 ? 1 : 2; // chunks per step
-  static constexpr int M = 16 * RT * RW;           // rows of the workgroup
-  static constexpr int NT = kKeyWaves * 64 * RW;   // threads
+  static constexpr int M = 16 * RT;           // rows of the workgroup
+  static constexpr int NT = kWaves * 64;           // threads
   static constexpr int TPR = NT / M;               // threads per row that build digits
   static constexpr int SPT = D / TPR;              // channels each
   static constexpr int DS = D + 16;                // bytes per row of a digit (padded)
@@ -73,7 +73,7 @@ struct RowsGeo {
   // outputs.
   static constexpr int kQ = 2 * kDig;
   static constexpr int kStream = kQ + M * AS * 4;
-  static constexpr int kAcc = kKeyWaves * M * AS * 4;
+  static constexpr int kAcc = kWaves * M * AS * 4;
   static constexpr int kSmem = kStream > kAcc ? kStream : kAcc;
   static_assert(TPR >= 4 && TPR <= 16 && (TPR & (TPR - 1)) == 0 && SPT % 4 == 0, "threads");
 };
@@ -100,12 +100,18 @@ __device__ __forceinline__ void load_query8(const void* q, int64_t i, int dt, bo
   }
 }
 
-// KW words of a key or value row: streamed (non-temporal) where one wave reads them,
-// through the caches where the second row group, or another tile's workgroup, does too.
+// KW words of a key or value row: streamed (non-temporal) where one workgroup reads them,
+// through the caches where the workgroups of other rows do too.
 template <int KW, bool STREAM>
 __device__ __forceinline__ KVec<KW> load_words(const uint8_t* p) {
   if constexpr (STREAM) return load_k<KW>(p);
   return *reinterpret_cast<const KVec<KW>*>(__builtin_assume_aligned(p, 4 * KW));
+}
+
+// Value of lane ^ 4: mirrored within 8 lanes, then within 4.
+__device__ __forceinline__ unsigned xchg4(unsigned x) {
+  return (unsigned)__builtin_amdgcn_mov_dpp(
+      __builtin_amdgcn_mov_dpp((int)x, 0x141, 0xF, 0xF, false), 0x1B, 0xF, 0xF, false);
 }
 
 // Maximum and sum over the four 16-lane groups.
@@ -131,14 +137,14 @@ __device__ __forceinline__ float over_groups_sum(float x) {
   return u2f(s[0]) + u2f(s[1]);
 }
 
-// RT row tiles a wave, RW row groups of four waves: wave w takes key chunks w % 4 and
-// row group w / 4. WIDE: float32 outputs (four digits of q*s, all 24 bits of a
-// probability); otherwise three digits and at least 16 bits.
-template <int D, int VDT, int RT, int RW, bool WIDE>
-__global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(RowsArgs a) {
+// RT: row tiles. WIDE: float32 outputs (four digits of q*s, all 24 bits of a
+// probability); otherwise three digits and at least 16 bits. STREAM: keys and values
+// are read by one workgroup only (non-temporal loads).
+template <int D, int VDT, int RT, bool WIDE, bool STREAM>
+__global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a) {
   constexpr int ND = WIDE ? 4 : 3;
   constexpr int TERMS = WIDE && VDT == kVBF16 ? 3 : 2;   // 16-bit terms of a probability
-  using G = RowsGeo<D, VDT, RT, RW, ND>;
+  using G = RowsGeo<D, VDT, RT, ND>;
   constexpr int NB = G::NB, CPS = G::CPS, NA = G::NA, M = G::M, NT = G::NT;
   constexpr int TPR = G::TPR, SPT = G::SPT, NS = 4 * CPS;
   // Shift of the probabilities: the largest is 2^kUp when the shift moves, and stays
@@ -152,9 +158,7 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
   const DecodeArgs& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kw = w & (kKeyWaves - 1), rg = w / kKeyWaves;
   const int n16 = lane & 15, grp = lane >> 4;
-  const int rbase = rg * 16 * RT;                  // first row of this wave's tiles
 
   // Tiles of one (sequence, kv-head, split) run on one XCD, one after the other: they
   // read the same pages.
@@ -172,12 +176,16 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
   const int live = min(rows - row0, M);            // rows of this workgroup
 
   __shared__ __align__(16) uint8_t smem[G::kSmem];
-  __shared__ __align__(16) float sz_s[2][2 * D];   // scaled scales, zero-points (slot order)
+  // Scaled scales, and zero-points times them, in slot order; four floats of padding
+  // every 16 keep the threads of a row, 16 channels apart, on different banks.
+  constexpr int kSz = D + D / 4;
+  auto sz_pos = [](int slot) { return slot + slot / 16 * 4; };
+  __shared__ __align__(16) float sz_s[2][2 * kSz];
   __shared__ float cs_s[2];                        // a group's scale unit
   __shared__ float2 cc_s[2][M];                    // a row's logit unit and constant
   __shared__ int low_s[M];                         // first cached token in a row's window
   __shared__ int ext_s[2];                         // smallest and largest of them
-  __shared__ float m_s[kKeyWaves][M], l_s[kKeyWaves][M];
+  __shared__ float m_s[kWaves][M], l_s[kWaves][M];
   __shared__ int bad_s;
   float* const q_s = reinterpret_cast<float*>(smem + G::kQ);
 
@@ -255,14 +263,20 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
   const uint8_t* vbase = reinterpret_cast<const uint8_t*>(c.v_pages) +
                          (int64_t)hk * c.v_head * G::VEB;
   const unsigned krow_b = (unsigned)c.k_row, vrow_b = (unsigned)(c.v_row * G::VEB);
+  // Offsets of this lane's key row and value rows in a full chunk; a partial one takes
+  // the smaller of these and the last valid row's.
   const unsigned k_lane = grp * (D / 8), v_lane = n16 * G::PB;
+  const unsigned k_full = k_lane + n16 * krow_b;
+  unsigned v_full[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v_full[i] = v_lane + (4 * grp + i) * vrow_b;
   // (An absent table is read at element 0 of some valid array and the value dropped.)
   const int32_t* table = c.page_table ? c.page_table + (int64_t)b * c.pt_b
                                       : reinterpret_cast<const int32_t*>(c.k_scale);
   const int table_mul = c.page_table ? 1 : 0;
 
   // ---- a step: CPS chunks of 16 rows of a group, for this wave ----
-  const int spg = (cpg + CPS * kKeyWaves - 1) / (CPS * kKeyWaves);
+  const int spg = (cpg + CPS * kWaves - 1) / (CPS * kWaves);
   // The table entries are loaded with the metadata and first used a step later.
   struct Meta {
     int entry[CPS], page[CPS], r0[CPS], nval[CPS], tok0[CPS];
@@ -273,7 +287,7 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
     const int g = group_of(min(li, it1 - 1));
 #pragma unroll
     for (int e = 0; e < CPS; ++e) {
-      const int j = (lp * CPS + e) * kKeyWaves + kw;
+      const int j = (lp * CPS + e) * kWaves + w;
       const int pj = fdiv(j, c.div_cpp);
       const int page = g * c.pages_per_group + pj;
       const int r0 = (j - pj * cpp) * 16;
@@ -310,11 +324,11 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
     for (int e = 0; e < CPS; ++e) {
       const uint8_t* kb = kbase + (phys_of(m, e) * (uint64_t)c.k_page +
                                    (uint64_t)(unsigned)m.r0[e] * krow_b);
-      const unsigned ko = k_lane + (unsigned)min(n16, max(m.nval[e] - 1, 0)) * krow_b;
+      const unsigned ko = min(k_full, k_lane + (unsigned)max(m.nval[e] - 1, 0) * krow_b);
       constexpr int KL = G::KW < 4 ? G::KW : 4;
 #pragma unroll
       for (int i = 0; i < G::KW / KL; ++i) {
-        const KVec<KL> x = load_words<KL, RW == 1>(kb + (ko + 16 * i));
+        const KVec<KL> x = load_words<KL, STREAM>(kb + (ko + 16 * i));
 #pragma unroll
         for (int k = 0; k < KL; ++k) f.w[e][KL * i + k] = x.w[k];
       }
@@ -323,16 +337,16 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
   auto load_values = [&](const Meta& m, Vals& f) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < CPS; ++e) {
-      const int last = max(m.nval[e] - 1, 0);
+      const unsigned v_last = v_lane + (unsigned)max(m.nval[e] - 1, 0) * vrow_b;
       const uint8_t* vb = vbase + (phys_of(m, e) * (uint64_t)(c.v_page * G::VEB) +
                                    (uint64_t)(unsigned)m.r0[e] * vrow_b);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const unsigned vo = v_lane + (unsigned)min(4 * grp + i, last) * vrow_b;
+        const unsigned vo = min(v_full[i], v_last);
 #pragma unroll
         for (int u = 0; u < G::NP; ++u) {
           const KVec<G::PB / 4> x =
-              load_words<G::PB / 4, RW == 1>(vb + (vo + 16 * G::PB * u));
+              load_words<G::PB / 4, STREAM>(vb + (vo + 16 * G::PB * u));
 #pragma unroll
           for (int k = 0; k < G::PB / 4; ++k) f.w[e][i][u][k] = x.w[k];
         }
@@ -341,50 +355,58 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
   };
 
   // ---- scales of a group to LDS, and the rows' digits ----
-  // Thread t < D / 4, all of wave 0, holds the scales and zero-points of channels 4t ..
+  // Lane l < D / 4 of every wave holds the scales and zero-points of channels 4l ..
   struct Scales {
     U32x4 s, z;
   };
   auto load_sz = [&](int it) __attribute__((always_inline)) -> Scales {
     const uint64_t off = (uint64_t)(unsigned)group_of(min(it, it1 - 1)) * (uint64_t)c.s_g +
-                         4 * (tid % (D / 4));
+                         4 * (lane % (D / 4));
     return Scales{ld16(sbase + off), ld16(zbase + off)};
   };
   // The scales in units of 2^-30 (2^-22) of the largest, and zero-points times them.
-  auto stage_sz = [&](const Scales& x, int buf) __attribute__((always_inline)) {
-    if (w != 0) return;
+  // (By wave `by`; powers of two, so that only the products with q round.)
+  constexpr int kBits = WIDE ? 30 : 22;
+  auto stage_sz = [&](const Scales& x, int buf, int by) __attribute__((always_inline)) {
+    if (w != by) return;
     unsigned mx = max(max(x.s.x & 0x7FFFFFFFu, x.s.y & 0x7FFFFFFFu),
                       max(x.s.z & 0x7FFFFFFFu, x.s.w & 0x7FFFFFFFu));
     mx = max(mx, xchg_u32<1>(mx));
     mx = max(mx, xchg_u32<2>(mx));
-    mx = max(mx, xchg_u32<4>(mx));
+    mx = max(mx, xchg4(mx));
     mx = max(mx, xchg_u32<8>(mx));
     if constexpr (D > 64) mx = max(mx, xchg_u32<16>(mx));
     if constexpr (D > 128) mx = max(mx, xchg_u32<32>(mx));
-    const float unit = u2f(max(mx, f2u(1e-28f))) * (WIDE ? 0x1p-30f : 0x1p-22f);
-    // (A little less than all the bits, so that no rounding reaches beyond them.)
-    const float inv = (1.f - 0x1p-20f) / unit;
-    if (tid == 0) cs_s[buf] = unit * (1.f + 0x1p-20f);
-    if (tid < D / 4) {
+    // All scales are below 2^kBits units. (An infinite or NaN one makes the rows NaN.)
+    const unsigned ex = (max(mx, f2u(1e-28f)) >> 23) + 1 - kBits;
+    const float inv = u2f((254 - ex) << 23);
+    if (lane == 0) cs_s[buf] = mx >= 0x7F800000u ? u2f(0x7FC00000u) : u2f(ex << 23);
+    if (lane < D / 4) {
       const float s0 = u2f(x.s.x) * inv, s1 = u2f(x.s.y) * inv, s2 = u2f(x.s.z) * inv,
                   s3 = u2f(x.s.w) * inv;
-      float* dst = sz_s[buf] + row_slot(4 * tid);
+      float* dst = sz_s[buf] + sz_pos(row_slot(4 * lane));
       *reinterpret_cast<float2*>(dst) = make_float2(s0, s2);
       *reinterpret_cast<float2*>(dst + 4) = make_float2(s1, s3);
-      *reinterpret_cast<float2*>(dst + D) = make_float2(u2f(x.z.x) * s0, u2f(x.z.z) * s2);
-      *reinterpret_cast<float2*>(dst + D + 4) = make_float2(u2f(x.z.y) * s1, u2f(x.z.w) * s3);
+      dst += kSz;
+      *reinterpret_cast<float2*>(dst) = make_float2(u2f(x.z.x) * s0, u2f(x.z.z) * s2);
+      *reinterpret_cast<float2*>(dst + 4) = make_float2(u2f(x.z.y) * s1, u2f(x.z.w) * s3);
     }
   };
   float qn[SPT], q_unit;                           // the row relative to its largest
   auto build = [&](int buf) __attribute__((always_inline)) {
-    const float* s = sz_s[buf] + part * SPT;
-    const float* z = s + D;
+    const float cs = cs_s[buf];
+    float4 sv[SPT / 4], zv[SPT / 4];
+#pragma unroll
+    for (int i = 0; i < SPT; i += 4) {
+      const float* src = sz_s[buf] + sz_pos(part * SPT + i);
+      sv[i / 4] = *reinterpret_cast<const float4*>(src);
+      zv[i / 4] = *reinterpret_cast<const float4*>(src + kSz);
+    }
     uint8_t* dst = smem + buf * G::kDig + brow * G::DS + part * SPT;
     float cg[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < SPT; i += 4) {
-      const float4 s4 = *reinterpret_cast<const float4*>(s + i);
-      const float4 z4 = *reinterpret_cast<const float4*>(z + i);
+      const float4 s4 = sv[i / 4], z4 = zv[i / 4];
       const float ss[4] = {s4.x, s4.y, s4.z, s4.w}, zz[4] = {z4.x, z4.y, z4.z, z4.w};
       unsigned x[4];
 #pragma unroll
@@ -414,21 +436,24 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
     float cgs = (cg[0] + cg[1]) + (cg[2] + cg[3]);
     cgs += xchg<1>(cgs);
     cgs += xchg<2>(cgs);
-    if constexpr (TPR > 4) cgs += xchg<4>(cgs);
+    if constexpr (TPR > 4) cgs += u2f(xchg4(f2u(cgs)));
     if constexpr (TPR > 8) cgs += xchg<8>(cgs);
     if (part == 0) {
-      const float c1 = q_unit * cs_s[buf] * kLog2e;
+      const float c1 = q_unit * cs * kLog2e;
       cc_s[buf][brow] = make_float2(c1, cgs * c1);
     }
   };
 
   // ---- softmax and values ----
-  float m_run[RT], l_run[RT];
+  // (The sum of a row's probabilities is one more output channel, of ones: as an
+  // accumulator of the 16-bit products, in every lane; per lane for float32 values.)
+  float m_run[RT];
+  v4f l_run[RT];
   v4f acc[RT][NA];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     m_run[rt] = kLeast;
-    l_run[rt] = 0.f;
+    l_run[rt] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int t = 0; t < NA; ++t) acc[rt][t] = v4f{0.f, 0.f, 0.f, 0.f};
   }
@@ -436,19 +461,22 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
   constexpr int PW = VDT == kVF32 ? 4 : 4 * TERMS;
   unsigned pr[RT][PW];
 
-  // Row tile rt and scores s (logit = s * c1 - cc, log2 units) of keys 4 grp + i of
-  // chunk e in s[4 e + i], of which those in vis are seen.
+  // Row tile rt and scores s (logit = s * c1 - cc, log2 units, c1 >= 0) of keys
+  // 4 grp + i of chunk e in s[4 e + i], of which, if masked, those in vis are seen.
   auto softmax = [&](int rt, const float* s, float c1, float cc, bool masked, unsigned vis)
       __attribute__((always_inline)) {
-    float p[NS], top = kLeast, ps = 0.f;
-#pragma unroll
-    for (int k = 0; k < NS; ++k) p[k] = __builtin_fmaf(s[k], c1, -cc);
+    float p[NS], top = kLeast;
     if (masked) {
 #pragma unroll
-      for (int k = 0; k < NS; ++k) p[k] = (vis >> k) & 1u ? p[k] : -INFINITY;
-    }
+      for (int k = 0; k < NS; ++k) {
+        p[k] = (vis >> k) & 1u ? __builtin_fmaf(s[k], c1, -cc) : -INFINITY;
+        top = fmaxf(top, p[k]);
+      }
+    } else {
 #pragma unroll
-    for (int k = 0; k < NS; ++k) top = fmaxf(top, p[k]);
+      for (int k = 0; k < NS; ++k) top = fmaxf(top, s[k]);
+      top = __builtin_fmaf(top, c1, -cc);
+    }
     top = over_groups_max(top);
     const bool up = top > m_run[rt] + (kUp + kSlack);
     if (__builtin_amdgcn_ballot_w64(up)) {
@@ -459,14 +487,20 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
 #pragma unroll
       for (int t = 0; t < NA; ++t) acc[rt][t] *= corr;
     }
+    if (masked) {
 #pragma unroll
-    for (int k = 0; k < NS; ++k) p[k] = __builtin_amdgcn_exp2f(p[k] - m_run[rt]);
+      for (int k = 0; k < NS; ++k) p[k] = __builtin_amdgcn_exp2f(p[k] - m_run[rt]);
+    } else {
+      const float sub = -cc - m_run[rt];
 #pragma unroll
-    for (int k = 0; k < NS; ++k) ps += p[k];
-    l_run[rt] += ps;
+      for (int k = 0; k < NS; ++k) p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], c1, sub));
+    }
     if constexpr (VDT == kVF32) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) pr[rt][k] = f2u(p[k]);
+      for (int k = 0; k < 4; ++k) {
+        pr[rt][k] = f2u(p[k]);
+        l_run[rt][0] += p[k];
+      }
     } else {
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
@@ -492,7 +526,25 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
     }
   };
 
+  auto prob = [&](int rt, int q) __attribute__((always_inline)) -> uint4 {
+    return make_uint4(pr[rt][4 * q], pr[rt][4 * q + 1], pr[rt][4 * q + 2], pr[rt][4 * q + 3]);
+  };
+  auto product = [](uint4 x, uint4 y, v4f o) __attribute__((always_inline)) -> v4f {
+    if constexpr (VDT == kVF16)
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, x),
+                                                    __builtin_bit_cast(v8h, y), o, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, x),
+                                                   __builtin_bit_cast(v8bf, y), o, 0, 0, 0);
+  };
   auto add_values = [&](const Vals& f) __attribute__((always_inline)) {
+    if constexpr (VDT != kVF32) {
+      constexpr unsigned kOnes = VDT == kVF16 ? 0x3C003C00u : 0x3F803F80u;
+      const uint4 ones = make_uint4(kOnes, kOnes, kOnes, kOnes);
+#pragma unroll
+      for (int q = 0; q < TERMS; ++q)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) l_run[rt] = product(ones, prob(rt, q), l_run[rt]);
+    }
 #pragma unroll
     for (int t = 0; t < NA; ++t) {
       const int u = t / G::CPP, j = t % G::CPP;
@@ -515,16 +567,7 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
 #pragma unroll
         for (int q = 0; q < TERMS; ++q)
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            const uint4 bv = make_uint4(pr[rt][4 * q], pr[rt][4 * q + 1], pr[rt][4 * q + 2],
-                                        pr[rt][4 * q + 3]);
-            if constexpr (VDT == kVF16)
-              acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                  __builtin_bit_cast(v8h, av), __builtin_bit_cast(v8h, bv), acc[rt][t], 0, 0, 0);
-            else
-              acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                  __builtin_bit_cast(v8bf, av), __builtin_bit_cast(v8bf, bv), acc[rt][t], 0, 0, 0);
-          }
+          for (int rt = 0; rt < RT; ++rt) acc[rt][t] = product(av, prob(rt, q), acc[rt][t]);
       }
     }
   };
@@ -580,8 +623,8 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
     }
     if (tid == 0) bad_s = 0;
     if (steps > 0) {
-      stage_sz(sz0, 0);
-      stage_sz(sz1, 1);
+      stage_sz(sz0, 0, 0);
+      stage_sz(sz1, 1, 1);
     }
     __syncthreads();
     if (steps > 0) {
@@ -591,11 +634,9 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
         const int buf = (it - it0) & 1;
         if (p == 0) {
           __syncthreads();
-          stage_sz(szr, buf);                      // of item it + 2
+          if (it + 1 < it1) build(buf ^ 1);
+          stage_sz(szr, buf, it & (kWaves - 1));   // of item it + 2
           szr = load_sz(it + 3);
-          if (RW == 1 || rg == 0) {
-            if (it + 1 < it1) build(buf ^ 1);
-          }
         }
         // Nibbles of key block kb of chunk e.
         auto key_op = [&](int e, int kb) __attribute__((always_inline)) -> v4i {
@@ -621,12 +662,11 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
                     ((cur.tok0[e] < low_max) & (cur.tok0[e] + 16 > a.sinks));
         }
         if (any) {
-          v4i ds_all[RT][CPS][ND];
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) {
-            const uint8_t* dg =
-                smem + buf * G::kDig + (rbase + rt * 16 + n16) * G::DS + grp * (D / 4);
-            v4i (&ds)[CPS][ND] = ds_all[rt];
+            const int r = rt * 16 + n16;
+            const uint8_t* dg = smem + buf * G::kDig + r * G::DS + grp * (D / 4);
+            v4i ds[CPS][ND];
 #pragma unroll
             for (int kb = 0; kb < NB; ++kb) {
               v4i kop[CPS];
@@ -641,12 +681,7 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
                       kop[e], bq, kb == 0 ? v4i{0, 0, 0, 0} : ds[e][k], 0, 0, 0);
               }
             }
-          }
-          if constexpr (RT == 1) load_keys(nxt, kf);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            const int r = rbase + rt * 16 + n16;
-            const v4i (&ds)[CPS][ND] = ds_all[rt];
+            if constexpr (RT == 1) load_keys(nxt, kf);
             float s[NS];
 #pragma unroll
             for (int e = 0; e < CPS; ++e)
@@ -699,8 +734,6 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
         const Meta ahead = next_meta();
         if (any) add_values(vf);
         load_values(nxt, vf);
-        // The second row group, on the same SIMDs, builds while the first multiplies.
-        if (RW > 1 && rg != 0 && p == 0 && it + 1 < it1) build(buf ^ 1);
         cur = nxt;
         nxt = ahead;
         if (++p == spg) {
@@ -712,7 +745,7 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
 
     // ---- drafts: 16 of them a wave and item, float32 products ----
     for (int item = dr0; item < dr1; ++item) {
-      const int j0 = (item * kKeyWaves + kw) * 16;
+      const int j0 = (item * kWaves + w) * 16;
       const int nval = min(16, a.nodes - j0);
       if (nval <= 0) break;
       const uint8_t* vb = a.vd + (int64_t)b * a.vd_b + (int64_t)hk * a.vd_h + v_lane;
@@ -740,7 +773,7 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           const float4 q4 = *reinterpret_cast<const float4*>(
-              q_s + (rbase + rt * 16 + n16) * G::AS + grp * (D / 4) + d);
+              q_s + (rt * 16 + n16) * G::AS + grp * (D / 4) + d);
           ds[rt] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.x, q4.x, ds[rt], 0, 0, 0);
           ds[rt] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.y, q4.y, ds[rt], 0, 0, 0);
           ds[rt] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.z, q4.z, ds[rt], 0, 0, 0);
@@ -749,7 +782,7 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
       }
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const int R = row0 + min(rbase + rt * 16 + n16, live - 1);
+        const int R = row0 + min(rt * 16 + n16, live - 1);
         const int node = R - fdiv(R, a.div_nodes) * a.nodes;
         const uint8_t* mk = a.mask + (int64_t)b * a.mk_b + (int64_t)node * a.mk_i + j0;
         unsigned vis = 0;
@@ -776,11 +809,11 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
     constexpr int CH = D / 64;
     float* part0 = reinterpret_cast<float*>(smem);
     __syncthreads();
-    for (int i = tid; i < kKeyWaves * M; i += NT) {
+    for (int i = tid; i < kWaves * M; i += NT) {
       m_s[i / M][i % M] = kLeast;
       l_s[i / M][i % M] = 0.f;
     }
-    for (int i = tid; i < kKeyWaves * M * G::AS; i += NT) part0[i] = 0.f;
+    for (int i = tid; i < kWaves * M * G::AS; i += NT) part0[i] = 0.f;
     __syncthreads();
     for (int r = w; r < live; r += NT / 64) {
       const int i = (row0 + r) % a.nodes;
@@ -841,21 +874,21 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
   // ---- the waves' parts ----
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const float l = over_groups_sum(l_run[rt]);
+    const float l = VDT == kVF32 ? over_groups_sum(l_run[rt][0]) : l_run[rt][0];
     if (grp == 0) {
-      m_s[kw][rbase + rt * 16 + n16] = m_run[rt];
-      l_s[kw][rbase + rt * 16 + n16] = l;
+      m_s[w][rt * 16 + n16] = m_run[rt];
+      l_s[w][rt * 16 + n16] = l;
     }
   }
   __syncthreads();                                 // (the digits are no longer read)
-  float* out_w = reinterpret_cast<float*>(smem) + kw * M * G::AS;
+  float* out_w = reinterpret_cast<float*>(smem) + w * M * G::AS;
   float any_nan = 0.f;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int r = rbase + rt * 16 + n16;
+    const int r = rt * 16 + n16;
     float top = m_s[0][r];
 #pragma unroll
-    for (int i = 1; i < kKeyWaves; ++i) top = fmaxf(top, m_s[i][r]);
+    for (int i = 1; i < kWaves; ++i) top = fmaxf(top, m_s[i][r]);
     const float f = __builtin_amdgcn_exp2f(m_run[rt] - top);
 #pragma unroll
     for (int u = 0; u < G::NP; ++u)
@@ -880,11 +913,11 @@ __global__ __launch_bounds__(kKeyWaves * 64 * RW, 2) void decode_rows_kernel(Row
     const int r = idx / D, d = idx % D;
     float top = m_s[0][r];
 #pragma unroll
-    for (int i = 1; i < kKeyWaves; ++i) top = fmaxf(top, m_s[i][r]);
+    for (int i = 1; i < kWaves; ++i) top = fmaxf(top, m_s[i][r]);
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < kKeyWaves; ++i) {
+    for (int i = 0; i < kWaves; ++i) {
       l = __builtin_fmaf(__builtin_amdgcn_exp2f(m_s[i][r] - top), l_s[i][r], l);
       const float4 x = *reinterpret_cast<const float4*>(parts + (i * M + r) * G::AS + d);
       o.x += x.x;
@@ -913,19 +946,20 @@ hipError_t launch_decode_rows(const RowsArgs& a, int D, int v_dtype, int batch, 
                       batch;
   if (wgs > INT32_MAX) return hipErrorInvalidValue;
   const bool wide = a.c.out_dtype == kEF32;
-#define FDI4_RW(DD, VV, RR, WW, OO)                                                       \
-  if (D == DD && v_dtype == VV && a.row_tiles == RR * WW && wide == OO) {                 \
-    hipLaunchKernelGGL((decode_rows_kernel<DD, VV, RR, WW, OO>), dim3((unsigned)wgs),      \
-                       dim3(kKeyWaves * 64 * WW), 0, st, a);                              \
+  const bool stream = a.tiles == 1;
+#define FDI4_RW(DD, VV, RR, OO, SS)                                                       \
+  if (D == DD && v_dtype == VV && a.row_tiles == RR && wide == OO && stream == SS) {      \
+    hipLaunchKernelGGL((decode_rows_kernel<DD, VV, RR, OO, SS>), dim3((unsigned)wgs),      \
+                       dim3(kWaves * 64), 0, st, a);                                      \
     return hipGetLastError();                                                             \
   }
-#define FDI4_RW_V(DD, RR, WW) \
-  FDI4_RW(DD, kVF32, RR, WW, false) FDI4_RW(DD, kVF16, RR, WW, false) \
-  FDI4_RW(DD, kVBF16, RR, WW, false) FDI4_RW(DD, kVF32, RR, WW, true) \
-  FDI4_RW(DD, kVF16, RR, WW, true) FDI4_RW(DD, kVBF16, RR, WW, true)
-  FDI4_RW_V(64, 1, 1) FDI4_RW_V(64, 2, 1) FDI4_RW_V(64, 2, 2)
-  FDI4_RW_V(128, 1, 1) FDI4_RW_V(128, 2, 1) FDI4_RW_V(128, 2, 2)
-  FDI4_RW_V(256, 1, 1) FDI4_RW_V(256, 1, 2)
+#define FDI4_RW_V(DD, RR, SS) \
+  FDI4_RW(DD, kVF32, RR, false, SS) FDI4_RW(DD, kVF16, RR, false, SS) \
+  FDI4_RW(DD, kVBF16, RR, false, SS) FDI4_RW(DD, kVF32, RR, true, SS) \
+  FDI4_RW(DD, kVF16, RR, true, SS) FDI4_RW(DD, kVBF16, RR, true, SS)
+  FDI4_RW_V(64, 1, true) FDI4_RW_V(64, 2, true) FDI4_RW_V(64, 2, false)
+  FDI4_RW_V(128, 1, true) FDI4_RW_V(128, 2, true) FDI4_RW_V(128, 2, false)
+  FDI4_RW_V(256, 1, true) FDI4_RW_V(256, 1, false)
 #undef FDI4_RW_V
 #undef FDI4_RW
   return hipErrorInvalidValue;
