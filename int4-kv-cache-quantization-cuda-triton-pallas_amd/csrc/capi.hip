@@ -951,6 +951,13 @@ int make_rows_args(const void* query, int q_dtype, int batch, int num_q_heads, i
   r->div_nodes = fdi4::make_fast_div(nodes);
   r->div_heads = fdi4::make_fast_div(cache->num_kv_heads);
   r->kv_heads = cache->num_kv_heads;
+  const int64_t vpb = cache->v_page_stride * (cache->v_dtype == FDI4_V_F32 ? 4 : 2);
+  if (cache->k_page_stride < 0 || cache->k_page_stride > UINT32_MAX || vpb < 0 ||
+      vpb > UINT32_MAX || cache->s_group_stride < 0 || cache->s_group_stride > UINT32_MAX)
+    return hipErrorInvalidValue;
+  r->k_page_b = (uint32_t)cache->k_page_stride;
+  r->v_page_b = (uint32_t)vpb;
+  r->s_group = (uint32_t)cache->s_group_stride;
   const int qeb = q_dtype == FDI4_K_F32 ? 4 : 2;
   r->q_vec = aligned(query, 16) && (q_batch_stride * qeb) % 16 == 0 &&
              (q_head_stride * qeb) % 16 == 0 && (q_node_stride * qeb) % 16 == 0;

@@ -52,6 +52,16 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kWaves = 4;
 
+// The kernel's arguments, read again from where they lie: a phase that follows the key
+// loop uses this copy, so that its arguments hold no scalar registers in the loop (those
+// that do not fit go to lanes of vector registers, which do not fit then).
+__device__ __forceinline__ const RowsArgs& late_args() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const RowsArgs*)p;
+}
+
+
 template <int D, int VDT, int RT, int ND>
 struct RowsGeo {
   static constexpr int NB = D / 64;                // 64-channel blocks of the key product
@@ -255,7 +265,6 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
   const int it0 = min(i0, ng), it1 = min(i1, ng);
   const int dr0 = max(i0, ng) - ng, dr1 = max(i1, ng) - ng;
   auto group_of = [&](int it) { return it < nsg ? it : it - nsg + gw0; };
-  const int64_t o0 = ((int64_t)b * c.num_q_heads + (int64_t)hk * c.hq_per_kv) * a.nodes + row0;
 
   const float* sbase = c.k_scale + (int64_t)b * c.s_b + (int64_t)hk * c.s_h;
   const float* zbase = c.k_zp + (int64_t)b * c.s_b + (int64_t)hk * c.s_h;
@@ -270,16 +279,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
   unsigned v_full[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) v_full[i] = v_lane + (4 * grp + i) * vrow_b;
-  // (An absent table is read at element 0 of some valid array and the value dropped.)
-  const int32_t* table = c.page_table ? c.page_table + (int64_t)b * c.pt_b
-                                      : reinterpret_cast<const int32_t*>(c.k_scale);
-  const int table_mul = c.page_table ? 1 : 0;
+  const int32_t* table = c.page_table ? c.page_table + (int64_t)b * c.pt_b : nullptr;
 
   // ---- a step: CPS chunks of 16 rows of a group, for this wave ----
   const int spg = (cpg + CPS * kWaves - 1) / (CPS * kWaves);
   // The table entries are loaded with the metadata and first used a step later.
   struct Meta {
-    int entry[CPS], page[CPS], r0[CPS], nval[CPS], tok0[CPS];
+    int entry[CPS], r0[CPS], nval[CPS], tok0[CPS];
   };
   int li = it0, lp = 0;                            // item and step of the next metadata
   auto next_meta = [&]() __attribute__((always_inline)) -> Meta {
@@ -295,8 +301,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
       int nval = j < cpg && li < it1 ? min(min(16, c.page_rows - r0), n - tok0) : 0;
       // Behind the sinks and before every row's window.
       if (tok0 >= a.sinks && tok0 + nval <= low_min) nval = 0;
-      m.page[e] = min(page, c.max_pages - 1);
-      m.entry[e] = ld_ro(table, __builtin_amdgcn_readfirstlane(m.page[e] * table_mul));
+      const int at = __builtin_amdgcn_readfirstlane(min(page, c.max_pages - 1));
+      m.entry[e] = at;
+      if (table) m.entry[e] = ld_ro(table, at);
       m.r0[e] = r0;
       m.nval[e] = __builtin_amdgcn_readfirstlane(nval);
       m.tok0[e] = __builtin_amdgcn_readfirstlane(tok0);
@@ -308,7 +315,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
     return m;
   };
   auto phys_of = [&](const Meta& m, int e) __attribute__((always_inline)) -> uint64_t {
-    return (uint64_t)(unsigned)min(max(table_mul ? m.entry[e] : m.page[e], 0), c.num_pages - 1);
+    return (unsigned)__builtin_amdgcn_readfirstlane(
+        min(max(m.entry[e], 0), c.num_pages - 1));
   };
 
   // Rows past the valid count are loaded from the last valid row, a chunk of none from
@@ -322,7 +330,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
   auto load_keys = [&](const Meta& m, Keys& f) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < CPS; ++e) {
-      const uint8_t* kb = kbase + (phys_of(m, e) * (uint64_t)c.k_page +
+      const uint8_t* kb = kbase + (phys_of(m, e) * a.k_page_b +
                                    (uint64_t)(unsigned)m.r0[e] * krow_b);
       const unsigned ko = min(k_full, k_lane + (unsigned)max(m.nval[e] - 1, 0) * krow_b);
       constexpr int KL = G::KW < 4 ? G::KW : 4;
@@ -338,7 +346,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
 #pragma unroll
     for (int e = 0; e < CPS; ++e) {
       const unsigned v_last = v_lane + (unsigned)max(m.nval[e] - 1, 0) * vrow_b;
-      const uint8_t* vb = vbase + (phys_of(m, e) * (uint64_t)(c.v_page * G::VEB) +
+      const uint8_t* vb = vbase + (phys_of(m, e) * a.v_page_b +
                                    (uint64_t)(unsigned)m.r0[e] * vrow_b);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -355,58 +363,65 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
   };
 
   // ---- scales of a group to LDS, and the rows' digits ----
-  // Lane l < D / 4 of every wave holds the scales and zero-points of channels 4l ..
+  // Lane l holds the scales and zero-points of channels SL * l .. (SL = D / 64).
+  constexpr int SL = D / 64;
   struct Scales {
-    U32x4 s, z;
+    float s[SL], z[SL];
   };
   auto load_sz = [&](int it) __attribute__((always_inline)) -> Scales {
-    const uint64_t off = (uint64_t)(unsigned)group_of(min(it, it1 - 1)) * (uint64_t)c.s_g +
-                         4 * (lane % (D / 4));
-    return Scales{ld16(sbase + off), ld16(zbase + off)};
+    const uint64_t off = (uint64_t)(unsigned)group_of(min(it, it1 - 1)) * a.s_group + SL * lane;
+    struct alignas(4 * SL) Part {
+      float v[SL];
+    };
+    const Part s = *reinterpret_cast<const Part*>(sbase + off);
+    const Part z = *reinterpret_cast<const Part*>(zbase + off);
+    Scales r;
+#pragma unroll
+    for (int k = 0; k < SL; ++k) {
+      r.s[k] = s.v[k];
+      r.z[k] = z.v[k];
+    }
+    return r;
   };
   // The scales in units of 2^-30 (2^-22) of the largest, and zero-points times them.
   // (By wave `by`; powers of two, so that only the products with q round.)
   constexpr int kBits = WIDE ? 30 : 22;
   auto stage_sz = [&](const Scales& x, int buf, int by) __attribute__((always_inline)) {
     if (w != by) return;
-    unsigned mx = max(max(x.s.x & 0x7FFFFFFFu, x.s.y & 0x7FFFFFFFu),
-                      max(x.s.z & 0x7FFFFFFFu, x.s.w & 0x7FFFFFFFu));
+    unsigned mx = 0;
+#pragma unroll
+    for (int k = 0; k < SL; ++k) mx = max(mx, f2u(x.s[k]) & 0x7FFFFFFFu);
     mx = max(mx, xchg_u32<1>(mx));
     mx = max(mx, xchg_u32<2>(mx));
     mx = max(mx, xchg4(mx));
     mx = max(mx, xchg_u32<8>(mx));
-    if constexpr (D > 64) mx = max(mx, xchg_u32<16>(mx));
-    if constexpr (D > 128) mx = max(mx, xchg_u32<32>(mx));
+    mx = max(mx, xchg_u32<16>(mx));
+    mx = max(mx, xchg_u32<32>(mx));
     // All scales are below 2^kBits units. (An infinite or NaN one makes the rows NaN.)
     const unsigned ex = (max(mx, f2u(1e-28f)) >> 23) + 1 - kBits;
     const float inv = u2f((254 - ex) << 23);
     if (lane == 0) cs_s[buf] = mx >= 0x7F800000u ? u2f(0x7FC00000u) : u2f(ex << 23);
-    if (lane < D / 4) {
-      const float s0 = u2f(x.s.x) * inv, s1 = u2f(x.s.y) * inv, s2 = u2f(x.s.z) * inv,
-                  s3 = u2f(x.s.w) * inv;
-      float* dst = sz_s[buf] + sz_pos(row_slot(4 * lane));
-      *reinterpret_cast<float2*>(dst) = make_float2(s0, s2);
-      *reinterpret_cast<float2*>(dst + 4) = make_float2(s1, s3);
-      dst += kSz;
-      *reinterpret_cast<float2*>(dst) = make_float2(u2f(x.z.x) * s0, u2f(x.z.z) * s2);
-      *reinterpret_cast<float2*>(dst + 4) = make_float2(u2f(x.z.y) * s1, u2f(x.z.w) * s3);
+    float* dst = sz_s[buf];
+#pragma unroll
+    for (int k = 0; k < SL; ++k) {
+      const float v = x.s[k] * inv;
+      const int at = sz_pos(row_slot(SL * lane + k));
+      dst[at] = v;
+      dst[kSz + at] = x.z[k] * v;
     }
   };
   float qn[SPT], q_unit;                           // the row relative to its largest
   auto build = [&](int buf) __attribute__((always_inline)) {
     const float cs = cs_s[buf];
-    float4 sv[SPT / 4], zv[SPT / 4];
+    uint8_t* dst = smem + buf * G::kDig + brow * G::DS + part * SPT;
+    float cg[4] = {0.f, 0.f, 0.f, 0.f};
+    unsigned out[ND][SPT / 4];
+    static_assert(SPT == 4 || SPT == 8 || SPT == 16, "digit stores");
 #pragma unroll
     for (int i = 0; i < SPT; i += 4) {
       const float* src = sz_s[buf] + sz_pos(part * SPT + i);
-      sv[i / 4] = *reinterpret_cast<const float4*>(src);
-      zv[i / 4] = *reinterpret_cast<const float4*>(src + kSz);
-    }
-    uint8_t* dst = smem + buf * G::kDig + brow * G::DS + part * SPT;
-    float cg[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < SPT; i += 4) {
-      const float4 s4 = sv[i / 4], z4 = zv[i / 4];
+      const float4 s4 = *reinterpret_cast<const float4*>(src);
+      const float4 z4 = *reinterpret_cast<const float4*>(src + kSz);
       const float ss[4] = {s4.x, s4.y, s4.z, s4.w}, zz[4] = {z4.x, z4.y, z4.z, z4.w};
       unsigned x[4];
 #pragma unroll
@@ -430,8 +445,17 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
                         __builtin_amdgcn_perm(u1, t1, 0x07060302u)};
       if constexpr (WIDE) dg[2] ^= 0x80808080u;
 #pragma unroll
-      for (int k = 0; k < ND; ++k)
-        *reinterpret_cast<unsigned*>(dst + k * M * G::DS + i) = dg[k];
+      for (int k = 0; k < ND; ++k) out[k][i / 4] = dg[k];
+    }
+#pragma unroll
+    for (int k = 0; k < ND; ++k) {
+      uint8_t* o = dst + k * M * G::DS;
+      if constexpr (SPT == 16)
+        *reinterpret_cast<uint4*>(o) = make_uint4(out[k][0], out[k][1], out[k][2], out[k][3]);
+      else if constexpr (SPT == 8)
+        *reinterpret_cast<uint2*>(o) = make_uint2(out[k][0], out[k][1]);
+      else
+        *reinterpret_cast<unsigned*>(o) = out[k][0];
     }
     float cgs = (cg[0] + cg[1]) + (cg[2] + cg[3]);
     cgs += xchg<1>(cgs);
@@ -744,6 +768,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
     }
 
     // ---- drafts: 16 of them a wave and item, float32 products ----
+    const RowsArgs& a = late_args();
     for (int item = dr0; item < dr1; ++item) {
       const int j0 = (item * kWaves + w) * 16;
       const int nval = min(16, a.nodes - j0);
@@ -806,6 +831,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
   // The range again for every row by itself, a wave a row and key after key, for the
   // rare workgroup with a NaN: a key that a row does not see takes no part in it.
   auto plain_rows = [&]() {
+    const RowsArgs& a = late_args();
+    const DecodeArgs& c = a.c;
+    const float* sbase = c.k_scale + (int64_t)b * c.s_b + (int64_t)hk * c.s_h;
+    const float* zbase = c.k_zp + (int64_t)b * c.s_b + (int64_t)hk * c.s_h;
+    const uint8_t* kbase = c.k_pages + (int64_t)hk * c.k_head;
+    const int32_t* table = c.page_table ? c.page_table + (int64_t)b * c.pt_b : nullptr;
+    const int group_rows = c.pages_per_group * c.page_rows;
     constexpr int CH = D / 64;
     float* part0 = reinterpret_cast<float*>(smem);
     __syncthreads();
@@ -841,7 +873,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
         for (int t = g * group_rows; t < min((g + 1) * group_rows, n); ++t) {
           if (t >= a.sinks && t < low_s[r]) continue;
           const int lp = fdiv(t, c.div_rows), tr = t - lp * c.page_rows;
-          const int64_t phys = min(max(table_mul ? table[lp] : lp, 0), c.num_pages - 1);
+          const int64_t phys = min(max(table ? table[lp] : lp, 0), c.num_pages - 1);
           const uint8_t* kp = kbase + phys * c.k_page + (int64_t)tr * c.k_row;
           const int64_t vo = phys * c.v_page + (int64_t)hk * c.v_head + (int64_t)tr * c.v_row;
           float k[CH], v[CH];
@@ -909,6 +941,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
   __syncthreads();
   if (bad_s) plain_rows();
   const float* parts = reinterpret_cast<const float*>(smem);
+  const RowsArgs& za = late_args();
+  const DecodeArgs& zc = za.c;
+  const int64_t o0 =
+      ((int64_t)b * zc.num_q_heads + (int64_t)hk * zc.hq_per_kv) * za.nodes + row0;
   for (int idx = tid * 4; idx < live * D; idx += NT * 4) {
     const int r = idx / D, d = idx % D;
     float top = m_s[0][r];
@@ -925,17 +961,17 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
       o.z += x.z;
       o.w += x.w;
     }
-    if (c.final_out) {
+    if (zc.final_out) {
       const float os[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        store_elem(c.out, (o0 + r) * D + d + k, c.out_dtype, l == 0.f ? 0.f : os[k] / l);
+        store_elem(zc.out, (o0 + r) * D + d + k, zc.out_dtype, l == 0.f ? 0.f : os[k] / l);
     } else {
-      const int64_t pi = (o0 + r) * c.num_splits + split;
-      *reinterpret_cast<float4*>(c.ws_acc + pi * D + d) = o;
+      const int64_t pi = (o0 + r) * zc.num_splits + split;
+      *reinterpret_cast<float4*>(zc.ws_acc + pi * D + d) = o;
       if (d == 0) {
-        c.ws_ml[2 * pi] = l == 0.f ? -INFINITY : (double)top * 0.6931471805599453;
-        c.ws_ml[2 * pi + 1] = (double)l;
+        zc.ws_ml[2 * pi] = l == 0.f ? -INFINITY : (double)top * 0.6931471805599453;
+        zc.ws_ml[2 * pi + 1] = (double)l;
       }
     }
   }

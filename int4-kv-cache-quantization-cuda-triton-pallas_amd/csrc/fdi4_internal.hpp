@@ -162,6 +162,8 @@ struct RowsArgs {
   FastDiv div_group;                    // by the rows of a scale group
   FastDiv div_nodes, div_heads;         // by nodes, kv_heads
   int kv_heads;
+  uint32_t k_page_b, v_page_b;          // page strides, bytes
+  uint32_t s_group;                     // scale group stride, elements
   int q_vec;                            // query rows start on 16-byte boundaries
   int row_tiles;                        // 16-row tiles per workgroup
   int tiles;                            // workgroups for the rows of a kv-head
