@@ -7,9 +7,10 @@
 // and zeros behind the sequence's end. The arithmetic is that of
 // dequant_kernel (reference src/quantize_int4_ref.py:87-136).
 //
-// One workgroup per (scale group, kv-head, sequence): a thread owns eight channels,
-// whose scales it loads once, and walks the group's rows. Bound by memory: every
-// byte is read once and written once.
+// A workgroup takes up to RPS * kReadRows rows of one scale group of one (sequence,
+// kv-head): a thread owns eight channels, whose scales it loads once, of kReadRows
+// rows, all of whose loads are in flight together (page-table entries, then codes and
+// values). Bound by memory: every byte is read once and written once.
 
 #include "decode_common.hpp"
 
@@ -41,65 +42,94 @@ __device__ __forceinline__ void store8(uint8_t* p, const float* x) {
   }
 }
 
+constexpr int kReadRows = 4;
+
 template <int D, int VDT, int OUT>
 __global__ __launch_bounds__(kReadThreads) void read_paged_kernel(ReadArgs a, int slots,
-                                                                  int heads) {
+                                                                  int pieces, int heads) {
   constexpr int TPR = D / 8;                  // threads per row
   constexpr int RPS = kReadThreads / TPR;     // rows per sweep
+  constexpr int U = kReadRows;
   constexpr int VEB = VDT == kVF32 ? 4 : 2;
   constexpr int OEB = OUT == kEF32 ? 4 : 2;
+  constexpr int VL = VDT == kVF32 ? 2 : 1;    // 16-byte value loads per row
   const DecodeArgs& c = a.c;
-  const int slot = (int)(blockIdx.x % (unsigned)slots);
-  const int h = (int)(blockIdx.x / (unsigned)slots % (unsigned)heads);
-  const int b = (int)(blockIdx.x / ((unsigned)slots * (unsigned)heads));
+  unsigned wi = blockIdx.x;
+  const int piece = (int)(wi % (unsigned)pieces);
+  wi /= (unsigned)pieces;
+  const int slot = (int)(wi % (unsigned)slots);
+  wi /= (unsigned)slots;
+  const int h = (int)(wi % (unsigned)heads), b = (int)(wi / (unsigned)heads);
   const int cap = c.max_pages * c.page_rows;
   const int G = c.pages_per_group * c.page_rows;
   const int start = a.start ? min(max(a.start[b], 0), cap) : a.start0;
   const int T = seq_len_of(c, b);
-  // Rows of this slot: the part of its group within the range (64 bits: a range
+  // Rows of this workgroup: its piece of its group, within the range (64 bits: a range
   // may end anywhere), counted from the range's start.
   const int g = start / G + slot;
-  const int64_t g0 = (int64_t)g * G;
-  const int i0 = (int)max(g0 - start, (int64_t)0);
-  const int i1 = (int)min(g0 + G - start, (int64_t)a.length);
+  const int64_t p0 = (int64_t)g * G + (int64_t)piece * (RPS * U);
+  const int64_t p1 = min(p0 + RPS * U, (int64_t)(g + 1) * G);
+  const int i0 = (int)max(p0 - start, (int64_t)0);
+  const int i1 = (int)min(p1 - start, (int64_t)a.length);
+  if (i0 >= i1) return;
   const int tid = threadIdx.x, oct = tid % TPR, rsub = tid / TPR;
   uint8_t* ko = reinterpret_cast<uint8_t*>(a.k_out) +
                 ((int64_t)b * a.ko_b + (int64_t)h * a.ko_h + 8 * oct) * OEB;
   uint8_t* vo = reinterpret_cast<uint8_t*>(a.v_out) +
                 ((int64_t)b * a.vo_b + (int64_t)h * a.vo_h + 8 * oct) * OEB;
-  float s[8], zs[8];
-  if (g0 < T) {
-    const int64_t so = (int64_t)b * c.s_b + (int64_t)h * c.s_h + (int64_t)g * c.s_g + 8 * oct;
+  float k[8], v[8];
+  if (start + (int64_t)i0 >= T) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      s[k] = c.k_scale[so + k];
-      zs[k] = __fmul_rn(c.k_zp[so + k], s[k]);
+    for (int j = 0; j < 8; ++j) k[j] = 0.f;
+    for (int i = i0 + rsub; i < i1; i += RPS) {
+      store8<OUT>(ko + (int64_t)i * a.ko_t * OEB, k);
+      store8<OUT>(vo + (int64_t)i * a.vo_t * OEB, k);
     }
+    return;
   }
-  for (int i = i0 + rsub; i < i1; i += RPS) {
-    const int t = start + i;
-    float k[8], v[8];
-    if (t < T) {
-      const int lp = fdiv(t, c.div_rows), row = t - lp * c.page_rows;
-      const int pg = c.page_table ? c.page_table[(int64_t)b * c.pt_b + lp] : lp;
-      const int64_t phys = (int64_t)min(max(pg, 0), c.num_pages - 1);
-      const unsigned q = __builtin_nontemporal_load(reinterpret_cast<const unsigned*>(
-          c.k_pages + phys * c.k_page + (int64_t)h * c.k_head + (int64_t)row * c.k_row + 4 * oct));
-      const uint8_t* vp = reinterpret_cast<const uint8_t*>(c.v_pages) +
-                          (phys * c.v_page + (int64_t)h * c.v_head + (int64_t)row * c.v_row +
-                           8 * oct) * VEB;
-      if constexpr (VDT == kVF32) {
-        widen_values<VDT>(ld16_stream(vp), v);
-        widen_values<VDT>(ld16_stream(vp + 16), v + 4);
-      } else {
-        widen_values<VDT>(ld16_stream(vp), v);
-      }
+  // Rows past the range or the sequence load the last valid one.
+  const int last = min(start + i1, T) - 1;
+  unsigned q[U];
+  U32x4 x[U][VL];
+  int phys[U], row[U];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        k[j] = __fsub_rn(__fmul_rn((float)((q >> (4 * j)) & 15u), s[j]), zs[j]);
-    } else {
+  for (int u = 0; u < U; ++u) {
+    const int t = min(start + i0 + rsub + u * RPS, last);
+    const int lp = fdiv(t, c.div_rows);
+    row[u] = t - lp * c.page_rows;
+    phys[u] = c.page_table ? c.page_table[(int64_t)b * c.pt_b + lp] : lp;
+  }
+  float s[8], zs[8];
+  const int64_t so = (int64_t)b * c.s_b + (int64_t)h * c.s_h + (int64_t)g * c.s_g + 8 * oct;
+  widen_values<kVF32>(ld16(c.k_scale + so), s);
+  widen_values<kVF32>(ld16(c.k_scale + so + 4), s + 4);
+  widen_values<kVF32>(ld16(c.k_zp + so), zs);
+  widen_values<kVF32>(ld16(c.k_zp + so + 4), zs + 4);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) k[j] = v[j] = 0.f;
+  for (int u = 0; u < U; ++u) {
+    const int64_t p = min(max(phys[u], 0), c.num_pages - 1);
+    q[u] = __builtin_nontemporal_load(reinterpret_cast<const unsigned*>(
+        c.k_pages + p * c.k_page + (int64_t)h * c.k_head + (int64_t)row[u] * c.k_row + 4 * oct));
+    const uint8_t* vp = reinterpret_cast<const uint8_t*>(c.v_pages) +
+                        (p * c.v_page + (int64_t)h * c.v_head + (int64_t)row[u] * c.v_row +
+                         8 * oct) * VEB;
+#pragma unroll
+    for (int i = 0; i < VL; ++i) x[u][i] = ld16_stream(vp + 16 * i);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) zs[j] = __fmul_rn(zs[j], s[j]);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = i0 + rsub + u * RPS;
+    if (i >= i1) continue;
+    const bool there = start + i < T;
+#pragma unroll
+    for (int w = 0; w < VL; ++w) widen_values<VDT>(x[u][w], v + w * 4);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      k[j] = __fsub_rn(__fmul_rn((float)((q[u] >> (4 * j)) & 15u), s[j]), zs[j]);
+      k[j] = there ? k[j] : 0.f;
+      v[j] = there ? v[j] : 0.f;
     }
     store8<OUT>(ko + (int64_t)i * a.ko_t * OEB, k);
     store8<OUT>(vo + (int64_t)i * a.vo_t * OEB, v);
@@ -110,14 +140,18 @@ hipError_t launch_read_paged(const ReadArgs& a, int D, int v_dtype, int batch, i
                              hipStream_t st) {
   if (batch == 0 || heads == 0 || a.length == 0) return hipSuccess;
   const int64_t G = (int64_t)a.c.pages_per_group * a.c.page_rows;
-  // Groups that a range of this length touches from any start.
-  const int64_t slots = (a.length + 2 * G - 2) / G;
-  const int64_t items = slots * heads * batch;
+  const int per = kReadThreads / (D / 8) * kReadRows;
+  // Groups that a range of this length touches from any start (all of them from this
+  // one), and workgroups for a group's rows (no more than the range needs).
+  const int64_t slots = a.start ? (a.length + 2 * G - 2) / G
+                                : (a.start0 + (int64_t)a.length - 1) / G - a.start0 / G + 1;
+  const int64_t pieces = (G + per - 1) / per;
+  const int64_t items = slots * pieces * heads * batch;
   if (items > INT32_MAX) return hipErrorInvalidValue;
 #define FDI4_RD(DD, VV, OO)                                                               \
   if (D == DD && v_dtype == VV && a.out_dtype == OO) {                                    \
     hipLaunchKernelGGL((read_paged_kernel<DD, VV, OO>), dim3((unsigned)items),            \
-                       dim3(kReadThreads), 0, st, a, (int)slots, heads);                  \
+                       dim3(kReadThreads), 0, st, a, (int)slots, (int)pieces, heads);     \
     return hipGetLastError();                                                             \
   }
 #define FDI4_RD_O(DD, VV) FDI4_RD(DD, VV, kEF32) FDI4_RD(DD, VV, kEF16) FDI4_RD(DD, VV, kEBF16)
