@@ -153,7 +153,8 @@ __device__ __forceinline__ float over_groups_sum(float x) {
 template <int D, int VDT, int RT, bool WIDE, bool STREAM>
 __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a) {
   constexpr int ND = WIDE ? 4 : 3;
-  constexpr int TERMS = WIDE && VDT == kVBF16 ? 3 : 2;   // 16-bit terms of a probability
+  // 16-bit terms of a probability.
+  constexpr int TERMS = VDT == kVF32 || (WIDE && VDT == kVBF16) ? 3 : 2;
   using G = RowsGeo<D, VDT, RT, ND>;
   constexpr int NB = G::NB, CPS = G::CPS, NA = G::NA, M = G::M, NT = G::NT;
   constexpr int TPR = G::TPR, SPT = G::SPT, NS = 4 * CPS;
@@ -482,8 +483,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
     for (int t = 0; t < NA; ++t) acc[rt][t] = v4f{0.f, 0.f, 0.f, 0.f};
   }
   // Probabilities of a step as the value product's operands.
-  constexpr int PW = VDT == kVF32 ? 4 : 4 * TERMS;
-  unsigned pr[RT][PW];
+  constexpr int PW = NS / 2;                       // registers per term
+  unsigned pr[RT][PW * TERMS];
 
   // Row tile rt and scores s (logit = s * c1 - cc, log2 units, c1 >= 0) of keys
   // 4 grp + i of chunk e in s[4 e + i], of which, if masked, those in vis are seen.
@@ -519,38 +520,34 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
 #pragma unroll
       for (int k = 0; k < NS; ++k) p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], c1, sub));
     }
-    if constexpr (VDT == kVF32) {
+    if constexpr (VDT == kVF32) l_run[rt][0] += (p[0] + p[1]) + (p[2] + p[3]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        pr[rt][k] = f2u(p[k]);
-        l_run[rt][0] += p[k];
-      }
-    } else {
+    for (int h = 0; h < PW; ++h) {
+      float y0 = p[2 * h], y1 = p[2 * h + 1];
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        float y0 = p[2 * h], y1 = p[2 * h + 1];
-#pragma unroll
-        for (int q = 0; q < TERMS; ++q) {
-          if constexpr (VDT == kVF16) {
-            const float h0 = q == TERMS - 1 ? y0 : u2f(f2u(y0) & 0xFFFFE000u);
-            const float h1 = q == TERMS - 1 ? y1 : u2f(f2u(y1) & 0xFFFFE000u);
-            pr[rt][4 * q + h] =
-                __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(h0, h1));
-            y0 -= h0;
-            y1 -= h1;
-          } else {
-            const unsigned r =
-                __builtin_bit_cast(unsigned, __builtin_convertvector(v2f{y0, y1}, v2bf));
-            pr[rt][4 * q + h] = r;
-            y0 -= u2f(r << 16);
-            y1 -= u2f(r & 0xFFFF0000u);
-          }
+      for (int q = 0; q < TERMS; ++q) {
+        if constexpr (VDT == kVF16) {
+          const float h0 = q == TERMS - 1 ? y0 : u2f(f2u(y0) & 0xFFFFE000u);
+          const float h1 = q == TERMS - 1 ? y1 : u2f(f2u(y1) & 0xFFFFE000u);
+          pr[rt][PW * q + h] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(h0, h1));
+          y0 -= h0;
+          y1 -= h1;
+        } else {
+          const unsigned r =
+              __builtin_bit_cast(unsigned, __builtin_convertvector(v2f{y0, y1}, v2bf));
+          pr[rt][PW * q + h] = r;
+          y0 -= u2f(r << 16);
+          y1 -= u2f(r & 0xFFFF0000u);
         }
       }
     }
   };
 
   auto prob = [&](int rt, int q) __attribute__((always_inline)) -> uint4 {
+    // (float32 values: terms 0 twice, 1 twice, then 0 and 2.)
+    if constexpr (VDT == kVF32)
+      return make_uint4(pr[rt][q % 2 * 2], pr[rt][q % 2 * 2 + 1], pr[rt][q * 2 % 6],
+                        pr[rt][q * 2 % 6 + 1]);
     return make_uint4(pr[rt][4 * q], pr[rt][4 * q + 1], pr[rt][4 * q + 2], pr[rt][4 * q + 3]);
   };
   auto product = [](uint4 x, uint4 y, v4f o) __attribute__((always_inline)) -> v4f {
@@ -573,12 +570,25 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
     for (int t = 0; t < NA; ++t) {
       const int u = t / G::CPP, j = t % G::CPP;
       if constexpr (VDT == kVF32) {
+        // A value is three bfloat16 terms of eight bits (cut off, so exactly), and of the
+        // nine products with those of p the six above 2^-24 count, two a product of 32.
+        unsigned x[4], tm[3][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) x[i] = f.w[0][i][u][j];
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+          tm[q][0] = __builtin_amdgcn_perm(x[1], x[0], 0x07060302u);
+          tm[q][1] = __builtin_amdgcn_perm(x[3], x[2], 0x07060302u);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = f2u(u2f(x[i]) - u2f(x[i] & 0xFFFF0000u));
+        }
+        const uint4 hi = make_uint4(tm[0][0], tm[0][1], tm[1][0], tm[1][1]);
+        const uint4 lo = make_uint4(tm[2][0], tm[2][1], tm[0][0], tm[0][1]);
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
-            acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                u2f(f.w[0][i][u][j]), u2f(pr[rt][i]), acc[rt][t], 0, 0, 0);
+            acc[rt][t] = product(q < 2 ? hi : lo, prob(rt, q), acc[rt][t]);
       } else {
         const unsigned sel = j & 1 ? 0x07060302u : 0x05040100u;
         const uint4 av =
@@ -937,7 +947,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
         }
       }
   }
-  if (!(any_nan == any_nan)) bad_s = 1;
+  if (!(any_nan - any_nan == 0.f)) bad_s = 1;      // (NaN, or beyond float32)
   __syncthreads();
   if (bad_s) plain_rows();
   const float* parts = reinterpret_cast<const float*>(smem);
