@@ -428,9 +428,12 @@ size_t fdi4_decode_rows_workspace_bytes(int batch, int num_q_heads, int nodes, i
  * sinks >= 0. Only the pages of those rows are read. The cache has group-indexed
  * scales (s_page_stride 0) and no page_lens. out is contiguous [batch,
  * num_q_heads, head_dim]; a sequence with no row gives zeros. lens_out as in
- * fdi4_decode_paged_advance, or NULL. float32 logits from
- * queries times scales held to 23 bits of their largest, probabilities and sums in
- * 24 bits or more (16 against 16-bit values that are rounded to 8 on output). */
+ * fdi4_decode_paged_advance, or NULL. float32 outputs:
+ * logits from queries times scales held to 29 bits of a group's largest, probabilities
+ * to 22 bits or more; 16-bit outputs: 21 and 16 bits; sums in float32. Refused besides
+ * what fdi4_decode_paged_ex refuses: more than 2^30 rows a sequence (max_pages *
+ * page_rows), and page or scale-group strides that are negative or do not fit 32 bits
+ * (bytes, scales in elements); pools may be larger than that. */
 int fdi4_decode_window(const void* query, int query_dtype, int batch, int num_q_heads,
                        int64_t q_batch_stride, int64_t q_head_stride,
                        const fdi4_paged_cache* cache, int window, int sinks, void* out,
@@ -448,7 +451,7 @@ int fdi4_decode_window(const void* query, int query_dtype, int batch, int num_q_
  * drafts, attends the cached rows t < sinks and t >= n + d_i - window: the last
  * `window` tokens of the sequence that it ends. out is contiguous [batch,
  * num_q_heads, nodes, head_dim]; a node that sees no row and no draft gives zeros.
- * The accepted drafts go to the cache with fdi4_extend_paged. */
+ * Precision and refusals are fdi4_decode_window's. The accepted drafts go to the cache with fdi4_extend_paged. */
 int fdi4_decode_tree(const void* query, int query_dtype, int batch, int num_q_heads, int nodes,
                      int64_t q_batch_stride, int64_t q_head_stride, int64_t q_node_stride,
                      const float* k_draft, int64_t kd_batch_stride, int64_t kd_head_stride,

@@ -915,6 +915,8 @@ RowsPlan plan_rows(int batch, int num_q_heads, int nodes, int window, int sinks,
   if (nodes > 1) items += (nodes + 63) / 64;
   items = std::max<int64_t>(items, 1);
   const int64_t streams = (int64_t)batch * cache->num_kv_heads * p.tiles;
+  // (Two workgroups fit a CU. 128 streams at 8192 tokens and 64 rows: 68 us with 4
+  // splits, 80 with 3, 83 with 5; 64 of 16 rows: 37 us with 4, 45 with 2, 43 with 8.)
   const int64_t slots = 2 * kCUs;
   const int64_t s = num_splits > 0 ? num_splits : slots / std::max<int64_t>(streams, 1);
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(s, items), kMaxSplits));

@@ -11,20 +11,25 @@
 //
 // A workgroup of four waves serves RT tiles of 16 rows of one kv-head over a range of
 // scale groups (and drafts, 64 an item, at the range's end). Its 16-row chunks of keys
-// go to the waves in turn, so the cache is read once for all rows, straight to
+// go to the waves in turn, so the cache is read once for all its rows, straight to
 // registers; the waves meet at the end, in LDS, and splits in the merge kernel.
 //
-//   digits: q . k_t = sum_d v_d (nib_td - zp_d), v = q*s. Per group and row, v is taken
-//      relative to the largest |q| of the row and the largest s of the group, as a
-//      32-bit integer |v| < 2^30 in four balanced base-256 digits; one product and
-//      one conversion per element, shared by the 128 keys of the group, where
-//      dequantized keys would need three 8-bit terms against three of the query.
-//      v_mfma_i32_16x16x64_i8 multiplies the nibbles of 16 keys (A) by a digit of 16
-//      rows (B); the digits' exact sums meet in float32 (28 bits of each pair), and
-//      the constant sum_d v_d zp_d, in float32, goes in with the exponent's FMA. A
-//      logit is off by what float32 products of q and k would be.
-//      The digits are built by the whole workgroup for the next group while the
-//      present one is multiplied (two LDS buffers, one barrier a group).
+//   digits: q . k_t = sum_d v_d (nib_td - zp_d), v = q*s. Per group and row, v is an
+//      integer in units of (the row's largest |q|) * (a power of two), the units of its
+//      largest possible v: below 2^22 in three balanced base-256 digits, or (WIDE:
+//      float32 outputs) below 2^30 in four. One product and one conversion per element,
+//      shared by the 128 keys of the group, where dequantized keys would need three
+//      8-bit terms against three of the query. v_mfma_i32_16x16x64_i8 multiplies the
+//      nibbles of 16 keys (A) by a digit of 16 rows (B); the digits' exact sums meet in
+//      float32, and the constant sum_d v_d zp_d, in float32, goes in with the exponent's
+//      FMA. Four digits are as good as float32 products of q and k; three leave a logit
+//      off by sum_d e_d nib_td units, |e_d| <= 1/2: over 128 channels 2^-16 of the largest
+//      product q*s in the root mean square, 2^-11 were all errors of one sign, where a
+//      16-bit output resolves 2^-8 or 2^-11 of a probability's share. The
+//      digits are built by the whole workgroup for the next group while the present one
+//      is multiplied (two LDS buffers, one barrier a group). Two float16 terms of v
+//      against nibbles read as float16's smallest numbers need a quarter less VALU work
+//      and took the same time: 72 us either way at the 64 rows below.
 //   softmax: lane (g, r) of a wave holds the logits of row r with keys 4g .. 4g+3, and
 //      the value product wants its B operand in the same lanes, so probabilities never
 //      leave their registers. The shift is a whole number that moves only when a logit
@@ -33,11 +38,31 @@
 //   values: lane (g, r) loads the channels 8r.. of rows 4g .. 4g+3, byte permutes pair
 //      the rows, and one product takes 32 keys. A probability is the sum of two
 //      (float16: 22 bits; bfloat16: 16) or three (bfloat16 values, float32 output:
-//      24) terms. float32 values: v_mfma_f32_16x16x4_f32.
+//      24) terms. float32 values are three bfloat16 terms like it: 58 us, where
+//      v_mfma_f32_16x16x4_f32 took 68 (100 drafts of four sequences of up to 3000
+//      tokens).
 //
 // A non-finite value times a probability of zero is NaN, though the row does not see
 // it: a workgroup that ends with a NaN goes through its range again, row by row and key
-// by key (rare, slow).
+// by key.
+//
+// What bounds it. Up to 32 rows a kv-head: memory. 8 sequences of 8 kv-heads with 128
+// bfloat16 channels and 16 rows read their tokens at 6.8 TB/s once they are many, on top
+// of 11 us (launch, the first loads' chain, the waves' and the splits' merges): 37 us at
+// 8192 tokens, 62 us at 16384, 5.5 TB/s in all. More rows: each further workgroup of 32
+// rows takes its keys again, from L2, and the time follows the rows: 126 us for 64 rows
+// at 16384 tokens, 221 us for 128, of which 115 and 203 us remain where all pages lie in
+// L2. A step (32 keys by 32 rows, a wave) takes about 7300 cycles, two waves a SIMD,
+// with the VALU busy for half of them, the matrix cores for a quarter, and the rest
+// waits for LDS, dependent results and the barrier.
+//
+// RT: one tile up to 16 rows (and at 256 channels, whose accumulators fill the registers
+// with one), two beyond: 32 rows in one workgroup read the cache once (75 us at 16384
+// tokens, 62 us for 16 rows). Four tiles in one workgroup of eight waves were slower
+// than two workgroups of two: one barrier for all of them.
+// STREAM: non-temporal loads where one workgroup reads a page, cached ones where the
+// workgroups of several tiles do, which run on one XCD one after the other.
+// Splits: as many as fill the chip twice over with workgroups (two fit a CU).
 
 #include "decode_common.hpp"
 
@@ -839,7 +864,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
   }
 
   // The range again for every row by itself, a wave a row and key after key, for the
-  // rare workgroup with a NaN: a key that a row does not see takes no part in it.
+  // rare workgroup with a NaN or an overflow: a key that a row does not see takes no
+  // part in it. (Masking the values of every product instead costs each step what this
+  // costs such a workgroup alone.)
   auto plain_rows = [&]() {
     const RowsArgs& a = late_args();
     const DecodeArgs& c = a.c;

@@ -10,7 +10,10 @@
 // A workgroup takes up to RPS * kReadRows rows of one scale group of one (sequence,
 // kv-head): a thread owns eight channels, whose scales it loads once, of kReadRows
 // rows, all of whose loads are in flight together (page-table entries, then codes and
-// values). Bound by memory: every byte is read once and written once.
+// values). Bound by memory: every byte is read once and written once, 5.4 TB/s over 440
+// MB of bfloat16 (81 us; a copy of 256 MB runs at 5.5). One row a thread at a time, and
+// a workgroup for the whole group, took 85 us there, 31 us against 25 for 1000 tokens
+// of 8 sequences (85 MB, to float32) and 15 against 10 for 16 sequences' open groups.
 
 #include "decode_common.hpp"
 
@@ -88,13 +91,15 @@ __global__ __launch_bounds__(kReadThreads) void read_paged_kernel(ReadArgs a, in
     return;
   }
   // Rows past the range or the sequence load the last valid one.
-  const int last = min(start + i1, T) - 1;
+  // (Sums of positions as unsigned: a capacity may be any 31-bit number.)
+  const unsigned s0 = (unsigned)start;
+  const unsigned last = min(s0 + (unsigned)i1, (unsigned)T) - 1;
   unsigned q[U];
   U32x4 x[U][VL];
   int phys[U], row[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int t = min(start + i0 + rsub + u * RPS, last);
+    const int t = (int)min(s0 + (unsigned)(i0 + rsub + u * RPS), last);
     const int lp = fdiv(t, c.div_rows);
     row[u] = t - lp * c.page_rows;
     phys[u] = c.page_table ? c.page_table[(int64_t)b * c.pt_b + lp] : lp;
@@ -122,7 +127,7 @@ __global__ __launch_bounds__(kReadThreads) void read_paged_kernel(ReadArgs a, in
   for (int u = 0; u < U; ++u) {
     const int i = i0 + rsub + u * RPS;
     if (i >= i1) continue;
-    const bool there = start + i < T;
+    const bool there = s0 + (unsigned)i < (unsigned)T;
 #pragma unroll
     for (int w = 0; w < VL; ++w) widen_values<VDT>(x[u][w], v + w * 4);
 #pragma unroll
