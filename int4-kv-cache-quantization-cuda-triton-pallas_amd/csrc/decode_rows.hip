@@ -251,7 +251,14 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
       const int R = row0 + min(brow, live - 1), node = R - fdiv(R, a.div_nodes) * a.nodes;
       const uint8_t* mk = a.mask + (int64_t)b * a.mk_b + (int64_t)node * a.mk_i;
       int mine = 0;
-      for (int j = part; j < a.nodes; j += TPR) mine += mk[j] != 0;
+      // (Eight in flight: one wait for memory up to 8 * TPR nodes.)
+      for (int j0 = part; j0 < a.nodes; j0 += 8 * TPR) {
+        uint8_t x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = mk[min(j0 + k * TPR, a.nodes - 1)];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mine += (x[k] != 0) & (j0 + k * TPR < a.nodes);
+      }
       mine += (int)xchg_u32<1>((unsigned)mine);
       mine += (int)xchg_u32<2>((unsigned)mine);
       if constexpr (TPR > 4) mine += (int)xchg_u32<4>((unsigned)mine);
@@ -803,6 +810,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
     }
 
     // ---- drafts: 16 of them a wave and item, float32 products ----
+    // (All of an item's loads are in flight before its first product: one wait for
+    // memory an item, at the end of a workgroup's chain.)
     const RowsArgs& a = late_args();
     for (int item = dr0; item < dr1; ++item) {
       const int j0 = (item * kWaves + w) * 16;
@@ -824,12 +833,25 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
           }
       const float* kd = a.kd + (int64_t)b * a.kd_b + (int64_t)hk * a.kd_h +
                         (int64_t)(j0 + min(n16, nval - 1)) * a.kd_n + grp * (D / 4);
+      float4 kx[D / 16];
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) kx[d] = *reinterpret_cast<const float4*>(kd + 4 * d);
+      uint8_t mb[RT][4];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int R = row0 + min(rt * 16 + n16, live - 1);
+        const int node = R - fdiv(R, a.div_nodes) * a.nodes;
+        const uint8_t* mk = a.mask + (int64_t)b * a.mk_b + (int64_t)node * a.mk_i + j0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mb[rt][k] = mk[min(4 * grp + k, nval - 1)];
+      }
+      __builtin_amdgcn_sched_barrier(0);
       v4f ds[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) ds[rt] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+#pragma unroll
       for (int d = 0; d < D / 4; d += 4) {
-        const float4 k4 = *reinterpret_cast<const float4*>(kd + d);
+        const float4 k4 = kx[d / 4];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           const float4 q4 = *reinterpret_cast<const float4*>(
@@ -842,17 +864,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
       }
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const int R = row0 + min(rt * 16 + n16, live - 1);
-        const int node = R - fdiv(R, a.div_nodes) * a.nodes;
-        const uint8_t* mk = a.mask + (int64_t)b * a.mk_b + (int64_t)node * a.mk_i + j0;
         unsigned vis = 0;
         float s[NS];
 #pragma unroll
         for (int k = 0; k < NS; ++k) s[k] = kLeast;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int r = 4 * grp + k;
-          vis |= (unsigned)((mk[min(r, nval - 1)] != 0) & (r < nval)) << k;
+          vis |= (unsigned)((mb[rt][k] != 0) & (4 * grp + k < nval)) << k;
           s[k] = ds[rt][k];
         }
         softmax(rt, s, kLog2e, 0.f, true, vis);
