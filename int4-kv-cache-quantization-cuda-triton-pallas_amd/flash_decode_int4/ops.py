@@ -24,6 +24,7 @@ sequence into it), ``dequantize_int4_paged`` (and out of it) and
 ``pack_int4_device``.
 """
 
+import operator
 from typing import List, Optional, Tuple
 
 import numpy as np
@@ -379,13 +380,14 @@ def flash_decode_paged(query, k_pages, v_pages, k_scale, k_zp, page_table, seq_l
 
 
 def _check_window(window: Optional[int], sinks: int, least: int = 1) -> None:
+    most = 2 ** 31 - 1
     if window is None:
         if sinks:
             raise ValueError("sinks need a window")
-    elif window < least:
-        raise ValueError(f"window must be at least {least}, got {window}")
-    if sinks < 0:
-        raise ValueError(f"sinks must not be negative, got {sinks}")
+    elif not least <= operator.index(window) <= most:
+        raise ValueError(f"window must be at least {least} and fit 32 bits, got {window}")
+    if not 0 <= operator.index(sinks) <= most:
+        raise ValueError(f"sinks must not be negative and fit 32 bits, got {sinks}")
 
 
 def flash_decode_paged_tree(query, k_draft, v_draft, mask, k_pages, v_pages, k_scale, k_zp,

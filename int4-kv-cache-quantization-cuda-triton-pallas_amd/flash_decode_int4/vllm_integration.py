@@ -24,6 +24,7 @@ packed size of the rows written), so code written against the reference's
 dicts keeps working.
 """
 
+import operator
 from typing import List
 
 import numpy as np
@@ -487,6 +488,9 @@ class INT4PagedSequenceCache:
             if index.dim() != 2 or tuple(index.shape) != (B, N):
                 raise ValueError("index must be [batch, tokens]")
             if not index.is_cuda:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("extend() with a host index cannot be captured into a "
+                                       "graph")
                 taken = torch.arange(N)[None] < torch.from_numpy(n)[:, None] if n is not None \
                     else torch.ones(B, N, dtype=torch.bool)
                 if ((index < 0) | (index >= N))[taken].any():
@@ -543,6 +547,15 @@ class INT4PagedSequenceCache:
         if len(short):
             raise RuntimeError(f"step() would write past the pages reserved for sequence "
                                f"{int(short[0])}; call reserve() first")
+        if window is not None:
+            import torch
+            # (Refused here, what the attention would refuse with the token appended.)
+            if query.dim() != 3 or query.shape[0] != B or query.shape[2] != self.head_dim or \
+                    query.shape[1] < 1 or query.shape[1] % self.num_kv_heads or \
+                    query.stride(2) != 1 or query.device != self.k_pages.device or \
+                    query.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+                raise ValueError("query must be float32, float16 or bfloat16 [batch, heads, "
+                                 "head_dim] on the cache's GPU, heads a multiple of kv_heads")
         self._unsynced_steps += 1
         if window is not None:
             C = load_binding()
@@ -614,11 +627,13 @@ class INT4PagedSequenceCache:
         of dtype (float32 by default): dequantized keys, stored values, zeros behind a
         sequence's end. start: an int, or int32 [batch] on the GPU (then length is
         needed)."""
+        import torch
         if not 0 <= batch <= self.max_seqs:
             raise ValueError(f"batch must lie in 0 .. {self.max_seqs}")
         if length is None:
-            if not isinstance(start, int):
+            if isinstance(start, torch.Tensor):
                 raise ValueError("length is needed with a start per sequence")
+            start = operator.index(start)
             self._sync_if_stepped()
             length = max(0, int(self._lens[:batch].max(initial=0)) - start)
         return ops.dequantize_int4_paged(

@@ -123,3 +123,24 @@ def test_python_arguments_refused():
         ops._check_window(7, 0, 8)
     ops._check_window(None, 0)
     ops._check_window(8, 100, 8)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(max_pages=(1 << 26) + 1), dict(k_page_stride=1 << 32), dict(k_page_stride=-1024),
+    dict(v_page_stride=1 << 31), dict(v_page_stride=-1024), dict(s_group_stride=1 << 32),
+    dict(s_group_stride=-128)],
+    ids=lambda d: "-".join(f"{k}={v}" for k, v in d.items()))
+def test_sizes_beyond_the_attentions_32_bits_refused(bad):
+    c = cache(**bad)
+    assert window(c) == INVALID
+    assert tree(c) == INVALID
+
+
+def test_python_windows_beyond_32_bits_refused():
+    from flash_decode_int4 import ops
+    for args in ((2 ** 31, 0), (8, 2 ** 31)):
+        with pytest.raises(ValueError):
+            ops._check_window(*args)
+    for args in ((8.5, 0), (8, 1.0)):
+        with pytest.raises(TypeError):
+            ops._check_window(*args)
