@@ -99,6 +99,13 @@ def _require_device(use_cuda: Optional[bool]) -> None:
                            "is False)")
 
 
+def _require_device_of(tensor) -> None:
+    """_require_device for a call on GPU tensors: one of them shows that there is a GPU
+    (asking the runtime takes 0.7 us of a 7 us call)."""
+    if not getattr(tensor, "is_cuda", False):
+        _require_device(None)
+
+
 def _sync(_out=None) -> None:
     torch.cuda.synchronize()
 
@@ -361,7 +368,7 @@ def flash_decode_paged(query, k_pages, v_pages, k_scale, k_zp, page_table, seq_l
     are not read. It needs seq_lens and the grouped scales, not page_lens.
     """
     _check_window(window, sinks)
-    _require_device(None)
+    _require_device_of(query)
     page_rows = k_pages.shape[2]
     if group_rows % page_rows:
         raise ValueError("group_rows must be a multiple of the page size")
@@ -416,7 +423,7 @@ def flash_decode_paged_tree(query, k_draft, v_draft, mask, k_pages, v_pages, k_s
         raise ValueError(f"query must be [batch, heads, nodes, head_dim], got "
                          f"{tuple(query.shape)}")
     _check_window(window, sinks, query.shape[2])
-    _require_device(None)
+    _require_device_of(query)
     page_rows = k_pages.shape[2]
     if group_rows % page_rows:
         raise ValueError("group_rows must be a multiple of the page size")
@@ -445,7 +452,7 @@ def extend_int4_paged(k_new, v_new, counts, k_stage, k_pages, v_pages, k_scale, 
     left for the caller to advance. A count that does not fit the pages mapped by
     page_table's columns takes nothing.
     """
-    _require_device(None)
+    _require_device_of(k_new)
     load_binding().extend_paged(k_new, v_new, counts, k_stage, k_pages, v_pages, k_scale, k_zp,
                                 page_table, seq_lens, lens_next, group_rows, index)
 
@@ -460,7 +467,7 @@ def dequantize_int4_paged(k_pages, v_pages, k_scale, k_zp, page_table, seq_lens,
     ``q*scale - zp*scale`` as ``dequantize_int4`` computes them, rounded once; values
     converted; zeros behind a sequence's end.
     """
-    _require_device(None)
+    _require_device_of(k_pages)
     page_rows = k_pages.shape[2]
     if group_rows % page_rows:
         raise ValueError("group_rows must be a multiple of the page size")
