@@ -238,3 +238,50 @@ def test_a_host_index_is_not_captured():
         graph.replay()
         torch.cuda.synchronize()
         assert cache.seq_lens.tolist() == [before[0] + 2 * (i + 1), before[1] + i + 1]
+
+
+@pytest.mark.parametrize("values,query,bits", [("float16", "float16", 21),
+                                               ("bfloat16", "bfloat16", 21),
+                                               ("float32", "float32", 29),
+                                               ("bfloat16", "float32", 29)])
+def test_outlier_channels(values, query, bits):
+    """One channel of large queries and another of large key scales, the worst for
+    products held relative to the largest of both. Such a product is off by at most half
+    a unit U = 2^-bits max|q| max s (the units are powers of two, so one bit of 22 or 30
+    goes), evenly spread: over D nibbles of up to 15 a logit's error has a standard
+    deviation below U sqrt(D / 12) 15; six of them and the float32 steps of the logit and
+    its constant (8 half steps of A, the largest sum |q| s (15 + |zp|)) bound it, twice
+    that times the largest value the output's; the rest is the rounding of the
+    probabilities (2^-17 at least) and of the output."""
+    import torch
+    c, t = case(8, values=values, N=5)
+    dt = getattr(torch, query)
+    c["s"][..., 17] *= 15
+    c["z"][..., 17] = 7.5
+    q = t["q"].float() * 0.3
+    q[..., 90] *= 30
+    t["q"] = q.to(dt)
+    from flash_decode_int4 import ops
+    out = ops.flash_decode_paged_tree(t["q"], t["kd"], t["vd"], t["m"], *args(c))
+    worst = 0.0
+    for b, n in enumerate(c["lens"].tolist()):
+        pages = c["table"][b].long()
+        raw = c["kp"][pages].permute(1, 0, 2, 3).reshape(2, -1, D // 2)[:, :n]
+        nib = torch.stack([raw & 15, raw >> 4], -1).reshape(2, n, D).double()
+        g = torch.arange(n, device="cuda") // G
+        k = (nib - c["z"][b].double()[:, g]) * c["s"][b].double()[:, g]
+        v = c["v"][pages].permute(1, 0, 2, 3).reshape(2, -1, D)[:, :n].double()
+        k = torch.cat([k, t["kd"][b].double()], 1).repeat_interleave(4, 0).contiguous()
+        v = torch.cat([v, t["vd"][b].double()], 1).repeat_interleave(4, 0).contiguous()
+        x = torch.stack([t["q"][b, h].double() @ k[h].t().contiguous() for h in range(8)])
+        x[:, :, n:].masked_fill_(~t["m"], float("-inf"))
+        want = torch.softmax(x, -1) @ v
+        worst = max(worst, (out[b].double() - want).abs().max().item())
+        vmax = v.abs().max().item()
+    qa, s = t["q"].double().abs(), c["s"].double()
+    U = 2.0 ** -bits * qa.max().item() * s.max().item()
+    A = (qa @ (s * (15 + c["z"].double().abs())).amax((0, 1, 2))).max().item()
+    logit = 6 * 15 * (D / 12) ** 0.5 * U + 8 * 2.0 ** -24 * A
+    half = torch.finfo(dt).eps / 2
+    p = 2.0 ** -17 if query == "bfloat16" else 2.0 ** -22
+    assert worst <= (2 * logit + p + half) * max(vmax, 5), (worst, logit)
