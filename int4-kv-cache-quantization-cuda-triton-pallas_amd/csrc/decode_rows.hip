@@ -14,22 +14,25 @@
 // go to the waves in turn, so the cache is read once for all its rows, straight to
 // registers; the waves meet at the end, in LDS, and splits in the merge kernel.
 //
-//   digits: q . k_t = sum_d v_d (nib_td - zp_d), v = q*s. Per group and row, v is an
-//      integer in units of (the row's largest |q|) * (a power of two), the units of its
-//      largest possible v: below 2^22 in three balanced base-256 digits, or (WIDE:
-//      float32 outputs) below 2^30 in four. One product and one conversion per element,
-//      shared by the 128 keys of the group, where dequantized keys would need three
-//      8-bit terms against three of the query. v_mfma_i32_16x16x64_i8 multiplies the
-//      nibbles of 16 keys (A) by a digit of 16 rows (B); the digits' exact sums meet in
-//      float32, and the constant sum_d v_d zp_d, in float32, goes in with the exponent's
-//      FMA. Four digits are as good as float32 products of q and k; three leave a logit
-//      off by sum_d e_d nib_td units, |e_d| <= 1/2: over 128 channels 2^-16 of the largest
-//      product q*s in the root mean square, 2^-11 were all errors of one sign, where a
-//      16-bit output resolves 2^-8 or 2^-11 of a probability's share. The
-//      digits are built by the whole workgroup for the next group while the present one
-//      is multiplied (two LDS buffers, one barrier a group). Two float16 terms of v
-//      against nibbles read as float16's smallest numbers need a quarter less VALU work
-//      and took the same time: 72 us either way at the 64 rows below.
+//   terms: q . k_t = sum_d v_d (nib_td - zp_d), v = q*s. Per group and row, v is made
+//      into a few narrow terms, once for the group's 128 keys, and multiplied by the
+//      nibbles as they are stored, where dequantized keys would need two or three terms
+//      against as many of the query; the constant sum_d v_d zp_d, in float32, goes in
+//      with the exponent's FMA. A product takes 16 keys (A) and 16 rows (B).
+//      16-bit outputs: two float16 terms, 21 bits of every v_d by itself (whatever
+//      outliers its row or group holds), scaled by powers of two and the row's largest
+//      |q| into float16's range. A nibble masked out of its word is a float16 of the
+//      smallest numbers, nib * 2^-24, or 16 times that; v_mfma_f32_16x16x32_f16.
+//      float32 outputs (WIDE): v as an integer below 2^30, in units of (the row's
+//      largest |q|) * (a power of two for the group's largest s), in four balanced
+//      base-256 digits for v_mfma_i32_16x16x64_i8, whose exact sums meet in float32: as
+//      good as float32 products of q and k. Three digits for 16-bit outputs were 2.5 %
+//      faster at 64 rows (68 us, 70) and as much slower with float32 values, but a
+//      channel of large q beside one of large s (30 and 15 times the others) made
+//      float16 outputs' error 7 % larger than the rounding's own.
+//      The terms are built by the whole workgroup for the next group while the present
+//      one is multiplied (two LDS buffers, one barrier a group), from scales that a wave
+//      stages for a group of its own every four.
 //   softmax: lane (g, r) of a wave holds the logits of row r with keys 4g .. 4g+3, and
 //      the value product wants its B operand in the same lanes, so probabilities never
 //      leave their registers. The shift is a whole number that moves only when a logit
@@ -86,9 +89,10 @@ __device__ __forceinline__ const RowsArgs& late_args() {
   return *(const RowsArgs*)p;
 }
 
-
-template <int D, int VDT, int RT, int ND>
+template <int D, int VDT, int RT, bool WIDE>
 struct RowsGeo {
+  static constexpr int ND = WIDE ? 4 : 2;          // terms of q*s
+  static constexpr int TB = WIDE ? 1 : 2;          // bytes of a term
   static constexpr int NB = D / 64;                // 64-channel blocks of the key product
   static constexpr int KW = D / 32;                // packed key words per lane per row
   static constexpr int VEB = VDT == kVF32 ? 4 : 2;
@@ -99,24 +103,31 @@ struct RowsGeo {
   static constexpr int CPS = VDT == kVF32 ? 1 : 2; // chunks per step
   static constexpr int M = 16 * RT;           // rows of the workgroup
   static constexpr int NT = kWaves * 64;           // threads
-  static constexpr int TPR = NT / M;               // threads per row that build digits
+  static constexpr int TPR = NT / M;               // threads per row that build terms
   static constexpr int SPT = D / TPR;              // channels each
-  static constexpr int DS = D + 16;                // bytes per row of a digit (padded)
-  static constexpr int kDig = ND * M * DS;         // a buffer of digits
+  static constexpr int DS = D * TB + 16;           // bytes per row of a term (padded)
+  static constexpr int kDig = ND * M * DS;         // a buffer of terms
   static constexpr int AS = D + 4;                 // floats per row of queries and outputs
-  // LDS: two buffers of digits and the queries while the keys stream, then the waves'
-  // outputs.
+  // Scaled scales, and zero-points times them, of a group, in slot order; four floats of
+  // padding every 16 keep the threads of a row, 16 channels apart, on different banks.
+  static constexpr int kSz = D + D / 4;
+  // LDS: two buffers of terms, the queries and twice kWaves groups' scales while the keys
+  // stream, then the waves' outputs.
   static constexpr int kQ = 2 * kDig;
-  static constexpr int kStream = kQ + M * AS * 4;
+  static constexpr int kScales = kQ + M * AS * 4;
+  static constexpr int kStream = kScales + 2 * kWaves * 2 * kSz * 4;
   static constexpr int kAcc = kWaves * M * AS * 4;
   static constexpr int kSmem = kStream > kAcc ? kStream : kAcc;
   static_assert(TPR >= 4 && TPR <= 16 && (TPR & (TPR - 1)) == 0 && SPT % 4 == 0, "threads");
 };
 
-// Position of channel d in the operands' order: of every eight channels (a word of
-// nibbles) the even ones (low nibbles) before the odd ones.
+// Position of channel d in the operands' order, of every eight channels (a word of
+// nibbles): digits, the even ones (low nibbles) before the odd ones; float16 terms, the
+// pairs (j, j + 4) of nibbles that lie 16 bits apart.
+template <bool WIDE>
 __device__ __forceinline__ int row_slot(int d) {
-  return (d & ~7) | ((d & 1) << 2) | ((d & 7) >> 1);
+  return WIDE ? (d & ~7) | ((d & 1) << 2) | ((d & 7) >> 1)
+              : (d & ~7) | ((d & 3) << 1) | ((d & 7) >> 2);
 }
 
 // Eight channels of a query as float32, from 16-byte loads (VEC) or element by element.
@@ -173,15 +184,14 @@ __device__ __forceinline__ float over_groups_sum(float x) {
 }
 
 // RT: row tiles. WIDE: float32 outputs (four digits of q*s, all 24 bits of a
-// probability); otherwise three digits and at least 16 bits. STREAM: keys and values
+// probability); otherwise two float16 terms and at least 16 bits. STREAM: keys and values
 // are read by one workgroup only (non-temporal loads).
 template <int D, int VDT, int RT, bool WIDE, bool STREAM>
 __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a) {
-  constexpr int ND = WIDE ? 4 : 3;
   // 16-bit terms of a probability.
   constexpr int TERMS = VDT == kVF32 || (WIDE && VDT == kVBF16) ? 3 : 2;
-  using G = RowsGeo<D, VDT, RT, ND>;
-  constexpr int NB = G::NB, CPS = G::CPS, NA = G::NA, M = G::M, NT = G::NT;
+  using G = RowsGeo<D, VDT, RT, WIDE>;
+  constexpr int ND = G::ND, NB = G::NB, CPS = G::CPS, NA = G::NA, M = G::M, NT = G::NT;
   constexpr int TPR = G::TPR, SPT = G::SPT, NS = 4 * CPS;
   // Shift of the probabilities: the largest is 2^kUp when the shift moves, and stays
   // below 2^(kUp + kSlack). float16 terms need the headroom (2^16) and the small end
@@ -212,20 +222,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
   const int live = min(rows - row0, M);            // rows of this workgroup
 
   __shared__ __align__(16) uint8_t smem[G::kSmem];
-  // Scaled scales, and zero-points times them, in slot order; four floats of padding
-  // every 16 keep the threads of a row, 16 channels apart, on different banks.
-  constexpr int kSz = D + D / 4;
+  constexpr int kSz = G::kSz;
   auto sz_pos = [](int slot) { return slot + slot / 16 * 4; };
-  __shared__ __align__(16) float sz_s[2][2 * kSz];
-  __shared__ float cs_s[2];                        // a group's scale unit
+  __shared__ float cs_s[2 * kWaves];               // a group's scale unit
   __shared__ float2 cc_s[2][M];                    // a row's logit unit and constant
   __shared__ int low_s[M];                         // first cached token in a row's window
   __shared__ int ext_s[2];                         // smallest and largest of them
   __shared__ float m_s[kWaves][M], l_s[kWaves][M];
   __shared__ int bad_s;
   float* const q_s = reinterpret_cast<float*>(smem + G::kQ);
+  float* const sz_s = reinterpret_cast<float*>(smem + G::kScales);
 
-  // This thread's part of a row of digits: brow's channels part * SPT .. (of eight, the
+  // This thread's part of a row of terms: brow's channels part * SPT .. (of eight, the
   // even or the odd ones where SPT is four).
   const int brow = tid / TPR, part = tid % TPR;
   constexpr int NQ = SPT / 8 > 0 ? SPT / 8 : 1;
@@ -395,7 +403,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
     }
   };
 
-  // ---- scales of a group to LDS, and the rows' digits ----
+  // ---- scales of a group to LDS, and the rows' terms ----
   // Lane l holds the scales and zero-points of channels SL * l .. (SL = D / 64).
   constexpr int SL = D / 64;
   struct Scales {
@@ -416,11 +424,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
     }
     return r;
   };
-  // The scales in units of 2^-30 (2^-22) of the largest, and zero-points times them.
-  // (By wave `by`; powers of two, so that only the products with q round.)
-  constexpr int kBits = WIDE ? 30 : 22;
-  auto stage_sz = [&](const Scales& x, int buf, int by) __attribute__((always_inline)) {
-    if (w != by) return;
+  // The scales in units of 2^-30 (2^-15) of the largest, and zero-points times them.
+  // (By one wave, to the slot of group it; powers of two, so that only the products with
+  // q round.)
+  constexpr int kBits = WIDE ? 30 : 15;
+  auto slot_of = [&](int it) { return (it - it0) & (2 * kWaves - 1); };
+  auto stage_sz = [&](const Scales& x, int it) __attribute__((always_inline)) {
+    const int slot = slot_of(it);
     unsigned mx = 0;
 #pragma unroll
     for (int k = 0; k < SL; ++k) mx = max(mx, f2u(x.s[k]) & 0x7FFFFFFFu);
@@ -433,62 +443,74 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
     // All scales are below 2^kBits units. (An infinite or NaN one makes the rows NaN.)
     const unsigned ex = (max(mx, f2u(1e-28f)) >> 23) + 1 - kBits;
     const float inv = u2f((254 - ex) << 23);
-    if (lane == 0) cs_s[buf] = mx >= 0x7F800000u ? u2f(0x7FC00000u) : u2f(ex << 23);
-    float* dst = sz_s[buf];
+    if (lane == 0) cs_s[slot] = mx >= 0x7F800000u ? u2f(0x7FC00000u) : u2f(ex << 23);
+    float* dst = sz_s + slot * 2 * kSz;
 #pragma unroll
     for (int k = 0; k < SL; ++k) {
       const float v = x.s[k] * inv;
-      const int at = sz_pos(row_slot(SL * lane + k));
-      dst[at] = v;
+      const int d = SL * lane + k, at = sz_pos(row_slot<WIDE>(d));
+      // (Odd channels' nibbles are multiplied where they lie, four bits up.)
+      dst[at] = !WIDE && (d & 1) ? v * 0.0625f : v;
       dst[kSz + at] = x.z[k] * v;
     }
   };
   float qn[SPT], q_unit;                           // the row relative to its largest
-  auto build = [&](int buf) __attribute__((always_inline)) {
-    const float cs = cs_s[buf];
-    uint8_t* dst = smem + buf * G::kDig + brow * G::DS + part * SPT;
+  auto build = [&](int it) __attribute__((always_inline)) {
+    const int buf = (it - it0) & 1, slot = slot_of(it);
+    const float cs = cs_s[slot];
+    const float* sz = sz_s + slot * 2 * kSz;
+    uint8_t* dst = smem + buf * G::kDig + brow * G::DS + part * SPT * G::TB;
     float cg[4] = {0.f, 0.f, 0.f, 0.f};
-    unsigned out[ND][SPT / 4];
-    static_assert(SPT == 4 || SPT == 8 || SPT == 16, "digit stores");
+    constexpr int OW = SPT * G::TB / 4;
+    unsigned out[ND][OW];
+    static_assert(SPT == 4 || SPT == 8 || SPT == 16, "operand stores");
 #pragma unroll
     for (int i = 0; i < SPT; i += 4) {
-      const float* src = sz_s[buf] + sz_pos(part * SPT + i);
+      const float* src = sz + sz_pos(part * SPT + i);
       const float4 s4 = *reinterpret_cast<const float4*>(src);
       const float4 z4 = *reinterpret_cast<const float4*>(src + kSz);
       const float ss[4] = {s4.x, s4.y, s4.z, s4.w}, zz[4] = {z4.x, z4.y, z4.z, z4.w};
-      unsigned x[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        cg[k] = __builtin_fmaf(qn[i + k], zz[k], cg[k]);
+      for (int k = 0; k < 4; ++k) cg[k] = __builtin_fmaf(qn[i + k], zz[k], cg[k]);
+      if constexpr (WIDE) {
         // The integer plus a bias that makes its lower bytes digits + 128.
-        if constexpr (WIDE) {
-          x[k] = (unsigned)(int)(qn[i + k] * ss[k]) + 0x808080u;
-        } else {
-          // (Rounded by the addition of 1.5 * 2^23, whose bits go again; |v| < 2^22.)
-          x[k] = f2u(__builtin_fmaf(qn[i + k], ss[k], 12582912.f)) - (0x4B400000u - 0x8080u);
+        unsigned x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = (unsigned)(int)(qn[i + k] * ss[k]) + 0x808080u;
+        const unsigned t0 = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u);
+        const unsigned u0 = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u);
+        const unsigned t1 = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u);
+        const unsigned u1 = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
+        out[0][i / 4] = __builtin_amdgcn_perm(u0, t0, 0x05040100u) ^ 0x80808080u;
+        out[1][i / 4] = __builtin_amdgcn_perm(u0, t0, 0x07060302u) ^ 0x80808080u;
+        out[2][i / 4] = __builtin_amdgcn_perm(u1, t1, 0x05040100u) ^ 0x80808080u;
+        out[3][i / 4] = __builtin_amdgcn_perm(u1, t1, 0x07060302u);
+      } else {
+        // (The second term is what the first cuts off, in the same units.)
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+          const float x0 = qn[i + k] * ss[k], x1 = qn[i + k + 1] * ss[k + 1];
+          const float h0 = u2f(f2u(x0) & 0xFFFFE000u), h1 = u2f(f2u(x1) & 0xFFFFE000u);
+          out[0][(i + k) / 2] =
+              __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(h0, h1));
+          out[1][(i + k) / 2] =
+              __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(x0 - h0, x1 - h1));
         }
       }
-      const unsigned t0 = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u);
-      const unsigned u0 = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u);
-      const unsigned t1 = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u);
-      const unsigned u1 = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
-      unsigned dg[4] = {__builtin_amdgcn_perm(u0, t0, 0x05040100u) ^ 0x80808080u,
-                        __builtin_amdgcn_perm(u0, t0, 0x07060302u) ^ 0x80808080u,
-                        __builtin_amdgcn_perm(u1, t1, 0x05040100u),
-                        __builtin_amdgcn_perm(u1, t1, 0x07060302u)};
-      if constexpr (WIDE) dg[2] ^= 0x80808080u;
-#pragma unroll
-      for (int k = 0; k < ND; ++k) out[k][i / 4] = dg[k];
     }
 #pragma unroll
     for (int k = 0; k < ND; ++k) {
       uint8_t* o = dst + k * M * G::DS;
-      if constexpr (SPT == 16)
-        *reinterpret_cast<uint4*>(o) = make_uint4(out[k][0], out[k][1], out[k][2], out[k][3]);
-      else if constexpr (SPT == 8)
+      if constexpr (OW == 2) {
         *reinterpret_cast<uint2*>(o) = make_uint2(out[k][0], out[k][1]);
-      else
+      } else if constexpr (OW == 1) {
         *reinterpret_cast<unsigned*>(o) = out[k][0];
+      } else {
+#pragma unroll
+        for (int i = 0; i < OW; i += 4)
+          *reinterpret_cast<uint4*>(o + 4 * i) =
+              make_uint4(out[k][i], out[k][i + 1], out[k][i + 2], out[k][i + 3]);
+      }
     }
     float cgs = (cg[0] + cg[1]) + (cg[2] + cg[3]);
     cgs += xchg<1>(cgs);
@@ -497,7 +519,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
     if constexpr (TPR > 8) cgs += xchg<8>(cgs);
     if (part == 0) {
       const float c1 = q_unit * cs * kLog2e;
-      cc_s[buf][brow] = make_float2(c1, cgs * c1);
+      cc_s[buf][brow] = make_float2(WIDE ? c1 : c1 * 16777216.f, cgs * c1);
     }
   };
 
@@ -518,58 +540,86 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
   constexpr int PW = NS / 2;                       // registers per term
   unsigned pr[RT][PW * TERMS];
 
-  // Row tile rt and scores s (logit = s * c1 - cc, log2 units, c1 >= 0) of keys
-  // 4 grp + i of chunk e in s[4 e + i], of which, if masked, those in vis are seen.
-  auto softmax = [&](int rt, const float* s, float c1, float cc, bool masked, unsigned vis)
-      __attribute__((always_inline)) {
-    float p[NS], top = kLeast;
+  // Scores s (logit = s * c1 - cc, log2 units, c1 >= 0) of keys 4 grp + i of chunk e in
+  // s[4 e + i], of which, if masked, those in vis are seen: of all row tiles together,
+  // whose chains of dependent instructions run side by side.
+  auto softmax = [&](float (*s)[NS], const float* c1, const float* cc, bool masked,
+                     const unsigned* vis) __attribute__((always_inline)) {
+    float top[RT], sub[RT];
     if (masked) {
 #pragma unroll
-      for (int k = 0; k < NS; ++k) {
-        p[k] = (vis >> k) & 1u ? __builtin_fmaf(s[k], c1, -cc) : -INFINITY;
-        top = fmaxf(top, p[k]);
+      for (int rt = 0; rt < RT; ++rt) {
+        top[rt] = kLeast;
+#pragma unroll
+        for (int k = 0; k < NS; ++k) {
+          s[rt][k] =
+              (vis[rt] >> k) & 1u ? __builtin_fmaf(s[rt][k], c1[rt], -cc[rt]) : -INFINITY;
+          top[rt] = fmaxf(top[rt], s[rt][k]);
+        }
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < NS; ++k) top = fmaxf(top, s[k]);
-      top = __builtin_fmaf(top, c1, -cc);
+      for (int rt = 0; rt < RT; ++rt) {
+        top[rt] = kLeast;
+#pragma unroll
+        for (int k = 0; k < NS; ++k) top[rt] = fmaxf(top[rt], s[rt][k]);
+        top[rt] = __builtin_fmaf(top[rt], c1[rt], -cc[rt]);
+      }
     }
-    top = over_groups_max(top);
-    const bool up = top > m_run[rt] + (kUp + kSlack);
-    if (__builtin_amdgcn_ballot_w64(up)) {
-      const float m_new = up ? __builtin_ceilf(top) - kUp : m_run[rt];
-      const float corr = __builtin_amdgcn_exp2f(m_run[rt] - m_new);
-      m_run[rt] = m_new;
-      l_run[rt] *= corr;
+    bool up[RT], some = false;
 #pragma unroll
-      for (int t = 0; t < NA; ++t) acc[rt][t] *= corr;
+    for (int rt = 0; rt < RT; ++rt) {
+      top[rt] = over_groups_max(top[rt]);
+      up[rt] = top[rt] > m_run[rt] + (kUp + kSlack);
+      some |= up[rt];
     }
-    if (masked) {
+    if (__builtin_amdgcn_ballot_w64(some)) {
 #pragma unroll
-      for (int k = 0; k < NS; ++k) p[k] = __builtin_amdgcn_exp2f(p[k] - m_run[rt]);
-    } else {
-      const float sub = -cc - m_run[rt];
+      for (int rt = 0; rt < RT; ++rt) {
+        const float m_new = up[rt] ? __builtin_ceilf(top[rt]) - kUp : m_run[rt];
+        const float corr = __builtin_amdgcn_exp2f(m_run[rt] - m_new);
+        m_run[rt] = m_new;
+        l_run[rt] *= corr;
 #pragma unroll
-      for (int k = 0; k < NS; ++k) p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], c1, sub));
+        for (int t = 0; t < NA; ++t) acc[rt][t] *= corr;
+      }
     }
-    if constexpr (VDT == kVF32) l_run[rt][0] += (p[0] + p[1]) + (p[2] + p[3]);
 #pragma unroll
-    for (int h = 0; h < PW; ++h) {
-      float y0 = p[2 * h], y1 = p[2 * h + 1];
+    for (int rt = 0; rt < RT; ++rt) {
+      if (masked) {
 #pragma unroll
-      for (int q = 0; q < TERMS; ++q) {
-        if constexpr (VDT == kVF16) {
-          const float h0 = q == TERMS - 1 ? y0 : u2f(f2u(y0) & 0xFFFFE000u);
-          const float h1 = q == TERMS - 1 ? y1 : u2f(f2u(y1) & 0xFFFFE000u);
-          pr[rt][PW * q + h] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(h0, h1));
-          y0 -= h0;
-          y1 -= h1;
-        } else {
-          const unsigned r =
-              __builtin_bit_cast(unsigned, __builtin_convertvector(v2f{y0, y1}, v2bf));
-          pr[rt][PW * q + h] = r;
-          y0 -= u2f(r << 16);
-          y1 -= u2f(r & 0xFFFF0000u);
+        for (int k = 0; k < NS; ++k) s[rt][k] -= m_run[rt];
+      } else {
+        sub[rt] = -cc[rt] - m_run[rt];
+#pragma unroll
+        for (int k = 0; k < NS; ++k) s[rt][k] = __builtin_fmaf(s[rt][k], c1[rt], sub[rt]);
+      }
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float* p = s[rt];
+#pragma unroll
+      for (int k = 0; k < NS; ++k) p[k] = __builtin_amdgcn_exp2f(p[k]);
+      if constexpr (VDT == kVF32) l_run[rt][0] += (p[0] + p[1]) + (p[2] + p[3]);
+#pragma unroll
+      for (int h = 0; h < PW; ++h) {
+        float y0 = p[2 * h], y1 = p[2 * h + 1];
+#pragma unroll
+        for (int q = 0; q < TERMS; ++q) {
+          if constexpr (VDT == kVF16) {
+            const float h0 = q == TERMS - 1 ? y0 : u2f(f2u(y0) & 0xFFFFE000u);
+            const float h1 = q == TERMS - 1 ? y1 : u2f(f2u(y1) & 0xFFFFE000u);
+            pr[rt][PW * q + h] =
+                __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(h0, h1));
+            y0 -= h0;
+            y1 -= h1;
+          } else {
+            const unsigned r =
+                __builtin_bit_cast(unsigned, __builtin_convertvector(v2f{y0, y1}, v2bf));
+            pr[rt][PW * q + h] = r;
+            y0 -= u2f(r << 16);
+            y1 -= u2f(r & 0xFFFF0000u);
+          }
         }
       }
     }
@@ -643,15 +693,14 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
     Keys kf;
     Vals vf;
     Meta cur, nxt;
-    Scales sz0, sz1, szr;
+    Scales sz0, szr;
     if (steps > 0) {
       cur = next_meta();
       nxt = next_meta();
-      sz0 = load_sz(it0);
+      sz0 = load_sz(it0 + w);
       load_keys(cur, kf);
       load_values(cur, vf);
-      sz1 = load_sz(it0 + 1);
-      szr = load_sz(it0 + 2);
+      szr = load_sz(it0 + kWaves + w);
     }
     // The row relative to its largest, in slot order (zeros behind the last row), and
     // as it is to LDS for the drafts.
@@ -672,11 +721,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
     const float inv = 1.f / q_unit;
 #pragma unroll
     for (int i = 0; i < SPT; ++i) {
+      // Channel of slot i of eight, for a thread of the lower and of the upper four.
+      auto of = [](int i) { return WIDE ? 2 * (i & 3) + (i >> 2) : 4 * (i & 1) + (i >> 1); };
       if constexpr (SPT >= 8) {
-        qn[i] = qv[i / 8][2 * (i % 4) + ((i >> 2) & 1)] * inv;
+        qn[i] = qv[i / 8][of(i % 8)] * inv;
       } else {
-        const unsigned odd = part & 1 ? ~0u : 0u;
-        qn[i] = u2f((f2u(qv[0][2 * i + 1]) & odd) | (f2u(qv[0][2 * i]) & ~odd)) * inv;
+        const unsigned up = part & 1 ? ~0u : 0u;
+        qn[i] = u2f((f2u(qv[0][of(i + 4)]) & up) | (f2u(qv[0][of(i)]) & ~up)) * inv;
       }
     }
     if (dr0 < dr1) {
@@ -688,36 +739,45 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
       }
     }
     if (tid == 0) bad_s = 0;
-    if (steps > 0) {
-      stage_sz(sz0, 0, 0);
-      stage_sz(sz1, 1, 1);
-    }
+    if (steps > 0) stage_sz(sz0, it0 + w);
     __syncthreads();
     if (steps > 0) {
-      build(0);
+      build(it0);
       int it = it0, p = 0;
       for (int done = 0; done < steps; ++done) {
         const int buf = (it - it0) & 1;
         if (p == 0) {
           __syncthreads();
-          if (it + 1 < it1) build(buf ^ 1);
-          stage_sz(szr, buf, it & (kWaves - 1));   // of item it + 2
-          szr = load_sz(it + 3);
+          if (it + 1 < it1) build(it + 1);
+          // Every kWaves items, a wave an item: of the next kWaves items the first is built
+          // in the last of these, and the slots held items built before.
+          if (((it - it0) & (kWaves - 1)) == 0) {
+            stage_sz(szr, it + kWaves + w);
+            szr = load_sz(it + 2 * kWaves + w);
+          }
         }
-        // Nibbles of key block kb of chunk e.
+        // Nibbles of key block kb of chunk e: as bytes, or (eight channels a block) as
+        // float16, of which a nibble in the lowest bits is one of the smallest numbers,
+        // nib * 2^-24, and one four bits up is 16 times that.
+        constexpr int KB = WIDE ? NB : G::KW;
         auto key_op = [&](int e, int kb) __attribute__((always_inline)) -> v4i {
-          const unsigned w0 = kf.w[e][2 * kb], w1 = kf.w[e][2 * kb + 1];
-          return v4i{(int)(w0 & 0x0F0F0F0Fu), (int)((w0 >> 4) & 0x0F0F0F0Fu),
-                     (int)(w1 & 0x0F0F0F0Fu), (int)((w1 >> 4) & 0x0F0F0F0Fu)};
+          if constexpr (WIDE) {
+            const unsigned w0 = kf.w[e][2 * kb], w1 = kf.w[e][2 * kb + 1];
+            return v4i{(int)(w0 & 0x0F0F0F0Fu), (int)((w0 >> 4) & 0x0F0F0F0Fu),
+                       (int)(w1 & 0x0F0F0F0Fu), (int)((w1 >> 4) & 0x0F0F0F0Fu)};
+          }
+          const unsigned w0 = kf.w[e][kb], w1 = w0 >> 8;
+          return v4i{(int)(w0 & 0x000F000Fu), (int)(w0 & 0x00F000F0u),
+                     (int)(w1 & 0x000F000Fu), (int)(w1 & 0x00F000F0u)};
         };
         // With one row tile they are made where they are used (registers), with two
         // once for both, and the next keys are loaded over the words.
-        v4i ak[CPS][NB];
+        v4i ak[CPS][KB];
         if constexpr (RT > 1) {
 #pragma unroll
           for (int e = 0; e < CPS; ++e)
 #pragma unroll
-            for (int kb = 0; kb < NB; ++kb) ak[e][kb] = key_op(e, kb);
+            for (int kb = 0; kb < KB; ++kb) ak[e][kb] = key_op(e, kb);
           load_keys(nxt, kf);
         }
         bool any = false, masked = false;
@@ -728,53 +788,85 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
                     ((cur.tok0[e] < low_max) & (cur.tok0[e] + 16 > a.sinks));
         }
         if (any) {
+          const uint8_t* dg = smem + buf * G::kDig + n16 * G::DS + grp * (D / 4 * G::TB);
+          float s[RT][NS];
+          if constexpr (WIDE) {
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            const int r = rt * 16 + n16;
-            const uint8_t* dg = smem + buf * G::kDig + r * G::DS + grp * (D / 4);
-            v4i ds[CPS][ND];
+            for (int rt = 0; rt < RT; ++rt) {
+              v4i ds[CPS][ND];
 #pragma unroll
-            for (int kb = 0; kb < NB; ++kb) {
+              for (int kb = 0; kb < KB; ++kb) {
+                v4i kop[CPS];
+#pragma unroll
+                for (int e = 0; e < CPS; ++e) kop[e] = RT > 1 ? ak[e][kb] : key_op(e, kb);
+#pragma unroll
+                for (int k = 0; k < ND; ++k) {
+                  const v4i bq = *reinterpret_cast<const v4i*>(
+                      dg + (k * M + rt * 16) * G::DS + 16 * kb);
+#pragma unroll
+                  for (int e = 0; e < CPS; ++e)
+                    ds[e][k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                        kop[e], bq, kb == 0 ? v4i{0, 0, 0, 0} : ds[e][k], 0, 0, 0);
+                }
+              }
+#pragma unroll
+              for (int e = 0; e < CPS; ++e)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  s[rt][4 * e + i] =
+                      __builtin_fmaf((float)((ds[e][3][i] << 8) + ds[e][2][i]), 65536.f,
+                                     (float)((ds[e][1][i] << 8) + ds[e][0][i]));
+            }
+          } else {
+            v4f ds[RT][CPS];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
               v4i kop[CPS];
 #pragma unroll
               for (int e = 0; e < CPS; ++e) kop[e] = RT > 1 ? ak[e][kb] : key_op(e, kb);
 #pragma unroll
-              for (int k = 0; k < ND; ++k) {
-                const v4i bq = *reinterpret_cast<const v4i*>(dg + k * M * G::DS + 16 * kb);
+              for (int k = ND - 1; k >= 0; --k)
 #pragma unroll
-                for (int e = 0; e < CPS; ++e)
-                  ds[e][k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-                      kop[e], bq, kb == 0 ? v4i{0, 0, 0, 0} : ds[e][k], 0, 0, 0);
-              }
+                for (int rt = 0; rt < RT; ++rt) {
+                  const v4i bq = *reinterpret_cast<const v4i*>(
+                      dg + (k * M + rt * 16) * G::DS + 16 * kb);
+#pragma unroll
+                  for (int e = 0; e < CPS; ++e)
+                    ds[rt][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        __builtin_bit_cast(v8h, kop[e]), __builtin_bit_cast(v8h, bq),
+                        kb == 0 && k == ND - 1 ? v4f{0.f, 0.f, 0.f, 0.f} : ds[rt][e], 0, 0, 0);
+                }
             }
-            if constexpr (RT == 1) load_keys(nxt, kf);
-            float s[NS];
 #pragma unroll
-            for (int e = 0; e < CPS; ++e)
+            for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float hi = (float)((ds[e][ND - 1][i] << 8) + ds[e][ND - 2][i]);
-                if constexpr (WIDE)
-                  s[4 * e + i] =
-                      __builtin_fmaf(hi, 65536.f, (float)((ds[e][1][i] << 8) + ds[e][0][i]));
-                else
-                  s[4 * e + i] = __builtin_fmaf(hi, 256.f, (float)ds[e][0][i]);
-              }
-            const float2 cc = cc_s[buf][r];
-            unsigned vis = 0;
-            if (masked) {
-              const int low = low_s[r];
+              for (int k = 0; k < NS; ++k) s[rt][k] = ds[rt][k / 4][k % 4];
+          }
+          if constexpr (RT == 1) load_keys(nxt, kf);
+          float c1[RT], cc[RT];
+          unsigned vis[RT];
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            const float2 x = cc_s[buf][rt * 16 + n16];
+            c1[rt] = x.x;
+            cc[rt] = x.y;
+            vis[rt] = 0;
+          }
+          if (masked) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+              const int low = low_s[rt * 16 + n16];
 #pragma unroll
               for (int e = 0; e < CPS; ++e)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   const int k = 4 * grp + i, t = cur.tok0[e] + k;
-                  vis |= (unsigned)((k < cur.nval[e]) & ((t < a.sinks) | (t >= low)))
-                         << (4 * e + i);
+                  vis[rt] |= (unsigned)((k < cur.nval[e]) & ((t < a.sinks) | (t >= low)))
+                             << (4 * e + i);
                 }
             }
-            softmax(rt, s, cc.x, cc.y, masked, vis);
           }
+          softmax(s, c1, cc, masked, vis);
           // Keys that no row sees keep no value: a probability of zero times what lies
           // there (a chunk of none holds anything) would be NaN where that is not
           // finite.
@@ -862,19 +954,22 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
           ds[rt] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.w, q4.w, ds[rt], 0, 0, 0);
         }
       }
+      float s[RT][NS], c1[RT], cc[RT];
+      unsigned vis[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        unsigned vis = 0;
-        float s[NS];
+        c1[rt] = kLog2e;
+        cc[rt] = 0.f;
+        vis[rt] = 0;
 #pragma unroll
-        for (int k = 0; k < NS; ++k) s[k] = kLeast;
+        for (int k = 0; k < NS; ++k) s[rt][k] = kLeast;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          vis |= (unsigned)((mb[rt][k] != 0) & (4 * grp + k < nval)) << k;
-          s[k] = ds[rt][k];
+          vis[rt] |= (unsigned)((mb[rt][k] != 0) & (4 * grp + k < nval)) << k;
+          s[rt][k] = ds[rt][k];
         }
-        softmax(rt, s, kLog2e, 0.f, true, vis);
       }
+      softmax(s, c1, cc, true, vis);
       add_values(vf);
     }
   } else if (tid == 0) {
@@ -967,7 +1062,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
       l_s[w][rt * 16 + n16] = l;
     }
   }
-  __syncthreads();                                 // (the digits are no longer read)
+  __syncthreads();                                 // (the terms are no longer read)
   float* out_w = reinterpret_cast<float*>(smem) + w * M * G::AS;
   float any_nan = 0.f;
 #pragma unroll
