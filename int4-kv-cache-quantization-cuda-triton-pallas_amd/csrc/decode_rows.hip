@@ -19,17 +19,14 @@
 //      nibbles as they are stored, where dequantized keys would need two or three terms
 //      against as many of the query; the constant sum_d v_d zp_d, in float32, goes in
 //      with the exponent's FMA. A product takes 16 keys (A) and 16 rows (B).
-//      16-bit outputs: two float16 terms, 21 bits of every v_d by itself (whatever
-//      outliers its row or group holds), scaled by powers of two and the row's largest
-//      |q| into float16's range. A nibble masked out of its word is a float16 of the
-//      smallest numbers, nib * 2^-24, or 16 times that; v_mfma_f32_16x16x32_f16.
-//      float32 outputs (WIDE): v as an integer below 2^30, in units of (the row's
-//      largest |q|) * (a power of two for the group's largest s), in four balanced
-//      base-256 digits for v_mfma_i32_16x16x64_i8, whose exact sums meet in float32: as
-//      good as float32 products of q and k. Three digits for 16-bit outputs were 2.5 %
-//      faster at 64 rows (68 us, 70) and as much slower with float32 values, but a
-//      channel of large q beside one of large s (30 and 15 times the others) made
-//      float16 outputs' error 7 % larger than the rounding's own.
+//      The terms are in units of a power of two for the largest |v| of the row and the
+//      group. 16-bit outputs: two float16 terms. A nibble masked out of its word is a
+//      float16 of the smallest numbers, nib * 2^-24, or 16 times that;
+//      v_mfma_f32_16x16x32_f16.
+//      float32 outputs (WIDE): an integer below 2^30, in four balanced base-256 digits
+//      for v_mfma_i32_16x16x64_i8, whose exact sums meet in float32: as good as float32
+//      products of q and k (2-norm error 3e-7 over 300 keys of 128 channels, 4e-7 with
+//      those).
 //      The terms are built by the whole workgroup for the next group while the present
 //      one is multiplied (two LDS buffers, one barrier a group), from scales that a wave
 //      stages for a group of its own every four.
@@ -108,7 +105,7 @@ struct RowsGeo {
   static constexpr int DS = D * TB + 16;           // bytes per row of a term (padded)
   static constexpr int kDig = ND * M * DS;         // a buffer of terms
   static constexpr int AS = D + 4;                 // floats per row of queries and outputs
-  // Scaled scales, and zero-points times them, of a group, in slot order; four floats of
+  // Scales, and zero-points times them, of a group, in slot order; four floats of
   // padding every 16 keep the threads of a row, 16 channels apart, on different banks.
   static constexpr int kSz = D + D / 4;
   // LDS: two buffers of terms, the queries and twice kWaves groups' scales while the keys
@@ -158,6 +155,14 @@ __device__ __forceinline__ KVec<KW> load_words(const uint8_t* p) {
 __device__ __forceinline__ unsigned xchg4(unsigned x) {
   return (unsigned)__builtin_amdgcn_mov_dpp(
       __builtin_amdgcn_mov_dpp((int)x, 0x141, 0xF, 0xF, false), 0x1B, 0xF, 0xF, false);
+}
+
+// A lane's number as a value of unknown origin: what is computed from it in a loop is
+// computed there. (Four digits leave no registers to keep a few addresses in: spilled,
+// they made 64 rows of 16-bit values and float32 outputs 85 us in place of 76.)
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 // Maximum and sum over the four 16-lane groups.
@@ -224,7 +229,6 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
   __shared__ __align__(16) uint8_t smem[G::kSmem];
   constexpr int kSz = G::kSz;
   auto sz_pos = [](int slot) { return slot + slot / 16 * 4; };
-  __shared__ float cs_s[2 * kWaves];               // a group's scale unit
   __shared__ float2 cc_s[2][M];                    // a row's logit unit and constant
   __shared__ int low_s[M];                         // first cached token in a row's window
   __shared__ int ext_s[2];                         // smallest and largest of them
@@ -410,7 +414,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
     float s[SL], z[SL];
   };
   auto load_sz = [&](int it) __attribute__((always_inline)) -> Scales {
-    const uint64_t off = (uint64_t)(unsigned)group_of(min(it, it1 - 1)) * a.s_group + SL * lane;
+    const uint64_t off = (uint64_t)(unsigned)group_of(min(it, it1 - 1)) * a.s_group +
+                         SL * (WIDE ? fresh(lane) : lane);
     struct alignas(4 * SL) Part {
       float v[SL];
     };
@@ -424,43 +429,31 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
     }
     return r;
   };
-  // The scales in units of 2^-30 (2^-15) of the largest, and zero-points times them.
-  // (By one wave, to the slot of group it; powers of two, so that only the products with
-  // q round.)
-  constexpr int kBits = WIDE ? 30 : 15;
+  // The scales, and zero-points times them, by one wave to the slot of group it.
   auto slot_of = [&](int it) { return (it - it0) & (2 * kWaves - 1); };
   auto stage_sz = [&](const Scales& x, int it) __attribute__((always_inline)) {
-    const int slot = slot_of(it);
-    unsigned mx = 0;
-#pragma unroll
-    for (int k = 0; k < SL; ++k) mx = max(mx, f2u(x.s[k]) & 0x7FFFFFFFu);
-    mx = max(mx, xchg_u32<1>(mx));
-    mx = max(mx, xchg_u32<2>(mx));
-    mx = max(mx, xchg4(mx));
-    mx = max(mx, xchg_u32<8>(mx));
-    mx = max(mx, xchg_u32<16>(mx));
-    mx = max(mx, xchg_u32<32>(mx));
-    // All scales are below 2^kBits units. (An infinite or NaN one makes the rows NaN.)
-    const unsigned ex = (max(mx, f2u(1e-28f)) >> 23) + 1 - kBits;
-    const float inv = u2f((254 - ex) << 23);
-    if (lane == 0) cs_s[slot] = mx >= 0x7F800000u ? u2f(0x7FC00000u) : u2f(ex << 23);
-    float* dst = sz_s + slot * 2 * kSz;
+    float* dst = sz_s + slot_of(it) * 2 * kSz;
+    const int d0 = SL * (WIDE ? fresh(lane) : lane);
 #pragma unroll
     for (int k = 0; k < SL; ++k) {
-      const float v = x.s[k] * inv;
-      const int d = SL * lane + k, at = sz_pos(row_slot<WIDE>(d));
+      const int d = d0 + k, at = sz_pos(row_slot<WIDE>(d));
       // (Odd channels' nibbles are multiplied where they lie, four bits up.)
-      dst[at] = !WIDE && (d & 1) ? v * 0.0625f : v;
-      dst[kSz + at] = x.z[k] * v;
+      dst[at] = !WIDE && (d & 1) ? x.s[k] * 0.0625f : x.s[k];
+      dst[kSz + at] = x.z[k] * x.s[k];
     }
   };
-  float qn[SPT], q_unit;                           // the row relative to its largest
+  float qn[SPT];                                   // the row's channels in slot order
+  // The row's products with the scales of group it as terms, in units of a power of two
+  // for the largest of them. (Not for the largest query times the largest scale, which
+  // may lie in different channels: one channel of r times the query and 1/r times the
+  // scale beside one of the opposite cost float32 outputs 2e-5 at r = 100 and 2e-3 at
+  // 1000, where float32 products have 4e-7.)
   auto build = [&](int it) __attribute__((always_inline)) {
-    const int buf = (it - it0) & 1, slot = slot_of(it);
-    const float cs = cs_s[slot];
-    const float* sz = sz_s + slot * 2 * kSz;
+    const int buf = (it - it0) & 1;
+    const float* sz = sz_s + slot_of(it) * 2 * kSz;
+    const int own = WIDE ? fresh(tid) : tid, brow = own / TPR, part = own % TPR;
     uint8_t* dst = smem + buf * G::kDig + brow * G::DS + part * SPT * G::TB;
-    float cg[4] = {0.f, 0.f, 0.f, 0.f};
+    float cg[4] = {0.f, 0.f, 0.f, 0.f}, mx[2] = {0.f, 0.f}, v[SPT];
     constexpr int OW = SPT * G::TB / 4;
     unsigned out[ND][OW];
     static_assert(SPT == 4 || SPT == 8 || SPT == 16, "operand stores");
@@ -471,12 +464,33 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
       const float4 z4 = *reinterpret_cast<const float4*>(src + kSz);
       const float ss[4] = {s4.x, s4.y, s4.z, s4.w}, zz[4] = {z4.x, z4.y, z4.z, z4.w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) cg[k] = __builtin_fmaf(qn[i + k], zz[k], cg[k]);
+      for (int k = 0; k < 4; ++k) {
+        cg[k] = __builtin_fmaf(qn[i + k], zz[k], cg[k]);
+        v[i + k] = qn[i + k] * ss[k];
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        mx[k] = fmaxf(mx[k], fmaxf(fabsf(v[i + k]), fabsf(v[i + k + 2])));
+    }
+    float top = fmaxf(mx[0], mx[1]);
+    top = fmaxf(top, xchg<1>(top));
+    top = fmaxf(top, xchg<2>(top));
+    if constexpr (TPR > 4) top = fmaxf(top, u2f(xchg4(f2u(top))));
+    if constexpr (TPR > 8) top = fmaxf(top, xchg<8>(top));
+    // All products are below 2^kBits units. (Of NaN, which the maximum passes over, the
+    // constant is NaN too.)
+    constexpr unsigned kBits = WIDE ? 30 : 15;
+    const unsigned ex = max(f2u(top) >> 23, 32u);
+    const float up = u2f((253 + kBits - ex) << 23);
+#pragma unroll
+    for (int i = 0; i < SPT; i += 4) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[i + k] *= up;
       if constexpr (WIDE) {
-        // The integer plus a bias that makes its lower bytes digits + 128.
+        // The nearest integer, plus a bias that makes its lower bytes digits + 128.
         unsigned x[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = (unsigned)(int)(qn[i + k] * ss[k]) + 0x808080u;
+        for (int k = 0; k < 4; ++k) x[k] = (unsigned)(int)__builtin_rintf(v[i + k]) + 0x808080u;
         const unsigned t0 = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u);
         const unsigned u0 = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u);
         const unsigned t1 = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u);
@@ -489,7 +503,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
         // (The second term is what the first cuts off, in the same units.)
 #pragma unroll
         for (int k = 0; k < 4; k += 2) {
-          const float x0 = qn[i + k] * ss[k], x1 = qn[i + k + 1] * ss[k + 1];
+          const float x0 = v[i + k], x1 = v[i + k + 1];
           const float h0 = u2f(f2u(x0) & 0xFFFFE000u), h1 = u2f(f2u(x1) & 0xFFFFE000u);
           out[0][(i + k) / 2] =
               __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(h0, h1));
@@ -518,8 +532,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
     if constexpr (TPR > 4) cgs += u2f(xchg4(f2u(cgs)));
     if constexpr (TPR > 8) cgs += xchg<8>(cgs);
     if (part == 0) {
-      const float c1 = q_unit * cs * kLog2e;
-      cc_s[buf][brow] = make_float2(WIDE ? c1 : c1 * 16777216.f, cgs * c1);
+      // (A product that is not finite makes the row NaN.)
+      const float unit = ex == 255u ? u2f(0x7FC00000u) : u2f((ex + 1 - kBits) << 23);
+      cc_s[buf][brow] =
+          make_float2(unit * (WIDE ? kLog2e : kLog2e * 16777216.f), cgs * kLog2e);
     }
   };
 
@@ -702,32 +718,21 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
       load_values(cur, vf);
       szr = load_sz(it0 + kWaves + w);
     }
-    // The row relative to its largest, in slot order (zeros behind the last row), and
-    // as it is to LDS for the drafts.
-    unsigned mx = 0;
+    // The row in slot order (zeros behind the last row), and as it is to LDS for the
+    // drafts.
 #pragma unroll
     for (int i = 0; i < NQ; ++i)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        qv[i][k] = brow < live ? qv[i][k] : 0.f;
-        mx = max(mx, f2u(qv[i][k]) & 0x7FFFFFFFu);
-      }
-    mx = max(mx, xchg_u32<1>(mx));
-    mx = max(mx, xchg_u32<2>(mx));
-    if constexpr (TPR > 4) mx = max(mx, xchg_u32<4>(mx));
-    if constexpr (TPR > 8) mx = max(mx, xchg_u32<8>(mx));
-    // (As bits, so that NaN is the largest and makes the row NaN.)
-    q_unit = u2f(max(mx, f2u(1e-30f)));
-    const float inv = 1.f / q_unit;
+      for (int k = 0; k < 8; ++k) qv[i][k] = brow < live ? qv[i][k] : 0.f;
 #pragma unroll
     for (int i = 0; i < SPT; ++i) {
       // Channel of slot i of eight, for a thread of the lower and of the upper four.
       auto of = [](int i) { return WIDE ? 2 * (i & 3) + (i >> 2) : 4 * (i & 1) + (i >> 1); };
       if constexpr (SPT >= 8) {
-        qn[i] = qv[i / 8][of(i % 8)] * inv;
+        qn[i] = qv[i / 8][of(i % 8)];
       } else {
         const unsigned up = part & 1 ? ~0u : 0u;
-        qn[i] = u2f((f2u(qv[0][of(i + 4)]) & up) | (f2u(qv[0][of(i)]) & ~up)) * inv;
+        qn[i] = u2f((f2u(qv[0][of(i + 4)]) & up) | (f2u(qv[0][of(i)]) & ~up));
       }
     }
     if (dr0 < dr1) {
