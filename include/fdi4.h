@@ -431,7 +431,7 @@ size_t fdi4_decode_rows_workspace_bytes(int batch, int num_q_heads, int nodes, i
  * fdi4_decode_paged_advance, or NULL. float32 outputs:
  * logits from products of queries and scales held to 29 bits of the largest of a row and
  * scale group, probabilities to 22 bits or more; 16-bit outputs: products to 21 bits
- * each, probabilities to 16 or more; sums in float32. Refused besides
+ * each and 24 of the largest, probabilities to 16 or more; sums in float32. Refused besides
  * what fdi4_decode_paged_ex refuses: more than 2^30 rows a sequence (max_pages *
  * page_rows), and page or scale-group strides that are negative or do not fit 32 bits
  * (bytes, scales in elements); pools may be larger than that. */

@@ -20,9 +20,13 @@
 //      against as many of the query; the constant sum_d v_d zp_d, in float32, goes in
 //      with the exponent's FMA. A product takes 16 keys (A) and 16 rows (B).
 //      The terms are in units of a power of two for the largest |v| of the row and the
-//      group. 16-bit outputs: two float16 terms. A nibble masked out of its word is a
-//      float16 of the smallest numbers, nib * 2^-24, or 16 times that;
-//      v_mfma_f32_16x16x32_f16.
+//      group. 16-bit outputs: two float16 terms of 11 bits (21 of v in all, and down to
+//      2^-39 of the largest), for v_mfma_f32_16x16x32_f16 with a nibble at bits 6 to 9 of
+//      a float16, the number nib * 2^-18. That instruction aligns a product of a number
+//      below 2^-14 as if it were 2^-14 and keeps 24 bits: nibbles in the lowest bits
+//      (nib * 2^-24) cost a sum of 32 2^-17 of its largest product, six bits up they cost
+//      2^-24, as float32 sums do. Three shifts a word more: 118 us in place of 116 for 64
+//      rows of bfloat16 at 16384 tokens.
 //      float32 outputs (WIDE): an integer below 2^30, in four balanced base-256 digits
 //      for v_mfma_i32_16x16x64_i8, whose exact sums meet in float32: as good as float32
 //      products of q and k (2-norm error 3e-7 over 300 keys of 128 channels, 4e-7 with
@@ -436,9 +440,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
     const int d0 = SL * (WIDE ? fresh(lane) : lane);
 #pragma unroll
     for (int k = 0; k < SL; ++k) {
-      const int d = d0 + k, at = sz_pos(row_slot<WIDE>(d));
-      // (Odd channels' nibbles are multiplied where they lie, four bits up.)
-      dst[at] = !WIDE && (d & 1) ? x.s[k] * 0.0625f : x.s[k];
+      const int at = sz_pos(row_slot<WIDE>(d0 + k));
+      dst[at] = x.s[k];
       dst[kSz + at] = x.z[k] * x.s[k];
     }
   };
@@ -535,7 +538,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
       // (A product that is not finite makes the row NaN.)
       const float unit = ex == 255u ? u2f(0x7FC00000u) : u2f((ex + 1 - kBits) << 23);
       cc_s[buf][brow] =
-          make_float2(unit * (WIDE ? kLog2e : kLog2e * 16777216.f), cgs * kLog2e);
+          make_float2(unit * (WIDE ? kLog2e : kLog2e * 262144.f), cgs * kLog2e);
     }
   };
 
@@ -762,8 +765,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
           }
         }
         // Nibbles of key block kb of chunk e: as bytes, or (eight channels a block) as
-        // float16, of which a nibble in the lowest bits is one of the smallest numbers,
-        // nib * 2^-24, and one four bits up is 16 times that.
+        // float16, nib * 2^-18.
         constexpr int KB = WIDE ? NB : G::KW;
         auto key_op = [&](int e, int kb) __attribute__((always_inline)) -> v4i {
           if constexpr (WIDE) {
@@ -771,9 +773,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
             return v4i{(int)(w0 & 0x0F0F0F0Fu), (int)((w0 >> 4) & 0x0F0F0F0Fu),
                        (int)(w1 & 0x0F0F0F0Fu), (int)((w1 >> 4) & 0x0F0F0F0Fu)};
           }
-          const unsigned w0 = kf.w[e][kb], w1 = w0 >> 8;
-          return v4i{(int)(w0 & 0x000F000Fu), (int)(w0 & 0x00F000F0u),
-                     (int)(w1 & 0x000F000Fu), (int)(w1 & 0x00F000F0u)};
+          const unsigned w0 = kf.w[e][kb];
+          return v4i{(int)(w0 << 6 & 0x03C003C0u), (int)(w0 << 2 & 0x03C003C0u),
+                     (int)(w0 >> 2 & 0x03C003C0u), (int)(w0 >> 6 & 0x03C003C0u)};
         };
         // With one row tile they are made where they are used (registers), with two
         // once for both, and the next keys are loaded over the words.
