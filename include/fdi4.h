@@ -427,7 +427,8 @@ size_t fdi4_decode_rows_workspace_bytes(int batch, int num_q_heads, int nodes, i
  * t >= n - window, n its length (the query is that of its last token); window >= 1,
  * sinks >= 0. Only the pages of those rows are read. The cache has group-indexed
  * scales (s_page_stride 0) and no page_lens. out is contiguous [batch,
- * num_q_heads, head_dim]; a sequence with no row gives zeros. lens_out as in
+ * num_q_heads, head_dim]; a sequence with no row gives zeros, rows whose logits are
+ * all -infinity, or whose query is not finite, NaN. lens_out as in
  * fdi4_decode_paged_advance, or NULL. float32 outputs:
  * logits from products of queries and scales held to 29 bits of the largest of a row and
  * scale group, probabilities to 22 bits or more; 16-bit outputs: products to 21 bits

@@ -622,7 +622,7 @@ __global__ __launch_bounds__(64) void merge_kernel(const float* __restrict__ ws_
 #pragma unroll
     for (int k = 0; k < CH; ++k) o[k] += (double)(t[0].v[k] + t[1].v[k]);
   }
-  const float r = fmaxf((float)l, 1e-10f);
+  const float r = ms == kNoFinite ? __builtin_nanf("") : fmaxf((float)l, 1e-10f);
 #pragma unroll
   for (int k = 0; k < CH; ++k)
     store_elem(out, (int64_t)b * o_b + (int64_t)h * o_h + lane * CH + k, out_dtype,

@@ -245,4 +245,8 @@ __device__ __forceinline__ float exp2_of(double x) {
   return __builtin_amdgcn_exp2f((float)(x * 1.4426950408889634));
 }
 
+// Maximum of a split partial whose row sees keys, all with logits of -infinity: it weighs
+// nothing beside a split with a finite logit, and without one the row is NaN.
+constexpr double kNoFinite = -1.7976931348623157e308;
+
 }  // namespace fdi4

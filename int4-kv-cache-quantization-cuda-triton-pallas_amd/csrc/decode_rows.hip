@@ -48,7 +48,8 @@
 //
 // A non-finite value times a probability of zero is NaN, though the row does not see
 // it: a workgroup that ends with a NaN goes through its range again, row by row and key
-// by key.
+// by key. Rows whose query is not finite are NaN without it, if they see anything: a
+// batch padded with such rows is no slower.
 //
 // What bounds it. Up to 32 rows a kv-head: memory. 8 sequences of 8 kv-heads with 128
 // bfloat16 channels and 16 rows read their tokens at 6.8 TB/s once they are many, on top
@@ -236,6 +237,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
   __shared__ float2 cc_s[2][M];                    // a row's logit unit and constant
   __shared__ int low_s[M];                         // first cached token in a row's window
   __shared__ int ext_s[2];                         // smallest and largest of them
+  __shared__ int seen_s[M];                        // a row sees a key of this range
+  __shared__ int wild_s[M];                        // its query is not finite
   __shared__ float m_s[kWaves][M], l_s[kWaves][M];
   __shared__ int bad_s;
   float* const q_s = reinterpret_cast<float*>(smem + G::kQ);
@@ -314,6 +317,16 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
   const int it0 = min(i0, ng), it1 = min(i1, ng);
   const int dr0 = max(i0, ng) - ng, dr1 = max(i1, ng) - ng;
   auto group_of = [&](int it) { return it < nsg ? it : it - nsg + gw0; };
+  // Whether a row sees a cached token of the range (a group of the sinks begins with
+  // one; those of the window follow one another), and no draft yet.
+  if (tid < M) {
+    const int w0 = max(it0, nsg), t0 = (w0 - nsg + gw0) * group_rows;
+    const int t1 = min((it1 - nsg + gw0) * group_rows, n);
+    seen_s[tid] = it0 < min(it1, nsg) ||
+                  (w0 < it1 && (max(t0, low_s[tid]) < t1 || t0 < min(a.sinks, t1)));
+    wild_s[tid] = 0;
+  }
+  if (tid == 0) bad_s = 0;
 
   const float* sbase = c.k_scale + (int64_t)b * c.s_b + (int64_t)hk * c.s_h;
   const float* zbase = c.k_zp + (int64_t)b * c.s_b + (int64_t)hk * c.s_h;
@@ -746,9 +759,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
         *reinterpret_cast<float4*>(dst + 4) = make_float4(qv[i][4], qv[i][5], qv[i][6], qv[i][7]);
       }
     }
-    if (tid == 0) bad_s = 0;
     if (steps > 0) stage_sz(sz0, it0 + w);
     __syncthreads();
+    // (Every logit of such a row is infinite or NaN, and the row NaN.)
+    unsigned big = 0;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) big = max(big, f2u(qv[i][k]) & 0x7FFFFFFFu);
+    if (big >= 0x7F800000u) wild_s[brow] = 1;
     if (steps > 0) {
       build(it0);
       int it = it0, p = 0;
@@ -975,12 +994,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
           vis[rt] |= (unsigned)((mb[rt][k] != 0) & (4 * grp + k < nval)) << k;
           s[rt][k] = ds[rt][k];
         }
+        if (vis[rt]) seen_s[rt * 16 + n16] = 1;
       }
       softmax(s, c1, cc, true, vis);
       add_values(vf);
     }
-  } else if (tid == 0) {
-    bad_s = 0;
   }
 
   // The range again for every row by itself, a wave a row and key after key, for the
@@ -1005,6 +1023,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
     for (int i = tid; i < kWaves * M * G::AS; i += NT) part0[i] = 0.f;
     __syncthreads();
     for (int r = w; r < live; r += NT / 64) {
+      if (wild_s[r]) continue;
       const int i = (row0 + r) % a.nodes;
       const int64_t q0 = (int64_t)b * c.q_b +
                          (int64_t)(hk * c.hq_per_kv + (row0 + r) / a.nodes) * c.q_h +
@@ -1079,6 +1098,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
 #pragma unroll
     for (int i = 1; i < kWaves; ++i) top = fmaxf(top, m_s[i][r]);
     const float f = __builtin_amdgcn_exp2f(m_run[rt] - top);
+    const bool wild = wild_s[r];
 #pragma unroll
     for (int u = 0; u < G::NP; ++u)
 #pragma unroll
@@ -1090,7 +1110,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
           const float4 x = make_float4(acc[rt][t][i] * f, acc[rt][t + 1][i] * f,
                                        acc[rt][t + 2][i] * f, acc[rt][t + 3][i] * f);
           *reinterpret_cast<float4*>(dst + j) = x;
-          any_nan += (x.x + x.y) + (x.z + x.w);
+          any_nan += wild ? 0.f : (x.x + x.y) + (x.z + x.w);
         }
       }
   }
@@ -1118,16 +1138,26 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
       o.z += x.z;
       o.w += x.w;
     }
+    if (wild_s[r]) {
+      l = 0.f;
+      o = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    // (No finite logit, hence no probability: zero where the row sees nothing, otherwise
+    // NaN, 0 / 0 as in the formula.)
+    const bool none = l == 0.f, seen = seen_s[r];
     if (zc.final_out) {
       const float os[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        store_elem(zc.out, (o0 + r) * D + d + k, zc.out_dtype, l == 0.f ? 0.f : os[k] / l);
+        store_elem(zc.out, (o0 + r) * D + d + k, zc.out_dtype,
+                   none && !seen ? 0.f : os[k] / l);
     } else {
       const int64_t pi = (o0 + r) * zc.num_splits + split;
       *reinterpret_cast<float4*>(zc.ws_acc + pi * D + d) = o;
       if (d == 0) {
-        zc.ws_ml[2 * pi] = l == 0.f ? -INFINITY : (double)top * 0.6931471805599453;
+        zc.ws_ml[2 * pi] = !none  ? (double)top * 0.6931471805599453
+                           : seen ? kNoFinite
+                                  : -INFINITY;
         zc.ws_ml[2 * pi + 1] = (double)l;
       }
     }
