@@ -997,6 +997,22 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
         if (vis[rt]) seen_s[rt * 16 + n16] = 1;
       }
       softmax(s, c1, cc, true, vis);
+      // Drafts that no row of the workgroup sees keep no value either (a batch of trees
+      // may be padded with anything).
+      unsigned any = vis[0];
+      if constexpr (RT > 1) any |= vis[1];
+      any |= xchg_u32<1>(any);
+      any |= xchg_u32<2>(any);
+      any |= xchg4(any);
+      any |= xchg_u32<8>(any);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned keep = any >> i & 1u ? ~0u : 0u;
+#pragma unroll
+        for (int u = 0; u < G::NP; ++u)
+#pragma unroll
+          for (int x = 0; x < G::PB / 4; ++x) vf.w[0][i][u][x] &= keep;
+      }
       add_values(vf);
     }
   }

@@ -135,3 +135,24 @@ def test_drafts_of_minus_infinity(splits):
     none[2] = False
     assert torch.equal(attend(c, q, kd=kd, vd=vd, mask=none, splits=splits)[0, :, 2],
                        out[0, :, 2])
+
+
+@pytest.mark.parametrize("values,query", [("float32", "float32"), ("float16", "float32"),
+                                          ("bfloat16", "float32"), ("bfloat16", "bfloat16")])
+@pytest.mark.parametrize("D,nodes,used", [(64, 7, 3), (128, 40, 33), (256, 20, 11), (64, 150, 70)])
+def test_values_of_drafts_that_no_node_sees(values, query, D, nodes, used):
+    """Keys and values of padding drafts may be anything: NaN in them gives the bits that
+    zeros give (a workgroup that had to go row by row would round otherwise)."""
+    import torch
+    c = make_cache(nodes, 2, 2, D, [300, 40], values)
+    q = queries(c, 4, nodes, query)
+    kd, vd = drafts(c, nodes)
+    mask = torch.ones(2, nodes, nodes, dtype=torch.bool, device="cuda").tril()
+    mask[:, :, used:] = False
+    outs = []
+    for fill in (0, float("nan"), INF):
+        kd[:, :, used:] = fill
+        vd[:, :, used:] = fill
+        outs.append(attend(c, q, kd=kd, vd=vd, mask=mask))
+    assert outs[0].isfinite().all()
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
