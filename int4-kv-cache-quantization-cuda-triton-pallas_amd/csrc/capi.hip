@@ -1111,11 +1111,9 @@ int fdi4_read_paged(const fdi4_paged_cache* cache, int batch, const int32_t* sta
   if (cache->s_page_stride != 0 || cache->page_lens || batch < 0 || batch > 65535 ||
       start0 < 0 || length < 0 || !valid_elem_dtype(out_dtype))
     return hipErrorInvalidValue;
-  const int64_t G = (int64_t)cache->pages_per_group * cache->page_rows;
   const int64_t cap = (int64_t)cache->max_pages * cache->page_rows;
-  // Token positions, and the groups that a range reaches past the end, in 32 bits.
-  if (G > INT32_MAX / 4 || std::max<int64_t>(cap, start0) + length > INT32_MAX - 2 * G)
-    return hipErrorInvalidValue;
+  // Token positions, and the rows of a workgroup behind the last, in 32 bits.
+  if (std::max<int64_t>(cap, start0) + length > INT32_MAX - 256) return hipErrorInvalidValue;
   if (batch == 0 || length == 0) return hipSuccess;
   const int oeb = out_dtype == FDI4_K_F32 ? 4 : 2;
   if (!k_out || !v_out || !aligned(k_out, 16) || !aligned(v_out, 16) ||
@@ -1126,6 +1124,8 @@ int fdi4_read_paged(const fdi4_paged_cache* cache, int batch, const int32_t* sta
   // The cache part of a decode's arguments (the query is not used).
   rc = make_decode_args(k_out, FDI4_K_F32, batch, cache->num_kv_heads, 0, 0, cache, 1, &a.c);
   if (rc != hipSuccess) return rc;
+  // A group larger than a sequence is the one group that the sequence has.
+  a.c.pages_per_group = std::min(cache->pages_per_group, std::max(cache->max_pages, 1));
   a.start = start;
   a.start0 = start0;
   a.length = length;

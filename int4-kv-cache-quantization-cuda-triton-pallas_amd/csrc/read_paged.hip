@@ -15,6 +15,8 @@
 // a workgroup for the whole group, took 85 us there, 31 us against 25 for 1000 tokens
 // of 8 sequences (85 MB, to float32) and 15 against 10 for 16 sequences' open groups.
 
+#include <algorithm>
+
 #include "decode_common.hpp"
 
 namespace fdi4 {
@@ -49,7 +51,7 @@ constexpr int kReadRows = 4;
 
 template <int D, int VDT, int OUT>
 __global__ __launch_bounds__(kReadThreads) void read_paged_kernel(ReadArgs a, int slots,
-                                                                  int pieces, int heads) {
+                                                                  int heads) {
   constexpr int TPR = D / 8;                  // threads per row
   constexpr int RPS = kReadThreads / TPR;     // rows per sweep
   constexpr int U = kReadRows;
@@ -58,8 +60,6 @@ __global__ __launch_bounds__(kReadThreads) void read_paged_kernel(ReadArgs a, in
   constexpr int VL = VDT == kVF32 ? 2 : 1;    // 16-byte value loads per row
   const DecodeArgs& c = a.c;
   unsigned wi = blockIdx.x;
-  const int piece = (int)(wi % (unsigned)pieces);
-  wi /= (unsigned)pieces;
   const int slot = (int)(wi % (unsigned)slots);
   wi /= (unsigned)slots;
   const int h = (int)(wi % (unsigned)heads), b = (int)(wi / (unsigned)heads);
@@ -67,10 +67,13 @@ __global__ __launch_bounds__(kReadThreads) void read_paged_kernel(ReadArgs a, in
   const int G = c.pages_per_group * c.page_rows;
   const int start = a.start ? min(max(a.start[b], 0), cap) : a.start0;
   const int T = seq_len_of(c, b);
-  // Rows of this workgroup: its piece of its group, within the range (64 bits: a range
-  // may end anywhere), counted from the range's start.
-  const int g = start / G + slot;
-  const int64_t p0 = (int64_t)g * G + (int64_t)piece * (RPS * U);
+  // Rows of this workgroup: a piece of a group, the slot-th from the one that holds the
+  // range's start, within the range (64 bits: a range may end anywhere), counted from
+  // its start.
+  const unsigned pieces = ((unsigned)G + RPS * U - 1) / (RPS * U);
+  const unsigned at = (unsigned)(start % G) / (RPS * U) + (unsigned)slot;
+  const int g = start / G + (int)(at / pieces);
+  const int64_t p0 = (int64_t)g * G + (int64_t)(at % pieces) * (RPS * U);
   const int64_t p1 = min(p0 + RPS * U, (int64_t)(g + 1) * G);
   const int i0 = (int)max(p0 - start, (int64_t)0);
   const int i1 = (int)min(p1 - start, (int64_t)a.length);
@@ -146,17 +149,24 @@ hipError_t launch_read_paged(const ReadArgs& a, int D, int v_dtype, int batch, i
   if (batch == 0 || heads == 0 || a.length == 0) return hipSuccess;
   const int64_t G = (int64_t)a.c.pages_per_group * a.c.page_rows;
   const int per = kReadThreads / (D / 8) * kReadRows;
-  // Groups that a range of this length touches from any start (all of them from this
-  // one), and workgroups for a group's rows (no more than the range needs).
-  const int64_t slots = a.start ? (a.length + 2 * G - 2) / G
-                                : (a.start0 + (int64_t)a.length - 1) / G - a.start0 / G + 1;
+  // Pieces that the range touches: of its groups' pieces as many as begin in it, at most
+  // one per `per` rows and one per further group, and the one that holds its start.
+  // (Counted from this start, or the most from any.)
   const int64_t pieces = (G + per - 1) / per;
-  const int64_t items = slots * pieces * heads * batch;
+  int64_t slots;
+  if (a.start) {
+    const int64_t groups = ((int64_t)a.length + 2 * G - 2) / G;
+    slots = std::min(groups * pieces, (a.length - 1) / per + 1 + groups);
+  } else {
+    const int64_t last = a.start0 + (int64_t)a.length - 1;
+    slots = (last / G - a.start0 / G) * pieces + last % G / per - a.start0 % G / per + 1;
+  }
+  const int64_t items = slots * heads * batch;
   if (items > INT32_MAX) return hipErrorInvalidValue;
 #define FDI4_RD(DD, VV, OO)                                                               \
   if (D == DD && v_dtype == VV && a.out_dtype == OO) {                                    \
     hipLaunchKernelGGL((read_paged_kernel<DD, VV, OO>), dim3((unsigned)items),            \
-                       dim3(kReadThreads), 0, st, a, (int)slots, (int)pieces, heads);     \
+                       dim3(kReadThreads), 0, st, a, (int)slots, heads);     \
     return hipGetLastError();                                                             \
   }
 #define FDI4_RD_O(DD, VV) FDI4_RD(DD, VV, kEF32) FDI4_RD(DD, VV, kEF16) FDI4_RD(DD, VV, kEBF16)
