@@ -336,6 +336,22 @@ class INT4PagedSequenceCache:
         if self._unsynced_steps:
             self.sync_lengths()
 
+    def _check_room(self, B: int, n: int, who: str) -> None:
+        """Raise unless the pages mapped for sequences 0..B-1 hold n more tokens each."""
+        import torch
+
+        def short():
+            return np.nonzero(self._lens[:B] + self._unsynced_steps + n > self._mapped[:B])[0]
+
+        at = short()
+        if len(at) and self._unsynced_steps and not torch.cuda.is_current_stream_capturing():
+            # Counts on the device may be smaller than what the host adds up for them.
+            self.sync_lengths()
+            at = short()
+        if len(at):
+            raise RuntimeError(f"{who} write past the pages reserved for sequence "
+                               f"{int(at[0])}; call reserve() first")
+
     def _release(self, b: int) -> None:
         """Host side of free(): sequence b's pages go back to the free list."""
         self._free.extend(reversed(self._pages[b]))
@@ -455,7 +471,10 @@ class INT4PagedSequenceCache:
         With counts on the host the pages are mapped here. With counts on the GPU
         nothing goes through the host, so the call can be captured into a graph; the
         pages of N tokens per sequence must be reserved (reserve), and the lengths
-        are known to the host only after sync_lengths(), as after step()."""
+        are known to the host only after sync_lengths(), as after step(). Until then the
+        host counts N tokens for every such call; an eager call that could by that count
+        pass the reservation reads the lengths from the device (a synchronization) before
+        it refuses."""
         import torch
         if k_new.dim() != 4 or k_new.shape[1] != self.num_kv_heads or \
                 k_new.shape[3] != self.head_dim or tuple(v_new.shape) != tuple(k_new.shape):
@@ -470,10 +489,7 @@ class INT4PagedSequenceCache:
         if on_device:
             if counts.dtype != torch.int32 or tuple(counts.shape) != (B,):
                 raise ValueError("counts on the GPU must be int32 [batch]")
-            short = np.nonzero(self._lens[:B] + self._unsynced_steps + N > self._mapped[:B])[0]
-            if len(short):
-                raise RuntimeError(f"extend() could write past the pages reserved for sequence "
-                                   f"{int(short[0])}; call reserve() first")
+            self._check_room(B, N, "extend() could")
             n = None
         else:
             if torch.cuda.is_current_stream_capturing():
@@ -543,10 +559,7 @@ class INT4PagedSequenceCache:
         B = k_new.shape[0]
         if B > self.max_seqs or tuple(k_new.shape) != (B, self.num_kv_heads, self.head_dim):
             raise ValueError("k_new must be [batch <= max_seqs, kv_heads, head_dim]")
-        short = np.nonzero(self._lens[:B] + self._unsynced_steps + 1 > self._mapped[:B])[0]
-        if len(short):
-            raise RuntimeError(f"step() would write past the pages reserved for sequence "
-                               f"{int(short[0])}; call reserve() first")
+        self._check_room(B, 1, "step() would")
         if window is not None:
             import torch
             # (Refused here, what the attention would refuse with the token appended.)
