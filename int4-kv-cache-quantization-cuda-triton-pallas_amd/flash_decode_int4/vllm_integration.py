@@ -284,8 +284,10 @@ class INT4PagedSequenceCache:
         self._lens = np.zeros(max_seqs, dtype=np.int64)
         self._mapped = np.zeros(max_seqs, dtype=np.int64)   # tokens the mapped pages hold
         # Eager step() calls since the host lengths were last read from the
-        # device (replays of a captured step() are not counted).
+        # device (replays of a captured step() are not counted), and whether one was
+        # captured: its replays may have moved the lengths at any time.
         self._unsynced_steps = 0
+        self._captured = False
 
     # ---- page bookkeeping (host) -------------------------------------------
 
@@ -333,7 +335,9 @@ class INT4PagedSequenceCache:
     def _sync_if_stepped(self) -> None:
         # step() advances the lengths on the device only; host-side page
         # mapping must start from the device's lengths.
-        if self._unsynced_steps:
+        import torch
+        if self._unsynced_steps or (self._captured
+                                    and not torch.cuda.is_current_stream_capturing()):
             self.sync_lengths()
 
     def _check_room(self, B: int, n: int, who: str) -> None:
@@ -344,7 +348,9 @@ class INT4PagedSequenceCache:
             return np.nonzero(self._lens[:B] + self._unsynced_steps + n > self._mapped[:B])[0]
 
         at = short()
-        if len(at) and self._unsynced_steps and not torch.cuda.is_current_stream_capturing():
+        capturing = torch.cuda.is_current_stream_capturing()
+        self._captured |= capturing
+        if len(at) and self._unsynced_steps and not capturing:
             # Counts on the device may be smaller than what the host adds up for them.
             self.sync_lengths()
             at = short()

@@ -63,3 +63,46 @@ def test_in_a_capture_the_count_of_the_host_stands():
         graph.replay()
         torch.cuda.synchronize()
         assert cache.seq_lens.tolist() == [3 * i + 3] * 2
+
+
+@pytest.mark.parametrize("how", ["extend", "append", "reserve", "read"])
+def test_replays_after_a_sync_are_seen(how):
+    """Replays of a captured extend move the lengths after the host last read them: a call
+    that maps pages or counts tokens on the host starts from the device's."""
+    import torch
+    cache = make()
+    k = tokens(16)
+    n = torch.tensor([16, 9], dtype=torch.int32, device="cuda")
+    cache.extend(k, k)
+    cache.reserve(2, 160)
+    cache.extend(k, k, n)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.extend(k, k, n)
+    cache.sync_lengths()
+    for _ in range(8):
+        graph.replay()
+    used = [16 + 16 * 9, 16 + 9 * 9]
+    big = tokens(70, seed=1)
+    if how == "extend":
+        cache.extend(big, big)
+        new, want = 70, big
+    elif how == "append":
+        cache.append(k[:, :, 0], k[:, :, 0])
+        new, want = 1, k[:, :, :1]
+    elif how == "reserve":
+        cache.reserve(2, 70)
+        cache.extend(big, big, torch.full((2,), 70, dtype=torch.int32, device="cuda"))
+        cache.sync_lengths()
+        new, want = 70, big
+    else:
+        new, want = 0, None
+    assert cache.read(2)[0].shape[2] == used[0] + new
+    assert cache.seq_lens.tolist() == cache.lengths().tolist() == [u + new for u in used]
+    pages = cache.page_table.cpu().numpy()
+    held = [pages[b, i] for b in range(2) for i in range(-(-(used[b] + new) // 16))]
+    assert len(set(held)) == len(held)
+    for b in range(2):
+        v = cache.read(2)[1][b, :, used[b]:used[b] + new]
+        assert want is None or torch.equal(v, want[b, :, :new])
