@@ -431,8 +431,10 @@ size_t fdi4_decode_rows_workspace_bytes(int batch, int num_q_heads, int nodes, i
  * all -infinity, or whose query is not finite, NaN. lens_out as in
  * fdi4_decode_paged_advance, or NULL. float32 outputs:
  * logits from products of queries and scales held to 29 bits of the largest of a row and
- * scale group, probabilities to 22 bits or more; 16-bit outputs: products to 21 bits
- * each and 24 of the largest, probabilities to 16 or more; sums in float32. Refused besides
+ * scale group, probabilities to 24 bits (float16 values: 22); 16-bit outputs: products
+ * to 21 bits each and 24 of the largest, probabilities to 16 bits with bfloat16 values,
+ * 22 with float16 and 24 with float32 ones; sums in float32. A workgroup in which a value
+ * that is not finite is seen takes its rows one by one, much more slowly. Refused besides
  * what fdi4_decode_paged_ex refuses: more than 2^30 rows a sequence (max_pages *
  * page_rows), and page or scale-group strides that are negative or do not fit 32 bits
  * (bytes, scales in elements); pools may be larger than that. */
@@ -453,7 +455,10 @@ int fdi4_decode_window(const void* query, int query_dtype, int batch, int num_q_
  * drafts, attends the cached rows t < sinks and t >= n + d_i - window: the last
  * `window` tokens of the sequence that it ends. out is contiguous [batch,
  * num_q_heads, nodes, head_dim]; a node that sees no row and no draft gives zeros.
- * Precision and refusals are fdi4_decode_window's. The accepted drafts go to the cache with fdi4_extend_paged. */
+ * Precision and refusals are fdi4_decode_window's. The drafts' keys are attended as
+ * they are, in float32; the accepted ones go to the cache, quantized, with
+ * fdi4_extend_paged. Drafts that no node sees and the queries of unused nodes may hold
+ * anything. */
 int fdi4_decode_tree(const void* query, int query_dtype, int batch, int num_q_heads, int nodes,
                      int64_t q_batch_stride, int64_t q_head_stride, int64_t q_node_stride,
                      const float* k_draft, int64_t kd_batch_stride, int64_t kd_head_stride,

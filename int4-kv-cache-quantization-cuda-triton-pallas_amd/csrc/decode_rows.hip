@@ -42,28 +42,31 @@
 //   values: lane (g, r) loads the channels 8r.. of rows 4g .. 4g+3, byte permutes pair
 //      the rows, and one product takes 32 keys. A probability is the sum of two
 //      (float16: 22 bits; bfloat16: 16) or three (bfloat16 values, float32 output:
-//      24) terms. float32 values are three bfloat16 terms like it: 58 us, where
+//      24) terms. (16 bits are off by a 64th of a float16 output's half step, a 512th of a
+//      bfloat16 one's; a third term took 128 us in place of 118 for 64 rows at 16384
+//      tokens, and changed one bfloat16 output in 1300.) float32 values are three bfloat16 terms like it: 58 us, where
 //      v_mfma_f32_16x16x4_f32 took 68 (100 drafts of four sequences of up to 3000
 //      tokens).
 //
 // A non-finite value times a probability of zero is NaN, though the row does not see
 // it: a workgroup that ends with a NaN goes through its range again, row by row and key
-// by key. Rows whose query is not finite are NaN without it, if they see anything: a
-// batch padded with such rows is no slower.
+// by key (14 ms where eight sequences of 8192 tokens all do, 71 us otherwise). Rows whose
+// query is not finite are NaN without it, if they see anything, and values that no row
+// sees are dropped: a batch padded with either is no slower.
 //
 // What bounds it. Up to 32 rows a kv-head: memory. 8 sequences of 8 kv-heads with 128
-// bfloat16 channels and 16 rows read their tokens at 6.8 TB/s once they are many, on top
+// bfloat16 channels and 16 rows read their tokens at 6.5 TB/s once they are many, on top
 // of 11 us (launch, the first loads' chain, the waves' and the splits' merges): 37 us at
-// 8192 tokens, 62 us at 16384, 5.5 TB/s in all. More rows: each further workgroup of 32
+// 8192 tokens, 64 us at 16384, 5.4 TB/s in all. More rows: each further workgroup of 32
 // rows takes its keys again, from L2, and the time follows the rows: 126 us for 64 rows
-// at 16384 tokens, 221 us for 128, of which 115 and 203 us remain where all pages lie in
-// L2. A step (32 keys by 32 rows, a wave) takes about 7300 cycles, two waves a SIMD,
-// with the VALU busy for half of them, the matrix cores for a quarter, and the rest
-// waits for LDS, dependent results and the barrier.
+// at 16384 tokens, 221 us for 128, of which 114 and 204 us remain where all pages lie in
+// L2. A step (32 keys by 32 rows, a wave) takes about 7800 cycles, two waves a SIMD,
+// with the VALU busy for 54 % of them, the matrix cores for 28 %; the rest waits for LDS,
+// dependent results and the barrier.
 //
 // RT: one tile up to 16 rows (and at 256 channels, whose accumulators fill the registers
-// with one), two beyond: 32 rows in one workgroup read the cache once (75 us at 16384
-// tokens, 62 us for 16 rows). Four tiles in one workgroup of eight waves were slower
+// with one), two beyond: 32 rows in one workgroup read the cache once (78 us at 16384
+// tokens, 64 us for 16 rows). Four tiles in one workgroup of eight waves were slower
 // than two workgroups of two: one barrier for all of them.
 // STREAM: non-temporal loads where one workgroup reads a page, cached ones where the
 // workgroups of several tiles do, which run on one XCD one after the other.

@@ -365,7 +365,17 @@ def flash_decode_paged(query, k_pages, v_pages, k_scale, k_zp, page_table, seq_l
 
     ``window``: attend only the last ``window`` tokens of each sequence (the
     query is that of its last token) and its first ``sinks``; the pages between
-    are not read. It needs seq_lens and the grouped scales, not page_lens.
+    are not read. It needs seq_lens and the grouped scales, not page_lens. With a
+    window (and in ``flash_decode_paged_tree``) sums are float32 and their factors
+    narrower: for float32 outputs products of queries and scales keep 29 bits of the
+    largest of a row and scale group, probabilities 24 (22 with float16 values); for
+    16-bit outputs the products 21 bits each, probabilities 22 (16 with bfloat16
+    values, 24 with float32 ones). Without it logits are float64 and probabilities
+    keep 24 bits.
+
+    Values that are not finite come out as the formula has them; where a query sees
+    one, the sequence's rows of that kv-head are computed one by one, which may take
+    a hundred times as long.
     """
     _check_window(window, sinks)
     _require_device_of(query)
@@ -409,8 +419,15 @@ def flash_decode_paged_tree(query, k_draft, v_draft, mask, k_pages, v_pages, k_s
     with rows on 16-byte boundaries); mask bool [N, N] or [B, N, N]: node i sees
     draft j where mask[.., i, j]. For a tree that is a node's ancestors and itself,
     for a chunk of a prompt the lower triangle; any mask is taken as it is. The
-    cache's tensors are those of ``flash_decode_paged``. Returns [B, Hq, N, D] in
-    the query's dtype; a node that sees no cached token and no draft gives zeros.
+    cache's tensors are those of ``flash_decode_paged``, and so is the precision.
+    Returns [B, Hq, N, D] in the query's dtype; a node that sees no cached token and
+    no draft gives zeros. Drafts that no node sees and queries of unused nodes may
+    hold anything.
+
+    The drafts' keys are attended as they are, in float32, and quantized only when
+    they are accepted: a node's output differs from that of the same tokens appended
+    one by one (``INT4PagedSequenceCache.step``), which attends each with its key
+    quantized, by the quantization error of the drafts that it sees.
 
     ``window`` (at least N): node i, seeing d drafts, attends the cache's last
     ``window - d`` tokens, which with its drafts are the last ``window`` tokens of

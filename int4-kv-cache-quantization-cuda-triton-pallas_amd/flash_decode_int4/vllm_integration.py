@@ -619,7 +619,7 @@ class INT4PagedSequenceCache:
         Hq a multiple of kv_heads) over sequences 0..B-1; returns [B, Hq, D] in
         the query's dtype (float32 arithmetic, one rounding at the end). With a
         window only over each sequence's last ``window`` and first ``sinks``
-        tokens."""
+        tokens (ops.flash_decode_paged says to how many bits)."""
         B = query.shape[0]
         return ops.flash_decode_paged(query, self.k_pages, self.v_pages, self.k_scale[:B],
                                       self.k_zp[:B], self.page_table[:B], self.seq_lens[:B],
@@ -633,7 +633,8 @@ class INT4PagedSequenceCache:
         and v_draft (the cache's value dtype) [B, kv_heads, N, D], over sequences
         0..B-1 and the drafts that mask ([N, N] or [B, N, N] bool) shows each of them
         (ops.flash_decode_paged_tree). Writes nothing; extend() takes the accepted
-        drafts."""
+        drafts, whose keys are quantized then: until then they are attended as they
+        are."""
         B = query.shape[0]
         return ops.flash_decode_paged_tree(
             query, k_draft, v_draft, mask, self.k_pages, self.v_pages, self.k_scale[:B],
