@@ -156,3 +156,63 @@ def test_values_of_drafts_that_no_node_sees(values, query, D, nodes, used):
         outs.append(attend(c, q, kd=kd, vd=vd, mask=mask))
     assert outs[0].isfinite().all()
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("bad", [INF, float("nan")])
+@pytest.mark.parametrize("values,query", [("float32", "float32"), ("bfloat16", "bfloat16"),
+                                          ("float16", "float32")])
+@pytest.mark.parametrize("D,splits", [(64, 0), (128, 1), (256, 3)])
+def test_scales_that_are_not_finite(D, splits, values, query, bad):
+    """A key scale of infinity or NaN in group 3 of one head of one sequence makes that
+    head's rows NaN that see the group; other heads and sequences keep their bits, and nodes
+    whose window begins behind the group their values."""
+    import torch
+    c = make_cache(D, 2, 2, D, [640, 600], values)
+    q = queries(c, 4, query=query)
+    want = attend(c, q, 300, 10, splits)
+    N = 9
+    qt = queries(c, 4, N, query)
+    kd, vd = drafts(c, N)
+    mask = torch.ones(N, N, dtype=torch.bool, device="cuda").tril()
+    # Node i attends from 640 + i + 1 - 133 on: nodes 0 .. 3 see tokens of group 3 (384 ..
+    # 511), the others none.
+    tree = attend(c, qt, 133, 0, splits, kd, vd, mask)
+    c["s"][0, 1, 3, 7] = bad
+    out = attend(c, q, 300, 10, splits)
+    assert out[0, 2:].isnan().all()
+    assert torch.equal(out[0, :2], want[0, :2]) and torch.equal(out[1], want[1])
+    out = attend(c, qt, 133, 0, splits, kd, vd, mask)
+    assert out[0, 2:, :4].isnan().all()
+    assert torch.equal(out[0, :2], tree[0, :2]) and torch.equal(out[1], tree[1])
+    a, b = out[0, 2:, 4:].float(), tree[0, 2:, 4:].float()
+    # (Row by row in float32 against the matrix cores: both within test_gpu_rows' bound of
+    # the definition, 8 * 2^-24 A * 5 of single elements, and rounded once each.)
+    A = (qt.abs().float().amax((0, 1, 2)) * torch.from_numpy(
+        np.where(np.isfinite(c["s"]), c["s"], 0).max((0, 1, 2))
+        * (15 + np.abs(c["z"]).max((0, 1, 2)))).cuda()).sum().item()
+    eps = {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -8}[query]
+    p = 2.0 ** -17 if query == "bfloat16" else 2.0 ** -22
+    vmax = max(1, b.abs().max().item())
+    assert (a - b).abs().max() <= 2 * (8 * 2.0 ** -24 * A * 5 + 5 * p + eps * vmax)
+
+
+@pytest.mark.parametrize("D,Hq", [(64, 4), (128, 16), (256, 4), (128, 4)])
+@pytest.mark.parametrize("splits", [0, 1, 4])
+def test_an_infinite_value_beside_a_query_that_is_not_finite(D, Hq, splits):
+    """The workgroup goes row by row for the value and leaves the bad row out."""
+    import torch
+    c = make_cache(D, 1, 1, D, [500], "bfloat16")
+    N = 5
+    q = queries(c, Hq, N)
+    kd, vd = drafts(c, N)
+    mask = torch.ones(N, N, dtype=torch.bool, device="cuda").tril()
+    q[:, 1, 2, 3] = INF
+    c["v"][c["table"][0, 499 // 16], :, 499 % 16, 9] = INF
+    vd[:, :, 4, 11] = -INF
+    out = attend(c, q, 100, 2, splits, kd, vd, mask)
+    assert out[:, 1, 2].isnan().all()
+    out[:, 1, 2] = out[:, 0, 2]
+    assert torch.isposinf(out[..., 9]).all() and torch.isneginf(out[:, :, 4, 11]).all()
+    out[..., 9] = 0
+    out[:, :, 4, 11] = 0
+    assert out.isfinite().all()
