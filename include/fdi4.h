@@ -469,6 +469,107 @@ int fdi4_decode_tree(const void* query, int query_dtype, int batch, int num_q_he
                      int out_dtype, int num_splits, void* workspace, size_t workspace_bytes,
                      hipStream_t stream);
 
+/* What fdi4_attend_paged's queries see and how they score it. A zeroed struct is plain
+ * causal attention by all queries.
+ *   counts       int32 [batch], the queries of each sequence (clamped to [0, queries]), or
+ *                NULL: queries
+ *   prefix_lens  int32 [batch] (clamped to [0, seq_lens[b]]), or NULL: none
+ *   slopes       float32 [num_q_heads], or NULL: none
+ *   window       last tokens that a query sees, 0: all
+ *   sinks        first tokens that it sees besides (needs a window)
+ *   logit_cap    0: none */
+typedef struct fdi4_attend_options {
+  const int32_t* counts;
+  const int32_t* prefix_lens;
+  const float* slopes;
+  int32_t window, sinks;
+  float logit_cap;
+} fdi4_attend_options;
+
+/* Workspace for fdi4_attend_paged with the same arguments (0: none needed; the options'
+ * pointers are not followed). num_splits <= 0 selects the split count. */
+size_t fdi4_attend_workspace_bytes(int batch, int num_q_heads, int queries,
+                                   const fdi4_attend_options* options, int num_splits,
+                                   const fdi4_paged_cache* cache);
+
+/* Attention of the last tokens of every sequence over the cache that holds them (written
+ * before, by fdi4_extend_paged or fdi4_append_paged): query [b, h, i] (i < queries; element
+ * strides, channel stride 1) of sequence b with n = seq_lens[b] tokens and c = counts[b] is
+ * that of the token at p = n - c + i, for i < c. It sees the tokens t <= p with t < sinks or
+ * t > p - window (all t <= p without a window), and every t < prefix_lens[b]. Its logits
+ * are
+ *   logit_cap * tanh(q.k_t / logit_cap)  (q.k_t without a cap),
+ *   less slopes[h] * |p - t|,
+ * unscaled otherwise. out is contiguous [batch, num_q_heads, queries, head_dim]; queries
+ * i >= c and those that see nothing give zeros, rows whose logits are all -infinity NaN.
+ * Sums are float32; each output element is rounded once. Refused besides what
+ * fdi4_decode_paged_ex refuses: scales attached to pages, page_lens, no seq_lens, scale
+ * groups that are neither a multiple of 64 rows nor as large as a sequence, more than 2^30
+ * rows a sequence, a cap that is negative or not finite. */
+int fdi4_attend_paged(const void* query, int query_dtype, int batch, int num_q_heads, int queries,
+                      int64_t q_batch_stride, int64_t q_head_stride, int64_t q_row_stride,
+                      const fdi4_paged_cache* cache, const fdi4_attend_options* options,
+                      void* out, int out_dtype, int num_splits, void* workspace,
+                      size_t workspace_bytes, hipStream_t stream);
+
+/* What fdi4_norm_rotary does to heads.
+ *   inv_freq      float32 [rotary_dim / 2]
+ *   q_weight, k_weight  [head_dim] of type weight_dtype (fdi4_key_dtype), or NULL: no norm
+ *   rotary_dim    rotated channels, even, 2 to head_dim
+ *   interleaved   0: channels j and j + rotary_dim / 2 are a pair; 1: 2j and 2j + 1 */
+typedef struct fdi4_rotary_options {
+  const float* inv_freq;
+  const void* q_weight;
+  const void* k_weight;
+  int32_t weight_dtype, rotary_dim, interleaved;
+  float eps, q_scale, rotary_scale;
+} fdi4_rotary_options;
+
+/* Norm of every query and key head and the position rotation, from q [b, h, i, :] and k
+ * [b, h, i, :] (dtype fdi4_key_dtype, element strides, channel stride 1; i < tokens) to q_out
+ * (the same dtype) and k_out (float32), both contiguous [batch, heads, tokens, head_dim]:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight[channel]   (no weight: y = x),
+ * then, for the pairs j < rotary_dim / 2 of channels, (a, b) -> (a cos u - b sin u, b cos u +
+ * a sin u) * rotary_scale with u = position * inv_freq[j] in 64 bits; the queries times
+ * q_scale. The position of token i is positions[b * p_batch_stride + i * p_token_stride], or
+ * with p_token_stride 0 positions[b * p_batch_stride] + i (int32: a cache's lengths before it
+ * is extended). head_dim is 64, 128 or 256. Statistics, products and k_out in float32; q_out
+ * rounded once. */
+int fdi4_norm_rotary(const void* q, const void* k, int dtype, int batch, int tokens,
+                     int num_q_heads, int num_kv_heads, int head_dim, int64_t q_batch_stride,
+                     int64_t q_head_stride, int64_t q_token_stride, int64_t k_batch_stride,
+                     int64_t k_head_stride, int64_t k_token_stride, const int32_t* positions,
+                     int64_t p_batch_stride, int64_t p_token_stride,
+                     const fdi4_rotary_options* options, void* q_out, float* k_out,
+                     hipStream_t stream);
+
+/* Most alternatives of fdi4_token_logprobs. */
+#define FDI4_MAX_TOP (64)
+
+/* What fdi4_token_logprobs takes from a row: top alternatives (at most FDI4_MAX_TOP and
+ * the vocabulary), of the softmax of logit_cap * tanh(x / logit_cap) (0: of x). */
+typedef struct fdi4_logprob_options {
+  int32_t top;
+  float logit_cap;
+} fdi4_logprob_options;
+
+/* Workspace for fdi4_token_logprobs (0: none needed). */
+size_t fdi4_token_logprobs_workspace_bytes(int64_t rows, int vocab, int top);
+
+/* Log probabilities of given tokens of rows of logits. Row r < outer * inner of logits
+ * (dtype fdi4_key_dtype, vocab elements, apart by 1) begins at element (r / inner) *
+ * outer_stride + (r % inner) * inner_stride. With x the row (capped) and p its softmax:
+ * logprobs[r] = log p[tokens[r]] (0 for a negative token, NaN for one past the vocabulary),
+ * entropy[r] = -sum p log p; with top > 0 top_ids[r, :] are the indices of the largest logits
+ * (as they are before the cap), ties to the lowest index, NaN first, and top_logprobs[r, :]
+ * their log p. Logits of -infinity have probability 0; rows with a NaN or +infinity, and
+ * rows of -infinity, give NaN. All sums in float32. */
+int fdi4_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner,
+                        int64_t outer_stride, int64_t inner_stride, int vocab,
+                        const int64_t* tokens, const fdi4_logprob_options* options,
+                        float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids,
+                        void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 /* fdi4_append_paged of several tokens: sequence b takes counts[b] (clamped to
  * [0, max_new]) of its new rows k_new[b, h, j] (float32) and v_new[b, h, j] (the
  * cache's value type) at positions seq_lens[b] .., in order, or, with index (int32

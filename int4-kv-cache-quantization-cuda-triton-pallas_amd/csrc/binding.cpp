@@ -758,6 +758,167 @@ torch::Tensor decode_tree(torch::Tensor query, torch::Tensor k_draft, torch::Ten
   return out;
 }
 
+// Attention of query [B, Hq, N, D], those of the last counts[b] tokens of every
+// sequence, over the cache that holds them (see fdi4_attend_paged); window 0: all earlier
+// tokens, logit_cap 0: none. Returns [B, Hq, N, D].
+torch::Tensor attend_paged(torch::Tensor query, torch::Tensor k_pages, torch::Tensor v_pages,
+                           torch::Tensor k_scale, torch::Tensor k_zp,
+                           c10::optional<torch::Tensor> page_table, torch::Tensor seq_lens,
+                           int64_t pages_per_group, int64_t max_pages,
+                           c10::optional<torch::Tensor> counts,
+                           c10::optional<torch::Tensor> prefix_lens, int64_t window,
+                           int64_t sinks, double logit_cap, c10::optional<torch::Tensor> slopes,
+                           int64_t num_splits) {
+  CHECK_DEV(query);
+  const int qcode = elem_code(query, "query");
+  TORCH_CHECK(query.dim() == 4 && query.stride(3) == 1,
+              "query must be [batch, heads, queries, head_dim] with contiguous rows");
+  const int64_t B = query.size(0), Hq = query.size(1), N = query.size(2);
+  TORCH_CHECK(query.size(3) == k_pages.size(3) * 2, "query head_dim must match the cache");
+  TORCH_CHECK(k_pages.size(1) >= 1 && Hq % k_pages.size(1) == 0,
+              "query heads must be a multiple of kv_heads");
+  TORCH_CHECK(window >= 0 && window <= INT32_MAX && sinks >= 0 && sinks <= INT32_MAX,
+              "window must be >= 1 and sinks >= 0");
+  TORCH_CHECK(window > 0 || sinks == 0, "sinks need a window");
+  CHECK_SAME_DEVICE(query, k_pages);
+  auto per_sequence = [&](const c10::optional<torch::Tensor>& t, const char* what) {
+    if (!t || !t->defined()) return static_cast<const int32_t*>(nullptr);
+    TORCH_CHECK(t->device() == query.device(), what, " must be on the device of query");
+    TORCH_CHECK(t->scalar_type() == torch::kInt32 && t->dim() == 1 && t->size(0) >= B &&
+                    (t->stride(0) == 1 || B <= 1),
+                what, " must be contiguous int32 [batch]");
+    return static_cast<const int32_t*>(t->data_ptr<int32_t>());
+  };
+  const int32_t* cnt = per_sequence(counts, "counts");
+  const int32_t* pre = per_sequence(prefix_lens, "prefix_lens");
+  const float* slp = nullptr;
+  if (slopes && slopes->defined()) {
+    CHECK_SAME_DEVICE(query, *slopes);
+    TORCH_CHECK(slopes->scalar_type() == torch::kFloat32 && slopes->dim() == 1 &&
+                    slopes->size(0) == Hq && slopes->is_contiguous(),
+                "slopes must be contiguous float32 [heads]");
+    slp = slopes->data_ptr<float>();
+  }
+  fdi4_paged_cache c = make_rows_cache(k_pages, v_pages, k_scale, k_zp, page_table, seq_lens,
+                                       pages_per_group, max_pages, B);
+  const DeviceGuard guard(query.device());
+  const int D = (int)query.size(3);
+  TORCH_CHECK(Hq * N <= INT32_MAX / 2 && B * Hq * N <= INT32_MAX, "too many queries");
+  auto out = torch::empty({B, Hq, N, D}, query.options());
+  if (out.numel() == 0) return out;
+  const fdi4_attend_options opt = {cnt, pre, slp, (int)window, (int)sinks, (float)logit_cap};
+  const size_t wsb = fdi4_attend_workspace_bytes((int)B, (int)Hq, (int)N, &opt, (int)num_splits,
+                                                 &c);
+  torch::Tensor ws;
+  if (wsb) ws = workspace(query, wsb);
+  check_rc(fdi4_attend_paged(query.data_ptr(), qcode, (int)B, (int)Hq, (int)N, query.stride(0),
+                             query.stride(1), query.stride(2), &c, &opt, out.data_ptr(), qcode,
+                             (int)num_splits, wsb ? ws.data_ptr() : nullptr, wsb, stream()),
+           "attend_paged");
+  return out;
+}
+
+// Head norms and rotation of q [B, Hq, N, D] and k [B, Hkv, N, D] (see fdi4_norm_rotary).
+// positions int32 [B] (token i at positions[b] + i) or [B, N]. Returns (q, k float32).
+std::vector<torch::Tensor> norm_rotary(torch::Tensor q, torch::Tensor k, torch::Tensor positions,
+                                       torch::Tensor inv_freq,
+                                       c10::optional<torch::Tensor> q_weight,
+                                       c10::optional<torch::Tensor> k_weight, double eps,
+                                       double q_scale, double rotary_scale, bool interleaved) {
+  CHECK_DEV(q);
+  CHECK_SAME_DEVICE(q, k);
+  CHECK_SAME_DEVICE(q, positions);
+  CHECK_SAME_DEVICE(q, inv_freq);
+  const int code = elem_code(q, "q");
+  TORCH_CHECK(k.scalar_type() == q.scalar_type(), "k must have q's dtype");
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && q.stride(3) == 1 && k.stride(3) == 1,
+              "q and k must be [batch, heads, tokens, head_dim] with contiguous rows");
+  const int64_t B = q.size(0), Hq = q.size(1), N = q.size(2), D = q.size(3), H = k.size(1);
+  TORCH_CHECK(k.size(0) == B && k.size(2) == N && k.size(3) == D,
+              "k must be [batch, kv_heads, tokens, head_dim] of q's batch, tokens and head_dim");
+  TORCH_CHECK(D == 64 || D == 128 || D == 256, "head_dim must be 64, 128 or 256, got ", D);
+  TORCH_CHECK(Hq >= 1 && H >= 1 && Hq <= 65535 && H <= 65535, "heads are out of range");
+  TORCH_CHECK(positions.scalar_type() == torch::kInt32 &&
+                  ((positions.dim() == 1 && positions.size(0) == B) ||
+                   (positions.dim() == 2 && positions.size(0) == B && positions.size(1) == N)),
+              "positions must be int32 [batch] or [batch, tokens]");
+  TORCH_CHECK(inv_freq.scalar_type() == torch::kFloat32 && inv_freq.dim() == 1 &&
+                  inv_freq.is_contiguous() && inv_freq.size(0) >= 1 && 2 * inv_freq.size(0) <= D,
+              "inv_freq must be contiguous float32 [1 to head_dim / 2]");
+  int wcode = FDI4_K_F32;
+  bool first = true;
+  auto weight = [&](const c10::optional<torch::Tensor>& w, const char* what) -> const void* {
+    if (!w || !w->defined()) return nullptr;
+    TORCH_CHECK(w->device() == q.device(), what, " must be on the device of q");
+    TORCH_CHECK(w->dim() == 1 && w->size(0) == D && w->is_contiguous(), what,
+                " must be contiguous [head_dim]");
+    const int code = elem_code(*w, what);
+    TORCH_CHECK(first || code == wcode, "q_weight and k_weight must have one dtype");
+    wcode = code;
+    first = false;
+    return w->data_ptr();
+  };
+  const void* qw = weight(q_weight, "q_weight");
+  const void* kw = weight(k_weight, "k_weight");
+  TORCH_CHECK(eps >= 0, "eps must not be negative");
+  TORCH_CHECK(B * N <= INT32_MAX / 2 && B * N * (Hq + H) <= INT32_MAX, "too many tokens");
+  const DeviceGuard guard(q.device());
+  auto qo = torch::empty({B, Hq, N, D}, q.options());
+  auto ko = torch::empty({B, H, N, D}, q.options().dtype(torch::kFloat32));
+  // (A row of explicit positions per sequence may be one token wide.)
+  const bool each = positions.dim() == 2 && N > 1;
+  TORCH_CHECK(!each || positions.stride(1) != 0, "positions of a row must not share an element");
+  const fdi4_rotary_options opt = {inv_freq.data_ptr<float>(), qw, kw, wcode,
+                                   (int)(2 * inv_freq.size(0)), interleaved ? 1 : 0, (float)eps,
+                                   (float)q_scale, (float)rotary_scale};
+  check_rc(fdi4_norm_rotary(q.data_ptr(), k.data_ptr(), code, (int)B, (int)N, (int)Hq, (int)H,
+                            (int)D, q.stride(0), q.stride(1), q.stride(2), k.stride(0),
+                            k.stride(1), k.stride(2), positions.data_ptr<int32_t>(),
+                            positions.stride(0), each ? positions.stride(1) : 0, &opt,
+                            qo.data_ptr(), ko.data_ptr<float>(), stream()),
+           "norm_rotary");
+  return {qo, ko};
+}
+
+// Log probabilities of tokens int64 [A, B] in logits [A, B, vocab] (see
+// fdi4_token_logprobs): (logprobs [A, B], entropy [A, B], top log probabilities and int64
+// indices [A, B, top]).
+std::vector<torch::Tensor> token_logprobs(torch::Tensor logits, torch::Tensor tokens,
+                                          double logit_cap, int64_t top) {
+  CHECK_DEV(logits);
+  CHECK_SAME_DEVICE(logits, tokens);
+  const int code = elem_code(logits, "logits");
+  TORCH_CHECK(logits.dim() == 3 && (logits.stride(2) == 1 || logits.size(2) == 1),
+              "logits must be [a, b, vocab] with contiguous rows");
+  const int64_t A = logits.size(0), B = logits.size(1), V = logits.size(2);
+  TORCH_CHECK(V >= 1 && V <= INT32_MAX, "the vocabulary must have 1 to 2^31 - 1 tokens, got ", V);
+  TORCH_CHECK(top >= 0 && top <= FDI4_MAX_TOP && top <= V, "top must lie in 0 .. min(",
+              FDI4_MAX_TOP, ", vocab), got ", top);
+  TORCH_CHECK(tokens.scalar_type() == torch::kInt64 && tokens.dim() == 2 && tokens.size(0) == A &&
+                  tokens.size(1) == B && tokens.is_contiguous(),
+              "tokens must be contiguous int64, one per row of logits");
+  TORCH_CHECK(B == 0 || A <= INT32_MAX / B, "too many rows");
+  const DeviceGuard guard(logits.device());
+  auto f32 = logits.options().dtype(torch::kFloat32);
+  auto lp = torch::empty({A, B}, f32), en = torch::empty({A, B}, f32);
+  auto tl = torch::empty({A, B, top}, f32);
+  auto ti = torch::empty({A, B, top}, logits.options().dtype(torch::kInt64));
+  if (A * B > 0) {
+    const fdi4_logprob_options opt = {(int)top, (float)logit_cap};
+    const size_t wsb = fdi4_token_logprobs_workspace_bytes(A * B, (int)V, (int)top);
+    torch::Tensor ws;
+    if (wsb) ws = workspace(logits, wsb);
+    check_rc(fdi4_token_logprobs(logits.data_ptr(), code, A, B, logits.stride(0),
+                                 logits.stride(1), (int)V, tokens.data_ptr<int64_t>(), &opt,
+                                 lp.data_ptr<float>(),
+                                 en.data_ptr<float>(), tl.data_ptr<float>(),
+                                 ti.data_ptr<int64_t>(), wsb ? ws.data_ptr() : nullptr, wsb,
+                                 stream()),
+             "token_logprobs");
+  }
+  return {lp, en, tl, ti};
+}
+
 // Several tokens per sequence into the cache (see fdi4_extend_paged).
 void extend_paged(torch::Tensor k_new, torch::Tensor v_new, torch::Tensor counts,
                   torch::Tensor k_stage, torch::Tensor k_pages, torch::Tensor v_pages,
@@ -1007,6 +1168,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "Decode over a sliding window and the first tokens of paged keys (HIP)");
   m.def("decode_tree", &decode_tree,
         "Attention of a tree of drafted tokens over paged keys and the drafts (HIP)");
+  m.def("attend_paged", &attend_paged,
+        "Attention of the last tokens of every sequence over the cache that holds them (HIP)");
+  m.def("norm_rotary", &norm_rotary, "Norm of query and key heads with the rotation (HIP)");
+  m.def("token_logprobs", &token_logprobs,
+        "Log probabilities of given tokens, entropy and alternatives (HIP)");
   m.def("extend_paged", &extend_paged,
         "Several tokens per sequence into the cache, touched groups re-quantized (HIP)");
   m.def("read_paged", &read_paged, "Rows of the cache as dense keys and values (HIP)");

@@ -1144,6 +1144,212 @@ int fdi4_read_paged(const fdi4_paged_cache* cache, int batch, const int32_t* sta
 
 }  // extern "C"
 
+// ---- queries of cached tokens, head norms with rotation, token log probabilities ----
+
+namespace {
+
+int attend_splits(int batch, int num_q_heads, int queries, int window, int sinks, int num_splits,
+                  const fdi4_paged_cache* cache) {
+  // The most 64-key tiles a row can see (a prefix apart).
+  const int64_t cap = (int64_t)cache->max_pages * cache->page_rows;
+  int64_t keys = cap;
+  if (window) keys = std::min<int64_t>(cap, (int64_t)window + queries + sinks + 128);
+  const int64_t items = std::max<int64_t>((keys + 63) / 64, 1);
+  const int64_t waves = (int64_t)batch * num_q_heads * queries;
+  int64_t s = num_splits > 0 ? num_splits : 4096 / std::max<int64_t>(waves, 1);
+  s = std::min<int64_t>(std::min<int64_t>(s, items), kMaxSplits);
+  return (int)std::max<int64_t>(s, 1);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fdi4_attend_workspace_bytes(int batch, int num_q_heads, int queries,
+                                   const fdi4_attend_options* options, int num_splits,
+                                   const fdi4_paged_cache* cache) {
+  if (!cache || !options) return 0;
+  const int window = options->window, sinks = options->sinks;
+  if (batch <= 0 || num_q_heads <= 0 || queries < 1 || window < 0 || sinks < 0 ||
+      cache->num_kv_heads < 1 || num_q_heads % cache->num_kv_heads || cache->page_rows < 1 ||
+      cache->max_pages < 0 || !valid_head_dim(cache->head_dim) ||
+      (int64_t)num_q_heads * queries > INT32_MAX)
+    return 0;
+  const int s = attend_splits(batch, num_q_heads, queries, window, sinks, num_splits, cache);
+  return s > 1 ? decode_ws_bytes(batch, num_q_heads * queries, cache->head_dim, s) : 0;
+}
+
+int fdi4_attend_paged(const void* query, int query_dtype, int batch, int num_q_heads, int queries,
+                      int64_t q_batch_stride, int64_t q_head_stride, int64_t q_row_stride,
+                      const fdi4_paged_cache* cache, const fdi4_attend_options* options,
+                      void* out, int out_dtype, int num_splits, void* workspace,
+                      size_t workspace_bytes, hipStream_t stream) {
+  if (!options) return hipErrorInvalidValue;
+  const int window = options->window, sinks = options->sinks;
+  const float logit_cap = options->logit_cap;
+  fdi4::AttendArgs a = {};
+  int rc = make_decode_args(query, query_dtype, batch, num_q_heads, q_batch_stride, q_head_stride,
+                            cache, 1, &a.c);
+  if (rc != hipSuccess) return rc;
+  if (cache->s_page_stride != 0 || cache->page_lens || !cache->seq_lens ||
+      !aligned(cache->seq_lens, 4))
+    return hipErrorInvalidValue;
+  const int64_t rows = (int64_t)cache->max_pages * cache->page_rows;
+  if (rows > (1 << 30)) return hipErrorInvalidValue;
+  if (queries < 1 || (int64_t)num_q_heads * queries > INT32_MAX / 2 || window < 0 || sinks < 0 ||
+      (sinks > 0 && window == 0) || !aligned(options->counts, 4) ||
+      !aligned(options->prefix_lens, 4) || !aligned(options->slopes, 4))
+    return hipErrorInvalidValue;
+  if (!(logit_cap >= 0.f) || logit_cap > 3.4028235e38f) return hipErrorInvalidValue;
+  if (!out || !valid_elem_dtype(out_dtype)) return hipErrorInvalidValue;
+  // A tile of 64 keys lies within one scale group. A group larger than a sequence is the
+  // one group that the sequence has.
+  const int64_t most = std::max<int64_t>((rows + 63) / 64 * 64, 64);
+  const int64_t group = (int64_t)cache->pages_per_group * cache->page_rows;
+  if (group < rows && group % 64) return hipErrorInvalidValue;
+  a.group_rows = (int)std::min(group < rows ? group : most, most);
+  a.div_group = fdi4::make_fast_div(a.group_rows);
+  a.queries = queries;
+  a.q_n = q_row_stride;
+  a.counts = options->counts;
+  a.prefix = options->prefix_lens;
+  a.window = std::min(window, 1 << 30);
+  a.sinks = std::min(sinks, 1 << 30);
+  a.cap = logit_cap;
+  a.slopes = options->slopes;
+  a.div_heads = fdi4::make_fast_div(cache->num_kv_heads);
+  a.kv_heads = cache->num_kv_heads;
+  const int qeb = query_dtype == FDI4_K_F32 ? 4 : 2;
+  a.q_vec = aligned(query, 16) && (q_batch_stride * qeb) % 16 == 0 &&
+            (q_head_stride * qeb) % 16 == 0 && (q_row_stride * qeb) % 16 == 0;
+  const int d = cache->head_dim, out_rows = num_q_heads * queries;
+  if ((int64_t)batch * out_rows > INT32_MAX) return hipErrorInvalidValue;
+  a.c.num_splits = attend_splits(batch, num_q_heads, queries, window, sinks, num_splits, cache);
+  a.c.div_splits = fdi4::make_fast_div(a.c.num_splits);
+  a.c.final_out = a.c.num_splits == 1 ? 1 : 0;
+  a.c.out = out;
+  a.c.out_dtype = out_dtype;
+  if (a.c.num_splits > 1) {
+    rc = carve_partials(workspace, workspace_bytes, batch, out_rows, d, &a.c);
+    if (rc != hipSuccess) return rc;
+  }
+  const hipError_t e = fdi4::launch_attend(a, d, cache->v_dtype, batch, stream);
+  if (e != hipSuccess || a.c.num_splits == 1) return e;
+  return fdi4::launch_merge(a.c.ws_acc, a.c.ws_ml, batch, out_rows, d, a.c.num_splits, out,
+                            out_dtype, (int64_t)out_rows * d, d, stream);
+}
+
+int fdi4_norm_rotary(const void* q, const void* k, int dtype, int batch, int tokens,
+                     int num_q_heads, int num_kv_heads, int head_dim, int64_t q_batch_stride,
+                     int64_t q_head_stride, int64_t q_token_stride, int64_t k_batch_stride,
+                     int64_t k_head_stride, int64_t k_token_stride, const int32_t* positions,
+                     int64_t p_batch_stride, int64_t p_token_stride,
+                     const fdi4_rotary_options* options, void* q_out, float* k_out,
+                     hipStream_t stream) {
+  if (!options) return hipErrorInvalidValue;
+  const int rotary_dim = options->rotary_dim, weight_dtype = options->weight_dtype;
+  const void *q_weight = options->q_weight, *k_weight = options->k_weight;
+  const float *inv_freq = options->inv_freq, eps = options->eps;
+  if (!valid_elem_dtype(dtype) || !valid_elem_dtype(weight_dtype) || !valid_head_dim(head_dim) ||
+      batch < 0 || tokens < 0 || num_q_heads < 1 || num_kv_heads < 1 || num_q_heads > 65535 ||
+      num_kv_heads > 65535 || rotary_dim < 2 || rotary_dim > head_dim || rotary_dim % 2 ||
+      !(eps >= 0.f))
+    return hipErrorInvalidValue;
+  if (batch == 0 || tokens == 0) return hipSuccess;
+  const int eb = dtype == FDI4_K_F32 ? 4 : 2, web = weight_dtype == FDI4_K_F32 ? 4 : 2;
+  if (!q || !k || !positions || !inv_freq || !q_out || !k_out || !aligned(q, eb) ||
+      !aligned(k, eb) || !aligned(positions, 4) || !aligned(inv_freq, 4) ||
+      !aligned(q_weight, web) || !aligned(k_weight, web) || !aligned(q_out, 16) ||
+      !aligned(k_out, 16))
+    return hipErrorInvalidValue;
+  // (Positions behind a start, and the grid, in 32 bits.)
+  if ((int64_t)batch * tokens > INT32_MAX / 2 ||
+      (int64_t)batch * tokens * (num_q_heads + num_kv_heads) > INT32_MAX)
+    return hipErrorInvalidValue;
+  fdi4::RotaryArgs a = {};
+  a.x[0] = q;
+  a.x[1] = k;
+  a.x_b[0] = q_batch_stride;
+  a.x_h[0] = q_head_stride;
+  a.x_t[0] = q_token_stride;
+  a.x_b[1] = k_batch_stride;
+  a.x_h[1] = k_head_stride;
+  a.x_t[1] = k_token_stride;
+  a.heads[0] = num_q_heads;
+  a.heads[1] = num_kv_heads;
+  a.weight[0] = q_weight;
+  a.weight[1] = k_weight;
+  a.scale[0] = options->q_scale;
+  a.scale[1] = 1.f;
+  a.out[0] = q_out;
+  a.out[1] = k_out;
+  a.dtype = dtype;
+  a.weight_dtype = weight_dtype;
+  a.batch = batch;
+  a.tokens = tokens;
+  a.head_dim = head_dim;
+  a.rotary = rotary_dim;
+  a.interleaved = options->interleaved != 0;
+  a.positions = positions;
+  a.p_b = p_batch_stride;
+  a.p_t = p_token_stride;
+  a.inv_freq = inv_freq;
+  a.eps = eps;
+  a.rotary_scale = options->rotary_scale;
+  a.vec = 1;
+  for (int i = 0; i < 2; ++i)
+    a.vec &= aligned(a.x[i], 16) && (a.x_b[i] * eb) % 16 == 0 && (a.x_h[i] * eb) % 16 == 0 &&
+             (a.x_t[i] * eb) % 16 == 0;
+  return fdi4::launch_norm_rotary(a, stream);
+}
+
+size_t fdi4_token_logprobs_workspace_bytes(int64_t rows, int vocab, int top) {
+  (void)rows;
+  (void)vocab;
+  (void)top;
+  return 0;
+}
+
+int fdi4_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner,
+                        int64_t outer_stride, int64_t inner_stride, int vocab,
+                        const int64_t* tokens, const fdi4_logprob_options* options,
+                        float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids,
+                        void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  if (!options) return hipErrorInvalidValue;
+  const int top = options->top;
+  const float logit_cap = options->logit_cap;
+  (void)workspace;
+  (void)workspace_bytes;
+  if (!valid_elem_dtype(dtype) || outer < 0 || inner < 0 || vocab < 1 || top < 0 ||
+      top > FDI4_MAX_TOP || top > vocab || !(logit_cap >= 0.f) || logit_cap > 3.4028235e38f)
+    return hipErrorInvalidValue;
+  if (outer == 0 || inner == 0) return hipSuccess;
+  if (outer > INT32_MAX / inner) return hipErrorInvalidValue;
+  const int eb = dtype == FDI4_K_F32 ? 4 : 2;
+  if (!logits || !tokens || !logprobs || !entropy || (top > 0 && (!top_logprobs || !top_ids)) ||
+      !aligned(logits, eb) || !aligned(tokens, 8) || !aligned(logprobs, 4) ||
+      !aligned(entropy, 4) || !aligned(top_logprobs, 4) || !aligned(top_ids, 8))
+    return hipErrorInvalidValue;
+  fdi4::LogprobArgs a = {};
+  a.x = logits;
+  a.dtype = dtype;
+  a.inner = inner;
+  a.s_outer = outer_stride;
+  a.s_inner = inner_stride;
+  a.rows = outer * inner;
+  a.vocab = vocab;
+  a.top = top;
+  a.cap = logit_cap;
+  a.tokens = tokens;
+  a.logprobs = logprobs;
+  a.entropy = entropy;
+  a.top_logprobs = top_logprobs;
+  a.top_ids = top_ids;
+  return fdi4::launch_token_logprobs(a, stream);
+}
+
+}  // extern "C"
+
 // ---- decode with its split partials in a static device array ------------------
 
 namespace {

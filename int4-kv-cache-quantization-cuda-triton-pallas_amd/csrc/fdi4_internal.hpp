@@ -169,6 +169,60 @@ struct RowsArgs {
   int tiles;                            // workgroups for the rows of a kv-head
 };
 
+// Queries of the last tokens of every sequence over the cache that holds them. Row R of
+// a kv-head is (query R / hq_per_kv, q-head R % hq_per_kv of its group); c holds the
+// cache, the queries and the split partials.
+struct AttendArgs {
+  DecodeArgs c;                         // out contiguous [B, Hq, queries, D]
+  int queries;                          // per sequence, the padding ones among them
+  int64_t q_n;                          // query stride, elements
+  const int32_t* counts;                // null: all of them; [B]
+  const int32_t* prefix;                // null: none; [B] tokens that every query sees
+  int window;                           // 0: all earlier tokens
+  int sinks;
+  float cap;                            // 0: none
+  const float* slopes;                  // null: none; [Hq]
+  FastDiv div_heads;                    // by kv_heads
+  int kv_heads;
+  int group_rows;                       // a multiple of 64
+  FastDiv div_group;
+  int q_vec;                            // query rows start on 16-byte boundaries
+  int tiles;                            // workgroups for the rows of a kv-head
+};
+
+// Norm of heads and position rotation: x [B, H, N, D] of q and k (element strides) to
+// q_out (q's type) and k_out (float32), contiguous.
+struct RotaryArgs {
+  const void* x[2];                     // q, k
+  int64_t x_b[2], x_h[2], x_t[2];       // elements
+  int heads[2];
+  const void* weight[2];                // null: no norm; [D]
+  float scale[2];                       // of the results
+  void* out[2];
+  int dtype, weight_dtype;              // EDtype
+  int batch, tokens, head_dim, rotary, interleaved;
+  const int32_t* positions;
+  int64_t p_b, p_t;                     // p_t 0: token i is at positions[b] + i
+  const float* inv_freq;                // [rotary / 2]
+  float eps, rotary_scale;
+  int vec;                              // rows start on 16-byte boundaries
+};
+
+// Log probabilities of given tokens of rows of logits.
+struct LogprobArgs {
+  const void* x;
+  int dtype;                            // EDtype
+  int64_t inner, s_outer, s_inner;      // row r: r / inner, r % inner; elements
+  int64_t rows;
+  int vocab, top;
+  float cap;                            // 0: none
+  const int64_t* tokens;                // [rows]
+  float* logprobs;                      // [rows]
+  float* entropy;                       // [rows]
+  float* top_logprobs;                  // [rows, top]
+  int64_t* top_ids;
+};
+
 // Several tokens per sequence appended: counts[b] of the new rows (by index when
 // given), the touched scale groups re-quantized, the open group staged.
 struct ExtendArgs {
@@ -250,6 +304,12 @@ hipError_t launch_merge(const float* ws_acc, const double* ws_ml, int batch, int
                         hipStream_t st);
 
 hipError_t launch_decode_rows(const RowsArgs& a, int D, int v_dtype, int batch, hipStream_t st);
+
+hipError_t launch_attend(const AttendArgs& a, int D, int v_dtype, int batch, hipStream_t st);
+
+hipError_t launch_norm_rotary(const RotaryArgs& a, hipStream_t st);
+
+hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t st);
 
 hipError_t launch_extend_paged(const ExtendArgs& a, int D, int group, int batch, int heads,
                                hipStream_t st);

@@ -23,6 +23,8 @@ SCALE_DIVIDE, SCALE_RECIPROCAL = 0, 1
 NOALLOC_SCRATCH_BYTES = 8 << 20
 #: FDI4_MAX_NODES: drafted tokens of fdi4_decode_tree.
 MAX_NODES = 1024
+#: FDI4_MAX_TOP: alternatives of fdi4_token_logprobs.
+MAX_TOP = 64
 #: fdi4_tuning_knob codes (launch-shape overrides for measurement and tests).
 TUNE = {"decode_vector_only": 0, "decode_waves": 1, "decode_heads_per_wg": 2,
         "decode_target_waves": 3, "fake_quant_split": 4}
@@ -52,6 +54,25 @@ class PagedCache(ctypes.Structure):
         ("max_pages", c_int32),
         ("num_pages", c_int32),
     ]
+
+
+class AttendOptions(ctypes.Structure):
+    """Mirror of ``fdi4_attend_options``."""
+    _fields_ = [("counts", c_void_p), ("prefix_lens", c_void_p), ("slopes", c_void_p),
+                ("window", c_int32), ("sinks", c_int32), ("logit_cap", ctypes.c_float)]
+
+
+class RotaryOptions(ctypes.Structure):
+    """Mirror of ``fdi4_rotary_options``."""
+    _fields_ = [("inv_freq", c_void_p), ("q_weight", c_void_p), ("k_weight", c_void_p),
+                ("weight_dtype", c_int32), ("rotary_dim", c_int32), ("interleaved", c_int32),
+                ("eps", ctypes.c_float), ("q_scale", ctypes.c_float),
+                ("rotary_scale", ctypes.c_float)]
+
+
+class LogprobOptions(ctypes.Structure):
+    """Mirror of ``fdi4_logprob_options``."""
+    _fields_ = [("top", c_int32), ("logit_cap", ctypes.c_float)]
 
 
 #: name -> (restype, argtypes); the complete exported surface of include/fdi4.h.
@@ -119,6 +140,20 @@ SIGNATURES = {
                                  c_int64, c_void_p, c_int64, c_int64, ctypes.POINTER(PagedCache),
                                  c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_size_t,
                                  c_void_p]),
+    "fdi4_attend_workspace_bytes": (c_size_t, [c_int, c_int, c_int,
+                                               ctypes.POINTER(AttendOptions), c_int,
+                                               ctypes.POINTER(PagedCache)]),
+    "fdi4_attend_paged": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64,
+                                  ctypes.POINTER(PagedCache), ctypes.POINTER(AttendOptions),
+                                  c_void_p, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "fdi4_norm_rotary": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
+                                 c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                                 c_int64, c_int64, ctypes.POINTER(RotaryOptions), c_void_p,
+                                 c_void_p, c_void_p]),
+    "fdi4_token_logprobs_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
+    "fdi4_token_logprobs": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int,
+                                    c_void_p, ctypes.POINTER(LogprobOptions), c_void_p, c_void_p,
+                                    c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "fdi4_extend_paged": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64,
                                   c_int64, c_int, c_int, c_void_p, c_void_p, c_int64, c_void_p,
                                   c_int64, c_int64, c_int64, c_int, ctypes.POINTER(PagedCache),

@@ -19,9 +19,10 @@ src/ops.py:90-108).
 Beyond the reference: ``quantize_int4_paged`` / ``flash_decode_paged`` (the
 per-sequence paged layout with 128-token scale groups and packed keys, the
 latter also over a sliding window with sinks), ``flash_decode_paged_tree``
-(drafted tokens over that cache), ``extend_int4_paged`` (several tokens per
-sequence into it), ``dequantize_int4_paged`` (and out of it) and
-``pack_int4_device``.
+(drafted tokens over that cache), ``flash_attend_paged`` (chunks of tokens that are in
+it, with capped or biased scores), ``norm_rotary`` (head norms and the rotation before
+it), ``extend_int4_paged`` (several tokens per sequence into it),
+``dequantize_int4_paged`` (and out of it) and ``pack_int4_device``.
 """
 
 import operator
@@ -352,7 +353,7 @@ def quantize_int4_paged(k, seq_lens, page_table, k_pages, k_scale, k_zp,
 def flash_decode_paged(query, k_pages, v_pages, k_scale, k_zp, page_table, seq_lens,
                        group_rows: int = 128, num_splits: int = 0, page_lens=None,
                        max_pages: Optional[int] = None, window: Optional[int] = None,
-                       sinks: int = 0):
+                       sinks: int = 0, logit_cap: Optional[float] = None, slopes=None):
     """Split-K fused INT4 flash decoding over the paged layout (all GPU tensors).
 
     query float32, float16 or bfloat16 [B, Hq, D]; k_pages uint8 [P, Hkv,
@@ -376,8 +377,20 @@ def flash_decode_paged(query, k_pages, v_pages, k_scale, k_zp, page_table, seq_l
     Values that are not finite come out as the formula has them; where a query sees
     one, the sequence's rows of that kv-head are computed one by one, which may take
     a hundred times as long.
+
+    ``logit_cap``, ``slopes``: capped scores and a distance bias, as
+    ``flash_attend_paged`` with one query has them (it is called; seq_lens and the
+    grouped scales are needed).
     """
     _check_window(window, sinks)
+    if logit_cap is not None or slopes is not None:
+        if page_lens is not None or seq_lens is None or query.dim() != 3:
+            raise ValueError("logit_cap and slopes need seq_lens and a query [batch, heads, "
+                             "head_dim], without page_lens")
+        return flash_attend_paged(query.unsqueeze(2), k_pages, v_pages, k_scale, k_zp, page_table,
+                                  seq_lens, group_rows=group_rows, window=window, sinks=sinks,
+                                  logit_cap=logit_cap, slopes=slopes, num_splits=num_splits,
+                                  max_pages=max_pages).squeeze(2)
     _require_device_of(query)
     page_rows = k_pages.shape[2]
     if group_rows % page_rows:
@@ -452,6 +465,85 @@ def flash_decode_paged_tree(query, k_draft, v_draft, mask, k_pages, v_pages, k_s
                                       k_zp, page_table, seq_lens, group_rows // page_rows,
                                       int(max_pages), int(window or 0), int(sinks),
                                       int(num_splits))
+
+
+def flash_attend_paged(query, k_pages, v_pages, k_scale, k_zp, page_table, seq_lens, counts=None,
+                       group_rows: int = 128, window: Optional[int] = None, sinks: int = 0,
+                       prefix_lens=None, logit_cap: Optional[float] = None, slopes=None,
+                       num_splits: int = 0, max_pages: Optional[int] = None):
+    """Attention of the last tokens of every sequence over the paged INT4 cache that
+    holds them: a chunk of a prompt after ``extend_int4_paged``, or one token.
+
+    query float32, float16 or bfloat16 [B, Hq, N, D] (any strides with contiguous rows);
+    counts int32 [B], the queries of each sequence (clamped to [0, N]; all N by
+    default): query i < counts[b] is that of the token at p = seq_lens[b] - counts[b] + i.
+    The cache's tensors are those of ``flash_decode_paged``, with scale groups of a
+    multiple of 64 rows (or one group).
+
+    A query sees the tokens up to its own; with ``window`` the last ``window`` of them
+    and the first ``sinks``; and with ``prefix_lens`` (int32 [B], clamped to the length)
+    every token below prefix_lens[b], also later ones. Logits are ``q.k`` (a caller scales
+    the query), with ``logit_cap`` ``logit_cap * tanh(q.k / logit_cap)``, and with
+    ``slopes`` (float32 [Hq]) less ``slopes[h] * |p - t|`` for the token at t.
+
+    Returns [B, Hq, N, D] in the query's dtype: float32 sums, one rounding of each output
+    element. Queries past a sequence's count, and those that see nothing, give zeros;
+    padding queries may hold anything. Values that are not finite come out as the formula has
+    them; the rows near one are then computed one by one, much more slowly. Nothing goes
+    through the host, so the call can be captured into a graph.
+    """
+    if query.dim() != 4:
+        raise ValueError(f"query must be [batch, heads, queries, head_dim], got "
+                         f"{tuple(query.shape)}")
+    _check_window(window, sinks)
+    cap = _checked_cap(logit_cap)
+    _require_device_of(query)
+    page_rows = k_pages.shape[2]
+    if group_rows % page_rows:
+        raise ValueError("group_rows must be a multiple of the page size")
+    if max_pages is None:
+        max_pages = page_table.shape[1] if page_table is not None else k_pages.shape[0]
+    if group_rows % 64 and group_rows < max_pages * page_rows:
+        raise ValueError(f"group_rows must be a multiple of 64, got {group_rows}")
+    return load_binding().attend_paged(query, k_pages, v_pages, k_scale, k_zp, page_table,
+                                       seq_lens, group_rows // page_rows, int(max_pages), counts,
+                                       prefix_lens, int(window or 0), int(sinks), cap, slopes,
+                                       int(num_splits))
+
+
+def _checked_cap(logit_cap: Optional[float]) -> float:
+    """A cap for the binding: 0 for none. (As float32, which the kernels take it in.)"""
+    if logit_cap is None:
+        return 0.0
+    if not 1e-30 <= float(logit_cap) <= 1e30:
+        raise ValueError(f"logit_cap must be positive and lie in 1e-30 .. 1e30, got {logit_cap}")
+    return float(logit_cap)
+
+
+def norm_rotary(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps: float = 1e-6,
+                q_scale: float = 1.0, rotary_scale: float = 1.0, interleaved: bool = False):
+    """Norm of every query and key head and the position rotation in one pass.
+
+    q [B, Hq, N, D] and k [B, Hkv, N, D], of one dtype (float32, float16 or bfloat16), any
+    strides with contiguous rows (views of a fused projection's output); D 64, 128 or
+    256. positions int32 [B] (token i of sequence b at positions[b] + i: a cache's lengths
+    before the tokens go in) or [B, N] (drafts of a tree). inv_freq float32 [R / 2]: the
+    first R channels are rotated, channel j with j + R / 2, or with ``interleaved``
+    neighbours, by position * inv_freq[j]; the others pass.
+
+    With a weight ([D], float32 or 16-bit) a head is first divided by the root of its mean
+    square plus eps and multiplied by the weight. rotary_scale multiplies the rotated
+    channels, q_scale the queries (the softmax scale, which the attention of this package
+    does not apply).
+
+    Returns (q, k): contiguous, q in its dtype, rounded once, k in float32, as
+    ``extend_int4_paged`` and ``flash_decode_paged_tree`` take it. Angles are formed in 64
+    bits.
+    """
+    _require_device_of(q)
+    out = load_binding().norm_rotary(q, k, positions, inv_freq, q_weight, k_weight, float(eps),
+                                     float(q_scale), float(rotary_scale), bool(interleaved))
+    return out[0], out[1]
 
 
 def extend_int4_paged(k_new, v_new, counts, k_stage, k_pages, v_pages, k_scale, k_zp, page_table,

@@ -1,4 +1,5 @@
-"""On-device INT4 fake quantization of keys, for quality studies.
+"""On-device INT4 fake quantization of keys, and the scores that a quality study reads off
+its logits (``token_logprobs``).
 
 Device form of the key quantize-dequantize of the reference's quality study
 (``fake_quantize_keys``, scripts/validate_llama.py:126-154, with its block
@@ -28,7 +29,7 @@ Keys must be finite GPU tensors of float32, float16 or bfloat16; there is no
 CPU path (the call raises without the HIP extension or a GPU).
 """
 
-from typing import Optional
+from typing import NamedTuple, Optional
 
 from ._lib import gpu_available, load_binding
 
@@ -121,3 +122,62 @@ def fake_quantize_keys(k, block_size: int = BLOCK_SIZE, rounding: str = "half_up
     load_binding().fake_quantize(_aligned_rows(k), out, block_size, ROUNDING_MODES[rounding],
                                  SCALE_OPS[scale_op])
     return out
+
+
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` returns (torch tensors on the GPU)."""
+    logprobs: object
+    entropy: object
+    top_logprobs: object
+    top_ids: object
+
+
+def token_logprobs(logits, tokens, top: int = 0, logit_cap: Optional[float] = None):
+    """Log probabilities of given tokens, the entropy of every row of logits, and its most
+    likely alternatives, from one read of the logits.
+
+    The mean of ``-logprobs`` over a text's tokens is the logarithm of the perplexity that
+    the quality study reports (scripts/validate_llama.py).
+
+    Args:
+        logits: [..., vocab] float32, float16 or bfloat16 on the GPU, rows contiguous
+           (``logits[:, :-1]`` of a batch is read where it lies).
+        tokens: integers [...], the token of every row; a negative one (a place without
+           a token) gives 0, one past the vocabulary NaN.
+        top: alternatives per row, 0 to 64.
+        logit_cap: softmax of ``logit_cap * tanh(logits / logit_cap)``.
+    Returns:
+        TokenLogprobs of logprobs float32 [...], entropy float32 [...] (in nats),
+        top_logprobs float32 [..., top] and top_ids int64 [..., top]: the largest logits,
+        ties to the lowest index. Logits of -infinity have probability zero; a row with a
+        NaN or +infinity, or of -infinity alone, gives NaN (its alternatives put NaN first).
+    """
+    import torch
+    from .ops import _checked_cap
+    if not isinstance(logits, torch.Tensor) or not isinstance(tokens, torch.Tensor):
+        raise TypeError("logits and tokens must be torch tensors")
+    if logits.dim() < 1 or tuple(logits.shape[:-1]) != tuple(tokens.shape):
+        raise ValueError(f"tokens must have one entry per row of logits, got "
+                         f"{tuple(tokens.shape)} for {tuple(logits.shape)}")
+    if logits.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f"logits must be float32, float16 or bfloat16, got {logits.dtype}")
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"tokens must be int32 or int64, got {tokens.dtype}")
+    top = int(top)
+    if not 0 <= top <= min(64, logits.shape[-1]):
+        raise ValueError(f"top must lie in 0 .. {min(64, logits.shape[-1])}, got {top}")
+    cap = _checked_cap(logit_cap)
+    binding = load_binding()  # raises with the reason when the extension is missing
+    if not logits.is_cuda or not tokens.is_cuda:
+        raise RuntimeError("logits and tokens must be GPU (cuda device) tensors; this package "
+                           "has no CPU path")
+    lead, vocab = tuple(logits.shape[:-1]), logits.shape[-1]
+    if logits.stride(-1) != 1 and vocab > 1:
+        logits = logits.contiguous()
+    outer = lead[0] if len(lead) > 1 else 1
+    rows = logits.reshape(outer, -1, vocab) if 0 not in lead else \
+        logits.new_empty((0, 0, vocab))
+    ids = tokens.to(torch.int64).reshape(rows.shape[:2]).contiguous()
+    lp, entropy, tl, ti = binding.token_logprobs(rows, ids, cap, top)
+    return TokenLogprobs(lp.view(lead), entropy.view(lead), tl.view(*lead, top),
+                         ti.view(*lead, top))

@@ -541,7 +541,8 @@ class INT4PagedSequenceCache:
         self._sync_if_stepped()
         self._grow_all((b, int(self._lens[b]) + n_tokens) for b in range(batch))
 
-    def step(self, k_new, v_new, query, num_splits: int = 0, window=None, sinks: int = 0):
+    def step(self, k_new, v_new, query, num_splits: int = 0, window=None, sinks: int = 0,
+             logit_cap=None, slopes=None):
         """One decode step on the device alone: append (k_new, v_new) [B,
         kv_heads, D] at each sequence's length, advance the lengths on the
         device, attend with query [B, Hq, D] (float32, float16 or bfloat16);
@@ -559,14 +560,16 @@ class INT4PagedSequenceCache:
         An eager call whose token would fall outside the reserved pages raises
         RuntimeError before anything is launched (the host knows the lengths up
         to the eager steps since the last sync; replays are the caller's to
-        keep within the reservation). window, sinks: attend as decode() does with
-        them."""
+        keep within the reservation). window, sinks, logit_cap, slopes: attend as
+        decode() does with them."""
         ops._check_window(window, sinks)
+        scored = logit_cap is not None or slopes is not None
+        ops._checked_cap(logit_cap)
         B = k_new.shape[0]
         if B > self.max_seqs or tuple(k_new.shape) != (B, self.num_kv_heads, self.head_dim):
             raise ValueError("k_new must be [batch <= max_seqs, kv_heads, head_dim]")
         self._check_room(B, 1, "step() would")
-        if window is not None:
+        if window is not None or scored:
             import torch
             # (Refused here, what the attention would refuse with the token appended.)
             if query.dim() != 3 or query.shape[0] != B or query.shape[2] != self.head_dim or \
@@ -575,7 +578,25 @@ class INT4PagedSequenceCache:
                     query.dtype not in (torch.float32, torch.float16, torch.bfloat16):
                 raise ValueError("query must be float32, float16 or bfloat16 [batch, heads, "
                                  "head_dim] on the cache's GPU, heads a multiple of kv_heads")
+            if slopes is not None and (
+                    not isinstance(slopes, torch.Tensor) or slopes.dtype != torch.float32 or
+                    tuple(slopes.shape) != (query.shape[1],) or not slopes.is_contiguous() or
+                    slopes.device != query.device):
+                raise ValueError("slopes must be contiguous float32 [heads] on the cache's GPU")
         self._unsynced_steps += 1
+        if scored:
+            C = load_binding()
+            C.append_paged_advance(k_new, v_new, self.k_stage[:B], self.k_pages, self.v_pages,
+                                   self.k_scale[:B], self.k_zp[:B], self.page_table[:B],
+                                   self.seq_lens[:B], self.group_rows, self._lens_next[:B])
+            out = ops.flash_decode_paged(
+                query, self.k_pages, self.v_pages, self.k_scale[:B], self.k_zp[:B],
+                self.page_table[:B], self._lens_next[:B], self.group_rows, num_splits,
+                max_pages=self.max_pages_per_seq, window=window, sinks=sinks,
+                logit_cap=logit_cap, slopes=slopes)
+            # (An addition, not a copy: a kernel of its own in a captured graph.)
+            torch.add(self._lens_next[:B], 0, out=self.seq_lens[:B])
+            return out
         if window is not None:
             C = load_binding()
             C.append_paged_advance(k_new, v_new, self.k_stage[:B], self.k_pages, self.v_pages,
@@ -614,18 +635,47 @@ class INT4PagedSequenceCache:
 
     # ---- reads -------------------------------------------------------------
 
-    def decode(self, query, num_splits: int = 0, window=None, sinks: int = 0):
+    def decode(self, query, num_splits: int = 0, window=None, sinks: int = 0, logit_cap=None,
+               slopes=None):
         """Fused INT4 attention of query [B, Hq, D] (float32, float16 or bfloat16;
         Hq a multiple of kv_heads) over sequences 0..B-1; returns [B, Hq, D] in
         the query's dtype (float32 arithmetic, one rounding at the end). With a
         window only over each sequence's last ``window`` and first ``sinks``
-        tokens (ops.flash_decode_paged says to how many bits)."""
+        tokens (ops.flash_decode_paged says to how many bits). logit_cap, slopes: scores
+        capped and biased as in attend()."""
         B = query.shape[0]
         return ops.flash_decode_paged(query, self.k_pages, self.v_pages, self.k_scale[:B],
                                       self.k_zp[:B], self.page_table[:B], self.seq_lens[:B],
                                       self.group_rows, num_splits,
                                       max_pages=self.max_pages_per_seq, window=window,
-                                      sinks=sinks)
+                                      sinks=sinks, logit_cap=logit_cap, slopes=slopes)
+
+    def rotate(self, q, k, inv_freq, q_weight=None, k_weight=None, eps: float = 1e-6,
+               q_scale: float = 1.0, rotary_scale: float = 1.0, interleaved: bool = False):
+        """Head norms and rotation (ops.norm_rotary) of the next tokens of sequences
+        0..B-1, q [B, q_heads, N, D] and k [B, kv_heads, N, D]: token i at the
+        sequence's device length plus i, so before they are written. Returns the queries
+        for attend() and the float32 keys for extend() ([:, :, 0] for step())."""
+        B = q.shape[0]
+        if B > self.max_seqs:
+            raise ValueError(f"{B} sequences, the cache holds {self.max_seqs}")
+        if k.dim() != 4 or (k.shape[1], k.shape[3]) != (self.num_kv_heads, self.head_dim):
+            raise ValueError("k must be [batch, kv_heads, tokens, head_dim] of this cache")
+        return ops.norm_rotary(q, k, self.seq_lens[:B], inv_freq, q_weight, k_weight, eps, q_scale,
+                               rotary_scale, interleaved)
+
+    def attend(self, query, counts=None, window=None, sinks: int = 0, prefix_lens=None,
+               logit_cap=None, slopes=None, num_splits: int = 0):
+        """Attention of query [B, q_heads, N, D], those of the last counts[b] (int32 on
+        the GPU; all N by default) tokens of sequences 0..B-1, over the cache that holds
+        them: a prompt's chunk after extend(), with the counts given to it. Causal, within a
+        window with sinks, with a prefix that every query sees, scores capped or lowered
+        by the distance (ops.flash_attend_paged)."""
+        B = query.shape[0]
+        return ops.flash_attend_paged(
+            query, self.k_pages, self.v_pages, self.k_scale[:B], self.k_zp[:B],
+            self.page_table[:B], self.seq_lens[:B], counts, self.group_rows, window, sinks,
+            prefix_lens, logit_cap, slopes, num_splits, max_pages=self.max_pages_per_seq)
 
     def tree_attention(self, query, k_draft, v_draft, mask, window=None, sinks: int = 0,
                        num_splits: int = 0):
