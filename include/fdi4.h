@@ -488,7 +488,7 @@ typedef struct fdi4_attend_options {
 
 /* Workspace for fdi4_attend_paged with the same arguments (0: none needed; the options'
  * pointers are not followed). num_splits <= 0 selects the split count. */
-size_t fdi4_attend_workspace_bytes(int batch, int num_q_heads, int queries,
+size_t fdi4_attend_workspace_bytes(int batch, int num_q_heads, int queries, int out_dtype,
                                    const fdi4_attend_options* options, int num_splits,
                                    const fdi4_paged_cache* cache);
 

@@ -48,6 +48,7 @@ hipError_t launch_attend_d(const AttendArgs& a, int v_dtype, int batch, hipStrea
 }
 
 hipError_t launch_attend(const AttendArgs& a, int D, int v_dtype, int batch, hipStream_t st) {
+  if (a.chunk) return launch_attend_chunk(a, D, v_dtype, batch, st);
   if (D == 64) return launch_attend_d<64>(a, v_dtype, batch, st);
   if (D == 128) return launch_attend_d<128>(a, v_dtype, batch, st);
   if (D == 256) return launch_attend_d<256>(a, v_dtype, batch, st);

@@ -81,6 +81,14 @@ __device__ __forceinline__ TileList tile_list(int head, int low, int pos) {
 
 // ---- a row by itself ------------------------------------------------------------
 
+// The kernel's arguments, read again from where they lie: what follows a kernel's loop
+// uses this copy, so that its arguments hold no scalar registers in the loop.
+__device__ __forceinline__ const AttendArgs& late_attend_args() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const AttendArgs*)p;
+}
+
 // Sums of one row over the tiles [j0, j1) of a list, by one wave: o[k] belongs to channel
 // lane * (D / 64) + k. Keys that the row does not see take no part at all, so values and
 // scales that are not finite come out as the formula has them. m = kLeastF and l = 0 if
@@ -91,7 +99,7 @@ struct RowSums {
 };
 
 template <int D, int VDT>
-__device__ __attribute__((noinline)) RowSums<D> plain_row(const AttendArgs& a, int b, int hk,
+__device__ __forceinline__ RowSums<D> plain_row(const AttendArgs& a, int b, int hk,
                                                           int R, int n, RowView view,
                                                           TileList list, int j0, int j1) {
   const DecodeArgs& c = a.c;
@@ -108,6 +116,7 @@ __device__ __attribute__((noinline)) RowSums<D> plain_row(const AttendArgs& a, i
   r.m = kLeastF;
   r.l = 0.f;
   for (int k = 0; k < CH; ++k) r.o[k] = 0.f;
+#pragma unroll 1
   for (int j = j0; j < j1; ++j) {
     const int t0 = list.tile(j) * kKeyTile, t = t0 + lane;
     const bool mine = t < n && sees(view, t);
@@ -120,6 +129,7 @@ __device__ __attribute__((noinline)) RowSums<D> plain_row(const AttendArgs& a, i
         c.k_pages + phys * c.k_page + (int64_t)hk * c.k_head + (int64_t)tr * c.k_row;
     const int64_t g = (int64_t)fdiv(t0, a.div_group) * c.s_g;
     float x = 0.f;
+#pragma unroll 1
     for (int d = 0; d < D; ++d) {
       const float s = sbase[g + d], z = zbase[g + d];
       const float k = (float)((kp[d >> 1] >> (4 * (d & 1))) & 15) * s - z * s;
@@ -141,6 +151,7 @@ __device__ __attribute__((noinline)) RowSums<D> plain_row(const AttendArgs& a, i
     for (int k = 0; k < CH; ++k) r.o[k] *= f;
     // Lane: its channels of every value.
     const int64_t vrow = phys * c.v_page + (int64_t)hk * c.v_head + (int64_t)tr * c.v_row;
+#pragma unroll 1
     for (int e = 0; e < kKeyTile; ++e) {
       if (!(who >> e & 1u)) continue;
       const float pe = __shfl(p, e, 64);

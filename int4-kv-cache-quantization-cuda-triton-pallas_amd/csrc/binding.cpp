@@ -807,8 +807,8 @@ torch::Tensor attend_paged(torch::Tensor query, torch::Tensor k_pages, torch::Te
   auto out = torch::empty({B, Hq, N, D}, query.options());
   if (out.numel() == 0) return out;
   const fdi4_attend_options opt = {cnt, pre, slp, (int)window, (int)sinks, (float)logit_cap};
-  const size_t wsb = fdi4_attend_workspace_bytes((int)B, (int)Hq, (int)N, &opt, (int)num_splits,
-                                                 &c);
+  const size_t wsb = fdi4_attend_workspace_bytes((int)B, (int)Hq, (int)N, qcode, &opt,
+                                                 (int)num_splits, &c);
   torch::Tensor ws;
   if (wsb) ws = workspace(query, wsb);
   check_rc(fdi4_attend_paged(query.data_ptr(), qcode, (int)B, (int)Hq, (int)N, query.stride(0),

@@ -1148,24 +1148,36 @@ int fdi4_read_paged(const fdi4_paged_cache* cache, int batch, const int32_t* sta
 
 namespace {
 
-int attend_splits(int batch, int num_q_heads, int queries, int window, int sinks, int num_splits,
-                  const fdi4_paged_cache* cache) {
-  // The most 64-key tiles a row can see (a prefix apart).
+// Launch shape of fdi4_attend_paged: the kernel, and splits of a sequence's 64-key tiles.
+struct AttendPlan {
+  int chunk, splits;
+};
+
+AttendPlan plan_attend(int batch, int num_q_heads, int queries, int window, int sinks, bool wide,
+                       int num_splits, const fdi4_paged_cache* cache) {
+  AttendPlan p;
+  const int64_t rows = (int64_t)(num_q_heads / cache->num_kv_heads) * queries;
+  p.chunk = rows > 16;
+  // The most 64-key tiles a row tile can see (a prefix apart).
   const int64_t cap = (int64_t)cache->max_pages * cache->page_rows;
   int64_t keys = cap;
   if (window) keys = std::min<int64_t>(cap, (int64_t)window + queries + sinks + 128);
   const int64_t items = std::max<int64_t>((keys + 63) / 64, 1);
-  const int64_t waves = (int64_t)batch * num_q_heads * queries;
-  int64_t s = num_splits > 0 ? num_splits : 4096 / std::max<int64_t>(waves, 1);
+  const int64_t m = wide || cache->head_dim == 256 ? 128 : 256;
+  const int64_t wgs = (int64_t)batch * cache->num_kv_heads * (p.chunk ? (rows + m - 1) / m : rows);
+  int64_t s = num_splits > 0 ? num_splits
+                             : std::min<int64_t>((p.chunk ? kCUs : 4096) / std::max<int64_t>(wgs, 1),
+                                                 (items + 3) / 4);
   s = std::min<int64_t>(std::min<int64_t>(s, items), kMaxSplits);
-  return (int)std::max<int64_t>(s, 1);
+  p.splits = (int)std::max<int64_t>(s, 1);
+  return p;
 }
 
 }  // namespace
 
 extern "C" {
 
-size_t fdi4_attend_workspace_bytes(int batch, int num_q_heads, int queries,
+size_t fdi4_attend_workspace_bytes(int batch, int num_q_heads, int queries, int out_dtype,
                                    const fdi4_attend_options* options, int num_splits,
                                    const fdi4_paged_cache* cache) {
   if (!cache || !options) return 0;
@@ -1175,7 +1187,8 @@ size_t fdi4_attend_workspace_bytes(int batch, int num_q_heads, int queries,
       cache->max_pages < 0 || !valid_head_dim(cache->head_dim) ||
       (int64_t)num_q_heads * queries > INT32_MAX)
     return 0;
-  const int s = attend_splits(batch, num_q_heads, queries, window, sinks, num_splits, cache);
+  const int s = plan_attend(batch, num_q_heads, queries, window, sinks,
+                            out_dtype == FDI4_K_F32, num_splits, cache).splits;
   return s > 1 ? decode_ws_bytes(batch, num_q_heads * queries, cache->head_dim, s) : 0;
 }
 
@@ -1224,7 +1237,10 @@ int fdi4_attend_paged(const void* query, int query_dtype, int batch, int num_q_h
             (q_head_stride * qeb) % 16 == 0 && (q_row_stride * qeb) % 16 == 0;
   const int d = cache->head_dim, out_rows = num_q_heads * queries;
   if ((int64_t)batch * out_rows > INT32_MAX) return hipErrorInvalidValue;
-  a.c.num_splits = attend_splits(batch, num_q_heads, queries, window, sinks, num_splits, cache);
+  const AttendPlan plan = plan_attend(batch, num_q_heads, queries, window, sinks,
+                                      out_dtype == FDI4_K_F32, num_splits, cache);
+  a.chunk = plan.chunk;
+  a.c.num_splits = plan.splits;
   a.c.div_splits = fdi4::make_fast_div(a.c.num_splits);
   a.c.final_out = a.c.num_splits == 1 ? 1 : 0;
   a.c.out = out;

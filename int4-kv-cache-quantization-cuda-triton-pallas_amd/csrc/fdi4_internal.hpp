@@ -187,7 +187,8 @@ struct AttendArgs {
   int group_rows;                       // a multiple of 64
   FastDiv div_group;
   int q_vec;                            // query rows start on 16-byte boundaries
-  int tiles;                            // workgroups for the rows of a kv-head
+  int chunk;                            // 1: the kernel of many rows
+  int tiles;                            // its workgroups for the rows of a kv-head
 };
 
 // Norm of heads and position rotation: x [B, H, N, D] of q and k (element strides) to
@@ -306,6 +307,9 @@ hipError_t launch_merge(const float* ws_acc, const double* ws_ml, int batch, int
 hipError_t launch_decode_rows(const RowsArgs& a, int D, int v_dtype, int batch, hipStream_t st);
 
 hipError_t launch_attend(const AttendArgs& a, int D, int v_dtype, int batch, hipStream_t st);
+
+hipError_t launch_attend_chunk(const AttendArgs& a, int D, int v_dtype, int batch,
+                               hipStream_t st);
 
 hipError_t launch_norm_rotary(const RotaryArgs& a, hipStream_t st);
 

@@ -140,7 +140,7 @@ SIGNATURES = {
                                  c_int64, c_void_p, c_int64, c_int64, ctypes.POINTER(PagedCache),
                                  c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_size_t,
                                  c_void_p]),
-    "fdi4_attend_workspace_bytes": (c_size_t, [c_int, c_int, c_int,
+    "fdi4_attend_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int,
                                                ctypes.POINTER(AttendOptions), c_int,
                                                ctypes.POINTER(PagedCache)]),
     "fdi4_attend_paged": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64,

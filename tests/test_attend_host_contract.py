@@ -54,7 +54,7 @@ def test_attend_workspace():
 
     def size(B, Hq, N, w, s, splits, c=c):
         return lib.fdi4_attend_workspace_bytes(
-            B, Hq, N, ctypes.byref(capi.AttendOptions(None, None, None, w, s, 0.0)), splits,
+            B, Hq, N, capi.K_BF16, ctypes.byref(capi.AttendOptions(None, None, None, w, s, 0.0)), splits,
             ctypes.byref(c) if c else None)
 
     assert size(2, 8, 5, 0, 0, 1) == 0
@@ -65,7 +65,7 @@ def test_attend_workspace():
                  (2, 8, 5, 0, -1, 4), (2, 8, 1 << 30, 0, 0, 4)):
         assert size(*args) == 0
     assert size(2, 8, 5, 0, 0, 4, None) == 0
-    assert lib.fdi4_attend_workspace_bytes(2, 8, 5, None, 4, ctypes.byref(c)) == 0
+    assert lib.fdi4_attend_workspace_bytes(2, 8, 5, capi.K_BF16, None, 4, ctypes.byref(c)) == 0
 
 
 @pytest.mark.parametrize("kw", [
