@@ -29,14 +29,8 @@
 
 namespace fdi4 {
 
-typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v16f __attribute__((ext_vector_type(16)));
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
-typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef short v4s __attribute__((ext_vector_type(4)));
-typedef unsigned v4u __attribute__((ext_vector_type(4)));
 
 template <int D, int VDT, bool WIDE>
 struct ChunkGeo {
@@ -65,26 +59,6 @@ struct ChunkGeo {
   static_assert(KT * SEG % NT == 0 && SEG <= 16, "threads");
 };
 
-__device__ __forceinline__ unsigned pack_f16(float x, float y) {
-  return __builtin_bit_cast(unsigned, __builtin_convertvector(v2f{x, y}, v2h));
-}
-
-__device__ __forceinline__ unsigned pack_bf16(float x, float y) {
-  return __builtin_bit_cast(unsigned, __builtin_convertvector(v2f{x, y}, v2bf));
-}
-
-// The upper halves of x and y: bfloat16 terms by truncation.
-__device__ __forceinline__ unsigned pack_high(float x, float y) {
-  return __builtin_amdgcn_perm(f2u(y), f2u(x), 0x07060302u);
-}
-
-__device__ __forceinline__ float less_high(float x) { return x - u2f(f2u(x) & 0xFFFF0000u); }
-
-// Exponent e of |x| < 2^(e + 1) from the bits of |x| (0 and subnormals: -126).
-__device__ __forceinline__ int exponent_of(unsigned bits) {
-  return max((int)(bits >> 23), 1) - 127;
-}
-
 __device__ __forceinline__ float over_halves_max(float x) {
   auto r = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
   return fmaxf(u2f(r[0]), u2f(r[1]));
@@ -93,16 +67,6 @@ __device__ __forceinline__ float over_halves_max(float x) {
 __device__ __forceinline__ float over_halves_sum(float x) {
   auto r = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
   return u2f(r[0]) + u2f(r[1]);
-}
-
-// Whether a row sees a key of the tiles [j0, j1) of a list.
-__device__ __forceinline__ bool sees_tiles(const RowView& v, const TileList& l, int j0, int j1) {
-  auto in = [&](int t0, int t1) {
-    return t0 < t1 && (t0 < v.head || max(t0, v.low) <= min(t1 - 1, v.pos));
-  };
-  const int f1 = min(j1, l.front), b0 = max(j0, l.front);
-  return in(j0 * kKeyTile, f1 * kKeyTile) ||
-         in((b0 - l.front + l.from) * kKeyTile, (j1 - l.front + l.from) * kKeyTile);
 }
 
 template <int D, int VDT, bool WIDE>

@@ -6,6 +6,13 @@
 
 namespace fdi4 {
 
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
+
 constexpr int kKeyTile = 64;             // keys of a tile, within one scale group
 constexpr float kLog2eF = 1.44269504088896f;
 constexpr float kLeastF = -3.4028235e38f;
@@ -77,6 +84,38 @@ __device__ __forceinline__ TileList tile_list(int head, int low, int pos) {
   l.from = max(low / kKeyTile, l.front);
   l.total = l.front + max(pos / kKeyTile + (pos >= 0) - l.from, 0);
   return l;
+}
+
+// Whether a row sees a key of the tiles [j0, j1) of a list.
+__device__ __forceinline__ bool sees_tiles(const RowView& v, const TileList& l, int j0, int j1) {
+  auto in = [&](int t0, int t1) {
+    return t0 < t1 && (t0 < v.head || max(t0, v.low) <= min(t1 - 1, v.pos));
+  };
+  const int f1 = min(j1, l.front), b0 = max(j0, l.front);
+  return in(j0 * kKeyTile, f1 * kKeyTile) ||
+         in((b0 - l.front + l.from) * kKeyTile, (j1 - l.front + l.from) * kKeyTile);
+}
+
+// ---- terms of 16 bits ---------------------------------------------------------
+
+__device__ __forceinline__ unsigned pack_f16(float x, float y) {
+  return __builtin_bit_cast(unsigned, __builtin_convertvector(v2f{x, y}, v2h));
+}
+
+__device__ __forceinline__ unsigned pack_bf16(float x, float y) {
+  return __builtin_bit_cast(unsigned, __builtin_convertvector(v2f{x, y}, v2bf));
+}
+
+// The upper halves of x and y: bfloat16 terms by truncation.
+__device__ __forceinline__ unsigned pack_high(float x, float y) {
+  return __builtin_amdgcn_perm(f2u(y), f2u(x), 0x07060302u);
+}
+
+__device__ __forceinline__ float less_high(float x) { return x - u2f(f2u(x) & 0xFFFF0000u); }
+
+// Exponent e of |x| < 2^(e + 1) from the bits of |x| (0 and subnormals: -126).
+__device__ __forceinline__ int exponent_of(unsigned bits) {
+  return max((int)(bits >> 23), 1) - 127;
 }
 
 // ---- a row by itself ------------------------------------------------------------

@@ -1164,10 +1164,10 @@ AttendPlan plan_attend(int batch, int num_q_heads, int queries, int window, int 
   if (window) keys = std::min<int64_t>(cap, (int64_t)window + queries + sinks + 128);
   const int64_t items = std::max<int64_t>((keys + 63) / 64, 1);
   const int64_t m = wide || cache->head_dim == 256 ? 128 : 256;
-  const int64_t wgs = (int64_t)batch * cache->num_kv_heads * (p.chunk ? (rows + m - 1) / m : rows);
+  const int64_t wgs = (int64_t)batch * cache->num_kv_heads * (p.chunk ? (rows + m - 1) / m : 1);
+  const int64_t slots = (p.chunk || cache->head_dim == 256 ? 1 : 2) * kCUs;
   int64_t s = num_splits > 0 ? num_splits
-                             : std::min<int64_t>((p.chunk ? kCUs : 4096) / std::max<int64_t>(wgs, 1),
-                                                 (items + 3) / 4);
+                             : std::min<int64_t>(slots / std::max<int64_t>(wgs, 1), (items + 3) / 4);
   s = std::min<int64_t>(std::min<int64_t>(s, items), kMaxSplits);
   p.splits = (int)std::max<int64_t>(s, 1);
   return p;
