@@ -1312,7 +1312,7 @@ int fdi4_norm_rotary(const void* q, const void* k, int dtype, int batch, int tok
   a.inv_freq = inv_freq;
   a.eps = eps;
   a.rotary_scale = options->rotary_scale;
-  a.vec = 1;
+  a.vec = aligned(q_weight, 16) && aligned(k_weight, 16);
   for (int i = 0; i < 2; ++i)
     a.vec &= aligned(a.x[i], 16) && (a.x_b[i] * eb) % 16 == 0 && (a.x_h[i] * eb) % 16 == 0 &&
              (a.x_t[i] * eb) % 16 == 0;
@@ -1320,10 +1320,10 @@ int fdi4_norm_rotary(const void* q, const void* k, int dtype, int batch, int tok
 }
 
 size_t fdi4_token_logprobs_workspace_bytes(int64_t rows, int vocab, int top) {
-  (void)rows;
-  (void)vocab;
-  (void)top;
-  return 0;
+  static_assert(FDI4_MAX_TOP == fdi4::kMaxTop, "alternatives");
+  if (rows < 1 || rows > INT32_MAX || vocab < 1 || top < 0 || top > FDI4_MAX_TOP) return 0;
+  const int s = fdi4::logprob_splits(rows, vocab);
+  return s > 1 ? (size_t)rows * s * (16 + 8 * (size_t)top) : 0;
 }
 
 int fdi4_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner,
@@ -1334,8 +1334,6 @@ int fdi4_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t in
   if (!options) return hipErrorInvalidValue;
   const int top = options->top;
   const float logit_cap = options->logit_cap;
-  (void)workspace;
-  (void)workspace_bytes;
   if (!valid_elem_dtype(dtype) || outer < 0 || inner < 0 || vocab < 1 || top < 0 ||
       top > FDI4_MAX_TOP || top > vocab || !(logit_cap >= 0.f) || logit_cap > 3.4028235e38f)
     return hipErrorInvalidValue;
@@ -1361,6 +1359,14 @@ int fdi4_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t in
   a.entropy = entropy;
   a.top_logprobs = top_logprobs;
   a.top_ids = top_ids;
+  a.splits = fdi4::logprob_splits(a.rows, vocab);
+  if (a.splits > 1) {
+    if (!workspace || !aligned(workspace, 16) ||
+        workspace_bytes < fdi4_token_logprobs_workspace_bytes(a.rows, vocab, top))
+      return hipErrorInvalidValue;
+    a.part_sums = static_cast<float4*>(workspace);
+    a.part_top = reinterpret_cast<uint64_t*>(a.part_sums + a.rows * a.splits);
+  }
   return fdi4::launch_token_logprobs(a, stream);
 }
 

@@ -93,6 +93,16 @@ def test_nothing_to_do():
     assert logprobs(outer=0, x=None) == 0 and logprobs(inner=0, lp=None) == 0
 
 
+def test_logprobs_workspace():
+    size = capi.load().fdi4_token_logprobs_workspace_bytes
+    assert size(5000, 128000, 5) == 0
+    need = size(6, 128000, 5)
+    assert need >= 6 * (16 + 5 * 8)
+    for kw in (dict(ws=None), dict(wsb=need - 1), dict(ws=P + 8)):
+        assert logprobs(vocab=128000, **kw) == INVALID
+    assert size(0, 1000, 5) == 0 and size(6, 0, 5) == 0 and size(6, 1000, 65) == 0
+
+
 @pytest.mark.parametrize("kw", [
     dict(x=None), dict(x=P + 1), dict(dt=4), dict(outer=-1), dict(inner=-1), dict(vocab=0),
     dict(tok=None), dict(tok=P + 4), dict(cap=-2.0), dict(cap=float("nan")), dict(top=-1),
