@@ -553,9 +553,6 @@ typedef struct fdi4_logprob_options {
   float logit_cap;
 } fdi4_logprob_options;
 
-/* Workspace for fdi4_token_logprobs (0: none needed). */
-size_t fdi4_token_logprobs_workspace_bytes(int64_t rows, int vocab, int top);
-
 /* Log probabilities of given tokens of rows of logits. Row r < outer * inner of logits
  * (dtype fdi4_key_dtype, vocab elements, apart by 1) begins at element (r / inner) *
  * outer_stride + (r % inner) * inner_stride. With x the row (capped) and p its softmax:
@@ -568,7 +565,7 @@ int fdi4_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t in
                         int64_t outer_stride, int64_t inner_stride, int vocab,
                         const int64_t* tokens, const fdi4_logprob_options* options,
                         float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids,
-                        void* workspace, size_t workspace_bytes, hipStream_t stream);
+                        hipStream_t stream);
 
 /* fdi4_append_paged of several tokens: sequence b takes counts[b] (clamped to
  * [0, max_new]) of its new rows k_new[b, h, j] (float32) and v_new[b, h, j] (the

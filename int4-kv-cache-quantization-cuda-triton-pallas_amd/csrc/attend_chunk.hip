@@ -316,7 +316,7 @@ void attend_chunk_kernel(AttendArgs a) {
     for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
   float m = kLeastF, l = 0.f;
   const float slope = a.slopes ? a.slopes[hk * c.hq_per_kv + qh] : 0.f;
-  const float inv_cap = 1.f / a.cap;
+  const float inv_cap = 1.f / a.cap, cap_scale = 2.f * kLog2eF / a.cap;
 
   auto compute = [&](int s, int buf) __attribute__((always_inline)) {
     const int t0 = key0_of(s);
@@ -348,7 +348,9 @@ void attend_chunk_kernel(AttendArgs a) {
       for (int e = 0; e < NS; ++e)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          x[e][i] = soft_cap(sv[e][i] * f, a.cap, inv_cap) * kLog2eF;
+          x[e][i] = (WIDE ? soft_cap(sv[e][i] * f, a.cap, inv_cap)
+                          : quick_cap(sv[e][i] * f, a.cap, cap_scale)) *
+                    kLog2eF;
     } else {
       const float f2 = f * kLog2eF;
 #pragma unroll

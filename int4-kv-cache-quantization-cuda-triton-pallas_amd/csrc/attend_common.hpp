@@ -51,13 +51,13 @@ __device__ __forceinline__ int prefix_of(const AttendArgs& a, int b, int n) {
   return a.prefix ? min(max(ld_ro(a.prefix, b), 0), n) : 0;
 }
 
-// cap * tanh(x / cap) in float32. With e = exp(-2|y|), tanh|y| = (1 - e) / (1 + e): its
-// error is that of 1 - e, 2^-24, so below |y| = 0.35 the odd Taylor series takes over
-// (to y^13: its next term is below 2^-28 of the sum).
+// cap * tanh(x / cap) in float32: with e = exp(-2|y|), y = x / cap, tanh|y| = (1 - e) / (1 +
+// e). Its error is that of 1 - e, 2^-24, so below |y| = 0.35 the odd Taylor series takes
+// over (to y^13: its next term is below 2^-28 of the sum).
 __device__ __forceinline__ float soft_cap(float x, float cap, float inv_cap) {
   const float y = x * inv_cap, z = fabsf(y);
   const float e = __builtin_amdgcn_exp2f(z * (-2.f * kLog2eF));
-  const float big = (1.f - e) / (1.f + e);
+  const float big = (1.f - e) * __builtin_amdgcn_rcpf(1.f + e);
   const float w = y * y;
   float s = 21844.f / 6081075.f;
   s = __builtin_fmaf(s, w, -1382.f / 155925.f);
@@ -68,6 +68,13 @@ __device__ __forceinline__ float soft_cap(float x, float cap, float inv_cap) {
   const float small = __builtin_fmaf(z * w, s, z);
   const float t = z < 0.35f ? small : big;       // (NaN: big)
   return cap * __builtin_copysignf(t, y);
+}
+
+// The same to 2^-23 of the cap, in five instructions: cap - 2 cap / (1 + exp(2 y)).
+// scale is 2 log2(e) / cap.
+__device__ __forceinline__ float quick_cap(float x, float cap, float scale) {
+  const float e = __builtin_amdgcn_exp2f(x * scale);
+  return __builtin_fmaf(-2.f * cap, __builtin_amdgcn_rcpf(1.f + e), cap);
 }
 
 // The tiles of kKeyTile keys that a range of rows needs: those of [0, head) and, behind

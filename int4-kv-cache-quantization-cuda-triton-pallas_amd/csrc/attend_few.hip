@@ -222,7 +222,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
       }
     }
     const float slope = a.slopes ? a.slopes[hk * c.hq_per_kv + qh] * kLog2eF : 0.f;
-    const float inv_cap = 1.f / a.cap;
+    const float inv_cap = 1.f / a.cap, cap_scale = 2.f * kLog2eF / a.cap;
 
 #pragma unroll 1
     for (int u = 0; u < steps; ++u) {
@@ -284,7 +284,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float y = sv[i / 4][i % 4];
-        x[i] = a.cap > 0.f ? soft_cap(y * f, a.cap, inv_cap) * kLog2eF : y * (f * kLog2eF);
+        if (a.cap > 0.f)
+          x[i] = (WIDE ? soft_cap(y * f, a.cap, inv_cap) : quick_cap(y * f, a.cap, cap_scale)) *
+                 kLog2eF;
+        else
+          x[i] = y * (f * kLog2eF);
         const int t = t0 + 16 * (i / 4) + 4 * g + i % 4;
         if (a.slopes) x[i] = __builtin_fmaf(-slope, fabsf((float)(view.pos - t)), x[i]);
         x[i] = sees(view, t) ? x[i] : -INFINITY;

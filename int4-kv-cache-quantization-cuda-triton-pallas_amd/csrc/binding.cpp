@@ -905,15 +905,11 @@ std::vector<torch::Tensor> token_logprobs(torch::Tensor logits, torch::Tensor to
   auto ti = torch::empty({A, B, top}, logits.options().dtype(torch::kInt64));
   if (A * B > 0) {
     const fdi4_logprob_options opt = {(int)top, (float)logit_cap};
-    const size_t wsb = fdi4_token_logprobs_workspace_bytes(A * B, (int)V, (int)top);
-    torch::Tensor ws;
-    if (wsb) ws = workspace(logits, wsb);
     check_rc(fdi4_token_logprobs(logits.data_ptr(), code, A, B, logits.stride(0),
                                  logits.stride(1), (int)V, tokens.data_ptr<int64_t>(), &opt,
                                  lp.data_ptr<float>(),
                                  en.data_ptr<float>(), tl.data_ptr<float>(),
-                                 ti.data_ptr<int64_t>(), wsb ? ws.data_ptr() : nullptr, wsb,
-                                 stream()),
+                                 ti.data_ptr<int64_t>(), stream()),
              "token_logprobs");
   }
   return {lp, en, tl, ti};

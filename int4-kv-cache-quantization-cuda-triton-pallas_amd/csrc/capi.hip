@@ -1319,18 +1319,12 @@ int fdi4_norm_rotary(const void* q, const void* k, int dtype, int batch, int tok
   return fdi4::launch_norm_rotary(a, stream);
 }
 
-size_t fdi4_token_logprobs_workspace_bytes(int64_t rows, int vocab, int top) {
-  static_assert(FDI4_MAX_TOP == fdi4::kMaxTop, "alternatives");
-  if (rows < 1 || rows > INT32_MAX || vocab < 1 || top < 0 || top > FDI4_MAX_TOP) return 0;
-  const int s = fdi4::logprob_splits(rows, vocab);
-  return s > 1 ? (size_t)rows * s * (16 + 8 * (size_t)top) : 0;
-}
-
 int fdi4_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner,
                         int64_t outer_stride, int64_t inner_stride, int vocab,
                         const int64_t* tokens, const fdi4_logprob_options* options,
                         float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids,
-                        void* workspace, size_t workspace_bytes, hipStream_t stream) {
+                        hipStream_t stream) {
+  static_assert(FDI4_MAX_TOP == fdi4::kMaxTop, "alternatives");
   if (!options) return hipErrorInvalidValue;
   const int top = options->top;
   const float logit_cap = options->logit_cap;
@@ -1359,14 +1353,6 @@ int fdi4_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t in
   a.entropy = entropy;
   a.top_logprobs = top_logprobs;
   a.top_ids = top_ids;
-  a.splits = fdi4::logprob_splits(a.rows, vocab);
-  if (a.splits > 1) {
-    if (!workspace || !aligned(workspace, 16) ||
-        workspace_bytes < fdi4_token_logprobs_workspace_bytes(a.rows, vocab, top))
-      return hipErrorInvalidValue;
-    a.part_sums = static_cast<float4*>(workspace);
-    a.part_top = reinterpret_cast<uint64_t*>(a.part_sums + a.rows * a.splits);
-  }
   return fdi4::launch_token_logprobs(a, stream);
 }
 

@@ -222,12 +222,8 @@ struct LogprobArgs {
   float* entropy;                       // [rows]
   float* top_logprobs;                  // [rows, top]
   int64_t* top_ids;
-  int splits;                           // workgroups of a row
-  float4* part_sums;                    // [rows, splits] with several
-  uint64_t* part_top;                   // [rows, splits, top]
 };
-constexpr int kMaxTop = 64, kMaxRowSplits = 64;
-int logprob_splits(int64_t rows, int vocab);
+constexpr int kMaxTop = 64;
 
 // Several tokens per sequence appended: counts[b] of the new rows (by index when
 // given), the touched scale groups re-quantized, the open group staged.

@@ -10,17 +10,14 @@
 // (a place without one), a token past the vocabulary NaN. NaN logits come first among the
 // alternatives.
 //
-// token_logprobs_kernel: workgroups of 256 threads take the row's segments of kSegment
-// 16-byte vectors in turn, a segment in registers: its maximum, then one exponential a
-// logit. A thread keeps its own m, l and s, and they meet at the end.
-// Alternatives: the K-th largest of the threads' maxima is at most the K-th largest logit,
-// so only logits from there on (and above the K kept so far) are candidates, a few
-// dozen a segment; they are ranked by counting. Segments with more (rows of ties) take
-// their alternatives one after the other.
-// Several workgroups a row (few rows) leave partials that merge_logprobs_kernel joins.
-// Bound: memory.
-
-#include <algorithm>
+// A workgroup of NT threads takes a row in segments of 8 NT 16-byte vectors, a segment in
+// registers: its maximum, then one exponential a logit. A thread keeps its own m, l and s,
+// and they meet at the end. Bound: memory.
+//
+// Alternatives: the K-th largest of 64 groups' maxima is at most the K-th largest logit, so
+// only logits from there on, and above the K kept so far, are candidates: a few dozen in
+// the first segment, hardly any later. They are ranked by counting. Segments with more
+// than kCandidates (rows of ties) take their alternatives one after the other.
 
 #include "attend_common.hpp"
 
@@ -28,6 +25,7 @@ namespace fdi4 {
 
 constexpr int kVectors = 8;              // 16-byte vectors of a thread in a segment
 constexpr int kCandidates = 1024;        // of a segment, besides those kept
+constexpr int kFewRows = 256;            // below: workgroups of 1024 threads
 
 // A logit as a number whose order is the alternatives'.
 __device__ __forceinline__ unsigned order_of(float x) {
@@ -49,12 +47,13 @@ __device__ __forceinline__ uint64_t candidate(float x, int i) {
 __device__ __forceinline__ uint64_t max_u64(uint64_t x, uint64_t y) { return x > y ? x : y; }
 
 // Ranks `count` different candidates by counting and keeps the largest `top` in order.
-// keys: LDS, kept: LDS, which may be part of keys. All threads of the workgroup.
+template <int NT>
 __device__ __forceinline__ void rank_candidates(const uint64_t* keys, int count, int top,
                                                 uint64_t* sorted) {
-  for (int i = threadIdx.x; i < count; i += 256) {
+  for (int i = threadIdx.x; i < count; i += NT) {
     const uint64_t x = keys[i];
     int rank = 0;
+#pragma unroll 4
     for (int k = 0; k < count; ++k) rank += keys[k] > x;
     if (rank < top) sorted[rank] = x;
   }
@@ -83,62 +82,40 @@ __device__ __forceinline__ LogSums join_lanes(LogSums a) {
   return join(a, b);
 }
 
-// Results of a row whose alternatives are sorted in LDS.
-__device__ __forceinline__ void finish_row(const LogprobArgs& a, int64_t row, int64_t x0,
-                                           LogSums t, const uint64_t* sorted) {
-  const float inv_cap = 1.f / a.cap, log_l = logf(t.l);
-  auto log_of = [&](float x) {
-    if (a.cap > 0.f) x = soft_cap(x, a.cap, inv_cap);
-    return x - t.m - log_l;
-  };
-  if (threadIdx.x == 0) {
-    const int64_t tok = a.tokens[row];
-    a.logprobs[row] = tok < 0 ? 0.f
-                      : tok >= a.vocab ? __builtin_nanf("")
-                                       : log_of(load_elem(a.x, x0 + tok, a.dtype));
-    a.entropy[row] = log_l - t.s / t.l;
-  }
-  for (int k = threadIdx.x; k < a.top; k += 256) {
-    const uint64_t x = sorted[k];
-    a.top_logprobs[row * a.top + k] = log_of(logit_of((unsigned)(x >> 32)));
-    a.top_ids[row * a.top + k] = (int)~(unsigned)x;
-  }
-}
-
-template <int DT, bool TOP>
-__global__ __launch_bounds__(256) void token_logprobs_kernel(LogprobArgs a) {
+template <int DT, bool TOP, int NT>
+__global__ __launch_bounds__(NT, 4) void token_logprobs_kernel(LogprobArgs a) {
   constexpr int EV = DT == kEF32 ? 4 : 8;              // elements of a vector
   constexpr int EB = DT == kEF32 ? 4 : 2;
   constexpr int NE = kVectors * EV;                    // of a thread in a segment
+  constexpr int NW = NT / 64, GL = NT / 64;            // waves; lanes of a group
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int64_t row = blockIdx.x / (unsigned)a.splits;
-  const int split = (int)(blockIdx.x - row * a.splits);
+  const int64_t row = blockIdx.x;
   const int64_t x0 = row / a.inner * a.s_outer + row % a.inner * a.s_inner;
   const char* base = static_cast<const char*>(a.x) + x0 * EB;
   // Element 0 of vector 0 is at -skew: vectors lie on 16-byte boundaries.
   const int skew = (int)((uintptr_t)base % 16) / EB;
   const int vectors = (int)(((int64_t)a.vocab + skew + EV - 1) / EV);
-  const int segments = (vectors + 256 * kVectors - 1) / (256 * kVectors);
-  const float inv_cap = 1.f / a.cap;
+  const int segments = (vectors + NT * kVectors - 1) / (NT * kVectors);
+  const float cap_scale = 2.f * kLog2eF / a.cap;
 
   __shared__ uint64_t list_s[TOP ? kMaxTop + kCandidates : 1];
   __shared__ uint64_t sorted_s[TOP ? kMaxTop : 1];
-  __shared__ unsigned max_s[TOP ? 256 : 1];
-  __shared__ unsigned floor_s;
+  __shared__ unsigned group_s[64];
+  __shared__ int more_s[NW];
   __shared__ int count_s;
-  __shared__ LogSums sums_s[4];
-  __shared__ uint64_t best_s[4];
+  __shared__ LogSums sums_s[NW];
+  __shared__ uint64_t best_s[NW];
   int kept = 0;                                        // alternatives so far
   uint64_t least = 0;                                  // the last of `top` of them
 
   LogSums t = {kLeastF, 0.f, 0.f};
 #pragma unroll 1
-  for (int seg = split; seg < segments; seg += a.splits) {
-    const int v0 = seg * 256 * kVectors + tid;
+  for (int seg = 0; seg < segments; ++seg) {
+    const int v0 = seg * NT * kVectors + tid;
     // (Only the row's first and last vectors may be cut.)
     const bool cut = (seg == 0 && skew) || seg == segments - 1;
     auto vector = [&](int k, float* x) __attribute__((always_inline)) {
-      const int64_t e0 = (int64_t)(v0 + 256 * k) * EV - skew;
+      const int64_t e0 = (int64_t)(v0 + NT * k) * EV - skew;
       if (!cut || (e0 >= 0 && e0 + EV <= a.vocab)) {
         const U32x4 y = ld16(base + e0 * EB);
         widen_values<DT == kEF32 ? kVF32 : DT == kEF16 ? kVF16 : kVBF16>(y, x);
@@ -155,19 +132,24 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(LogprobArgs a) {
 #pragma unroll
     for (int k = 1; k < NE; ++k) mx = fmaxf(mx, x[k]);
     // (Of the logits as they are; a cap rises with them.)
-    const float mn = fmaxf(t.m, a.cap > 0.f ? soft_cap(mx, a.cap, inv_cap) : mx);
+    const float mn = fmaxf(t.m, a.cap > 0.f ? quick_cap(mx, a.cap, cap_scale) : mx);
     const float dm = t.m - mn, g = __builtin_amdgcn_exp2f(dm * kLog2eF);
     t.s = __builtin_fmaf(t.l, dm, t.s) * g;
     t.l *= g;
     t.m = mn;
     float l2[2] = {0.f, 0.f}, s2[2] = {0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < NE; ++k) {
-      const float y = a.cap > 0.f ? soft_cap(x[k], a.cap, inv_cap) : x[k];
+    auto add = [&](int k, float y) __attribute__((always_inline)) {
       const float d = y - mn, e = __builtin_amdgcn_exp2f(d * kLog2eF);
       l2[k & 1] += e;
       // (-infinity weighs nothing: 0 times a finite number.)
       s2[k & 1] = __builtin_fmaf(e, fmaxf(d, -1e30f), s2[k & 1]);
+    };
+    if (a.cap > 0.f) {
+#pragma unroll
+      for (int k = 0; k < NE; ++k) add(k, quick_cap(x[k], a.cap, cap_scale));
+    } else {
+#pragma unroll
+      for (int k = 0; k < NE; ++k) add(k, x[k]);
     }
     const float lt = l2[0] + l2[1];
     t.l += lt;
@@ -183,43 +165,59 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(LogprobArgs a) {
         for (int k = 0; k < kVectors; ++k) {
           float y[EV];
           vector(k, y);
-          const int64_t e0 = (int64_t)(v0 + 256 * k) * EV - skew;
+          const int64_t e0 = (int64_t)(v0 + NT * k) * EV - skew;
 #pragma unroll
           for (int j = 0; j < EV; ++j)
             if (e0 + j >= 0 && e0 + j < a.vocab) f(candidate(y[j], (int)(e0 + j)));
         }
       };
-      // Whether this segment can change anything.
-      if (!__syncthreads_or(mine > (unsigned)(least >> 32))) continue;
-      max_s[tid] = mine;
-      if (tid == 0) {
-        floor_s = 0;
-        count_s = kept;
-      }
+      // The threads with a logit above those kept, and the groups' maxima.
+      const unsigned floor = (unsigned)(least >> 32);
+      const int more = __builtin_popcountll(__builtin_amdgcn_ballot_w64(mine > floor));
+      unsigned gm = mine;
+      if constexpr (GL >= 2) gm = max(gm, xchg_u32<1>(gm));
+      if constexpr (GL >= 4) gm = max(gm, xchg_u32<2>(gm));
+      if constexpr (GL >= 8) gm = max(gm, xchg_u32<4>(gm));
+      if constexpr (GL >= 16) gm = max(gm, xchg_u32<8>(gm));
+      if (lane == 0) more_s[w] = more;
+      if (tid % GL == 0) group_s[tid / GL] = gm;
+      if (tid == 0) count_s = kept;
       if (tid < kept) list_s[tid] = sorted_s[tid];
       __syncthreads();
-      // The top-th largest of the threads' maxima (any of equal ones).
-      int above = 0, equal = 0;
-#pragma unroll 8
-      for (int k = 0; k < 256; ++k) {
-        above += max_s[k] > mine;
-        equal += max_s[k] == mine;
+      int all = 0;
+#pragma unroll
+      for (int k = 0; k < NW; ++k) all += more_s[k];
+      if (all == 0) {
+        // (group_s and more_s are written again behind this.)
+        __syncthreads();
+        continue;
       }
-      if (above < a.top && above + equal >= a.top) floor_s = mine;
-      __syncthreads();
-      const unsigned low = max(floor_s, (unsigned)(least >> 32));
-      if (mine >= low) {
+      unsigned low = floor;
+      if (all * NE > kCandidates) {
+        // The top-th largest group maximum (any of equal ones), found by every wave.
+        const unsigned v = group_s[lane];
+        int above = 0, equal = 0;
+#pragma unroll
+        for (int k = 0; k < 64; ++k) {
+          const unsigned o = (unsigned)__builtin_amdgcn_readlane((int)v, k);
+          above += o > v;
+          equal += o == v;
+        }
+        const uint64_t at =
+            __builtin_amdgcn_ballot_w64(above < a.top && above + equal >= a.top);
+        low = max(low, (unsigned)__builtin_amdgcn_readlane((int)v, __builtin_ctzll(at)));
+      }
+      if (mine >= low)
         each([&](uint64_t key) {
           if ((unsigned)(key >> 32) >= low && key > least) {
             const int at = atomicAdd(&count_s, 1);
             if (at < kMaxTop + kCandidates) list_s[at] = key;
           }
         });
-      }
       __syncthreads();
       const int count = count_s;
       if (count <= kMaxTop + kCandidates) {
-        rank_candidates(list_s, count, a.top, sorted_s);
+        rank_candidates<NT>(list_s, count, a.top, sorted_s);
         kept = min(count, a.top);
       } else {
         // Rows of ties: the best that is left, `top` times, of the segment and those kept.
@@ -228,11 +226,13 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(LogprobArgs a) {
         kept = 0;
         while (kept < a.top) {
           uint64_t best = tid < had && list_s[tid] < last ? list_s[tid] : 0;
-          if (mine >= low) each([&](uint64_t key) { best = key < last ? max_u64(best, key) : best; });
+          if (mine >= low)
+            each([&](uint64_t key) { best = key < last ? max_u64(best, key) : best; });
           for (int o = 1; o < 64; o *= 2) best = max_u64(best, __shfl_xor(best, o, 64));
           if (lane == 0) best_s[w] = best;
           __syncthreads();
-          last = max_u64(max_u64(best_s[0], best_s[1]), max_u64(best_s[2], best_s[3]));
+          last = best_s[0];
+          for (int k = 1; k < NW; ++k) last = max_u64(last, best_s[k]);
           if (tid == 0) sorted_s[kept] = last;
           ++kept;
           __syncthreads();
@@ -251,59 +251,44 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(LogprobArgs a) {
   t = join_lanes<32>(t);
   if (lane == 0) sums_s[w] = t;
   __syncthreads();
-  t = join(join(sums_s[0], sums_s[1]), join(sums_s[2], sums_s[3]));
-  if (a.splits == 1) {
-    finish_row(a, row, x0, t, sorted_s);
-    return;
+  t = sums_s[0];
+#pragma unroll
+  for (int k = 1; k < NW; ++k) t = join(t, sums_s[k]);
+  const float log_l = logf(t.l);
+  auto log_of = [&](float x) {
+    return (a.cap > 0.f ? quick_cap(x, a.cap, cap_scale) : x) - t.m - log_l;
+  };
+  if (tid == 0) {
+    const int64_t tok = a.tokens[row];
+    a.logprobs[row] = tok < 0 ? 0.f
+                      : tok >= a.vocab ? __builtin_nanf("")
+                                       : log_of(load_elem(a.x, x0 + tok, a.dtype));
+    a.entropy[row] = log_l - t.s / t.l;
   }
-  if (tid == 0) a.part_sums[blockIdx.x] = make_float4(t.m, t.l, t.s, 0.f);
-  if constexpr (TOP)
-    for (int k = tid; k < a.top; k += 256)
-      a.part_top[(int64_t)blockIdx.x * a.top + k] = k < kept ? sorted_s[k] : 0;
+  if constexpr (TOP) {
+    if (tid < a.top) {
+      const uint64_t x = sorted_s[tid];
+      a.top_logprobs[row * a.top + tid] = log_of(logit_of((unsigned)(x >> 32)));
+      a.top_ids[row * a.top + tid] = (int)~(unsigned)x;
+    }
+  }
 }
 
-__global__ __launch_bounds__(256) void merge_logprobs_kernel(LogprobArgs a) {
-  __shared__ uint64_t list_s[kMaxRowSplits * kMaxTop];
-  __shared__ uint64_t sorted_s[kMaxTop];
-  __shared__ int count_s;
-  const int64_t row = blockIdx.x;
-  const int64_t x0 = row / a.inner * a.s_outer + row % a.inner * a.s_inner;
-  if (threadIdx.x == 0) count_s = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.splits * a.top; i += 256) {
-    const uint64_t x = a.part_top[row * a.splits * a.top + i];
-    if (x) list_s[atomicAdd(&count_s, 1)] = x;
-  }
-  LogSums t = {kLeastF, 0.f, 0.f};
-  for (int i = 0; i < a.splits; ++i) {
-    const float4 x = a.part_sums[row * a.splits + i];
-    t = join(t, LogSums{x.x, x.y, x.z});
-  }
-  __syncthreads();
-  rank_candidates(list_s, count_s, a.top, sorted_s);
-  __syncthreads();
-  finish_row(a, row, x0, t, sorted_s);
-}
-
-// Workgroups a row: as many as fill the chip four times, one segment each at most.
-int logprob_splits(int64_t rows, int vocab) {
-  const int64_t segments = ((int64_t)vocab + 256 * kVectors * 4 - 1) / (256 * kVectors * 4);
-  return (int)std::max<int64_t>(
-      1, std::min<int64_t>(std::min<int64_t>(segments, kMaxRowSplits), 1024 / rows));
+template <int DT, int NT>
+void launch_logprobs(const LogprobArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)a.rows);
+  if (a.top)
+    hipLaunchKernelGGL((token_logprobs_kernel<DT, true, NT>), grid, dim3(NT), 0, st, a);
+  else
+    hipLaunchKernelGGL((token_logprobs_kernel<DT, false, NT>), grid, dim3(NT), 0, st, a);
 }
 
 hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)(a.rows * a.splits));
-#define FDI4_LP(DT)                                                                          \
-  if (a.dtype == DT) {                                                                       \
-    if (a.top) hipLaunchKernelGGL((token_logprobs_kernel<DT, true>), grid, dim3(256), 0, st, a); \
-    else hipLaunchKernelGGL((token_logprobs_kernel<DT, false>), grid, dim3(256), 0, st, a);  \
-  }
-  FDI4_LP(kEF32) FDI4_LP(kEF16) FDI4_LP(kEBF16)
-#undef FDI4_LP
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.splits == 1) return e;
-  hipLaunchKernelGGL(merge_logprobs_kernel, dim3((unsigned)a.rows), dim3(256), 0, st, a);
+  const bool few = a.rows < kFewRows;
+  if (a.dtype == kEF32) few ? launch_logprobs<kEF32, 1024>(a, st) : launch_logprobs<kEF32, 256>(a, st);
+  if (a.dtype == kEF16) few ? launch_logprobs<kEF16, 1024>(a, st) : launch_logprobs<kEF16, 256>(a, st);
+  if (a.dtype == kEBF16)
+    few ? launch_logprobs<kEBF16, 1024>(a, st) : launch_logprobs<kEBF16, 256>(a, st);
   return hipGetLastError();
 }
 

@@ -150,10 +150,9 @@ SIGNATURES = {
                                  c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
                                  c_int64, c_int64, ctypes.POINTER(RotaryOptions), c_void_p,
                                  c_void_p, c_void_p]),
-    "fdi4_token_logprobs_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
     "fdi4_token_logprobs": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int,
                                     c_void_p, ctypes.POINTER(LogprobOptions), c_void_p, c_void_p,
-                                    c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+                                    c_void_p, c_void_p, c_void_p]),
     "fdi4_extend_paged": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64,
                                   c_int64, c_int, c_int, c_void_p, c_void_p, c_int64, c_void_p,
                                   c_int64, c_int64, c_int64, c_int, ctypes.POINTER(PagedCache),

@@ -27,10 +27,10 @@ def rotary(q=P, k=P, dt=capi.K_BF16, B=2, N=3, Hq=8, H=2, D=128, pos=P, pb=1, pt
 
 
 def logprobs(x=P, dt=capi.K_BF16, outer=2, inner=3, vocab=1000, tok=P, cap=0.0, top=5, lp=P,
-             en=P, tl=P, ti=P, ws=P, wsb=1 << 40):
+             en=P, tl=P, ti=P):
     return capi.load().fdi4_token_logprobs(x, dt, outer, inner, 3000, 1000, vocab, tok,
                                            ctypes.byref(capi.LogprobOptions(top, cap)), lp, en,
-                                           tl, ti, ws, wsb, None)
+                                           tl, ti, None)
 
 
 @pytest.mark.parametrize("bad", BAD_CACHES + [dict(seq_lens=None), dict(pages_per_group=3),
@@ -84,23 +84,13 @@ def test_options_are_needed():
                                  capi.K_BF16, 0, P, 1 << 40, None) == INVALID
     assert lib.fdi4_norm_rotary(P, P, 0, 2, 3, 8, 2, 128, 0, 0, 0, 0, 0, 0, P, 1, 0, None, P, P,
                                 None) == INVALID
-    assert lib.fdi4_token_logprobs(P, 0, 2, 3, 3000, 1000, 1000, P, None, P, P, P, P, P, 1 << 40,
+    assert lib.fdi4_token_logprobs(P, 0, 2, 3, 3000, 1000, 1000, P, None, P, P, P, P,
                                    None) == INVALID
 
 
 def test_nothing_to_do():
     assert rotary(B=0, q=None) == 0 and rotary(N=0, qo=None) == 0
     assert logprobs(outer=0, x=None) == 0 and logprobs(inner=0, lp=None) == 0
-
-
-def test_logprobs_workspace():
-    size = capi.load().fdi4_token_logprobs_workspace_bytes
-    assert size(5000, 128000, 5) == 0
-    need = size(6, 128000, 5)
-    assert need >= 6 * (16 + 5 * 8)
-    for kw in (dict(ws=None), dict(wsb=need - 1), dict(ws=P + 8)):
-        assert logprobs(vocab=128000, **kw) == INVALID
-    assert size(0, 1000, 5) == 0 and size(6, 0, 5) == 0 and size(6, 1000, 65) == 0
 
 
 @pytest.mark.parametrize("kw", [
