@@ -559,8 +559,8 @@ typedef struct fdi4_logprob_options {
  * logprobs[r] = log p[tokens[r]] (0 for a negative token, NaN for one past the vocabulary),
  * entropy[r] = -sum p log p; with top > 0 top_ids[r, :] are the indices of the largest logits
  * (as they are before the cap), ties to the lowest index, NaN first, and top_logprobs[r, :]
- * their log p. Logits of -infinity have probability 0; rows with a NaN or +infinity, and
- * rows of -infinity, give NaN. All sums in float32. */
+ * their log p. Logits of -infinity have probability 0, also under a cap; rows with a NaN or
+ * +infinity, and rows of -infinity, give NaN. All sums in float32. */
 int fdi4_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner,
                         int64_t outer_stride, int64_t inner_stride, int vocab,
                         const int64_t* tokens, const fdi4_logprob_options* options,

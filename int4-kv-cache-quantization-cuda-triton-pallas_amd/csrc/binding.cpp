@@ -880,38 +880,60 @@ std::vector<torch::Tensor> norm_rotary(torch::Tensor q, torch::Tensor k, torch::
   return {qo, ko};
 }
 
-// Log probabilities of tokens int64 [A, B] in logits [A, B, vocab] (see
-// fdi4_token_logprobs): (logprobs [A, B], entropy [A, B], top log probabilities and int64
-// indices [A, B, top]).
+// Log probabilities of tokens [...] in logits [..., vocab] (see fdi4_token_logprobs):
+// (logprobs [...], entropy [...], top log probabilities and int64 indices [..., top]).
 std::vector<torch::Tensor> token_logprobs(torch::Tensor logits, torch::Tensor tokens,
                                           double logit_cap, int64_t top) {
   CHECK_DEV(logits);
   CHECK_SAME_DEVICE(logits, tokens);
   const int code = elem_code(logits, "logits");
-  TORCH_CHECK(logits.dim() == 3 && (logits.stride(2) == 1 || logits.size(2) == 1),
-              "logits must be [a, b, vocab] with contiguous rows");
-  const int64_t A = logits.size(0), B = logits.size(1), V = logits.size(2);
+  TORCH_CHECK(logits.dim() >= 1, "logits must be [..., vocab]");
+  const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+  TORCH_CHECK(tokens.sizes() == lead, "tokens must have one entry per row of logits");
+  TORCH_CHECK(tokens.scalar_type() == torch::kInt64 || tokens.scalar_type() == torch::kInt32,
+              "tokens must be int32 or int64");
+  const int64_t V = logits.size(-1), R = tokens.numel();
   TORCH_CHECK(V >= 1 && V <= INT32_MAX, "the vocabulary must have 1 to 2^31 - 1 tokens, got ", V);
   TORCH_CHECK(top >= 0 && top <= FDI4_MAX_TOP && top <= V, "top must lie in 0 .. min(",
               FDI4_MAX_TOP, ", vocab), got ", top);
-  TORCH_CHECK(tokens.scalar_type() == torch::kInt64 && tokens.dim() == 2 && tokens.size(0) == A &&
-                  tokens.size(1) == B && tokens.is_contiguous(),
-              "tokens must be contiguous int64, one per row of logits");
-  TORCH_CHECK(B == 0 || A <= INT32_MAX / B, "too many rows");
+  TORCH_CHECK(R <= INT32_MAX, "too many rows");
   const DeviceGuard guard(logits.device());
   auto f32 = logits.options().dtype(torch::kFloat32);
-  auto lp = torch::empty({A, B}, f32), en = torch::empty({A, B}, f32);
-  auto tl = torch::empty({A, B, top}, f32);
-  auto ti = torch::empty({A, B, top}, logits.options().dtype(torch::kInt64));
-  if (A * B > 0) {
-    const fdi4_logprob_options opt = {(int)top, (float)logit_cap};
-    check_rc(fdi4_token_logprobs(logits.data_ptr(), code, A, B, logits.stride(0),
-                                 logits.stride(1), (int)V, tokens.data_ptr<int64_t>(), &opt,
-                                 lp.data_ptr<float>(),
-                                 en.data_ptr<float>(), tl.data_ptr<float>(),
-                                 ti.data_ptr<int64_t>(), stream()),
-             "token_logprobs");
+  auto lp = torch::empty(lead, f32), en = torch::empty(lead, f32);
+  std::vector<int64_t> wide(lead.begin(), lead.end());
+  wide.push_back(top);
+  auto tl = torch::empty(wide, f32);
+  auto ti = torch::empty(wide, logits.options().dtype(torch::kInt64));
+  if (R == 0) return {lp, en, tl, ti};
+  if (logits.stride(-1) != 1 && V > 1) logits = logits.contiguous();
+  // Two strides reach the rows of logits[:, :-1] where they lie; what needs more is copied.
+  const int64_t outer = lead.size() > 1 ? lead[0] : 1, inner = R / outer;
+  int64_t so = lead.size() > 1 ? logits.stride(0) : 0, si = V;
+  bool two = true;
+  int64_t step = 0;
+  for (int64_t d = (int64_t)lead.size() - 1; d >= (lead.size() > 1 ? 1 : 0); --d) {
+    if (lead[d] == 1) continue;
+    if (step == 0) {
+      si = logits.stride(d);
+      step = si;
+    } else if (logits.stride(d) != step) {
+      two = false;
+    }
+    step *= lead[d];
   }
+  if (!two) {
+    logits = logits.contiguous();
+    so = inner * V;
+    si = V;
+  }
+  if (tokens.scalar_type() != torch::kInt64) tokens = tokens.to(torch::kInt64);
+  tokens = tokens.contiguous();
+  const fdi4_logprob_options opt = {(int)top, (float)logit_cap};
+  check_rc(fdi4_token_logprobs(logits.data_ptr(), code, outer, inner, so, si, (int)V,
+                               tokens.data_ptr<int64_t>(), &opt, lp.data_ptr<float>(),
+                               en.data_ptr<float>(), tl.data_ptr<float>(),
+                               ti.data_ptr<int64_t>(), stream()),
+           "token_logprobs");
   return {lp, en, tl, ti};
 }
 

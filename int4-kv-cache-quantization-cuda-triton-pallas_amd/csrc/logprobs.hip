@@ -5,8 +5,8 @@
 //   logprob = x[token] - m - log l,   entropy = log l - s / l
 //   alternatives: the largest logits, ties to the lowest index, as log probabilities
 //
-// A logit of -infinity has the probability zero and adds nothing to the entropy; a NaN,
-// +infinity or a row of -infinity makes the row's results NaN. A negative token gives 0
+// A logit of -infinity has the probability zero, also under a cap, and adds nothing to the
+// entropy; a NaN, +infinity or a row of -infinity makes the row's results NaN. A negative token gives 0
 // (a place without one), a token past the vocabulary NaN. NaN logits come first among the
 // alternatives.
 //
@@ -14,17 +14,19 @@
 // registers: its maximum, then one exponential a logit. A thread keeps its own m, l and s,
 // and they meet at the end. Bound: memory.
 //
-// Alternatives: the K-th largest of 64 groups' maxima is at most the K-th largest logit, so
-// only logits from there on, and above the K kept so far, are candidates: a few dozen in
-// the first segment, hardly any later. They are ranked by counting. Segments with more
-// than kCandidates (rows of ties) take their alternatives one after the other.
+// Alternatives: a thread also keeps the largest logit that it has met. The K-th largest of 64
+// groups' such maxima is at most the K-th largest logit, so only logits from there on are
+// candidates; every wave finds that bound by itself (18 of its bits, with ballots), and few
+// vectors hold one. The candidates (some K a segment, fewer as the bound rises) are ranked
+// once, by counting. Rows with more than kCandidates of them (thousands of ties) are read
+// again for each alternative.
 
 #include "attend_common.hpp"
 
 namespace fdi4 {
 
 constexpr int kVectors = 8;              // 16-byte vectors of a thread in a segment
-constexpr int kCandidates = 1024;        // of a segment, besides those kept
+constexpr int kCandidates = 2048;
 constexpr int kFewRows = 256;            // below: workgroups of 1024 threads
 
 // A logit as a number whose order is the alternatives'.
@@ -42,6 +44,12 @@ __device__ __forceinline__ float logit_of(unsigned o) {
 // An alternative: larger is better, of equal logits the lower index.
 __device__ __forceinline__ uint64_t candidate(float x, int i) {
   return (uint64_t)order_of(x) << 32 | (unsigned)~i;
+}
+
+// A capped logit; infinite ones stay so (a product with the smallest number adds nothing to
+// others).
+__device__ __forceinline__ float cap_logit(float x, float cap, float scale) {
+  return __builtin_fmaf(x, 1.4e-45f, quick_cap(x, cap, scale));
 }
 
 __device__ __forceinline__ uint64_t max_u64(uint64_t x, uint64_t y) { return x > y ? x : y; }
@@ -86,8 +94,9 @@ template <int DT, bool TOP, int NT>
 __global__ __launch_bounds__(NT, 4) void token_logprobs_kernel(LogprobArgs a) {
   constexpr int EV = DT == kEF32 ? 4 : 8;              // elements of a vector
   constexpr int EB = DT == kEF32 ? 4 : 2;
-  constexpr int NE = kVectors * EV;                    // of a thread in a segment
   constexpr int NW = NT / 64, GL = NT / 64;            // waves; lanes of a group
+  // -infinity in both halves of a word (float32: in the word).
+  constexpr unsigned kNone = DT == kEF32 ? 0xFF800000u : DT == kEF16 ? 0xFC00FC00u : 0xFF80FF80u;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int64_t row = blockIdx.x;
   const int64_t x0 = row / a.inner * a.s_outer + row % a.inner * a.s_inner;
@@ -98,148 +107,131 @@ __global__ __launch_bounds__(NT, 4) void token_logprobs_kernel(LogprobArgs a) {
   const int segments = (vectors + NT * kVectors - 1) / (NT * kVectors);
   const float cap_scale = 2.f * kLog2eF / a.cap;
 
-  __shared__ uint64_t list_s[TOP ? kMaxTop + kCandidates : 1];
+  __shared__ uint64_t list_s[TOP ? kCandidates : 1];
   __shared__ uint64_t sorted_s[TOP ? kMaxTop : 1];
-  __shared__ unsigned group_s[64];
-  __shared__ int more_s[NW];
+  __shared__ unsigned group_s[2][64];
   __shared__ int count_s;
   __shared__ LogSums sums_s[NW];
   __shared__ uint64_t best_s[NW];
-  int kept = 0;                                        // alternatives so far
-  uint64_t least = 0;                                  // the last of `top` of them
+  unsigned largest = 0, low = 0;                       // of this thread; the bound
+  if (TOP && tid == 0) count_s = 0;
+
+  auto widen = [](U32x4 v, float* x) __attribute__((always_inline)) {
+    widen_values<DT == kEF32 ? kVF32 : DT == kEF16 ? kVF16 : kVBF16>(v, x);
+  };
+  // Vector v of the row, -infinity for what lies before and behind it.
+  auto load = [&](int v) __attribute__((always_inline)) -> U32x4 {
+    const int64_t e0 = (int64_t)v * EV - skew;
+    if (e0 >= 0 && e0 + EV <= a.vocab) return ld16(base + e0 * EB);
+    unsigned y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (DT == kEF32) {
+        y[j] = e0 + j >= 0 && e0 + j < a.vocab
+                   ? reinterpret_cast<const unsigned*>(base)[e0 + j] : kNone;
+      } else {
+        const unsigned short* p = reinterpret_cast<const unsigned short*>(base);
+        const int64_t e = e0 + 2 * j;
+        y[j] = (e >= 0 && e < a.vocab ? p[e] : kNone & 0xFFFFu) |
+               (e + 1 >= 0 && e + 1 < a.vocab ? (unsigned)p[e + 1] << 16 : kNone << 16);
+      }
+    }
+    return U32x4{y[0], y[1], y[2], y[3]};
+  };
 
   LogSums t = {kLeastF, 0.f, 0.f};
 #pragma unroll 1
   for (int seg = 0; seg < segments; ++seg) {
     const int v0 = seg * NT * kVectors + tid;
-    // (Only the row's first and last vectors may be cut.)
-    const bool cut = (seg == 0 && skew) || seg == segments - 1;
-    auto vector = [&](int k, float* x) __attribute__((always_inline)) {
-      const int64_t e0 = (int64_t)(v0 + NT * k) * EV - skew;
-      if (!cut || (e0 >= 0 && e0 + EV <= a.vocab)) {
-        const U32x4 y = ld16(base + e0 * EB);
-        widen_values<DT == kEF32 ? kVF32 : DT == kEF16 ? kVF16 : kVBF16>(y, x);
-      } else {
+    // Vectors a thread has here (uniform; the last may be behind the row).
+    const int nk = min(kVectors, (vectors - seg * NT * kVectors + NT - 1) / NT);
+    U32x4 raw[kVectors];
+    if (seg + 1 < segments && (seg > 0 || skew == 0)) {
 #pragma unroll
-        for (int j = 0; j < EV; ++j)
-          x[j] = e0 + j >= 0 && e0 + j < a.vocab ? load_elem(base, e0 + j, DT) : -INFINITY;
+      for (int k = 0; k < kVectors; ++k)
+        raw[k] = ld16(base + ((int64_t)(v0 + NT * k) * EV - skew) * EB);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kVectors; ++k)
+        if (k < nk) raw[k] = load(v0 + NT * k);
+    }
+    float mv[kVectors], mx = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k)
+      if (k < nk) {
+        float x[EV];
+        widen(raw[k], x);
+        mv[k] = x[0];
+#pragma unroll
+        for (int j = 1; j < EV; ++j) mv[k] = fmaxf(mv[k], x[j]);
+        mx = fmaxf(mx, mv[k]);
       }
-    };
-    float x[NE];
-#pragma unroll
-    for (int k = 0; k < kVectors; ++k) vector(k, x + EV * k);
-    float mx = x[0];
-#pragma unroll
-    for (int k = 1; k < NE; ++k) mx = fmaxf(mx, x[k]);
     // (Of the logits as they are; a cap rises with them.)
-    const float mn = fmaxf(t.m, a.cap > 0.f ? quick_cap(mx, a.cap, cap_scale) : mx);
+    const float mn = fmaxf(t.m, a.cap > 0.f ? cap_logit(mx, a.cap, cap_scale) : mx);
     const float dm = t.m - mn, g = __builtin_amdgcn_exp2f(dm * kLog2eF);
     t.s = __builtin_fmaf(t.l, dm, t.s) * g;
     t.l *= g;
     t.m = mn;
     float l2[2] = {0.f, 0.f}, s2[2] = {0.f, 0.f};
-    auto add = [&](int k, float y) __attribute__((always_inline)) {
-      const float d = y - mn, e = __builtin_amdgcn_exp2f(d * kLog2eF);
-      l2[k & 1] += e;
-      // (-infinity weighs nothing: 0 times a finite number.)
-      s2[k & 1] = __builtin_fmaf(e, fmaxf(d, -1e30f), s2[k & 1]);
-    };
-    if (a.cap > 0.f) {
 #pragma unroll
-      for (int k = 0; k < NE; ++k) add(k, quick_cap(x[k], a.cap, cap_scale));
-    } else {
+    for (int k = 0; k < kVectors; ++k)
+      if (k < nk) {
+        float x[EV];
+        widen(raw[k], x);
+        if (a.cap > 0.f) {
 #pragma unroll
-      for (int k = 0; k < NE; ++k) add(k, x[k]);
-    }
+          for (int j = 0; j < EV; ++j) x[j] = cap_logit(x[j], a.cap, cap_scale);
+        }
+#pragma unroll
+        for (int j = 0; j < EV; ++j) {
+          const float d = x[j] - mn, e = __builtin_amdgcn_exp2f(d * kLog2eF);
+          l2[j & 1] += e;
+          // (-infinity weighs nothing: 0 times a finite number.)
+          s2[j & 1] = __builtin_fmaf(e, fmaxf(d, -1e30f), s2[j & 1]);
+        }
+      }
     const float lt = l2[0] + l2[1];
     t.l += lt;
     t.s += s2[0] + s2[1];
 
     if constexpr (TOP) {
       // A NaN among the thread's logits comes before all (its sum is NaN too).
-      const unsigned mine = lt != lt ? 0xFFFFFFFFu : order_of(mx);
-      // This thread's logits once more (few threads have a candidate; the segment is in
-      // the caches, and registers that held it for them would cost every wave).
-      auto each = [&](auto&& f) {
-#pragma unroll 1
-        for (int k = 0; k < kVectors; ++k) {
-          float y[EV];
-          vector(k, y);
-          const int64_t e0 = (int64_t)(v0 + NT * k) * EV - skew;
-#pragma unroll
-          for (int j = 0; j < EV; ++j)
-            if (e0 + j >= 0 && e0 + j < a.vocab) f(candidate(y[j], (int)(e0 + j)));
-        }
-      };
-      // The threads with a logit above those kept, and the groups' maxima.
-      const unsigned floor = (unsigned)(least >> 32);
-      const int more = __builtin_popcountll(__builtin_amdgcn_ballot_w64(mine > floor));
-      unsigned gm = mine;
+      const bool nan = lt != lt;
+      const unsigned mine = nan ? 0xFFFFFFFFu : order_of(mx);
+      largest = max(largest, mine);
+      unsigned gm = largest;
       if constexpr (GL >= 2) gm = max(gm, xchg_u32<1>(gm));
       if constexpr (GL >= 4) gm = max(gm, xchg_u32<2>(gm));
       if constexpr (GL >= 8) gm = max(gm, xchg_u32<4>(gm));
       if constexpr (GL >= 16) gm = max(gm, xchg_u32<8>(gm));
-      if (lane == 0) more_s[w] = more;
-      if (tid % GL == 0) group_s[tid / GL] = gm;
-      if (tid == 0) count_s = kept;
-      if (tid < kept) list_s[tid] = sorted_s[tid];
+      if (tid % GL == 0) group_s[seg & 1][tid / GL] = gm;
+      // (The other buffer may still be read by a wave that is a segment behind.)
       __syncthreads();
-      int all = 0;
+      if (__builtin_amdgcn_ballot_w64(mine >= low)) {
+        const unsigned v = group_s[seg & 1][lane];
+        unsigned bound = 0;
 #pragma unroll
-      for (int k = 0; k < NW; ++k) all += more_s[k];
-      if (all == 0) {
-        // (group_s and more_s are written again behind this.)
-        __syncthreads();
-        continue;
-      }
-      unsigned low = floor;
-      if (all * NE > kCandidates) {
-        // The top-th largest group maximum (any of equal ones), found by every wave.
-        const unsigned v = group_s[lane];
-        int above = 0, equal = 0;
-#pragma unroll
-        for (int k = 0; k < 64; ++k) {
-          const unsigned o = (unsigned)__builtin_amdgcn_readlane((int)v, k);
-          above += o > v;
-          equal += o == v;
+        for (int bit = 31; bit >= 14; --bit) {
+          const unsigned more = bound | 1u << bit;
+          if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(v >= more)) >= a.top) bound = more;
         }
-        const uint64_t at =
-            __builtin_amdgcn_ballot_w64(above < a.top && above + equal >= a.top);
-        low = max(low, (unsigned)__builtin_amdgcn_readlane((int)v, __builtin_ctzll(at)));
-      }
-      if (mine >= low)
-        each([&](uint64_t key) {
-          if ((unsigned)(key >> 32) >= low && key > least) {
-            const int at = atomicAdd(&count_s, 1);
-            if (at < kMaxTop + kCandidates) list_s[at] = key;
-          }
-        });
-      __syncthreads();
-      const int count = count_s;
-      if (count <= kMaxTop + kCandidates) {
-        rank_candidates<NT>(list_s, count, a.top, sorted_s);
-        kept = min(count, a.top);
-      } else {
-        // Rows of ties: the best that is left, `top` times, of the segment and those kept.
-        const int had = kept;
-        uint64_t last = ~0ull;
-        kept = 0;
-        while (kept < a.top) {
-          uint64_t best = tid < had && list_s[tid] < last ? list_s[tid] : 0;
-          if (mine >= low)
-            each([&](uint64_t key) { best = key < last ? max_u64(best, key) : best; });
-          for (int o = 1; o < 64; o *= 2) best = max_u64(best, __shfl_xor(best, o, 64));
-          if (lane == 0) best_s[w] = best;
-          __syncthreads();
-          last = best_s[0];
-          for (int k = 1; k < NW; ++k) last = max_u64(last, best_s[k]);
-          if (tid == 0) sorted_s[kept] = last;
-          ++kept;
-          __syncthreads();
+        low = max(low, bound);
+        if (mine >= low) {
+#pragma unroll
+          for (int k = 0; k < kVectors; ++k)
+            if (k < nk && (nan || order_of(mv[k]) >= low)) {
+              float x[EV];
+              widen(raw[k], x);
+              const int64_t e0 = (int64_t)(v0 + NT * k) * EV - skew;
+#pragma unroll
+              for (int j = 0; j < EV; ++j)
+                if (e0 + j >= 0 && e0 + j < a.vocab && order_of(x[j]) >= low) {
+                  const int at = atomicAdd(&count_s, 1);
+                  if (at < kCandidates) list_s[at] = candidate(x[j], (int)(e0 + j));
+                }
+            }
         }
       }
-      __syncthreads();
-      least = kept == a.top ? sorted_s[a.top - 1] : 0;
     }
   }
 
@@ -256,7 +248,7 @@ __global__ __launch_bounds__(NT, 4) void token_logprobs_kernel(LogprobArgs a) {
   for (int k = 1; k < NW; ++k) t = join(t, sums_s[k]);
   const float log_l = logf(t.l);
   auto log_of = [&](float x) {
-    return (a.cap > 0.f ? quick_cap(x, a.cap, cap_scale) : x) - t.m - log_l;
+    return (a.cap > 0.f ? cap_logit(x, a.cap, cap_scale) : x) - t.m - log_l;
   };
   if (tid == 0) {
     const int64_t tok = a.tokens[row];
@@ -266,6 +258,35 @@ __global__ __launch_bounds__(NT, 4) void token_logprobs_kernel(LogprobArgs a) {
     a.entropy[row] = log_l - t.s / t.l;
   }
   if constexpr (TOP) {
+    if (count_s <= kCandidates) {
+      rank_candidates<NT>(list_s, count_s, a.top, sorted_s);
+    } else {
+      // The best that is left, `top` times.
+      uint64_t last = ~0ull;
+#pragma unroll 1
+      for (int i = 0; i < a.top; ++i) {
+        uint64_t best = 0;
+#pragma unroll 1
+        for (int v = tid; v < vectors; v += NT) {
+          float x[EV];
+          widen(load(v), x);
+          const int64_t e0 = (int64_t)v * EV - skew;
+#pragma unroll
+          for (int j = 0; j < EV; ++j) {
+            const uint64_t key = candidate(x[j], (int)(e0 + j));
+            if (e0 + j >= 0 && e0 + j < a.vocab && key < last) best = max_u64(best, key);
+          }
+        }
+        for (int o = 1; o < 64; o *= 2) best = max_u64(best, __shfl_xor(best, o, 64));
+        if (lane == 0) best_s[w] = best;
+        __syncthreads();
+        last = best_s[0];
+        for (int k = 1; k < NW; ++k) last = max_u64(last, best_s[k]);
+        if (tid == 0) sorted_s[i] = last;
+        __syncthreads();
+      }
+    }
+    __syncthreads();
     if (tid < a.top) {
       const uint64_t x = sorted_s[tid];
       a.top_logprobs[row * a.top + tid] = log_of(logit_of((unsigned)(x >> 32)));

@@ -149,8 +149,8 @@ def token_logprobs(logits, tokens, top: int = 0, logit_cap: Optional[float] = No
     Returns:
         TokenLogprobs of logprobs float32 [...], entropy float32 [...] (in nats),
         top_logprobs float32 [..., top] and top_ids int64 [..., top]: the largest logits,
-        ties to the lowest index. Logits of -infinity have probability zero; a row with a
-        NaN or +infinity, or of -infinity alone, gives NaN (its alternatives put NaN first).
+        ties to the lowest index. Logits of -infinity have probability zero, also under a
+        cap; a row with a NaN or +infinity, or of -infinity alone, gives NaN (its alternatives put NaN first).
     """
     import torch
     from .ops import _checked_cap
@@ -171,13 +171,4 @@ def token_logprobs(logits, tokens, top: int = 0, logit_cap: Optional[float] = No
     if not logits.is_cuda or not tokens.is_cuda:
         raise RuntimeError("logits and tokens must be GPU (cuda device) tensors; this package "
                            "has no CPU path")
-    lead, vocab = tuple(logits.shape[:-1]), logits.shape[-1]
-    if logits.stride(-1) != 1 and vocab > 1:
-        logits = logits.contiguous()
-    outer = lead[0] if len(lead) > 1 else 1
-    rows = logits.reshape(outer, -1, vocab) if 0 not in lead else \
-        logits.new_empty((0, 0, vocab))
-    ids = tokens.to(torch.int64).reshape(rows.shape[:2]).contiguous()
-    lp, entropy, tl, ti = binding.token_logprobs(rows, ids, cap, top)
-    return TokenLogprobs(lp.view(lead), entropy.view(lead), tl.view(*lead, top),
-                         ti.view(*lead, top))
+    return TokenLogprobs(*binding.token_logprobs(logits, tokens, cap, top))

@@ -154,6 +154,29 @@ def test_infinities_and_nan():
     check(type(out)(*[t[7:] for t in out]), x[7:], tok[7:], 6)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("vocab", [5, 999, 33001])
+def test_small_caps_and_masked_logits(vocab, dtype):
+    """Logits of -infinity stay masked under a cap that would make them count, and nothing
+    behind a row does."""
+    import torch
+    from flash_decode_int4.quality import token_logprobs
+    x, tok = make((9,), vocab, dtype)
+    check(token_logprobs(x, tok, 4, logit_cap=0.5), x, tok, 4, 0.5)
+    x[:, 2::3] = -float("inf")
+    tok[:] = 1
+    out = token_logprobs(x, tok, 3, logit_cap=0.5)
+    kept = [i for i in range(vocab) if i % 3 != 2]
+    part = x[:, kept].contiguous()
+    lp, ent, tl, ids, m = oracle(part, tok, 3, 0.5)
+    base = (64 + 45) * U + 2.0 ** -22 * 0.5 + 4 * U * 31
+    for got, want in ((out.logprobs, lp), (out.entropy, ent)):
+        g = got.double().cpu().numpy()
+        assert (np.abs(g - want) <= 2 * base + 4 * U * np.abs(want) + base * np.abs(ent)).all()
+    assert (out.top_ids.cpu().numpy() == np.asarray(kept)[ids]).all()
+    assert (token_logprobs(x, tok + 1, 0, logit_cap=0.5).logprobs == -float("inf")).all()
+
+
 def test_places_without_a_token():
     import torch
     from flash_decode_int4.quality import token_logprobs
