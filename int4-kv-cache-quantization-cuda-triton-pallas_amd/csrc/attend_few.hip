@@ -1,20 +1,26 @@
-// Attention of a few cached tokens (gfx950): up to 16 rows a kv-head, one token of a decode
+// Attention of a few cached tokens (gfx950): up to 32 rows a kv-head, one token of a decode
 // step above all. Memory bound: what counts is that the cache is read once, in long runs.
 //
-// A workgroup of four waves takes the rows of one kv-head over a range of 64-key tiles,
-// which go to the waves in turn. A wave loads 32 keys straight to registers and dequantizes
-// them there (k = nib*s - zp*s as float16 in units of a power of two for the scale group's
-// largest). The next keys are loaded as soon as these are multiplied, the next values as
-// soon as these are. Waves meet at the end, in LDS, and splits in the merge kernel.
+// A workgroup of four waves takes 16 rows of one kv-head over a range of 64-key tiles,
+// which go to the waves in pairs. A wave loads 32 keys straight to registers; the next keys
+// are loaded as soon as these are multiplied, the next values as soon as these are. Waves
+// meet at the end, in LDS, and splits in the merge kernel.
 //
+//   terms: q . k_t = sum_d v_d (nib_td - zp_d), v = q*s. Per scale group and row, v is made
+//      into two float16 terms (22 bits, in units of a power of two for the largest), once for
+//      the group's keys, and multiplied by the nibbles as they are stored: a nibble at bits 6
+//      to 9 of a float16 is the number nib * 2^-18. The constant sum_d v_d zp_d, in
+//      float32, goes in with the exponent's FMA. Dequantized keys, in two terms as well, took
+//      900 instructions of the vector units for 32 keys in place of 350, and 155 us in
+//      place of XXX for 16 sequences of 16384 bfloat16 tokens and 8 kv-heads.
 //   scores: v_mfma_f32_16x16x32_f16 of 16 keys (A) and 16 rows (B): lane (g, r) loads the
 //      channels g * D/4 .. of key r and of row r, eight of them a product.
 //   values: lane (g, r) holds the scores of row r with keys 4g .. 4g + 3 of both 16-key
 //      halves, which is the B operand of a product of 32 keys, and loads the channels r *
 //      D/16 .. of the same keys: byte permutes pair them.
 //
-// Terms as the kernel of many rows (attend_chunk.hip) has them, but two of keys also for
-// 16-bit outputs: the vector units have time.
+// Probabilities are in as many terms as in the kernel of many rows (attend_chunk.hip). PAGED:
+// pages hold whole runs of 16 rows, so that a run's address is the same for all lanes.
 
 #include "attend_common.hpp"
 
@@ -24,7 +30,6 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 
 template <int D, int VDT, bool WIDE>
 struct FewGeo {
-  static constexpr int TQ = WIDE ? 2 : 1;
   static constexpr int TV = VDT == kVF32 ? (WIDE ? 3 : 2) : 1;
   static constexpr int TP = VDT == kVF16 ? (WIDE ? 2 : 1) : (WIDE ? 3 : 1);
   static constexpr int VEB = VDT == kVF32 ? 4 : 2;
@@ -79,7 +84,7 @@ __device__ __forceinline__ Words<N> load_stream(const uint8_t* p) {
   return r;
 }
 
-template <int D, int VDT, bool WIDE>
+template <int D, int VDT, bool WIDE, bool PAGED>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(AttendArgs a) {
   using G = FewGeo<D, VDT, WIDE>;
   constexpr int kWaves = 4;
@@ -88,24 +93,35 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
   const DecodeArgs& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wi = (int)blockIdx.x, wj = fdiv(wi, c.div_splits), split = wi - wj * c.num_splits;
+  // The groups of 16 rows of one (sequence, kv-head, split) run on one XCD.
+  const int L = a.tiles > 1 ? (int)xcd_run_item(blockIdx.x, gridDim.x, (unsigned)a.tiles)
+                            : (int)blockIdx.x;
+  const int wi = a.tiles > 1 ? L / a.tiles : L, row0 = 16 * (L - wi * a.tiles);
+  const int wj = fdiv(wi, c.div_splits), split = wi - wj * c.num_splits;
   const int b = fdiv(wj, a.div_heads), hk = wj - b * a.kv_heads;
-  const int rows = c.hq_per_kv * a.queries;
+  const int all_rows = c.hq_per_kv * a.queries, rows = min(all_rows - row0, 16);
   const int n = seq_len_of(c, b), cnt = count_of(a, b), prefix = prefix_of(a, b, n);
 
   __shared__ __align__(16) float acc_s[kWaves][16][G::AS];
   __shared__ float m_s[kWaves][16], l_s[kWaves][16];
+  __shared__ __align__(16) float q_s[16][G::AS];       // the rows' queries
+  __shared__ __align__(16) float sz_s[kWaves][2][D];   // a wave's scales and zero-points
 
   // ---- this lane's row ----
-  const int R = min(r16, rows - 1), qi = fdiv(R, c.div_hpk), qh = R - qi * c.hq_per_kv;
+  const int R = row0 + min(r16, rows - 1), qi = fdiv(R, c.div_hpk), qh = R - qi * c.hq_per_kv;
   const bool live = r16 < rows && qi < cnt;
   const RowView view = row_view(a, n, cnt, prefix, live ? qi : a.queries);
-  const RowView v_lo = row_view(a, n, cnt, prefix, 0);
-  const RowView v_hi = row_view(a, n, cnt, prefix, max(cnt - 1, 0));
+  const int i_lo = fdiv(row0, c.div_hpk), i_hi = min(fdiv(row0 + rows - 1, c.div_hpk), cnt - 1);
+  const RowView v_lo = row_view(a, n, cnt, prefix, i_lo);
+  const RowView v_hi = row_view(a, n, cnt, prefix, max(i_hi, 0));
   TileList list = tile_list(v_hi.head, v_lo.low, v_hi.pos);
-  if (cnt == 0) list.total = 0;
-  const int j0 = (int)((int64_t)split * list.total / c.num_splits);
-  const int j1 = (int)((int64_t)(split + 1) * list.total / c.num_splits);
+  if (i_hi < i_lo) list.total = 0;
+  // Pairs of tiles, which mostly lie in one scale group, to splits and waves; single ones
+  // where a wave would be without.
+  const int pairs = (list.total + 1) >> 1;
+  const int j0 = 2 * (int)((int64_t)split * pairs / c.num_splits);
+  const int j1 = min(2 * (int)((int64_t)(split + 1) * pairs / c.num_splits), list.total);
+  const int item = j1 - j0 > kWaves ? 2 : 1;
   bool wild = false;
 
   v4f acc[G::NA];
@@ -113,58 +129,78 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
 #pragma unroll
   for (int t = 0; t < G::NA; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
 
-  const float* sbase = c.k_scale + (int64_t)b * c.s_b + (int64_t)hk * c.s_h + g * G::CH;
-  const float* zbase = c.k_zp + (int64_t)b * c.s_b + (int64_t)hk * c.s_h + g * G::CH;
-  const uint8_t* kbase = c.k_pages + (int64_t)hk * c.k_head + g * (D / 8);
-  const uint8_t* vbase = static_cast<const uint8_t*>(c.v_pages) +
-                         ((int64_t)hk * c.v_head + r16 * G::NA) * G::VEB;
+  const float* sbase = c.k_scale + (int64_t)b * c.s_b + (int64_t)hk * c.s_h;
+  const float* zbase = c.k_zp + (int64_t)b * c.s_b + (int64_t)hk * c.s_h;
+  const uint8_t* kbase = c.k_pages + (int64_t)hk * c.k_head;
+  const uint8_t* vbase = static_cast<const uint8_t*>(c.v_pages) + (int64_t)hk * c.v_head * G::VEB;
+  const int k_lane = g * (D / 8), v_lane = r16 * G::NA * G::VEB;
   const int32_t* table = c.page_table ? c.page_table + (int64_t)b * c.pt_b : nullptr;
 
   // Step u of this wave: 32 keys, two to a tile.
-  const int mine = max(j1 - j0 - w + kWaves - 1, 0) / kWaves, steps = 2 * mine;
-  auto key0_of = [&](int u) { return list.tile(j0 + w + kWaves * (u >> 1)) * kKeyTile + 32 * (u & 1); };
+  const int rounds = max(j1 - j0 - w * item + kWaves * item - 1, 0) / (kWaves * item);
+  const int last = j0 + (w + kWaves * (rounds - 1)) * item;   // its last item's first tile
+  const int steps =
+      rounds > 0 ? 2 * (item * (rounds - 1) + min(item, j1 - last)) : 0;
+  auto key0_of = [&](int u) {
+    const int k = u >> 1, round = item == 2 ? k >> 1 : k;
+    const int j = j0 + (w + kWaves * round) * item + (item == 2 ? k & 1 : 0);
+    return list.tile(j) * kKeyTile + 32 * (u & 1);
+  };
 
   Words<G::NK> kf[2];
   Words<G::VW> vf[2][4];
-  // This lane's key of both halves of a step: page and row within it; the entries of the
-  // table a step ahead.
+  // PAGED: a run's place, the same for all lanes. Otherwise this lane's key of both halves
+  // of a step, its page and row; the entries of the table a step ahead.
   int entry[2], phys[2], prow[2];
+  auto key_at = [&](int u, int h) {
+    const int t = key0_of(min(u, steps - 1)) + 16 * h;
+    return PAGED ? min(t, (n - 1) & ~15) : min(t + r16, n - 1);
+  };
   auto load_entries = [&](int u) __attribute__((always_inline)) {
-    const int t0 = key0_of(min(u, steps - 1));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int lp = fdiv(min(t0 + 16 * h + r16, n - 1), c.div_rows);
-      entry[h] = table ? table[lp] : lp;
+      const int lp = fdiv(key_at(u, h), c.div_rows);
+      if constexpr (PAGED) entry[h] = table ? ld_ro(table, lp) : lp;
+      else entry[h] = table ? table[lp] : lp;
     }
   };
   auto load_keys = [&](int u) __attribute__((always_inline)) {
-    const int t0 = key0_of(min(u, steps - 1));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int t = min(t0 + 16 * h + r16, n - 1);
+      const int t = key_at(u, h);
       prow[h] = t - fdiv(t, c.div_rows) * c.page_rows;
       phys[h] = min(max(entry[h], 0), c.num_pages - 1);
-      kf[h] = load_stream<G::NK>(kbase + (int64_t)phys[h] * c.k_page + (int64_t)prow[h] * c.k_row);
+      const uint8_t* at = kbase + ((int64_t)phys[h] * c.k_page + (int64_t)prow[h] * c.k_row);
+      kf[h] = load_stream<G::NK>(at + (PAGED ? k_lane + r16 * (int)c.k_row : k_lane));
     }
   };
   auto load_values = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h) {
+      const uint8_t* at =
+          vbase + ((int64_t)phys[h] * c.v_page + (int64_t)prow[h] * c.v_row) * G::VEB;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int pv = __shfl(phys[h], 4 * g + i, 16), rv = __shfl(prow[h], 4 * g + i, 16);
-        vf[h][i] = load_stream<G::VW>(
-            vbase + ((int64_t)pv * c.v_page + (int64_t)rv * c.v_row) * G::VEB);
+        if constexpr (PAGED) {
+          vf[h][i] = load_stream<G::VW>(at + (v_lane + (4 * g + i) * (int)(c.v_row * G::VEB)));
+        } else {
+          const int pv = __shfl(phys[h], 4 * g + i, 16), rv = __shfl(prow[h], 4 * g + i, 16);
+          vf[h][i] = load_stream<G::VW>(
+              vbase + (((int64_t)pv * c.v_page + (int64_t)rv * c.v_row) * G::VEB + v_lane));
+        }
       }
+    }
   };
-  float sc[G::CH], zs[G::CH];
-  int unit = 0;
-  auto load_scales = [&](int u) __attribute__((always_inline)) {
-    const int64_t at = (int64_t)fdiv(key0_of(min(u, steps - 1)), a.div_group) * c.s_g;
+  // Scales and zero-points of a group, D / 64 channels a lane (they go through LDS).
+  constexpr int SL = D / 64;
+  float sc[SL], zp[SL];
+  auto group_at = [&](int u) { return fdiv(key0_of(min(u, steps - 1)), a.div_group); };
+  auto load_scales = [&](int group) __attribute__((always_inline)) {
+    const int64_t at = (int64_t)group * c.s_g + SL * lane;
 #pragma unroll
-    for (int k = 0; k < G::CH; k += 4) {
-      widen_values<kVF32>(ld16(sbase + at + k), sc + k);
-      widen_values<kVF32>(ld16(zbase + at + k), zs + k);
+    for (int k = 0; k < SL; ++k) {
+      sc[k] = sbase[at + k];
+      zp[k] = zbase[at + k];
     }
   };
 
@@ -172,55 +208,81 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
     load_entries(0);
     load_keys(0);
     load_values();
-    load_scales(0);
+    load_scales(group_at(0));
     load_entries(1);
+  }
 
-    // ---- the queries, B operands in units of a power of two for the row's largest ----
-    v8h qop[G::TQ][G::NK];
-    int q_unit;
-    {
-      const int64_t q0 = (int64_t)b * c.q_b + (int64_t)(hk * c.hq_per_kv + qh) * c.q_h +
-                         (int64_t)qi * a.q_n + g * G::CH;
-      float x[G::CH];
+  // ---- the queries to LDS: sixteen threads a row; zeros for rows that are not there ----
+  {
+    const int row = tid >> 4, rr = row0 + min(row, rows - 1), i = fdiv(rr, c.div_hpk);
+    const int d0 = (tid & 15) * G::NA;
+    const int64_t q0 = (int64_t)b * c.q_b +
+                       (int64_t)(hk * c.hq_per_kv + rr - i * c.hq_per_kv) * c.q_h +
+                       (int64_t)i * a.q_n + d0;
+    const bool there = row < rows && i < cnt;
 #pragma unroll
-      for (int s = 0; s < G::CH; s += 8) {
-        if (!a.q_vec) {
+    for (int k = 0; k < G::NA; k += 4) {
+      float x[4];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) x[s + k] = load_elem(c.q, q0 + s + k, c.q_dtype);
-        } else if (c.q_dtype == kEF32) {
-          const float* p = static_cast<const float*>(c.q) + q0 + s;
-          widen_values<kVF32>(ld16(p), x + s);
-          widen_values<kVF32>(ld16(p + 4), x + s + 4);
-        } else {
-          const U32x4 v = ld16(static_cast<const unsigned short*>(c.q) + q0 + s);
-          if (c.q_dtype == kEF16) widen_values<kVF16>(v, x + s);
-          else widen_values<kVBF16>(v, x + s);
+      for (int j = 0; j < 4; ++j) {
+        x[j] = there ? load_elem(c.q, q0 + k + j, c.q_dtype) : 0.f;
+        wild |= (f2u(x[j]) & 0x7FFFFFFFu) >= 0x7F800000u;
+      }
+      *reinterpret_cast<float4*>(&q_s[row][d0 + k]) = make_float4(x[0], x[1], x[2], x[3]);
+    }
+  }
+  __syncthreads();
+
+  if (steps > 0) {
+
+    // Terms of a group: eight channels a product, in the order in which a shift brings
+    // nibbles to bits 6 to 9 and 22 to 25 of a word. A score is S * unit - shift.
+    v8h term[2][G::NK];
+    float unit = 0.f, shift = 0.f;
+    auto make_terms = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int k = 0; k < SL; ++k) {
+        sz_s[w][0][SL * lane + k] = sc[k];
+        sz_s[w][1][SL * lane + k] = zp[k];
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      unsigned big = 0;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f}, v[G::CH];
+#pragma unroll
+      for (int k = 0; k < G::CH; k += 4) {
+        const float4 qx = *reinterpret_cast<const float4*>(&q_s[r16][g * G::CH + k]);
+        const float4 sx = *reinterpret_cast<const float4*>(&sz_s[w][0][g * G::CH + k]);
+        const float4 zx = *reinterpret_cast<const float4*>(&sz_s[w][1][g * G::CH + k]);
+        const float q4[4] = {qx.x, qx.y, qx.z, qx.w}, s4[4] = {sx.x, sx.y, sx.z, sx.w};
+        const float z4[4] = {zx.x, zx.y, zx.z, zx.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[k + j] = q4[j] * s4[j];
+          big = max(big, f2u(v[k + j]) & 0x7FFFFFFFu);
+          sum[j] = __builtin_fmaf(v[k + j], z4[j], sum[j]);
         }
       }
-      unsigned big = 0;
-#pragma unroll
-      for (int k = 0; k < G::CH; ++k) {
-        x[k] = live ? x[k] : 0.f;
-        big = max(big, f2u(x[k]) & 0x7FFFFFFFu);
-      }
       big = over_quarters_umax(big);
-      wild |= big >= 0x7F800000u;
-      q_unit = exponent_of(min(big, 0x7F7FFFFFu)) - 7;
+      shift = over_quarters_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
+      wild |= big >= 0x7F800000u || (f2u(shift) & 0x7FFFFFFFu) >= 0x7F800000u;
+      const int e = exponent_of(min(big, 0x7F7FFFFFu)) - 14;
+      unit = ldexpf(1.f, min(max(e + 18, -120), 120));
 #pragma unroll
       for (int s = 0; s < G::NK; ++s) {
         v4u t[2];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float y0 = ldexpf(x[8 * s + 2 * k], -q_unit);
-          const float y1 = ldexpf(x[8 * s + 2 * k + 1], -q_unit);
+          const float y0 = ldexpf(v[8 * s + k], -e), y1 = ldexpf(v[8 * s + k + 4], -e);
           t[0][k] = pack_f16(y0, y1);
           const v2h h = __builtin_bit_cast(v2h, (unsigned)t[0][k]);
           t[1][k] = pack_f16(y0 - (float)h[0], y1 - (float)h[1]);
         }
-#pragma unroll
-        for (int k = 0; k < G::TQ; ++k) qop[k][s] = __builtin_bit_cast(v8h, t[k]);
+        term[0][s] = __builtin_bit_cast(v8h, t[0]);
+        term[1][s] = __builtin_bit_cast(v8h, t[1]);
       }
-    }
+    };
+    int group = -1;
     const float slope = a.slopes ? a.slopes[hk * c.hq_per_kv + qh] * kLog2eF : 0.f;
     const float inv_cap = 1.f / a.cap, cap_scale = 2.f * kLog2eF / a.cap;
 
@@ -228,20 +290,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
     for (int u = 0; u < steps; ++u) {
       const int t0 = key0_of(u);
       if ((u & 1) == 0) {
-        unsigned big = 0;
-#pragma unroll
-        for (int k = 0; k < G::CH; ++k) {
-          zs[k] *= sc[k];
-          big = max(big, max(f2u(zs[k]) & 0x7FFFFFFFu,
-                             f2u(__builtin_fmaf(15.f, sc[k], -zs[k])) & 0x7FFFFFFFu));
-        }
-        big = over_quarters_umax(big);
-        wild |= big >= 0x7F800000u;
-        unit = __builtin_amdgcn_readfirstlane(exponent_of(min(big, 0x7F7FFFFFu)) - 7);
-#pragma unroll
-        for (int k = 0; k < G::CH; ++k) {
-          sc[k] = ldexpf(sc[k], -unit);
-          zs[k] = ldexpf(zs[k], -unit);
+        const int now = group_at(u);
+        if (now != group) {
+          make_terms();
+          group = now;
+          // (The next group's scales come under this one's products.)
+          int v = u + 2;
+          if (item == 2 && v < steps && group_at(v) == now) v += 2;
+          if (v < steps) load_scales(group_at(v));
         }
       }
       // ---- scores ----
@@ -252,46 +308,43 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
       for (int s = 0; s < G::NK; ++s)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const unsigned lo = kf[h].w[s] & 0x0F0F0F0Fu, hi = (kf[h].w[s] >> 4) & 0x0F0F0F0Fu;
-          v4u t[2];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int ch = 8 * s + 2 * j;
-            const float y0 = __builtin_fmaf((float)((lo >> (8 * j)) & 0xFFu), sc[ch], -zs[ch]);
-            const float y1 =
-                __builtin_fmaf((float)((hi >> (8 * j)) & 0xFFu), sc[ch + 1], -zs[ch + 1]);
-            t[0][j] = pack_f16(y0, y1);
-            const v2h x = __builtin_bit_cast(v2h, (unsigned)t[0][j]);
-            t[1][j] = pack_f16(y0 - (float)x[0], y1 - (float)x[1]);
-          }
-          const v8h k0 = __builtin_bit_cast(v8h, t[0]), k1 = __builtin_bit_cast(v8h, t[1]);
-          sv[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qop[0][s], sv[h], 0, 0, 0);
-          if constexpr (WIDE)
-            sv[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qop[1][s], sv[h], 0, 0, 0);
-          sv[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qop[0][s], sv[h], 0, 0, 0);
+          const unsigned x = kf[h].w[s];
+          const v4u nib = {x << 6 & 0x03C003C0u, x << 2 & 0x03C003C0u, x >> 2 & 0x03C003C0u,
+                           x >> 6 & 0x03C003C0u};
+          const v8h k0 = __builtin_bit_cast(v8h, nib);
+          sv[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, term[1][s], sv[h], 0, 0, 0);
+          sv[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, term[0][s], sv[h], 0, 0, 0);
         }
       if (u + 1 < steps) {
         load_keys(u + 1);
         load_entries(u + 2);
       }
-      // (Of this tile the scales are used: the next one's are loaded under the rest.)
-      const int key_unit = unit;
-      if ((u & 1) && u + 1 < steps) load_scales(u + 1);
 
       v4u p[G::TP];
-      const float f = ldexpf(1.f, min(max(q_unit + key_unit, -120), 120));
+      // Scores in units of log2.
       float x[8];
+      if (a.cap > 0.f) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float y = sv[i / 4][i % 4];
-        if (a.cap > 0.f)
-          x[i] = (WIDE ? soft_cap(y * f, a.cap, inv_cap) : quick_cap(y * f, a.cap, cap_scale)) *
-                 kLog2eF;
-        else
-          x[i] = y * (f * kLog2eF);
-        const int t = t0 + 16 * (i / 4) + 4 * g + i % 4;
-        if (a.slopes) x[i] = __builtin_fmaf(-slope, fabsf((float)(view.pos - t)), x[i]);
-        x[i] = sees(view, t) ? x[i] : -INFINITY;
+        for (int i = 0; i < 8; ++i) {
+          const float y = __builtin_fmaf(sv[i / 4][i % 4], unit, -shift);
+          x[i] = (WIDE ? soft_cap(y, a.cap, inv_cap) : quick_cap(y, a.cap, cap_scale)) * kLog2eF;
+        }
+      } else {
+        const float f2 = unit * kLog2eF, s2 = shift * kLog2eF;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __builtin_fmaf(sv[i / 4][i % 4], f2, -s2);
+      }
+      // (Element i is key 16 (i / 4) + 4 g + i % 4.)
+      if (a.slopes) {
+        const float d0 = (float)(view.pos - t0 - 4 * g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          x[i] = __builtin_fmaf(-slope, fabsf(d0 - (float)(16 * (i / 4) + i % 4)), x[i]);
+      }
+      if (!(t0 + 32 <= v_lo.head || (t0 + 31 <= v_lo.pos && t0 >= v_hi.low))) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          x[i] = sees(view, t0 + 16 * (i / 4) + 4 * g + i % 4) ? x[i] : -INFINITY;
       }
       float top = x[0];
 #pragma unroll
@@ -417,13 +470,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
     weight[k] = __builtin_amdgcn_exp2f(m_s[k][row] - top);
     total = __builtin_fmaf(weight[k], l_s[k][row], total);
   }
-  const int oi = fdiv(min(row, rows - 1), c.div_hpk), oh = min(row, rows - 1) - oi * c.hq_per_kv;
+  const int oR = row0 + min(row, rows - 1), oi = fdiv(oR, c.div_hpk), oh = oR - oi * c.hq_per_kv;
   const bool seen = row < rows && sees_tiles(row_view(a, n, cnt, prefix, oi), list, j0, j1);
   if (__syncthreads_or(bad || (seen && !(total > 0.f)))) {
     const AttendArgs& a = late_attend_args();
     const DecodeArgs& c = a.c;
 #pragma unroll 1
-    for (int r = w; r < rows; r += kWaves) {
+    for (int r = row0 + w; r < row0 + rows; r += kWaves) {
       const RowView v = row_view(a, n, cnt, prefix, r / c.hq_per_kv);
       const RowSums<D> x = plain_row<D, VDT>(a, b, hk, r, n, v, list, j0, j1);
       store_plain_row<D>(a, b, hk, r, split, x, x.m != kLeastF);
@@ -460,19 +513,22 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
   }
 }
 
-template <int D, int VDT>
-hipError_t launch_few(const AttendArgs& a, int batch, hipStream_t st) {
-  const dim3 grid((unsigned)(a.c.num_splits * batch * a.kv_heads));
-  if (a.c.out_dtype == kEF32)
-    hipLaunchKernelGGL((attend_few_kernel<D, VDT, true>), grid, dim3(256), 0, st, a);
+template <int D, int VDT, bool WIDE>
+hipError_t launch_few(AttendArgs a, int batch, hipStream_t st) {
+  a.tiles = (a.c.hq_per_kv * a.queries + 15) / 16;
+  const dim3 grid((unsigned)(a.tiles * a.c.num_splits * batch * a.kv_heads));
+  if (a.c.page_rows % 16 == 0)
+    hipLaunchKernelGGL((attend_few_kernel<D, VDT, WIDE, true>), grid, dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((attend_few_kernel<D, VDT, false>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attend_few_kernel<D, VDT, WIDE, false>), grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
 hipError_t launch_attend_few(const AttendArgs& a, int D, int v_dtype, int batch, hipStream_t st) {
 #define FDI4_FEW(DD, VV) \
-  if (D == DD && v_dtype == VV) return launch_few<DD, VV>(a, batch, st);
+  if (D == DD && v_dtype == VV)                                   \
+    return a.c.out_dtype == kEF32 ? launch_few<DD, VV, true>(a, batch, st) \
+                                  : launch_few<DD, VV, false>(a, batch, st);
   FDI4_FEW(64, kVF32) FDI4_FEW(64, kVF16) FDI4_FEW(64, kVBF16)
   FDI4_FEW(128, kVF32) FDI4_FEW(128, kVF16) FDI4_FEW(128, kVBF16)
   FDI4_FEW(256, kVF32) FDI4_FEW(256, kVF16) FDI4_FEW(256, kVBF16)

@@ -27,7 +27,7 @@ namespace fdi4 {
 
 constexpr int kVectors = 8;              // 16-byte vectors of a thread in a segment
 constexpr int kCandidates = 2048;
-constexpr int kFewRows = 256;            // below: workgroups of 1024 threads
+constexpr int kFewRows = 256;            // up to it: workgroups of 1024 threads
 
 // A logit as a number whose order is the alternatives'.
 __device__ __forceinline__ unsigned order_of(float x) {
@@ -305,7 +305,7 @@ void launch_logprobs(const LogprobArgs& a, hipStream_t st) {
 }
 
 hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t st) {
-  const bool few = a.rows < kFewRows;
+  const bool few = a.rows <= kFewRows;
   if (a.dtype == kEF32) few ? launch_logprobs<kEF32, 1024>(a, st) : launch_logprobs<kEF32, 256>(a, st);
   if (a.dtype == kEF16) few ? launch_logprobs<kEF16, 1024>(a, st) : launch_logprobs<kEF16, 256>(a, st);
   if (a.dtype == kEBF16)
