@@ -37,7 +37,11 @@ struct ChunkGeo {
   static constexpr int WAVES = WIDE || D == 256 ? 4 : 8;
   static constexpr int NT = WAVES * 64;
   static constexpr int M = WAVES * 32;                 // rows of a workgroup
-  static constexpr int KT = WIDE || D == 256 ? 32 : 64;   // keys of a staged tile
+  // Keys of a staged tile. Of float32 outputs 64 keys pay at 128 channels (8 sequences, 512
+  // queries over 2048 tokens, bfloat16 values: 475 us, 547 with 32), while at 64 channels 32
+  // leave registers for a second workgroup on a CU (229 us, 305 with 64); at 256 the buffers
+  // and registers hold 64 with 16-bit values and outputs only.
+  static constexpr int KT = WIDE ? (D == 128 ? 64 : 32) : (D == 256 && VDT == kVF32 ? 32 : 64);
   static constexpr int NBUF = WIDE ? 1 : 2;
   static constexpr int TK = WIDE ? 2 : 1;              // terms of keys and queries
   static constexpr int TV = VDT == kVF32 ? (WIDE ? 3 : 2) : 1;
@@ -58,6 +62,13 @@ struct ChunkGeo {
   static constexpr int NK = D / 16;                    // channel steps of a score
   static_assert(KT * SEG % NT == 0 && SEG <= 16, "threads");
 };
+
+// The largest of three (the instruction quiets operands itself).
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+  return r;
+}
 
 __device__ __forceinline__ float over_halves_max(float x) {
   auto r = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
@@ -318,72 +329,31 @@ void attend_chunk_kernel(AttendArgs a) {
   const float slope = a.slopes ? a.slopes[hk * c.hq_per_kv + qh] : 0.f;
   const float inv_cap = 1.f / a.cap, cap_scale = 2.f * kLog2eF / a.cap;
 
-  auto compute = [&](int s, int buf) __attribute__((always_inline)) {
-    const int t0 = key0_of(s);
-    if (idle || !(t0 < w_hi.head || (t0 <= w_hi.pos && t0 + KT > w_lo.low))) return;
-    const bool whole = t0 + KT <= w_lo.head || (t0 + KT - 1 <= w_lo.pos && t0 >= w_hi.low);
-    const uint8_t* kl = smem + buf * G::kBuf + r32 * G::KS + half * 16;
-    v16f sv[NS];
+  // ---- one step: KT keys, blocks of 32 ----
+  // Scores of block e of a buffer: 16 of a row's 32 (element i is key 8 (i / 4) + 4 half + i % 4).
+  auto scores = [&](int buf, int e, v16f& sv) __attribute__((always_inline)) {
+    const uint8_t* kl = smem + buf * G::kBuf + (32 * e + r32) * G::KS + half * 16;
 #pragma unroll
-    for (int e = 0; e < NS; ++e) {
+    for (int i = 0; i < 16; ++i) sv[i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sv[e][i] = 0.f;
-#pragma unroll
-      for (int k = 0; k < G::NK; ++k) {
-        const v8h k0 = *reinterpret_cast<const v8h*>(kl + 32 * e * G::KS + 32 * k);
-        if constexpr (WIDE) {
-          const v8h k1 = *reinterpret_cast<const v8h*>(kl + (KT + 32 * e) * G::KS + 32 * k);
-          sv[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qop[0][k], sv[e], 0, 0, 0);
-          sv[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qop[G::TK - 1][k], sv[e], 0, 0, 0);
-        }
-        sv[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qop[0][k], sv[e], 0, 0, 0);
+    for (int k = 0; k < G::NK; ++k) {
+      const v8h k0 = *reinterpret_cast<const v8h*>(kl + 32 * k);
+      if constexpr (WIDE) {
+        const v8h k1 = *reinterpret_cast<const v8h*>(kl + KT * G::KS + 32 * k);
+        sv = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qop[0][k], sv, 0, 0, 0);
+        sv = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qop[G::TK - 1][k], sv, 0, 0, 0);
       }
+      sv = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qop[0][k], sv, 0, 0, 0);
     }
-    // Scores in units of log2.
-    const int e2 = min(max(q_unit + __builtin_amdgcn_readfirstlane(unit_s[buf]), -120), 120);
-    const float f = ldexpf(1.f, e2);
-    float x[NS][16];
-    if (a.cap > 0.f) {
+  };
+  auto largest = [&](const v16f& x, float top) __attribute__((always_inline)) {
 #pragma unroll
-      for (int e = 0; e < NS; ++e)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          x[e][i] = (WIDE ? soft_cap(sv[e][i] * f, a.cap, inv_cap)
-                          : quick_cap(sv[e][i] * f, a.cap, cap_scale)) *
-                    kLog2eF;
-    } else {
-      const float f2 = f * kLog2eF;
-#pragma unroll
-      for (int e = 0; e < NS; ++e)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[e][i] = sv[e][i] * f2;
-    }
-    // Element i of block e is key 32 e + 8 (i / 4) + 4 half + i % 4.
-    if (a.slopes) {
-      const float d0 = (float)(view.pos - t0 - 4 * half), s2 = slope * kLog2eF;
-#pragma unroll
-      for (int e = 0; e < NS; ++e)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          x[e][i] = __builtin_fmaf(-s2, fabsf(d0 - (float)(32 * e + 8 * (i / 4) + i % 4)),
-                                   x[e][i]);
-    }
-    if (!whole) {
-#pragma unroll
-      for (int e = 0; e < NS; ++e)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int t = t0 + 4 * half + 32 * e + 8 * (i / 4) + i % 4;
-          x[e][i] = sees(view, t) ? x[e][i] : -INFINITY;
-        }
-    }
-    float top = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < NS; ++e)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, x[e][i]);
-    top = over_halves_max(top) - kUp;
-    if (__builtin_amdgcn_ballot_w64(top > m + kSlack)) {
+    for (int i = 0; i < 16; i += 2) top = max3(top, x[i], x[i + 1]);
+    return top;
+  };
+  // The shift follows the rows' largest score, and the sums it.
+  auto raise = [&](float top) __attribute__((always_inline)) {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0, 0)) {
       const float mn = fmaxf(m, top);
       const float g = __builtin_amdgcn_exp2f(m - mn);
       m = mn;
@@ -393,76 +363,138 @@ void attend_chunk_kernel(AttendArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[t][i] *= g;
     }
+  };
+  // Probabilities of a block, B operands of its two products of 16 keys; their sum.
+  struct Prob {
+    v4u p[2][G::TP];
+  };
+  auto weigh = [&](const v16f& x, float f2, Prob& r) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < NS; ++e)
+    for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[e][i] = __builtin_amdgcn_exp2f(x[e][i] - m);
-    if constexpr (WIDE) {
-#pragma unroll
-      for (int e = 0; e < NS; ++e)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) l += x[e][i];
-    }
-    // Values: 16 keys a product, in the order of the scores' elements.
-    const int l16 = lane & 15;
-    const uint8_t* vl = smem + buf * G::kBuf + G::kKeys + (4 * half + (l16 >> 2)) * G::VS +
-                        ((lane & 16) + 4 * (l16 & 3)) * 2;
-#pragma unroll
-    for (int e = 0; e < NS; ++e)
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        v4u p[G::TP];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float y0 = x[e][8 * ks + 2 * k], y1 = x[e][8 * ks + 2 * k + 1];
-          if constexpr (VDT == kVF16) {
-            p[0][k] = pack_f16(y0, y1);
-            if constexpr (WIDE) {
-              const v2h h = __builtin_bit_cast(v2h, (unsigned)p[0][k]);
-              p[1][k] = pack_f16(y0 - (float)h[0], y1 - (float)h[1]);
-            } else {
-              l = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, (unsigned)p[0][k]),
-                                         v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
-            }
-          } else if constexpr (WIDE) {
-#pragma unroll
-            for (int q = 0; q < 3; ++q) {
-              p[q][k] = pack_high(y0, y1);
-              y0 = less_high(y0);
-              y1 = less_high(y1);
-            }
+      for (int k = 0; k < 4; ++k) {
+        float y0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * ks + 2 * k], f2, -m));
+        float y1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * ks + 2 * k + 1], f2, -m));
+        if constexpr (WIDE) l += y0 + y1;
+        if constexpr (VDT == kVF16) {
+          r.p[ks][0][k] = pack_f16(y0, y1);
+          if constexpr (WIDE) {
+            const v2h h = __builtin_bit_cast(v2h, (unsigned)r.p[ks][0][k]);
+            r.p[ks][1][k] = pack_f16(y0 - (float)h[0], y1 - (float)h[1]);
           } else {
-            p[0][k] = pack_bf16(y0, y1);
-            l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, (unsigned)p[0][k]),
-                                                v2bf{(__bf16)1.f, (__bf16)1.f}, l, false);
+            l = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, (unsigned)r.p[ks][0][k]),
+                                       v2h{(_Float16)1.f, (_Float16)1.f}, l, false);
           }
+        } else if constexpr (WIDE) {
+#pragma unroll
+          for (int q = 0; q < 3; ++q) {
+            r.p[ks][q][k] = pack_high(y0, y1);
+            y0 = less_high(y0);
+            y1 = less_high(y1);
+          }
+        } else {
+          r.p[ks][0][k] = pack_bf16(y0, y1);
+          l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, (unsigned)r.p[ks][0][k]),
+                                              v2bf{(__bf16)1.f, (__bf16)1.f}, l, false);
         }
+      }
+  };
+  const int l16 = lane & 15;
+  const int v_lane = (4 * half + (l16 >> 2)) * G::VS + ((lane & 16) + 4 * (l16 & 3)) * 2;
+  auto values = [&](int buf, int e, const Prob& r) __attribute__((always_inline)) {
+    const uint8_t* vl = smem + buf * G::kBuf + G::kKeys + v_lane;
 #pragma unroll
-        for (int t = 0; t < G::NA; ++t)
+    for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-          for (int q = 0; q < G::TV; ++q) {
-            const uint8_t* at = vl + (q * KT + 32 * e + 16 * ks) * G::VS + 64 * t;
-            typedef __attribute__((address_space(3))) v4s lds_v4s;
-            const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_v4s*)(__attribute__((address_space(3))) void*)at);
-            const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_v4s*)(__attribute__((address_space(3))) void*)(at + 8 * G::VS));
-            typedef short v8s __attribute__((ext_vector_type(8)));
-            const v8s av = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            // (Of the float32 values' terms q and the probabilities' z those with q + z < 3.)
+      for (int t = 0; t < G::NA; ++t)
 #pragma unroll
-            for (int z = 0; z < G::TP; ++z)
-              if (z + q < 3) {
-                if constexpr (VDT == kVF16)
-                  acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                      __builtin_bit_cast(v8h, av), __builtin_bit_cast(v8h, p[z]), acc[t], 0, 0, 0);
-                else
-                  acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                      __builtin_bit_cast(v8bf, av), __builtin_bit_cast(v8bf, p[z]), acc[t], 0, 0,
-                      0);
-              }
+        for (int q = 0; q < G::TV; ++q) {
+          const uint8_t* at = vl + (q * KT + 32 * e + 16 * ks) * G::VS + 64 * t;
+          typedef __attribute__((address_space(3))) v4s lds_v4s;
+          const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_v4s*)(__attribute__((address_space(3))) void*)at);
+          const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_v4s*)(__attribute__((address_space(3))) void*)(at + 8 * G::VS));
+          typedef short v8s __attribute__((ext_vector_type(8)));
+          const v8s av = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          // (Of the float32 values' terms q and the probabilities' z those with q + z < 3.)
+#pragma unroll
+          for (int z = 0; z < G::TP; ++z)
+            if (z + q < 3) {
+              if constexpr (VDT == kVF16)
+                acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                    __builtin_bit_cast(v8h, av), __builtin_bit_cast(v8h, r.p[ks][z]), acc[t], 0, 0,
+                    0);
+              else
+                acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                    __builtin_bit_cast(v8bf, av), __builtin_bit_cast(v8bf, r.p[ks][z]), acc[t], 0,
+                    0, 0);
+            }
+        }
+  };
+  // Whether a step counts for this wave, and needs no mask.
+  auto skipped = [&](int t0) {
+    return idle || !(t0 < w_hi.head || (t0 <= w_hi.pos && t0 + KT > w_lo.low));
+  };
+  auto whole_at = [&](int t0) {
+    return t0 + KT <= w_lo.head || (t0 + KT - 1 <= w_lo.pos && t0 >= w_hi.low);
+  };
+  const bool scored = a.cap > 0.f || a.slopes;
+  auto factor = [&](int buf) {
+    const int e2 = min(max(q_unit + __builtin_amdgcn_readfirstlane(unit_s[buf]), -120), 120);
+    return ldexpf(1.f, e2);
+  };
+
+  // A step. The second block's weights go with the first one's values.
+  auto compute = [&](int s, int buf) __attribute__((always_inline)) {
+    const int t0 = key0_of(s);
+    if (skipped(t0)) return;
+    v16f x[NS];
+#pragma unroll
+    for (int e = 0; e < NS; ++e) scores(buf, e, x[e]);
+    const float f = factor(buf);
+    float f2 = f * kLog2eF;                            // to units of log2
+    if (scored || !whole_at(t0)) {
+      if (a.cap > 0.f) {
+#pragma unroll
+        for (int e = 0; e < NS; ++e)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            x[e][i] = WIDE ? soft_cap(x[e][i] * f, a.cap, inv_cap)
+                           : quick_cap(x[e][i], a.cap, cap_scale * f);
+        f2 = kLog2eF;
+      }
+      if (a.slopes) {
+        const float d0 = (float)(view.pos - t0 - 4 * half), s2 = slope * kLog2eF;
+#pragma unroll
+        for (int e = 0; e < NS; ++e)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            x[e][i] = __builtin_fmaf(-s2, fabsf(d0 - (float)(32 * e + 8 * (i / 4) + i % 4)),
+                                     x[e][i] * f2);
+        f2 = 1.f;
+      }
+      if (!whole_at(t0)) {
+#pragma unroll
+        for (int e = 0; e < NS; ++e)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int t = t0 + 4 * half + 32 * e + 8 * (i / 4) + i % 4;
+            x[e][i] = sees(view, t) ? x[e][i] : -INFINITY;
           }
       }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < NS; ++e) top = largest(x[e], top);
+    raise(over_halves_max(top) * f2 - kUp);
+    Prob p[NS];
+    weigh(x[0], f2, p[0]);
+#pragma unroll
+    for (int e = 0; e < NS; ++e) {
+      if (e + 1 < NS) weigh(x[e + 1], f2, p[e + 1]);
+      values(buf, e, p[e]);
+    }
   };
 
   if (s0 < s1) {
@@ -476,12 +508,18 @@ void attend_chunk_kernel(AttendArgs a) {
       __syncthreads();
       for (int s = s0; s < s1; ++s) {
         const int buf = (s - s0) & 1;
+        // Half the waves stage the next step before they compute, half behind it: the waves
+        // of a SIMD are not in the same part of a step.
+        auto stage = [&]() __attribute__((always_inline)) {
+          if (s + 1 < s1) {
+            write_tile(s + 1, buf ^ 1);
+            load_tile(s + 2);
+            load_entries(s + 3);
+          }
+        };
+        if (w >= G::WAVES / 2) stage();
         compute(s, buf);
-        if (s + 1 < s1) {
-          write_tile(s + 1, buf ^ 1);
-          load_tile(s + 2);
-          load_entries(s + 3);
-        }
+        if (w < G::WAVES / 2) stage();
         __syncthreads();
       }
     } else {
