@@ -15,12 +15,14 @@
 //      fixed order of keys, and the transposing LDS reads (ds_read_b64_tr_b16) bring V^T
 //      in the same order: probabilities never leave their registers.
 //
-// Terms. 16-bit outputs: one float16 term of keys (2^-11 of a product at most; a float16
-// holds 3 bits more than the bfloat16 of a dequantizing cache) and of queries (bfloat16 fits
-// exactly), one term of probabilities in the values' type (their sum takes them rounded),
-// float32 values in two bfloat16 terms. float32 outputs (WIDE): two terms of both, without
-// the product of the second ones, probabilities in two float16 or three bfloat16 terms,
-// float32 values in three.
+// Terms. bfloat16 outputs: one float16 term of keys (2^-11 of a product at most; a float16
+// holds 3 bits more than the bfloat16 of a dequantizing cache) and of queries (16-bit ones
+// fit exactly), one term of probabilities in the values' type (their sum takes them
+// rounded), float32 values in two bfloat16 terms: 0.0021 in the 2-norm in place of the 0.0017
+// of the output's own rounding. float16 values: two terms of keys (with one 5.1e-4, with two
+// 2.3e-4, of which 2.1e-4 are the output's). WIDE, for float32 outputs, and for float16 ones
+// of other values: two terms of both, without the product of the second ones, probabilities
+// in two float16 or three bfloat16 terms, float32 values in three.
 //
 // A workgroup that ends with a NaN, or meets a query or a scale that is not finite, takes its
 // rows one by one: a value that a row does not see would otherwise reach it as 0 * inf.
@@ -40,10 +42,11 @@ struct ChunkGeo {
   // Keys of a staged tile. Of float32 outputs 64 keys pay at 128 channels (8 sequences, 512
   // queries over 2048 tokens, bfloat16 values: 475 us, 547 with 32), while at 64 channels 32
   // leave registers for a second workgroup on a CU (229 us, 305 with 64); at 256 the buffers
-  // and registers hold 64 with 16-bit values and outputs only.
-  static constexpr int KT = WIDE ? (D == 128 ? 64 : 32) : (D == 256 && VDT == kVF32 ? 32 : 64);
+  // and registers hold 64 with bfloat16 values and 16-bit outputs only.
+  static constexpr int KT = WIDE ? (D == 128 ? 64 : 32) : (D == 256 && VDT != kVBF16 ? 32 : 64);
   static constexpr int NBUF = WIDE ? 1 : 2;
-  static constexpr int TK = WIDE ? 2 : 1;              // terms of keys and queries
+  static constexpr int TK = WIDE || VDT == kVF16 ? 2 : 1;   // terms of keys
+  static constexpr int TQ = WIDE ? 2 : 1;              // and of queries
   static constexpr int TV = VDT == kVF32 ? (WIDE ? 3 : 2) : 1;
   static constexpr int TP = !WIDE ? 1 : VDT == kVF16 ? 2 : 3;
   static constexpr int VEB = VDT == kVF32 ? 4 : 2;
@@ -133,7 +136,7 @@ void attend_chunk_kernel(AttendArgs a) {
   __syncthreads();
 
   // ---- the queries: B operands, channels 16 s + 8 half .. of the row ----
-  v8h qop[G::TK][G::NK];
+  v8h qop[G::TQ][G::NK];
   int q_unit = 0;
   if (j0 < j1) {
     const int64_t q0 = (int64_t)b * c.q_b + (int64_t)(hk * c.hq_per_kv + qh) * c.q_h +
@@ -178,7 +181,7 @@ void attend_chunk_kernel(AttendArgs a) {
             }
           }
 #pragma unroll
-          for (int k = 0; k < G::TK; ++k) qop[k][s] = __builtin_bit_cast(v8h, t[k]);
+          for (int k = 0; k < G::TQ; ++k) qop[k][s] = __builtin_bit_cast(v8h, t[k]);
         }
       }
     }
@@ -284,7 +287,7 @@ void attend_chunk_kernel(AttendArgs a) {
           const float y1 =
               __builtin_fmaf((float)((hi >> (8 * j)) & 0xFFu), sc[ch + 1], -zs[ch + 1]);
           t[0][j] = pack_f16(y0, y1);
-          if constexpr (WIDE) {
+          if constexpr (G::TK == 2) {
             const v2h h = __builtin_bit_cast(v2h, (unsigned)t[0][j]);
             t[1][j] = pack_f16(y0 - (float)h[0], y1 - (float)h[1]);
           }
@@ -338,11 +341,12 @@ void attend_chunk_kernel(AttendArgs a) {
 #pragma unroll
     for (int k = 0; k < G::NK; ++k) {
       const v8h k0 = *reinterpret_cast<const v8h*>(kl + 32 * k);
-      if constexpr (WIDE) {
+      if constexpr (G::TK == 2) {
         const v8h k1 = *reinterpret_cast<const v8h*>(kl + KT * G::KS + 32 * k);
         sv = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qop[0][k], sv, 0, 0, 0);
-        sv = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qop[G::TK - 1][k], sv, 0, 0, 0);
       }
+      if constexpr (G::TQ == 2)
+        sv = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qop[1][k], sv, 0, 0, 0);
       sv = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qop[0][k], sv, 0, 0, 0);
     }
   };
@@ -609,7 +613,7 @@ hipError_t launch_chunk(AttendArgs a, int batch, hipStream_t st) {
 
 hipError_t launch_attend_chunk(const AttendArgs& a, int D, int v_dtype, int batch,
                                hipStream_t st) {
-  const bool wide = a.c.out_dtype == kEF32;
+  const bool wide = attend_wide(a.c.out_dtype, v_dtype);
 #define FDI4_CHUNK(DD, VV)                                                        \
   if (D == DD && v_dtype == VV)                                                   \
     return wide ? launch_chunk<DD, VV, true>(a, batch, st) : launch_chunk<DD, VV, false>(a, batch, st);

@@ -1194,7 +1194,7 @@ size_t fdi4_attend_workspace_bytes(int batch, int num_q_heads, int queries, int 
       (int64_t)num_q_heads * queries > INT32_MAX)
     return 0;
   const int s = plan_attend(batch, num_q_heads, queries, window, sinks,
-                            out_dtype == FDI4_K_F32, num_splits, cache).splits;
+                            fdi4::attend_wide(out_dtype, cache->v_dtype), num_splits, cache).splits;
   return s > 1 ? decode_ws_bytes(batch, num_q_heads * queries, cache->head_dim, s) : 0;
 }
 
@@ -1244,7 +1244,8 @@ int fdi4_attend_paged(const void* query, int query_dtype, int batch, int num_q_h
   const int d = cache->head_dim, out_rows = num_q_heads * queries;
   if ((int64_t)batch * out_rows > INT32_MAX) return hipErrorInvalidValue;
   const AttendPlan plan = plan_attend(batch, num_q_heads, queries, window, sinks,
-                                      out_dtype == FDI4_K_F32, num_splits, cache);
+                                      fdi4::attend_wide(out_dtype, cache->v_dtype), num_splits,
+                                      cache);
   a.chunk = plan.chunk;
   a.c.num_splits = plan.splits;
   a.c.div_splits = fdi4::make_fast_div(a.c.num_splits);

@@ -191,6 +191,12 @@ struct AttendArgs {
   int tiles;                            // its workgroups for the rows of a kv-head
 };
 
+// Whether the kernels of an attention keep more than 16 bits of a probability: for float32
+// outputs, and for float16 ones of values whose type holds fewer.
+inline bool attend_wide(int out_dtype, int v_dtype) {
+  return out_dtype == kEF32 || (out_dtype == kEF16 && v_dtype != kVF16);
+}
+
 // Norm of heads and position rotation: x [B, H, N, D] of q and k (element strides) to
 // q_out (q's type) and k_out (float32), contiguous.
 struct RotaryArgs {

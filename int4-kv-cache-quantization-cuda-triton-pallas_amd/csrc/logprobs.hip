@@ -12,7 +12,9 @@
 //
 // A workgroup of NT threads takes a row in segments of 8 NT 16-byte vectors, a segment in
 // registers: its maximum, then one exponential a logit. A thread keeps its own m, l and s,
-// and they meet at the end. Bound: memory.
+// and they meet at the end. Bound: memory with 16-bit logits and no cap (2048 rows of 128000
+// bfloat16 logits: 97 us, 5.4 TB/s); with a cap the vector units, which take some 20
+// instructions a logit, two of them a quarter as fast (777 rows of 50021, 20 alternatives: 52 us).
 //
 // Alternatives: a thread also keeps the largest logit that it has met. The K-th largest of 64
 // groups' such maxima is at most the K-th largest logit, so only logits from there on are
@@ -27,7 +29,9 @@ namespace fdi4 {
 
 constexpr int kVectors = 8;              // 16-byte vectors of a thread in a segment
 constexpr int kCandidates = 2048;
-constexpr int kFewRows = 256;            // up to it: workgroups of 1024 threads
+// Up to so many rows (one a CU) workgroups of 1024 threads: 4 rows of 32000 float32 logits with
+// five alternatives 8.7 us, with 256 threads 15.7; 300 rows 20.6 and 20.1.
+constexpr int kFewRows = 256;
 
 // A logit as a number whose order is the alternatives'.
 __device__ __forceinline__ unsigned order_of(float x) {

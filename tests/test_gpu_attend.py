@@ -388,6 +388,25 @@ def test_one_hot_and_huge_logits():
                 assert np.abs(out[0, h, i] - v[0][x.argmax()]).max() <= 1e-5
 
 
+@pytest.mark.parametrize("D,values,N", [(128, "float16", 1), (128, "float16", 200),
+                                        (256, "float16", 150), (64, "bfloat16", 100),
+                                        (128, "float32", 100), (64, "bfloat16", 1)])
+def test_float16_outputs_keep_their_bits(D, values, N):
+    """Two terms of keys, and of probabilities where the values' type is no float16: the
+    2-norm of the error is that of the output's rounding and of one rounding of the
+    probabilities, each at most 2^-11 / sqrt(3) of a uniform error: 4.0e-4 as squares. (One
+    term of keys alone made it 5e-4.)"""
+    c = make_cache(23, 2, 2, D, [900, 700], values)
+    import torch
+    from flash_decode_int4 import ops
+    q, q64 = make_queries(np.random.RandomState(6), 2, 4, N, D, "float16")
+    cnt = [N, N]
+    out = ops.flash_attend_paged(q, *device_args(c), counts=torch.tensor(cnt).int().cuda())
+    want = oracle(c, q64, cnt, query="float16", values="float16")[0]
+    rel = np.linalg.norm(out.double().cpu().numpy() - want) / np.linalg.norm(want)
+    assert rel <= np.sqrt(2 / 3) * 2.0 ** -11, rel
+
+
 def test_streams_devices_and_a_graph():
     import torch
     from flash_decode_int4 import ops
