@@ -9,7 +9,7 @@
 //
 // A row that sees nothing, and the queries i >= c, are zero.
 //
-// Up to 16 rows a kv-head: attend_few.hip; more: attend_chunk.hip.
+// Up to 32 rows a kv-head: attend_few.hip; more: attend_chunk.hip.
 
 #include "attend_common.hpp"
 

@@ -4,7 +4,10 @@
 // A workgroup takes 32 rows a wave, and keys in tiles that the whole workgroup stages into
 // LDS: keys dequantized once for all rows (k = nib*s - zp*s as float16 in units of a power
 // of two for the scale group's largest), values as they are. The next tile is loaded to
-// registers while the present one is computed, two LDS buffers, one barrier a tile.
+// registers while the present one is computed, two LDS buffers, one barrier a tile. Half of
+// the waves stage the next tile before they compute, half behind it, so that the two waves
+// of a SIMD are in different parts of a step (1295 us, 1206 so, for 8 sequences, 8 kv-heads
+// and 32 q-heads of 128 bfloat16 channels, 1024 queries over 8192 tokens; 856 TFLOP/s).
 //
 //   scores: S^T = K Q^T by v_mfma_f32_32x32x16_f16, keys as A from LDS, queries as B in
 //      registers for the whole call (in units of a power of two for the row's largest):
@@ -23,6 +26,10 @@
 // 2.3e-4, of which 2.1e-4 are the output's). WIDE, for float32 outputs, and for float16 ones
 // of other values: two terms of both, without the product of the second ones, probabilities
 // in two float16 or three bfloat16 terms, float32 values in three.
+//
+// What bounds it: at that size the matrix cores are busy for 39 % of the time, the vector
+// units for 59 and LDS for 25 (no bank conflicts): the two mostly work in turns, as the
+// registers of accumulators, queries and scores leave two waves a SIMD (one with 256 channels).
 //
 // A workgroup that ends with a NaN, or meets a query or a scale that is not finite, takes its
 // rows one by one: a value that a row does not see would otherwise reach it as 0 * inf.

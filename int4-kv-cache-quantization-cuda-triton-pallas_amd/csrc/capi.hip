@@ -1153,6 +1153,8 @@ struct AttendPlan {
   int chunk, splits;
 };
 
+// Rows a kv-head up to which the kernel of few rows is taken (4 q-heads a kv-head: 8 queries
+// 54 us there, 75 in the other; 12 queries 102 and 79).
 constexpr int kFewRows = 32;
 
 AttendPlan plan_attend(int batch, int num_q_heads, int queries, int window, int sinks, bool wide,
@@ -1248,6 +1250,9 @@ int fdi4_attend_paged(const void* query, int query_dtype, int batch, int num_q_h
                                       cache);
   a.chunk = plan.chunk;
   a.c.num_splits = plan.splits;
+  // (Workgroups in 32 bits: at most one a row and split.)
+  if ((int64_t)batch * out_rows * plan.splits > INT32_MAX && plan.splits > 1)
+    return hipErrorInvalidValue;
   a.c.div_splits = fdi4::make_fast_div(a.c.num_splits);
   a.c.final_out = a.c.num_splits == 1 ? 1 : 0;
   a.c.out = out;
@@ -1287,7 +1292,7 @@ int fdi4_norm_rotary(const void* q, const void* k, int dtype, int batch, int tok
     return hipErrorInvalidValue;
   // (Positions behind a start, and the grid, in 32 bits.)
   if ((int64_t)batch * tokens > INT32_MAX / 2 ||
-      (int64_t)batch * tokens * (num_q_heads + num_kv_heads) > INT32_MAX)
+      (int64_t)batch * tokens * (num_q_heads + num_kv_heads) > INT32_MAX - 1024)
     return hipErrorInvalidValue;
   fdi4::RotaryArgs a = {};
   a.x[0] = q;
