@@ -199,9 +199,20 @@ __global__ __launch_bounds__(NT, 4) void token_logprobs_kernel(LogprobArgs a) {
     t.s += s2[0] + s2[1];
 
     if constexpr (TOP) {
-      // A NaN among the thread's logits comes before all (its sum is NaN too).
-      const bool nan = lt != lt;
-      const unsigned mine = nan ? 0xFFFFFFFFu : order_of(mx);
+      // A NaN among the thread's logits comes before all. Its sum is NaN then, but so is that
+      // with +infinity alone.
+      unsigned mine = order_of(mx);
+      if (lt != lt) {
+#pragma unroll
+        for (int k = 0; k < kVectors; ++k)
+          if (k < nk) {
+            float x[EV];
+            widen(raw[k], x);
+#pragma unroll
+            for (int j = 0; j < EV; ++j) mine = max(mine, order_of(x[j]));
+          }
+      }
+      const bool nan = mine == 0xFFFFFFFFu;
       largest = max(largest, mine);
       unsigned gm = largest;
       if constexpr (GL >= 2) gm = max(gm, xchg_u32<1>(gm));

@@ -222,3 +222,28 @@ def test_refused():
                         (RuntimeError, (x, tok.cpu()))):
         with pytest.raises(error):
             token_logprobs(*args)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("rows,vocab", [(4, 700), (4, 20011), (300, 9001)])
+@pytest.mark.parametrize("cap", [None, 2.0])
+def test_alternatives_with_infinities(rows, vocab, dtype, cap):
+    """+infinity is the largest logit, behind NaN alone."""
+    import torch
+    from flash_decode_int4.quality import token_logprobs
+    x, tok = make((rows,), vocab, dtype)
+    inf = float("inf")
+    x[0, vocab // 2] = inf
+    x[1, 5::3] = inf
+    x[2, 9] = float("nan")
+    x[2, vocab - 2] = inf
+    x[3, 1::2] = -inf
+    x[3, 8] = inf
+    raw = x.double().cpu().numpy()
+    raw[2, 9] = 2e300                      # above infinity for the order
+    order = np.where(np.isposinf(raw), 1e300, raw)
+    want = np.argsort(-order, axis=1, kind="stable")
+    for top in (1, 2, 33, 64):
+        out = token_logprobs(x, tok, top, logit_cap=cap)
+        assert (out.top_ids.cpu().numpy() == want[:, :top]).all()
+        assert torch.isnan(out.top_logprobs[:3]).all() and torch.isnan(out.logprobs[:4]).all()
