@@ -911,9 +911,11 @@ std::vector<torch::Tensor> token_logprobs(torch::Tensor logits, torch::Tensor to
   int64_t so = lead.size() > 1 ? logits.stride(0) : 0, si = V;
   bool two = true;
   int64_t step = 0;
+  bool any = false;                      // (A stride of 0 is one, too: expanded logits.)
   for (int64_t d = (int64_t)lead.size() - 1; d >= (lead.size() > 1 ? 1 : 0); --d) {
     if (lead[d] == 1) continue;
-    if (step == 0) {
+    if (!any) {
+      any = true;
       si = logits.stride(d);
       step = si;
     } else if (logits.stride(d) != step) {

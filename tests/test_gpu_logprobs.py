@@ -247,3 +247,12 @@ def test_alternatives_with_infinities(rows, vocab, dtype, cap):
         out = token_logprobs(x, tok, top, logit_cap=cap)
         assert (out.top_ids.cpu().numpy() == want[:, :top]).all()
         assert torch.isnan(out.top_logprobs[:3]).all() and torch.isnan(out.logprobs[:4]).all()
+
+
+def test_expanded_rows():
+    from flash_decode_int4.quality import token_logprobs
+    x, _ = make((2, 3, 1), 515, "float32")
+    _, tok = make((2, 3, 4), 515, "float32")
+    for view, ids in ((x.expand(2, 3, 4, 515), tok), (x[:, :1].expand(2, 3, 4, 515), tok),
+                      (x[:, 0].expand(2, 4, 515), tok[:, 0]), (x[0, :1, 0].expand(4, 515), tok[0, 0])):
+        check(token_logprobs(view, ids, 3), view, ids, 3)
