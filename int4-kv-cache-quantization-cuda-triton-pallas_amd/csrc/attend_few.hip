@@ -285,7 +285,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
         term[1][s] = __builtin_bit_cast(v8h, t[1]);
       }
     };
-    int group = -1;
+    int group = -1, held = group_at(0);   // of the terms; of sc and zp
     const float slope = a.slopes ? a.slopes[hk * c.hq_per_kv + qh] * kLog2eF : 0.f;
     const float inv_cap = 1.f / a.cap, cap_scale = 2.f * kLog2eF / a.cap;
 
@@ -297,10 +297,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
         if (now != group) {
           make_terms();
           group = now;
-          // (The next group's scales come under this one's products.)
-          int v = u + 2;
-          if (item == 2 && v < steps && group_at(v) == now) v += 2;
-          if (v < steps) load_scales(group_at(v));
+        }
+        // (The next group's scales come under this one's products: those of the next tile,
+        // or of the one behind it, where the next one is in this group.)
+        int v = u + 2;
+        if (item == 2 && v < steps && group_at(v) == now) v += 2;
+        const int next = v < steps ? group_at(v) : now;
+        if (next != now && next != held) {
+          load_scales(next);
+          held = next;
         }
       }
       // ---- scores ----

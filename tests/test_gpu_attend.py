@@ -195,6 +195,18 @@ def test_chunks_of_several_tiles(query, values, D, N, Hq, H):
     run(c, Hq, N, [N - 1, N], query, values, seed=3)
 
 
+@pytest.mark.parametrize("group,page_rows", [(512, 16), (1024, 16), (1024, 8), (2048, 16),
+                                             (704, 16)])
+@pytest.mark.parametrize("N", [1, 40])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (3000, 70)])
+def test_groups_of_many_tiles(group, page_rows, N, window, sinks):
+    """A wave takes several tiles of a group, and several groups, at whatever tile the
+    window begins."""
+    c = make_cache(17, 1, 1, 64, [6001, 4900], "float32", page_rows=page_rows, group=group)
+    run(c, 1, N, [N, N], window=window, sinks=sinks, num_splits=1)
+    run(c, 1, N, [N, N], window=window, sinks=sinks)
+
+
 def test_many_heads_for_one_and_odd_groups():
     c = make_cache(10, 2, 1, 64, [333, 70], "bfloat16")
     run(c, 71, 1, [1, 1], "bfloat16", "bfloat16")
