@@ -75,10 +75,15 @@ struct LogSums {
   float m, l, s;                         // sum exp(x - m), sum exp(x - m) (x - m)
 };
 
+// How far a maximum lies below another one, as sums are rescaled by it: exp(-200) is zero, and
+// where a row is masked with the type's lowest value the difference times a sum would be
+// infinite, and zero times that NaN.
+__device__ __forceinline__ float below(float m, float top) { return fmaxf(m - top, -200.f); }
+
 __device__ __forceinline__ LogSums join(LogSums a, LogSums b) {
   LogSums r;
   r.m = fmaxf(a.m, b.m);
-  const float da = a.m - r.m, db = b.m - r.m;
+  const float da = below(a.m, r.m), db = below(b.m, r.m);
   const float ea = __builtin_amdgcn_exp2f(da * kLog2eF), eb = __builtin_amdgcn_exp2f(db * kLog2eF);
   r.l = __builtin_fmaf(a.l, ea, b.l * eb);
   r.s = __builtin_fmaf(__builtin_fmaf(a.l, da, a.s), ea, __builtin_fmaf(b.l, db, b.s) * eb);
@@ -172,7 +177,7 @@ __global__ __launch_bounds__(NT, 4) void token_logprobs_kernel(LogprobArgs a) {
       }
     // (Of the logits as they are; a cap rises with them.)
     const float mn = fmaxf(t.m, a.cap > 0.f ? cap_logit(mx, a.cap, cap_scale) : mx);
-    const float dm = t.m - mn, g = __builtin_amdgcn_exp2f(dm * kLog2eF);
+    const float dm = below(t.m, mn), g = __builtin_amdgcn_exp2f(dm * kLog2eF);
     t.s = __builtin_fmaf(t.l, dm, t.s) * g;
     t.l *= g;
     t.m = mn;
