@@ -281,7 +281,7 @@ __global__ __launch_bounds__(NT, 4) void token_logprobs_kernel(LogprobArgs a) {
     if (count_s <= kCandidates) {
       rank_candidates<NT>(list_s, count_s, a.top, sorted_s);
     } else {
-      // The best that is left, `top` times.
+      // The best that is left, `top` times. (The first may be any: NaN at index 0 is ~0.)
       uint64_t last = ~0ull;
 #pragma unroll 1
       for (int i = 0; i < a.top; ++i) {
@@ -294,7 +294,8 @@ __global__ __launch_bounds__(NT, 4) void token_logprobs_kernel(LogprobArgs a) {
 #pragma unroll
           for (int j = 0; j < EV; ++j) {
             const uint64_t key = candidate(x[j], (int)(e0 + j));
-            if (e0 + j >= 0 && e0 + j < a.vocab && key < last) best = max_u64(best, key);
+            if (e0 + j >= 0 && e0 + j < a.vocab && (i == 0 || key < last))
+              best = max_u64(best, key);
           }
         }
         for (int o = 1; o < 64; o *= 2) best = max_u64(best, __shfl_xor(best, o, 64));

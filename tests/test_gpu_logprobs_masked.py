@@ -70,3 +70,24 @@ def test_huge_logits(rows, vocab, dtype):
         out = token_logprobs(x, at, 1)
         assert not out.logprobs.any() and not out.entropy.any()
         assert torch.equal(out.top_ids[:, 0], at) and not out.top_logprobs.any()
+
+
+@pytest.mark.parametrize("rows,vocab", [(3, 700), (3, 5000), (300, 5000), (2, 40000)])
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_nan_at_the_front_of_many_candidates(rows, vocab, dtype):
+    """NaN first, ties to the lowest index, also where a row has more NaN or equal logits
+    than are ranked at once."""
+    import torch
+    from flash_decode_int4.quality import token_logprobs
+    nan = float("nan")
+    tok = torch.zeros(rows, dtype=torch.long, device="cuda")
+    for seen, first in ((slice(None), []), (slice(0, 1), [0]), ([0, 17, vocab - 1], [0, 17, vocab - 1]),
+                        (slice(1, None, 2), list(range(1, vocab, 2)))):
+        x = torch.zeros(rows, vocab, device="cuda", dtype=getattr(torch, dtype))
+        x[:, seen] = nan
+        rest = [i for i in range(200) if i not in set(first[:200])]
+        want = (first + rest)[:64]
+        for top in (1, 5, 64):
+            out = token_logprobs(x, tok, top)
+            assert (out.top_ids.cpu().numpy() == np.array(want[:top])).all()
+            assert torch.isnan(out.top_logprobs).all() and torch.isnan(out.entropy).all()
