@@ -23,9 +23,9 @@
 // fit exactly), one term of probabilities in the values' type (their sum takes them
 // rounded), float32 values in two bfloat16 terms: 0.0021 in the 2-norm in place of the 0.0017
 // of the output's own rounding. float16 values: two terms of keys (with one 5.1e-4, with two
-// 2.3e-4, of which 2.1e-4 are the output's). WIDE, for float32 outputs, and for float16 ones
-// of other values: two terms of both, without the product of the second ones, probabilities
-// in two float16 or three bfloat16 terms, float32 values in three.
+// 2.3e-4, of which 2.1e-4 are the output's). WIDE, for float32 outputs, for float16 ones
+// of other values, and under caps beyond 512: two terms of both, without the product of the
+// second ones, probabilities in two float16 or three bfloat16 terms, float32 values in three.
 //
 // What bounds it: at that size the matrix cores are busy for 39 % of the time, the vector
 // units for 59 and LDS for 25 (no bank conflicts): the two mostly work in turns, as the
@@ -620,7 +620,7 @@ hipError_t launch_chunk(AttendArgs a, int batch, hipStream_t st) {
 
 hipError_t launch_attend_chunk(const AttendArgs& a, int D, int v_dtype, int batch,
                                hipStream_t st) {
-  const bool wide = attend_wide(a.c.out_dtype, v_dtype);
+  const bool wide = attend_wide(a.c.out_dtype, v_dtype, a.cap);
 #define FDI4_CHUNK(DD, VV)                                                        \
   if (D == DD && v_dtype == VV)                                                   \
     return wide ? launch_chunk<DD, VV, true>(a, batch, st) : launch_chunk<DD, VV, false>(a, batch, st);

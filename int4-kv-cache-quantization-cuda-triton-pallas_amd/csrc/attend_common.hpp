@@ -51,7 +51,7 @@ __device__ __forceinline__ int prefix_of(const AttendArgs& a, int b, int n) {
   return a.prefix ? min(max(ld_ro(a.prefix, b), 0), n) : 0;
 }
 
-// cap * tanh(x / cap) in float32: with e = exp(-2|y|), y = x / cap, tanh|y| = (1 - e) / (1 +
+// cap * tanh(x / cap) in float32, to 2^-20 of itself: with e = exp(-2|y|), y = x / cap, tanh|y| = (1 - e) / (1 +
 // e). Its error is that of 1 - e, 2^-24, so below |y| = 0.35 the odd Taylor series takes
 // over (to y^13: its next term is below 2^-28 of the sum).
 __device__ __forceinline__ float soft_cap(float x, float cap, float inv_cap) {
@@ -70,8 +70,9 @@ __device__ __forceinline__ float soft_cap(float x, float cap, float inv_cap) {
   return cap * __builtin_copysignf(t, y);
 }
 
-// The same to 2^-23 of the cap, in five instructions: cap - 2 cap / (1 + exp(2 y)).
-// scale is 2 log2(e) / cap.
+// The same to 2^-22 of the cap, in five instructions: cap - 2 cap / (1 + exp(2 y)). scale is 2
+// log2(e) / cap. That error has the size of the cap, not of the score: 0.1 for a cap of 1e6. So
+// the kernels take it up to a cap of their own (attend_wide, and the token log probabilities').
 __device__ __forceinline__ float quick_cap(float x, float cap, float scale) {
   const float e = __builtin_amdgcn_exp2f(x * scale);
   return __builtin_fmaf(-2.f * cap, __builtin_amdgcn_rcpf(1.f + e), cap);

@@ -535,7 +535,7 @@ hipError_t launch_few(AttendArgs a, int batch, hipStream_t st) {
 hipError_t launch_attend_few(const AttendArgs& a, int D, int v_dtype, int batch, hipStream_t st) {
 #define FDI4_FEW(DD, VV) \
   if (D == DD && v_dtype == VV)                                   \
-    return attend_wide(a.c.out_dtype, v_dtype) ? launch_few<DD, VV, true>(a, batch, st) \
+    return attend_wide(a.c.out_dtype, v_dtype, a.cap) ? launch_few<DD, VV, true>(a, batch, st) \
                                                : launch_few<DD, VV, false>(a, batch, st);
   FDI4_FEW(64, kVF32) FDI4_FEW(64, kVF16) FDI4_FEW(64, kVBF16)
   FDI4_FEW(128, kVF32) FDI4_FEW(128, kVF16) FDI4_FEW(128, kVBF16)

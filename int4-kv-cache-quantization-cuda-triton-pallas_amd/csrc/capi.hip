@@ -1196,7 +1196,8 @@ size_t fdi4_attend_workspace_bytes(int batch, int num_q_heads, int queries, int 
       (int64_t)num_q_heads * queries > INT32_MAX)
     return 0;
   const int s = plan_attend(batch, num_q_heads, queries, window, sinks,
-                            fdi4::attend_wide(out_dtype, cache->v_dtype), num_splits, cache).splits;
+                            fdi4::attend_wide(out_dtype, cache->v_dtype, options->logit_cap),
+                            num_splits, cache).splits;
   return s > 1 ? decode_ws_bytes(batch, num_q_heads * queries, cache->head_dim, s) : 0;
 }
 
@@ -1246,8 +1247,8 @@ int fdi4_attend_paged(const void* query, int query_dtype, int batch, int num_q_h
   const int d = cache->head_dim, out_rows = num_q_heads * queries;
   if ((int64_t)batch * out_rows > INT32_MAX) return hipErrorInvalidValue;
   const AttendPlan plan = plan_attend(batch, num_q_heads, queries, window, sinks,
-                                      fdi4::attend_wide(out_dtype, cache->v_dtype), num_splits,
-                                      cache);
+                                      fdi4::attend_wide(out_dtype, cache->v_dtype, logit_cap),
+                                      num_splits, cache);
   a.chunk = plan.chunk;
   a.c.num_splits = plan.splits;
   // (Workgroups in 32 bits: at most one a row and split.)

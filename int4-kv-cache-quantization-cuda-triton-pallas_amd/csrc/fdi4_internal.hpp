@@ -191,10 +191,15 @@ struct AttendArgs {
   int tiles;                            // its workgroups for the rows of a kv-head
 };
 
-// Whether the kernels of an attention keep more than 16 bits of a probability: for float32
-// outputs, and for float16 ones of values whose type holds fewer.
-inline bool attend_wide(int out_dtype, int v_dtype) {
-  return out_dtype == kEF32 || (out_dtype == kEF16 && v_dtype != kVF16);
+// Whether the kernels of an attention keep more than 16 bits of a probability, and cap scores
+// to 2^-20 of themselves: for float32 outputs, for float16 ones of values whose type holds
+// fewer, and under caps beyond 512. (The others cap to 2^-22 of the cap, 2^-13 at 512, where a
+// probability is rounded by up to 2^-11. Scores capped so in the other kernels too, by a branch,
+// made their chunks slower without any cap: 1256 us in place of 1212 for 8 sequences, 8 kv-heads
+// and 32 q-heads of 128 bfloat16 channels, 1024 queries over 8192 tokens. Under a cap of 50 it
+// takes 1581 us, under one of 600 4862.)
+inline bool attend_wide(int out_dtype, int v_dtype, float cap) {
+  return out_dtype == kEF32 || (out_dtype == kEF16 && v_dtype != kVF16) || cap > 512.f;
 }
 
 // Norm of heads and position rotation: x [B, H, N, D] of q and k (element strides) to
