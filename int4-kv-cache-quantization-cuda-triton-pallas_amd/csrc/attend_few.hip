@@ -268,8 +268,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
       }
       big = over_quarters_umax(big);
       shift = over_quarters_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
-      wild |= big >= 0x7F800000u || (f2u(shift) & 0x7FFFFFFFu) >= 0x7F800000u;
+      // (Also from 2^117 on, where the unit would pass 2^120: row by row.)
+      wild |= big >= (117u + 127u) << 23 || (f2u(shift) & 0x7FFFFFFFu) >= 0x7F800000u;
       const int e = exponent_of(min(big, 0x7F7FFFFFu)) - 14;
+      // (Scores below 2^-100 are as good as 0, and their unit may be larger than it is.)
       unit = ldexpf(1.f, min(max(e + 18, -120), 120));
 #pragma unroll
       for (int s = 0; s < G::NK; ++s) {
