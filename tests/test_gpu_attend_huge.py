@@ -87,3 +87,24 @@ def test_the_sign_of_such_scores_under_a_cap(types):
             tol = attend_test.EPS[types[0]] * np.abs(want) + 400 * 2.0 ** -24 * (
                 p @ np.abs(v[0][:399 + i]))
             assert (np.abs(out[0, h, i] - want) <= tol + 1e-6).all()
+
+
+@pytest.mark.parametrize("types", [("bfloat16", "bfloat16"), ("float32", "float32"),
+                                   ("float32", "bfloat16"), ("bfloat16", "float32")])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_largest_channels_that_do_not_meet(D, types):
+    """Many rows: queries of 2^68 in one channel and keys of 2^71 in another, so that the
+    product of their units passes 2^120 and the scores do not."""
+    import torch
+    c = make_cache(43, 1, 1, D, [500], types[1])
+    rng = np.random.RandomState(D)
+    c["s"] *= np.float32(2.0 ** 43)
+    c["s"][..., 1] = np.array([2.0 ** 68, 2.0 ** 64, 2.0 ** 66, 2.0 ** 63])[None, None]
+    q = rng.randn(1, 4, 40, D) * 2.0 ** 46
+    q[..., 0] = 2.0 ** 68 * np.sign(rng.randn(1, 4, 40))
+    q[..., 1] = 2.0 ** 50 * rng.uniform(0.5, 1.0, size=(1, 4, 40)) * np.sign(rng.randn(1, 4, 40))
+    # Zero-points of one channel, so that a group's best score is that of its best code.
+    c["z"][..., 1] = [5.3, 7.1, 6.2, 8.4]
+    q = torch.from_numpy(q.astype(np.float32))
+    check(c, q, types, least=0.05)
+    check(c, q, types, least=0.05, num_splits=3)
