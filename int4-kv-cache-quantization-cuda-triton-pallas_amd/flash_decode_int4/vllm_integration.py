@@ -565,11 +565,12 @@ class INT4PagedSequenceCache:
         ops._check_window(window, sinks)
         scored = logit_cap is not None or slopes is not None
         ops._checked_cap(logit_cap)
+        num_splits = int(num_splits or 0)
         B = k_new.shape[0]
         if B > self.max_seqs or tuple(k_new.shape) != (B, self.num_kv_heads, self.head_dim):
             raise ValueError("k_new must be [batch <= max_seqs, kv_heads, head_dim]")
         self._check_room(B, 1, "step() would")
-        if window is not None or scored:
+        if window is not None or scored or num_splits:
             import torch
             # (Refused here, what the attention would refuse with the token appended.)
             if query.dim() != 3 or query.shape[0] != B or query.shape[2] != self.head_dim or \
@@ -583,12 +584,14 @@ class INT4PagedSequenceCache:
                     tuple(slopes.shape) != (query.shape[1],) or not slopes.is_contiguous() or
                     slopes.device != query.device):
                 raise ValueError("slopes must be contiguous float32 [heads] on the cache's GPU")
-        self._unsynced_steps += 1
-        if scored:
-            C = load_binding()
+        C = load_binding()
+        if scored or window is not None or num_splits:
+            # The append writes seq_lens + 1 to _lens_next; the attention is over those.
             C.append_paged_advance(k_new, v_new, self.k_stage[:B], self.k_pages, self.v_pages,
                                    self.k_scale[:B], self.k_zp[:B], self.page_table[:B],
                                    self.seq_lens[:B], self.group_rows, self._lens_next[:B])
+            self._unsynced_steps += 1
+        if scored:
             out = ops.flash_decode_paged(
                 query, self.k_pages, self.v_pages, self.k_scale[:B], self.k_zp[:B],
                 self.page_table[:B], self._lens_next[:B], self.group_rows, num_splits,
@@ -598,35 +601,27 @@ class INT4PagedSequenceCache:
             torch.add(self._lens_next[:B], 0, out=self.seq_lens[:B])
             return out
         if window is not None:
-            C = load_binding()
-            C.append_paged_advance(k_new, v_new, self.k_stage[:B], self.k_pages, self.v_pages,
-                                   self.k_scale[:B], self.k_zp[:B], self.page_table[:B],
-                                   self.seq_lens[:B], self.group_rows, self._lens_next[:B])
             return C.decode_window(query, self.k_pages, self.v_pages, self.k_scale[:B],
                                    self.k_zp[:B], self.page_table[:B], self._lens_next[:B],
                                    self.group_rows // self.page_rows, self.max_pages_per_seq,
-                                   int(window), int(sinks), int(num_splits), self.seq_lens[:B])
+                                   int(window), int(sinks), num_splits, self.seq_lens[:B])
         if num_splits:
-            # An explicit split count: the two-launch form (the append writes
-            # seq_lens + 1 to _lens_next, the decode attends over it with the
-            # given splits and copies it back to seq_lens when it ends).
-            C = load_binding()
-            C.append_paged_advance(k_new, v_new, self.k_stage[:B], self.k_pages, self.v_pages,
-                                   self.k_scale[:B], self.k_zp[:B], self.page_table[:B],
-                                   self.seq_lens[:B], self.group_rows, self._lens_next[:B])
+            # An explicit split count: the two-launch form (the decode attends with the
+            # given splits and copies _lens_next back to seq_lens when it ends).
             return C.decode_paged_advance(query, self.k_pages, self.v_pages, self.k_scale[:B],
                                           self.k_zp[:B], self.page_table[:B],
                                           self._lens_next[:B],
                                           self.group_rows // self.page_rows,
-                                          self.max_pages_per_seq, int(num_splits),
+                                          self.max_pages_per_seq, num_splits,
                                           self.seq_lens[:B])
         # One launch (plus the split merge) with one q-head per kv-head when
         # the splits hold whole scale groups, two otherwise (fdi4_decode_step
         # decides).
-        return load_binding().decode_step(query, k_new, v_new, self.k_stage, self.k_pages,
-                                          self.v_pages, self.k_scale, self.k_zp,
-                                          self.page_table, self.seq_lens, self.group_rows,
-                                          self._step_counters, self._lens_next)
+        out = C.decode_step(query, k_new, v_new, self.k_stage, self.k_pages, self.v_pages,
+                            self.k_scale, self.k_zp, self.page_table, self.seq_lens,
+                            self.group_rows, self._step_counters, self._lens_next)
+        self._unsynced_steps += 1
+        return out
 
     def sync_lengths(self) -> None:
         """Refresh the host copy of the lengths from the device (after step())."""
