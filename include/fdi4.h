@@ -477,7 +477,7 @@ int fdi4_decode_tree(const void* query, int query_dtype, int batch, int num_q_he
  *   slopes       float32 [num_q_heads], or NULL: none
  *   window       last tokens that a query sees, 0: all
  *   sinks        first tokens that it sees besides (needs a window)
- *   logit_cap    0: none */
+ *   logit_cap    0: none, or 1e-30 to 1e30 */
 typedef struct fdi4_attend_options {
   const int32_t* counts;
   const int32_t* prefix_lens;
@@ -505,7 +505,7 @@ size_t fdi4_attend_workspace_bytes(int batch, int num_q_heads, int queries, int 
  * Sums are float32; each output element is rounded once. Refused besides what
  * fdi4_decode_paged_ex refuses: scales attached to pages, page_lens, no seq_lens, scale
  * groups that are neither a multiple of 64 rows nor as large as a sequence, more than 2^30
- * rows a sequence, a cap that is negative or not finite. */
+ * rows a sequence, another cap. */
 int fdi4_attend_paged(const void* query, int query_dtype, int batch, int num_q_heads, int queries,
                       int64_t q_batch_stride, int64_t q_head_stride, int64_t q_row_stride,
                       const fdi4_paged_cache* cache, const fdi4_attend_options* options,
@@ -547,7 +547,8 @@ int fdi4_norm_rotary(const void* q, const void* k, int dtype, int batch, int tok
 #define FDI4_MAX_TOP (64)
 
 /* What fdi4_token_logprobs takes from a row: top alternatives (at most FDI4_MAX_TOP and
- * the vocabulary), of the softmax of logit_cap * tanh(x / logit_cap) (0: of x). */
+ * the vocabulary), of the softmax of logit_cap * tanh(x / logit_cap) (1e-30 to 1e30; 0: of
+ * x). */
 typedef struct fdi4_logprob_options {
   int32_t top;
   float logit_cap;

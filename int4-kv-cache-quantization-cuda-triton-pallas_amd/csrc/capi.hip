@@ -1148,6 +1148,9 @@ int fdi4_read_paged(const fdi4_paged_cache* cache, int batch, const int32_t* sta
 
 namespace {
 
+// A cap of scores or logits: 0 for none, or one whose reciprocal and double are usual numbers.
+bool valid_cap(float cap) { return cap == 0.f || (cap >= 1e-30f && cap <= 1e30f); }
+
 // Launch shape of fdi4_attend_paged: the kernel, and splits of a sequence's 64-key tiles.
 struct AttendPlan {
   int chunk, splits;
@@ -1222,7 +1225,7 @@ int fdi4_attend_paged(const void* query, int query_dtype, int batch, int num_q_h
       (sinks > 0 && window == 0) || !aligned(options->counts, 4) ||
       !aligned(options->prefix_lens, 4) || !aligned(options->slopes, 4))
     return hipErrorInvalidValue;
-  if (!(logit_cap >= 0.f) || logit_cap > 3.4028235e38f) return hipErrorInvalidValue;
+  if (!valid_cap(logit_cap)) return hipErrorInvalidValue;
   if (!out || !valid_elem_dtype(out_dtype)) return hipErrorInvalidValue;
   // A tile of 64 keys lies within one scale group. A group larger than a sequence is the
   // one group that the sequence has.
@@ -1342,7 +1345,7 @@ int fdi4_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t in
   const int top = options->top;
   const float logit_cap = options->logit_cap;
   if (!valid_elem_dtype(dtype) || outer < 0 || inner < 0 || vocab < 1 || top < 0 ||
-      top > FDI4_MAX_TOP || top > vocab || !(logit_cap >= 0.f) || logit_cap > 3.4028235e38f)
+      top > FDI4_MAX_TOP || top > vocab || !valid_cap(logit_cap))
     return hipErrorInvalidValue;
   if (outer == 0 || inner == 0) return hipSuccess;
   if (outer > INT32_MAX / inner) return hipErrorInvalidValue;
