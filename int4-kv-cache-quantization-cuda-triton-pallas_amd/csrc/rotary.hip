@@ -25,7 +25,7 @@
 namespace fdi4 {
 
 // Cosine and sine of position t times frequency f.
-__device__ __forceinline__ void turn_of(int t, float f, float& cs, float& sn) {
+__device__ __forceinline__ void turn_of(int64_t t, float f, float& cs, float& sn) {
   const double turns = (double)t * ((double)f * 0.15915494309189535);
   const float part = (float)(turns - rint(turns));
   sincospif(2.f * part, &sn, &cs);
@@ -82,7 +82,8 @@ __global__ __launch_bounds__(256) void norm_rotary_kernel(RotaryArgs a, int chun
   const int d1 = turns && !a.interleaved ? half + 8 * j : 16 * j + 8;
 
   // The token's turns, pair 8 j + k of lane j's k-th.
-  const int t = a.positions[(int64_t)b * a.p_b + (int64_t)i * a.p_t] + (a.p_t ? 0 : i);
+  const int64_t t =
+      (int64_t)a.positions[(int64_t)b * a.p_b + (int64_t)i * a.p_t] + (a.p_t ? 0 : i);
   float cs[8], sn[8];
 #pragma unroll
   for (int k = 0; k < D / 2; k += 64) {
@@ -179,7 +180,8 @@ __global__ __launch_bounds__(256) void norm_rotary_any_kernel(RotaryArgs a) {
   const int side = hh >= a.heads[0], h = side ? hh - a.heads[0] : hh;
   const int64_t x0 = (int64_t)b * a.x_b[side] + (int64_t)h * a.x_h[side] + (int64_t)i * a.x_t[side];
   const int64_t o0 = (((int64_t)b * a.heads[side] + h) * a.tokens + i) * D;
-  const int t = a.positions[(int64_t)b * a.p_b + (int64_t)i * a.p_t] + (a.p_t ? 0 : i);
+  const int64_t t =
+      (int64_t)a.positions[(int64_t)b * a.p_b + (int64_t)i * a.p_t] + (a.p_t ? 0 : i);
   float norm = 1.f;
   if (a.weight[side]) {
     float s = 0.f;
