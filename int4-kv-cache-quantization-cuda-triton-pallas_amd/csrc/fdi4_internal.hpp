@@ -169,6 +169,12 @@ struct RowsArgs {
   int tiles;                            // workgroups for the rows of a kv-head
 };
 
+// A launch's threads along a grid's dimension are counted in 32 bits, and of a larger number
+// the rest is launched, without an error: what a kernel does not loop over is refused.
+inline bool grid_fits(int64_t workgroups, int threads) {
+  return workgroups <= (int64_t)UINT32_MAX / threads;
+}
+
 // Queries of the last tokens of every sequence over the cache that holds them. Row R of
 // a kv-head is (query R / hq_per_kv, q-head R % hq_per_kv of its group); c holds the
 // cache, the queries and the split partials.
@@ -218,6 +224,7 @@ struct RotaryArgs {
   const float* inv_freq;                // [rotary / 2]
   float eps, rotary_scale;
   int vec;                              // rows start on 16-byte boundaries
+  int first;                            // of this launch: its first wave's item
 };
 
 // Log probabilities of given tokens of rows of logits.
@@ -226,6 +233,7 @@ struct LogprobArgs {
   int dtype;                            // EDtype
   int64_t inner, s_outer, s_inner;      // row r: r / inner, r % inner; elements
   int64_t rows;
+  int64_t first;                        // row of this launch's first workgroup
   int vocab, top;
   float cap;                            // 0: none
   const int64_t* tokens;                // [rows]
@@ -325,7 +333,7 @@ hipError_t launch_attend_few(const AttendArgs& a, int D, int v_dtype, int batch,
 hipError_t launch_attend_chunk(const AttendArgs& a, int D, int v_dtype, int batch,
                                hipStream_t st);
 
-hipError_t launch_norm_rotary(const RotaryArgs& a, hipStream_t st);
+hipError_t launch_norm_rotary(RotaryArgs a, hipStream_t st);
 
 hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t st);
 

@@ -23,6 +23,8 @@
 // once, by counting. Rows with more than kCandidates of them (thousands of ties) are read
 // again for each alternative.
 
+#include <algorithm>
+
 #include "attend_common.hpp"
 
 namespace fdi4 {
@@ -114,7 +116,7 @@ __global__ __launch_bounds__(NT, 4) void token_logprobs_kernel(LogprobArgs a) {
   // -infinity in both halves of a word (float32: in the word).
   constexpr unsigned kNone = DT == kEF32 ? 0xFF800000u : DT == kEF16 ? 0xFC00FC00u : 0xFF80FF80u;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int64_t row = blockIdx.x;
+  const int64_t row = a.first + blockIdx.x;
   const int64_t x0 = row / a.inner * a.s_outer + row % a.inner * a.s_inner;
   const char* base = static_cast<const char*>(a.x) + x0 * EB;
   // Element 0 of vector 0 is at -skew: vectors lie on 16-byte boundaries.
@@ -330,13 +332,18 @@ __global__ __launch_bounds__(NT, 4) void token_logprobs_kernel(LogprobArgs a) {
   }
 }
 
+// Rows of a launch; more take another one.
+constexpr int kMostRows = 1 << 22;
+
 template <int DT, int NT>
-void launch_logprobs(const LogprobArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)a.rows);
-  if (a.top)
-    hipLaunchKernelGGL((token_logprobs_kernel<DT, true, NT>), grid, dim3(NT), 0, st, a);
-  else
-    hipLaunchKernelGGL((token_logprobs_kernel<DT, false, NT>), grid, dim3(NT), 0, st, a);
+void launch_logprobs(LogprobArgs a, hipStream_t st) {
+  for (a.first = 0; a.first < a.rows; a.first += kMostRows) {
+    const dim3 grid((unsigned)std::min<int64_t>(a.rows - a.first, kMostRows));
+    if (a.top)
+      hipLaunchKernelGGL((token_logprobs_kernel<DT, true, NT>), grid, dim3(NT), 0, st, a);
+    else
+      hipLaunchKernelGGL((token_logprobs_kernel<DT, false, NT>), grid, dim3(NT), 0, st, a);
+  }
 }
 
 hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t st) {

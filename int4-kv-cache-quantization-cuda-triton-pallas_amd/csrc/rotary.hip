@@ -63,13 +63,16 @@ __device__ __forceinline__ void store8(void* p, int64_t i, const float* x) {
   }
 }
 
+// Waves of a launch; more take another one.
+constexpr int kMostWaves = 1 << 25;
+
 // Item of a wave: (token, group of `chunk` rounds of heads).
 template <int D, int DT>
 __global__ __launch_bounds__(256) void norm_rotary_kernel(RotaryArgs a, int chunks, int rounds) {
   constexpr int LPR = D / 16, RPW = 64 / LPR;      // lanes a head, heads a round
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int j = lane % LPR, r = lane / LPR;
-  const int item = (int)blockIdx.x * 4 + w;
+  const int item = a.first + (int)blockIdx.x * 4 + w;
   const int bt = item / chunks, chunk = item - bt * chunks;
   __shared__ float2 turn_s[4][D / 2];
   if (bt >= a.batch * a.tokens) return;
@@ -173,7 +176,7 @@ __global__ __launch_bounds__(256) void norm_rotary_kernel(RotaryArgs a, int chun
 __global__ __launch_bounds__(256) void norm_rotary_any_kernel(RotaryArgs a) {
   const int lane = threadIdx.x & 63, D = a.head_dim, half = a.rotary / 2;
   const int all = a.heads[0] + a.heads[1];
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t row = a.first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= (int64_t)a.batch * a.tokens * all) return;
   const int64_t bt = row / all;
   const int hh = (int)(row - bt * all), b = (int)(bt / a.tokens), i = (int)(bt % a.tokens);
@@ -215,23 +218,27 @@ __global__ __launch_bounds__(256) void norm_rotary_any_kernel(RotaryArgs a) {
 }
 
 template <int D>
-hipError_t launch_rotary(const RotaryArgs& a, hipStream_t st) {
+hipError_t launch_rotary(RotaryArgs a, hipStream_t st) {
   const int all = a.heads[0] + a.heads[1], total = (all * D + 1023) / 1024;
   const int64_t tokens = (int64_t)a.batch * a.tokens;
   // Rounds of heads a wave: one while that leaves waves for fewer than 16 a SIMD.
   const int rounds = (int)std::min<int64_t>(std::max<int64_t>(tokens * total / 16384, 1), total);
   const int chunks = (total + rounds - 1) / rounds;
-  const dim3 grid((unsigned)((tokens * chunks + 3) / 4));
-  if (a.dtype == kEF32)
-    hipLaunchKernelGGL((norm_rotary_kernel<D, kEF32>), grid, dim3(256), 0, st, a, chunks, rounds);
-  else if (a.dtype == kEF16)
-    hipLaunchKernelGGL((norm_rotary_kernel<D, kEF16>), grid, dim3(256), 0, st, a, chunks, rounds);
-  else
-    hipLaunchKernelGGL((norm_rotary_kernel<D, kEBF16>), grid, dim3(256), 0, st, a, chunks, rounds);
+  for (int64_t i = 0; i < tokens * chunks; i += kMostWaves) {
+    a.first = (int)i;
+    const dim3 grid((unsigned)((std::min<int64_t>(tokens * chunks - i, kMostWaves) + 3) / 4));
+    if (a.dtype == kEF32)
+      hipLaunchKernelGGL((norm_rotary_kernel<D, kEF32>), grid, dim3(256), 0, st, a, chunks, rounds);
+    else if (a.dtype == kEF16)
+      hipLaunchKernelGGL((norm_rotary_kernel<D, kEF16>), grid, dim3(256), 0, st, a, chunks, rounds);
+    else
+      hipLaunchKernelGGL((norm_rotary_kernel<D, kEBF16>), grid, dim3(256), 0, st, a, chunks,
+                         rounds);
+  }
   return hipGetLastError();
 }
 
-hipError_t launch_norm_rotary(const RotaryArgs& a, hipStream_t st) {
+hipError_t launch_norm_rotary(RotaryArgs a, hipStream_t st) {
   // Rows and weights by 16-byte loads, sixteen rotated channels a lane.
   if (a.vec && a.rotary % 16 == 0) {
     if (a.head_dim == 64) return launch_rotary<64>(a, st);
@@ -239,7 +246,11 @@ hipError_t launch_norm_rotary(const RotaryArgs& a, hipStream_t st) {
     return launch_rotary<256>(a, st);
   }
   const int64_t rows = (int64_t)a.batch * a.tokens * (a.heads[0] + a.heads[1]);
-  hipLaunchKernelGGL(norm_rotary_any_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+  for (int64_t i = 0; i < rows; i += kMostWaves) {
+    a.first = (int)i;
+    const dim3 grid((unsigned)((std::min<int64_t>(rows - i, kMostWaves) + 3) / 4));
+    hipLaunchKernelGGL(norm_rotary_any_kernel, grid, dim3(256), 0, st, a);
+  }
   return hipGetLastError();
 }
 
