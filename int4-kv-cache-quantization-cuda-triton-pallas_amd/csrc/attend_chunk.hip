@@ -613,8 +613,10 @@ hipError_t launch_chunk(AttendArgs a, int batch, hipStream_t st) {
   using G = ChunkGeo<D, VDT, WIDE>;
   const int rows = a.c.hq_per_kv * a.queries;
   a.tiles = (rows + G::M - 1) / G::M;
-  const unsigned grid = (unsigned)a.tiles * a.c.num_splits * batch * a.kv_heads;
-  hipLaunchKernelGGL((attend_chunk_kernel<D, VDT, WIDE>), dim3(grid), dim3(G::NT), 0, st, a);
+  const int64_t wgs = (int64_t)a.tiles * a.c.num_splits * batch * a.kv_heads;
+  if (!grid_fits(wgs, G::NT)) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((attend_chunk_kernel<D, VDT, WIDE>), dim3((unsigned)wgs), dim3(G::NT), 0, st,
+                     a);
   return hipGetLastError();
 }
 

@@ -526,7 +526,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
 template <int D, int VDT, bool WIDE>
 hipError_t launch_few(AttendArgs a, int batch, hipStream_t st) {
   a.tiles = (a.c.hq_per_kv * a.queries + 15) / 16;
-  const dim3 grid((unsigned)(a.tiles * a.c.num_splits * batch * a.kv_heads));
+  const int64_t wgs = (int64_t)a.tiles * a.c.num_splits * batch * a.kv_heads;
+  if (!grid_fits(wgs, 256)) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)wgs);
   if (a.c.page_rows % 16 == 0)
     hipLaunchKernelGGL((attend_few_kernel<D, VDT, WIDE, true>), grid, dim3(256), 0, st, a);
   else

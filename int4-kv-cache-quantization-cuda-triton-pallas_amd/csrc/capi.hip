@@ -1254,8 +1254,9 @@ int fdi4_attend_paged(const void* query, int query_dtype, int batch, int num_q_h
                                       num_splits, cache);
   a.chunk = plan.chunk;
   a.c.num_splits = plan.splits;
-  // (Workgroups in 32 bits: at most one a row and split.)
-  if ((int64_t)batch * out_rows * plan.splits > INT32_MAX && plan.splits > 1)
+  // (Rows of partials in 32 bits, and the merge's grid.)
+  if (plan.splits > 1 && ((int64_t)batch * out_rows * plan.splits > INT32_MAX ||
+                          !fdi4::grid_fits(out_rows, 64)))
     return hipErrorInvalidValue;
   a.c.div_splits = fdi4::make_fast_div(a.c.num_splits);
   a.c.final_out = a.c.num_splits == 1 ? 1 : 0;
@@ -1294,7 +1295,7 @@ int fdi4_norm_rotary(const void* q, const void* k, int dtype, int batch, int tok
       !aligned(q_weight, web) || !aligned(k_weight, web) || !aligned(q_out, 16) ||
       !aligned(k_out, 16))
     return hipErrorInvalidValue;
-  // (Positions behind a start, and the grid, in 32 bits.)
+  // (Tokens and heads in 32 bits.)
   if ((int64_t)batch * tokens > INT32_MAX / 2 ||
       (int64_t)batch * tokens * (num_q_heads + num_kv_heads) > INT32_MAX - 1024)
     return hipErrorInvalidValue;
