@@ -666,11 +666,12 @@ hipError_t launch_merge(const float* ws_acc, const double* ws_ml, int batch, int
 }
 
 // Copy rows of `cols` floats into rows of `d_cols` floats, zero-filling the tail.
-__global__ __launch_bounds__(256) void pad_rows_kernel(const float* __restrict__ src, int64_t rows,
+__global__ __launch_bounds__(256) void pad_rows_kernel(int64_t first,
+                                                       const float* __restrict__ src, int64_t rows,
                                                        int cols, int64_t s_stride,
                                                        float* __restrict__ dst, int64_t d_stride,
                                                        int d_cols) {
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t idx = first + (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (idx >= rows * d_cols) return;
   const int64_t r = idx / d_cols;
   const int c = (int)(idx % d_cols);
@@ -681,8 +682,11 @@ hipError_t launch_pad_rows(const float* src, int64_t rows, int cols, int64_t s_s
                            int64_t d_stride, int d_cols, hipStream_t st) {
   const int64_t total = rows * d_cols;
   if (total == 0) return hipSuccess;
-  hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st,
-                     src, rows, cols, s_stride, dst, d_stride, d_cols);
+  for (int64_t i = 0; i < total; i += kMostElements) {
+    const int64_t blocks = (std::min(total - i, kMostElements) + 255) / 256;
+    hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, st, i, src, rows,
+                       cols, s_stride, dst, d_stride, d_cols);
+  }
   return hipGetLastError();
 }
 

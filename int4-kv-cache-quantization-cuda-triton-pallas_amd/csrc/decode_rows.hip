@@ -1186,7 +1186,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_rows_kernel(RowsArgs a)
 hipError_t launch_decode_rows(const RowsArgs& a, int D, int v_dtype, int batch, hipStream_t st) {
   const int64_t wgs = (int64_t)a.tiles * a.c.num_splits * (a.c.num_q_heads / a.c.hq_per_kv) *
                       batch;
-  if (wgs > INT32_MAX) return hipErrorInvalidValue;
+  if (!grid_fits(wgs, kWaves * 64)) return hipErrorInvalidValue;
   const bool wide = a.c.out_dtype == kEF32;
   const bool stream = a.tiles == 1;
 #define FDI4_RW(DD, VV, RR, OO, SS)                                                       \

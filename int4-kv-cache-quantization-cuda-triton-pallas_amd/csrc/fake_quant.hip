@@ -287,9 +287,10 @@ hipError_t launch_fake_quant(const FakeQuantArgs& args, int key_dtype, int round
   const int forced = tuning(FDI4_TUNE_FAKE_QUANT_SPLIT);
   int split = forced > 0 ? forced : (row_bytes >= 128 ? row_bytes / 128 : 1);
   while (split > 1 && (a.head_dim % split || (a.head_dim / split * esz) % 16 ||
-                       nblk * split > INT32_MAX))
+                       !grid_fits(nblk * split, kFqThreads)))
     --split;
   a.nsplit = max(split, 1);
+  if (!grid_fits(nblk * a.nsplit, kFqThreads)) return hipErrorInvalidValue;
   a.cw = a.head_dim / a.nsplit;
   a.vpr = a.cw * esz / 16;
   a.rpp = kFqThreads / a.vpr;

@@ -174,6 +174,8 @@ struct RowsArgs {
 inline bool grid_fits(int64_t workgroups, int threads) {
   return workgroups <= (int64_t)UINT32_MAX / threads;
 }
+// Elements of a launch of a thread an element; more take another launch.
+constexpr int64_t kMostElements = 1ll << 31;
 
 // Queries of the last tokens of every sequence over the cache that holds them. Row R of
 // a kv-head is (query R / hq_per_kv, q-head R % hq_per_kv of its group); c holds the

@@ -985,7 +985,7 @@ hipError_t launch_extend_paged(const ExtendArgs& a, int D, int group, int batch,
   // Groups that max_tokens new ones can touch from any position in a group.
   const int slots = (int)(((int64_t)a.q.max_tokens + 2 * group - 2) / group);
   const int64_t items = (int64_t)std::max(slots, 1) * heads * batch;
-  if (items > INT32_MAX) return hipErrorInvalidValue;
+  if (!grid_fits(items, kQThreads)) return hipErrorInvalidValue;
   dim3 grid((unsigned)items);
 #define FDI4_EX(DD, GG)                                                                  \
   if (D == DD && group == GG) {                                                          \
@@ -1005,7 +1005,7 @@ hipError_t launch_quantize_paged(const QuantPagedArgs& a, int D, int group, int 
   const int ngroups = (max_tokens + group - 1) / group;
   if (ngroups == 0 || batch == 0 || heads == 0) return hipSuccess;
   const int64_t items = (int64_t)ngroups * heads * batch;
-  if (items > INT32_MAX) return hipErrorInvalidValue;
+  if (!grid_fits(items, kQThreads)) return hipErrorInvalidValue;
   dim3 grid((unsigned)items);
 #define FDI4_QP(DD, GG)                                                             \
   if (D == DD && group == GG) {                                                     \
@@ -1026,7 +1026,7 @@ hipError_t launch_prefill_paged(const PrefillArgs& a, int D, int group, int batc
   const int ngroups = max_len > 0 ? (max_len + group - 1) / group : 1;
   if (batch == 0 || heads == 0) return hipSuccess;
   const int64_t items = (int64_t)ngroups * heads * batch;
-  if (items > INT32_MAX) return hipErrorInvalidValue;
+  if (!grid_fits(items, kQThreads)) return hipErrorInvalidValue;
   dim3 grid((unsigned)items);
 #define FDI4_PF(DD, GG)                                                                   \
   if (D == DD && group == GG) {                                                           \
@@ -1062,11 +1062,12 @@ hipError_t launch_append_paged(const AppendArgs& a, int D, int group, int batch,
 // j < ceil(C/2); bytes ceil(C/2) .. out_cols-1 are zero (row padding).
 // ---------------------------------------------------------------------------
 
-__global__ __launch_bounds__(256) void pack_kernel(const uint8_t* __restrict__ q, int64_t rows,
+__global__ __launch_bounds__(256) void pack_kernel(int64_t first,
+                                                   const uint8_t* __restrict__ q, int64_t rows,
                                                    int C, int64_t q_stride,
                                                    uint8_t* __restrict__ out, int64_t o_stride,
                                                    int out_cols) {
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t idx = first + (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t total = rows * out_cols;
   if (idx >= total) return;
   const int64_t r = idx / out_cols;
@@ -1082,9 +1083,11 @@ hipError_t launch_pack(const uint8_t* q, int64_t rows, int C, int64_t q_stride, 
                        int64_t o_stride, int out_cols, hipStream_t st) {
   const int64_t total = rows * out_cols;
   if (total == 0) return hipSuccess;
-  const int64_t blocks = (total + 255) / 256;
-  hipLaunchKernelGGL(pack_kernel, dim3((unsigned)blocks), dim3(256), 0, st, q, rows, C, q_stride,
-                     out, o_stride, out_cols);
+  for (int64_t i = 0; i < total; i += kMostElements) {
+    const int64_t blocks = (std::min(total - i, kMostElements) + 255) / 256;
+    hipLaunchKernelGGL(pack_kernel, dim3((unsigned)blocks), dim3(256), 0, st, i, q, rows, C,
+                       q_stride, out, o_stride, out_cols);
+  }
   return hipGetLastError();
 }
 
@@ -1098,13 +1101,14 @@ hipError_t launch_pack(const uint8_t* q, int64_t rows, int C, int64_t q_stride, 
 // even, the high nibble when odd). One thread per output element.
 // ---------------------------------------------------------------------------
 
-__global__ __launch_bounds__(256) void dequant_kernel(const uint8_t* __restrict__ q, int64_t rows,
+__global__ __launch_bounds__(256) void dequant_kernel(int64_t first,
+                                                      const uint8_t* __restrict__ q, int64_t rows,
                                                       int C, int64_t q_stride, int packed,
                                                       const float* __restrict__ scale,
                                                       const float* __restrict__ zp, int64_t s_rs,
                                                       int64_t s_cs, float* __restrict__ out,
                                                       int64_t o_stride) {
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t idx = first + (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (idx >= rows * C) return;
   const int64_t r = idx / C;
   const int c = (int)(idx - r * C);
@@ -1124,10 +1128,11 @@ hipError_t launch_dequantize(const uint8_t* q, int64_t rows, int C, int64_t q_st
                              float* out, int64_t o_stride, hipStream_t st) {
   const int64_t total = rows * C;
   if (total == 0) return hipSuccess;
-  const int64_t blocks = (total + 255) / 256;
-  if (blocks > INT32_MAX) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(dequant_kernel, dim3((unsigned)blocks), dim3(256), 0, st, q, rows, C,
-                     q_stride, packed, scale, zp, s_rs, s_cs, out, o_stride);
+  for (int64_t i = 0; i < total; i += kMostElements) {
+    const int64_t blocks = (std::min(total - i, kMostElements) + 255) / 256;
+    hipLaunchKernelGGL(dequant_kernel, dim3((unsigned)blocks), dim3(256), 0, st, i, q, rows, C,
+                       q_stride, packed, scale, zp, s_rs, s_cs, out, o_stride);
+  }
   return hipGetLastError();
 }
 

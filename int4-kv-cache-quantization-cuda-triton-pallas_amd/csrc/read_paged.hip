@@ -162,7 +162,7 @@ hipError_t launch_read_paged(const ReadArgs& a, int D, int v_dtype, int batch, i
     slots = (last / G - a.start0 / G) * pieces + last % G / per - a.start0 % G / per + 1;
   }
   const int64_t items = slots * heads * batch;
-  if (items > INT32_MAX) return hipErrorInvalidValue;
+  if (!grid_fits(items, kReadThreads)) return hipErrorInvalidValue;
 #define FDI4_RD(DD, VV, OO)                                                               \
   if (D == DD && v_dtype == VV && a.out_dtype == OO) {                                    \
     hipLaunchKernelGGL((read_paged_kernel<DD, VV, OO>), dim3((unsigned)items),            \

@@ -43,3 +43,19 @@ def test_heads(R, N, Hq, H):
         b = ops.norm_rotary(q[:, :, at:at + 1000], k[:, :, at:at + 1000], start + at, inv, w, w)
         for x, y in zip(a, b):
             assert bool(torch.equal(x[:, :, at:at + 1000], y))
+
+
+def test_packed_and_dequantized_elements():
+    import torch
+    from flash_decode_int4 import ops
+    C, rows = 128, (1 << 26) + 1003                 # 2^33 values, 2^32 bytes of them
+    q = torch.empty(rows, C, dtype=torch.uint8, device="cuda").random_(0, 16)
+    p = ops.pack_int4_device(q)
+    for at in (slice(0, 1000), slice(rows // 2, rows // 2 + 1000), slice(rows - 2000, rows)):
+        assert bool(torch.equal(p[at], q[at, 0::2] | q[at, 1::2] << 4))
+    del q
+    s, z = (torch.rand(C, device="cuda") for _ in range(2))
+    x = ops.dequantize_int4(p, s, z, packed=True)
+    assert tuple(x.shape) == (rows, C)
+    for at in (slice(0, 1000), slice(rows // 2, rows // 2 + 1000), slice(rows - 2000, rows)):
+        assert bool(torch.equal(x[at], ops.dequantize_int4(p[at].contiguous(), s, z, packed=True)))

@@ -13,3 +13,14 @@ from test_rows_host_contract import INVALID, cache
     dict(B=1, Hq=64, N=1100000, splits=2)], ids=str)     # 70 million rows to merge
 def test_attend(kw):
     assert attend(cache(num_kv_heads=64), wsb=1 << 50, **kw) == INVALID
+
+
+def test_reads():
+    import ctypes
+
+    from flash_decode_int4 import capi
+    from test_rows_host_contract import P
+    c = cache(num_kv_heads=512)
+    assert capi.load().fdi4_read_paged(
+        ctypes.byref(c), 65535, None, 0, 1, P, 512 * 128, 128, 128, P, 512 * 128, 128, 128,
+        capi.K_F32, None) == INVALID
