@@ -1,5 +1,17 @@
-// Pieces shared by the kernels that attend with queries of cached tokens: what a row
-// sees, its logits, and the computation of a row by itself.
+// Attention of the last tokens of every sequence over the paged INT4 cache that holds
+// them (gfx950). Query i of sequence b, with n cached tokens and c queries, is at
+// position p = n - c + i and sees the tokens
+//
+//   t < prefix,  t <= p with t < sinks or t > p - window;
+//
+//   x_t = cap * tanh(q . k_t / cap) - slope * |p - t|,  k_t = nib*scale - zp*scale,
+//   out = sum_t p_t v_t / sum_t p_t,  p_t = exp(x_t - max).
+//
+// A row that sees nothing, and the queries i >= c, are zero.
+//
+// Here: what the two kernels share (up to 32 rows a kv-head: attend_few.hip; more:
+// attend_chunk.hip), namely what a row sees, its logits, and the computation of a row by
+// itself.
 #pragma once
 
 #include "decode_common.hpp"

@@ -1158,13 +1158,13 @@ struct AttendPlan {
 
 // Rows a kv-head up to which the kernel of few rows is taken (4 q-heads a kv-head: 8 queries
 // 54 us there, 75 in the other; 12 queries 102 and 79).
-constexpr int kFewRows = 32;
+constexpr int kFewRowsOfHead = 32;
 
 AttendPlan plan_attend(int batch, int num_q_heads, int queries, int window, int sinks, bool wide,
                        int num_splits, const fdi4_paged_cache* cache) {
   AttendPlan p;
   const int64_t rows = (int64_t)(num_q_heads / cache->num_kv_heads) * queries;
-  p.chunk = rows > kFewRows;
+  p.chunk = rows > kFewRowsOfHead;
   // The most 64-key tiles a row tile can see (a prefix apart).
   const int64_t cap = (int64_t)cache->max_pages * cache->page_rows;
   int64_t keys = cap;
@@ -1266,7 +1266,8 @@ int fdi4_attend_paged(const void* query, int query_dtype, int batch, int num_q_h
     rc = carve_partials(workspace, workspace_bytes, batch, out_rows, d, &a.c);
     if (rc != hipSuccess) return rc;
   }
-  const hipError_t e = fdi4::launch_attend(a, d, cache->v_dtype, batch, stream);
+  const hipError_t e = (a.chunk ? fdi4::launch_attend_chunk : fdi4::launch_attend_few)(
+      a, d, cache->v_dtype, batch, stream);
   if (e != hipSuccess || a.c.num_splits == 1) return e;
   return fdi4::launch_merge(a.c.ws_acc, a.c.ws_ml, batch, out_rows, d, a.c.num_splits, out,
                             out_dtype, (int64_t)out_rows * d, d, stream);

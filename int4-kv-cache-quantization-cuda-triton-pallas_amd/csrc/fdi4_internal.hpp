@@ -328,8 +328,6 @@ hipError_t launch_merge(const float* ws_acc, const double* ws_ml, int batch, int
 
 hipError_t launch_decode_rows(const RowsArgs& a, int D, int v_dtype, int batch, hipStream_t st);
 
-hipError_t launch_attend(const AttendArgs& a, int D, int v_dtype, int batch, hipStream_t st);
-
 hipError_t launch_attend_few(const AttendArgs& a, int D, int v_dtype, int batch, hipStream_t st);
 
 hipError_t launch_attend_chunk(const AttendArgs& a, int D, int v_dtype, int batch,

@@ -33,7 +33,7 @@ constexpr int kVectors = 8;              // 16-byte vectors of a thread in a seg
 constexpr int kCandidates = 2048;
 // Up to so many rows (one a CU) workgroups of 1024 threads: 4 rows of 32000 float32 logits with
 // five alternatives 8.7 us, with 256 threads 15.7; 300 rows 20.6 and 20.1.
-constexpr int kFewRows = 256;
+constexpr int kFewLogitRows = 256;
 
 // A logit as a number whose order is the alternatives'.
 __device__ __forceinline__ unsigned order_of(float x) {
@@ -347,7 +347,7 @@ void launch_logprobs(LogprobArgs a, hipStream_t st) {
 }
 
 hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t st) {
-  const bool few = a.rows <= kFewRows;
+  const bool few = a.rows <= kFewLogitRows;
   if (a.dtype == kEF32) few ? launch_logprobs<kEF32, 1024>(a, st) : launch_logprobs<kEF32, 256>(a, st);
   if (a.dtype == kEF16) few ? launch_logprobs<kEF16, 1024>(a, st) : launch_logprobs<kEF16, 256>(a, st);
   if (a.dtype == kEBF16)

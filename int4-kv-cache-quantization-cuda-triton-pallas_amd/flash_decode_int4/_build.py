@@ -26,9 +26,8 @@ INCLUDE = os.path.join(os.path.dirname(ROOT_DIR), "include")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 HIP_SOURCES = ("quantize.hip", "decode.hip", "decode_gqa.hip", "decode_mfma.hip",
-               "decode_rows.hip", "read_paged.hip", "fake_quant.hip", "attend.hip",
-               "attend_few.hip", "attend_chunk.hip", "rotary.hip", "logprobs.hip",
-               "capi.hip")
+               "decode_rows.hip", "read_paged.hip", "fake_quant.hip", "attend_few.hip",
+               "attend_chunk.hip", "rotary.hip", "logprobs.hip", "capi.hip")
 LIB_PATH = os.path.join(PKG_DIR, "libfdi4.so")
 EXT_PATH = os.path.join(PKG_DIR, "_C.so")
 
