@@ -22,8 +22,13 @@
 // 16 sequences of 16384 tokens, 8 kv-heads, 32 q-heads, 128 bfloat16 channels, capped: 113 us,
 // 6.1 TB/s, 109 in the kernel and the rest in the merge; the vector units are busy for 39 %.
 //
-// Probabilities are in as many terms as in the kernel of many rows (attend_chunk.hip). PAGED:
-// pages hold whole runs of 16 rows, so that a run's address is the same for all lanes.
+// Probabilities: two terms of the values' type for 16-bit outputs (16 bits of them with bfloat16
+// and float32 values, the latter in two bfloat16 terms themselves; 22 with float16 ones). One
+// was 0 to 4 % faster (149.9 us in place of 151.8 for 24 sequences of 6000 float16 tokens, 16
+// heads of 128) and rounded a quarter of the outputs to a neighbour, where two do so with 0.5
+// %. WIDE, for what attend_chunk.hip says: two float16 or three bfloat16 terms, float32 values
+// in three. PAGED: pages hold whole runs of 16 rows, so that a run's address is the same for
+// all lanes.
 
 #include "attend_common.hpp"
 
@@ -34,7 +39,7 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 template <int D, int VDT, bool WIDE>
 struct FewGeo {
   static constexpr int TV = VDT == kVF32 ? (WIDE ? 3 : 2) : 1;
-  static constexpr int TP = VDT == kVF16 ? (WIDE ? 2 : 1) : (WIDE ? 3 : 1);
+  static constexpr int TP = VDT == kVF16 || !WIDE ? 2 : 3;
   static constexpr int VEB = VDT == kVF32 ? 4 : 2;
   static constexpr int NK = D / 32;                    // products of a score; packed words a lane
   static constexpr int CH = D / 4;                     // key channels of a lane
@@ -374,22 +379,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
       for (int k = 0; k < 4; ++k) {
         float y0 = __builtin_amdgcn_exp2f(x[2 * k] - m);
         float y1 = __builtin_amdgcn_exp2f(x[2 * k + 1] - m);
-        if constexpr (WIDE) l += y0 + y1;
+        l += y0 + y1;
         if constexpr (VDT == kVF16) {
           p[0][k] = pack_f16(y0, y1);
           const v2h h = __builtin_bit_cast(v2h, (unsigned)p[0][k]);
-          if constexpr (WIDE) p[1][k] = pack_f16(y0 - (float)h[0], y1 - (float)h[1]);
-          else l += (float)h[0] + (float)h[1];
-        } else if constexpr (WIDE) {
+          p[1][k] = pack_f16(y0 - (float)h[0], y1 - (float)h[1]);
+        } else {
 #pragma unroll
-          for (int q = 0; q < 3; ++q) {
+          for (int q = 0; q + 1 < G::TP; ++q) {
             p[q][k] = pack_high(y0, y1);
             y0 = less_high(y0);
             y1 = less_high(y1);
           }
-        } else {
-          p[0][k] = pack_bf16(y0, y1);
-          l += u2f(p[0][k] << 16) + u2f(p[0][k] & 0xFFFF0000u);
+          p[G::TP - 1][k] = WIDE ? pack_high(y0, y1) : pack_bf16(y0, y1);
         }
       }
       // Values behind the sequence's end may be anything: zeros.
