@@ -502,10 +502,21 @@ size_t fdi4_attend_workspace_bytes(int batch, int num_q_heads, int queries, int 
  *   less slopes[h] * |p - t|,
  * unscaled otherwise. out is contiguous [batch, num_q_heads, queries, head_dim]; queries
  * i >= c and those that see nothing give zeros, rows whose logits are all -infinity NaN.
- * Sums are float32; each output element is rounded once. Refused besides what
- * fdi4_decode_paged_ex refuses: scales attached to pages, page_lens, no seq_lens, scale
- * groups that are neither a multiple of 64 rows nor as large as a sequence, more than 2^30
- * rows a sequence, another cap. */
+ * Sums are float32; each output element is rounded once; factors hold fewer bits. Up to 32
+ * rows (queries times q-heads) a kv-head: products of queries and scales 22 bits of the largest
+ * of a row and scale group, probabilities 24 for float32 outputs (22 with float16 values), 16
+ * for 16-bit ones (22 with float16 values; float32 values 16). More rows: for float32
+ * outputs keys and queries 22 bits, probabilities as before; for 16-bit outputs keys and
+ * queries 11 bits (16-bit queries as they are, keys 22 with float16 values), probabilities the
+ * 8 or 11 of the values' type (8 with float32 values, which keep 16): errors of 0.0021 of
+ * bfloat16 outputs in the 2-norm and 2.5e-4 of float16 ones, whose rounding is 0.0017 and
+ * 2.1e-4. float16 outputs of other values, and outputs capped beyond 512, are computed as
+ * float32 ones. Caps are exact to 2^-20 of a score, up to 512 for 16-bit outputs to 2^-22 of
+ * the cap. Rows near a query, scale or value that is not finite are taken one by one, 25 to
+ * 130 times as slowly. Refused besides what fdi4_decode_paged_ex refuses: scales attached to
+ * pages, page_lens, no seq_lens, scale groups that are neither a multiple of 64 rows nor as
+ * large as a sequence, more than 2^30 rows a sequence, another cap, more than 2^32 - 1
+ * threads. */
 int fdi4_attend_paged(const void* query, int query_dtype, int batch, int num_q_heads, int queries,
                       int64_t q_batch_stride, int64_t q_head_stride, int64_t q_row_stride,
                       const fdi4_paged_cache* cache, const fdi4_attend_options* options,
@@ -561,7 +572,9 @@ typedef struct fdi4_logprob_options {
  * entropy[r] = -sum p log p; with top > 0 top_ids[r, :] are the indices of the largest logits
  * (as they are before the cap), ties to the lowest index, NaN first, and top_logprobs[r, :]
  * their log p. Logits of -infinity have probability 0, also under a cap; rows with a NaN or
- * +infinity, and rows of -infinity, give NaN. All sums in float32. */
+ * +infinity, and rows of -infinity, give NaN. All sums in float32; caps up to 64 to 2^-22 of
+ * the cap, larger ones to 2^-20 of the logit. A row with more than 2048 logits as large as
+ * its last alternative is read again for each alternative. */
 int fdi4_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner,
                         int64_t outer_stride, int64_t inner_stride, int vocab,
                         const int64_t* tokens, const fdi4_logprob_options* options,

@@ -6,8 +6,9 @@
 // of two for the scale group's largest), values as they are. The next tile is loaded to
 // registers while the present one is computed, two LDS buffers, one barrier a tile. Half of
 // the waves stage the next tile before they compute, half behind it, so that the two waves
-// of a SIMD are in different parts of a step (1295 us, 1206 so, for 8 sequences, 8 kv-heads
-// and 32 q-heads of 128 bfloat16 channels, 1024 queries over 8192 tokens; 856 TFLOP/s).
+// of a SIMD are in different parts of a step (1295 us, 1203 to 1266 so on several cards, for 8
+// sequences, 8 kv-heads and 32 q-heads of 128 bfloat16 channels, 1024 queries over 8192 tokens;
+// 813 to 856 TFLOP/s).
 //
 //   scores: S^T = K Q^T by v_mfma_f32_32x32x16_f16, keys as A from LDS, queries as B in
 //      registers for the whole call (in units of a power of two for the row's largest):
@@ -23,16 +24,20 @@
 // fit exactly), one term of probabilities in the values' type (their sum takes them
 // rounded), float32 values in two bfloat16 terms: 0.0021 in the 2-norm in place of the 0.0017
 // of the output's own rounding. float16 values: two terms of keys (with one 5.1e-4, with two
-// 2.3e-4, of which 2.1e-4 are the output's). WIDE, for float32 outputs, for float16 ones
+// 2.3e-4, of which 2.1e-4 are the output's). Two terms of probabilities would leave the output's
+// rounding alone and take 1575 us in place of 1236 at the size above, 1953 in place of 1641 with
+// float16 values. WIDE, for float32 outputs, for float16 ones
 // of other values, and under caps beyond 512: two terms of both, without the product of the
 // second ones, probabilities in two float16 or three bfloat16 terms, float32 values in three.
 //
 // What bounds it: at that size the matrix cores are busy for 39 % of the time, the vector
-// units for 59 and LDS for 25 (no bank conflicts): the two mostly work in turns, as the
-// registers of accumulators, queries and scores leave two waves a SIMD (one with 256 channels).
+// units for 59 and LDS for 25 (no bank conflicts): the two mostly work in turns. A step has all
+// its scores before its weights, and the registers of accumulators, queries and scores leave two
+// waves a SIMD (one with 256 channels).
 //
 // A workgroup that ends with a NaN, or meets a query or a scale that is not finite, takes its
-// rows one by one: a value that a row does not see would otherwise reach it as 0 * inf.
+// rows one by one: a value that a row does not see would otherwise reach it as 0 * inf. (One NaN
+// among the values above: 151 ms.)
 
 #include "attend_common.hpp"
 

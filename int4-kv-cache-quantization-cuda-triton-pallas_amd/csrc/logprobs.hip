@@ -20,8 +20,10 @@
 // groups' such maxima is at most the K-th largest logit, so only logits from there on are
 // candidates; every wave finds that bound by itself (18 of its bits, with ballots), and few
 // vectors hold one. The candidates (some K a segment, fewer as the bound rises) are ranked
-// once, by counting. Rows with more than kCandidates of them (thousands of ties) are read
-// again for each alternative.
+// once, by counting. Rows with more than kCandidates of them are read again for each
+// alternative: those with thousands of ties, and those masked with a finite value where fewer
+// than K of the groups hold another logit (4 rows of 32000 float32 logits, all but five at the
+// lowest number: 13 us for 5 alternatives, 138 for 20, where usual rows take 11 and 10).
 
 #include <algorithm>
 

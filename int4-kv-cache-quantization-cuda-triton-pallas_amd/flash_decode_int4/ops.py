@@ -361,8 +361,9 @@ def flash_decode_paged(query, k_pages, v_pages, k_scale, k_zp, page_table, seq_l
     D]; k_scale/k_zp [B, Hkv, G, D]; page_table int32 [B, max_pages] (or None
     for identity); seq_lens int32 [B] (or None with page_lens). q-head h reads
     kv-head h // (Hq // Hkv). Returns [B, Hq, D] on the GPU in the query's
-    dtype: float32 arithmetic, 16-bit queries widened exactly, one rounding
-    (to nearest even) of each output element.
+    dtype: float32 arithmetic (but see ``window`` and ``logit_cap``), 16-bit
+    queries widened exactly, one rounding (to nearest even) of each output
+    element.
 
     ``window``: attend only the last ``window`` tokens of each sequence (the
     query is that of its last token) and its first ``sinks``; the pages between
@@ -371,16 +372,16 @@ def flash_decode_paged(query, k_pages, v_pages, k_scale, k_zp, page_table, seq_l
     narrower: for float32 outputs products of queries and scales keep 29 bits of the
     largest of a row and scale group, probabilities 24 (22 with float16 values); for
     16-bit outputs the products 21 bits each, probabilities 22 (16 with bfloat16
-    values, 24 with float32 ones). Without it logits are float64 and probabilities
-    keep 24 bits.
+    values, 24 with float32 ones). Without it, a cap and slopes logits are float64 and
+    probabilities keep 24 bits.
 
     Values that are not finite come out as the formula has them; where a query sees
     one, the sequence's rows of that kv-head are computed one by one, which may take
     a hundred times as long.
 
     ``logit_cap``, ``slopes``: capped scores and a distance bias, as
-    ``flash_attend_paged`` with one query has them (it is called; seq_lens and the
-    grouped scales are needed).
+    ``flash_attend_paged`` with one query has them, and to as many bits (it is called;
+    seq_lens and the grouped scales are needed).
     """
     _check_window(window, sinks)
     if logit_cap is not None or slopes is not None:
@@ -486,11 +487,27 @@ def flash_attend_paged(query, k_pages, v_pages, k_scale, k_zp, page_table, seq_l
     the query), with ``logit_cap`` ``logit_cap * tanh(q.k / logit_cap)``, and with
     ``slopes`` (float32 [Hq]) less ``slopes[h] * |p - t|`` for the token at t.
 
-    Returns [B, Hq, N, D] in the query's dtype: float32 sums, one rounding of each output
-    element. Queries past a sequence's count, and those that see nothing, give zeros;
-    padding queries may hold anything. Values that are not finite come out as the formula has
-    them; the rows near one are then computed one by one, much more slowly. Nothing goes
-    through the host, so the call can be captured into a graph.
+    Returns [B, Hq, N, D] in the query's dtype. Queries past a sequence's count, and those
+    that see nothing, give zeros; padding queries may hold anything. Nothing goes through the
+    host, so the call can be captured into a graph.
+
+    Sums are float32 and each output element is rounded once; factors hold fewer bits. With
+    up to 32 rows (queries times q-heads) a kv-head, products of queries and scales hold 22
+    of the largest of a row and scale group, and probabilities 24 for float32 outputs (22 with
+    float16 values), for 16-bit ones 16 (22 with float16 values; float32 values 16 there).
+    With more rows float32 outputs have keys and queries of 22 bits and the same
+    probabilities; 16-bit outputs have keys of 11 bits (22 with float16 values) and
+    probabilities of the 8 or 11 bits of the values' type (8 with float32 values, which keep
+    16): errors of 0.0021 of bfloat16 outputs in the 2-norm and 2.5e-4 of float16 ones, whose
+    own rounding is 0.0017 and 2.1e-4 of it. float16 outputs of other values are computed as
+    float32 ones are, and so are capped ones beyond a cap of 512. Caps are exact to 2^-20
+    of a score, up to 512 for 16-bit outputs to 2^-22 of the cap.
+
+    Values that are not finite come out as the formula has them. Where a query, a scale or a
+    value that is seen is not finite, the rows near it (16, or up to 256 with more than 32 a
+    kv-head) are computed one by one: 25 to 130 times as long, 3 ms for one token of 16
+    sequences of 16384 and 150 ms for a chunk of 1024 over 8 of 8192. So are rows whose
+    queries times scales reach 2^117.
     """
     if query.dim() != 4:
         raise ValueError(f"query must be [batch, heads, queries, head_dim], got "

@@ -145,12 +145,15 @@ def token_logprobs(logits, tokens, top: int = 0, logit_cap: Optional[float] = No
         tokens: integers [...], the token of every row; a negative one (a place without
            a token) gives 0, one past the vocabulary NaN.
         top: alternatives per row, 0 to 64.
-        logit_cap: softmax of ``logit_cap * tanh(logits / logit_cap)``.
+        logit_cap: softmax of ``logit_cap * tanh(logits / logit_cap)``, a cap to 64 to
+           2^-22 of it, a larger one to 2^-20 of the logit.
     Returns:
         TokenLogprobs of logprobs float32 [...], entropy float32 [...] (in nats),
         top_logprobs float32 [..., top] and top_ids int64 [..., top]: the largest logits,
         ties to the lowest index. Logits of -infinity have probability zero, also under a
-        cap; a row with a NaN or +infinity, or of -infinity alone, gives NaN (its alternatives put NaN first).
+        cap; a row with a NaN or +infinity, or of -infinity alone, gives NaN (its alternatives
+        put NaN first). More than 2048 logits as large as the last alternative, as where fewer
+        than ``top`` are not masked, make a row be read ``top`` times.
     """
     import torch
     from .ops import _checked_cap

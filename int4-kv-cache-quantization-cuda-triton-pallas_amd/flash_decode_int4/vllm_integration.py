@@ -634,10 +634,11 @@ class INT4PagedSequenceCache:
                slopes=None):
         """Fused INT4 attention of query [B, Hq, D] (float32, float16 or bfloat16;
         Hq a multiple of kv_heads) over sequences 0..B-1; returns [B, Hq, D] in
-        the query's dtype (float32 arithmetic, one rounding at the end). With a
-        window only over each sequence's last ``window`` and first ``sinks``
-        tokens (ops.flash_decode_paged says to how many bits). logit_cap, slopes: scores
-        capped and biased as in attend()."""
+        the query's dtype (float32 arithmetic, one rounding at the end; with a window, a
+        cap or slopes factors of fewer bits, as ops.flash_decode_paged and
+        ops.flash_attend_paged say). With a window only over each sequence's last
+        ``window`` and first ``sinks`` tokens. logit_cap, slopes: scores capped and biased
+        as in attend()."""
         B = query.shape[0]
         return ops.flash_decode_paged(query, self.k_pages, self.v_pages, self.k_scale[:B],
                                       self.k_zp[:B], self.page_table[:B], self.seq_lens[:B],
@@ -665,7 +666,7 @@ class INT4PagedSequenceCache:
         the GPU; all N by default) tokens of sequences 0..B-1, over the cache that holds
         them: a prompt's chunk after extend(), with the counts given to it. Causal, within a
         window with sinks, with a prefix that every query sees, scores capped or lowered
-        by the distance (ops.flash_attend_paged)."""
+        by the distance (ops.flash_attend_paged, also for how many bits it keeps)."""
         B = query.shape[0]
         return ops.flash_attend_paged(
             query, self.k_pages, self.v_pages, self.k_scale[:B], self.k_zp[:B],
