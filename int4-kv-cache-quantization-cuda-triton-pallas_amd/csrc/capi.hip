@@ -1156,8 +1156,9 @@ struct AttendPlan {
   int chunk, splits;
 };
 
-// Rows a kv-head up to which the kernel of few rows is taken (4 q-heads a kv-head: 8 queries
-// 54 us there, 75 in the other; 12 queries 102 and 79).
+// Rows a kv-head up to which the kernel of few rows is taken (8 sequences of 8192 tokens, 8
+// kv-heads and 32 q-heads of 128 bfloat16 channels: 8 queries 52 us there, 67 in the other; 12
+// queries 106 and 70).
 constexpr int kFewRowsOfHead = 32;
 
 AttendPlan plan_attend(int batch, int num_q_heads, int queries, int window, int sinks, bool wide,
@@ -1175,8 +1176,8 @@ AttendPlan plan_attend(int batch, int num_q_heads, int queries, int window, int 
                       (p.chunk ? (rows + m - 1) / m : (rows + 15) / 16);
   const int64_t slots = (p.chunk || cache->head_dim == 256 ? 1 : 2) * kCUs;
   // Splits that fill the chip. Of few rows one more rather than one less: 384 workgroups
-  // of ragged sequences up to 6000 tokens take 78 us with two splits and 104 with one (of
-  // equal ones 138 and 127).
+  // of ragged sequences up to 6000 tokens take 81 us with two splits and 112 with one (of
+  // equal ones 137 and 131).
   const int64_t fill = p.chunk ? slots / wgs : (slots + wgs - 1) / wgs;
   int64_t s = num_splits > 0 ? num_splits : std::min<int64_t>(fill, (items + 3) / 4);
   s = std::min<int64_t>(std::min<int64_t>(s, items), kMaxSplits);
