@@ -544,8 +544,8 @@ typedef struct fdi4_rotary_options {
  * a sin u) * rotary_scale with u = position * inv_freq[j] in 64 bits; the queries times
  * q_scale. The position of token i is positions[b * p_batch_stride + i * p_token_stride], or
  * with p_token_stride 0 positions[b * p_batch_stride] + i (int32: a cache's lengths before it
- * is extended). head_dim is 64, 128 or 256. Statistics, products and k_out in float32; q_out
- * rounded once. */
+ * is extended). head_dim is 64, 128 or 256. Statistics, products and k_out in float32 (a head
+ * whose squares leave it, from 1e19 on, is normed to zeros); q_out rounded once. */
 int fdi4_norm_rotary(const void* q, const void* k, int dtype, int batch, int tokens,
                      int num_q_heads, int num_kv_heads, int head_dim, int64_t q_batch_stride,
                      int64_t q_head_stride, int64_t q_token_stride, int64_t k_batch_stride,

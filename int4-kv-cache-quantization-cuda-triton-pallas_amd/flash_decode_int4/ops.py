@@ -555,7 +555,7 @@ def norm_rotary(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps: fl
 
     Returns (q, k): contiguous, q in its dtype, rounded once, k in float32, as
     ``extend_int4_paged`` and ``flash_decode_paged_tree`` take it. Angles are formed in 64
-    bits.
+    bits, the mean of squares in float32: a head beyond 1e19 is normed to zeros.
     """
     _require_device_of(q)
     out = load_binding().norm_rotary(q, k, positions, inv_freq, q_weight, k_weight, float(eps),
